@@ -484,6 +484,78 @@ int ttlh_sdpa_fwd(const void* Q, const void* K, const void* V, void* O,
 #define TTLH_SDPA_EIGHT_WAVES 8
 int ttlh_sdpa_fwd_form(int64_t B, int64_t H, int64_t S, int64_t D, int causal);
 
+/* ------------------------------------------------------------------------
+ * Serving from an 8-bit key/value cache (no counterpart in the reference).
+ *
+ * The cache: pages of `page` tokens (16, 32, 64 or 128), for K and for V codes
+ * [pages, heads, page, dim] (contiguous, 16-byte aligned; dim 64 or 128) in int8
+ * or OCP e4m3, and one fp32 scale for each page and head; a value is code * scale.
+ * Position p of sequence b is token p % page of page table[b][p / page] (int32
+ * [seqs, width], rows table_ld apart).  lengths[b] (int32): its tokens, the new
+ * ones of the call among them.  New tokens are packed in `tokens` rows, sequence
+ * b's at starts[b] .. starts[b + 1] (int32 [seqs + 1]; null: tokens = seqs, one
+ * each); the last one is at position lengths[b] - 1.
+ * The three arrays are device memory, read by the kernels, which bound what they
+ * find: a position outside the table or on a page outside the cache is nowhere
+ * (not written, not attended to), tokens outside the packed rows do not exist.   */
+#define TTLH_CACHE_INT8 0
+#define TTLH_CACHE_E4M3 1
+
+typedef struct ttlh_kv_cache {
+  void* k;
+  void* v;
+  float* k_scale;
+  float* v_scale;
+  const int32_t* table;
+  const int32_t* lengths;
+  const int32_t* starts;
+  int64_t table_ld;
+  int64_t pages;
+  int64_t width;
+  int64_t heads;
+  int64_t seqs;
+  int64_t tokens;
+  int32_t page;
+  int32_t dim;
+  int32_t format;
+  int32_t pad;
+} ttlh_kv_cache;
+
+/* k, v: bf16 or f32 [tokens, heads, dim], strides (in elements) for tokens and
+ * heads.  Each goes to its position, as code = x / s rounded to nearest even (ties
+ * to even).  s is the smallest power of two >= 2^-126 with max |x| <= top * s (top:
+ * 127, 448) over the new tokens of the page and head, or the page's scale where it
+ * holds earlier tokens under a larger one; where it holds them under a smaller
+ * one their codes are scaled down and rounded again.  A value that is not finite
+ * makes the scale NaN (and new codes 0): what reads that page and head is NaN.
+ * A page belongs to one sequence in a call.                                      */
+int ttlh_kv_cache_write(const ttlh_kv_cache* cache, const void* k, const void* v, int dtype,
+                        int64_t k_token, int64_t k_head, int64_t v_token, int64_t v_head,
+                        void* stream);
+
+/* O[t, h] = softmax over the positions j that token t (at position p) sees of
+ * cap(scale Q[t, h] . K[j, h / (q_heads / heads)]) V[j, ..], with j <= p, and
+ * j > p - window where window > 0; cap(x) = softcap tanh(x / softcap), or x where
+ * softcap = 0.  A token that sees nothing gets zeros.  Q, O: bf16 [tokens, q_heads,
+ * dim], 16-byte aligned, strides multiples of 8.  fp32 scores and statistics.
+ * `workspace`: ttlh_sdpa_cached_workspace_bytes of device memory, 16-byte aligned. */
+int64_t ttlh_sdpa_cached_workspace_bytes(const ttlh_kv_cache* cache, int64_t q_heads);
+int ttlh_sdpa_cached(const ttlh_kv_cache* cache, const void* Q, void* O, int64_t q_heads,
+                     int64_t q_token, int64_t q_head, int64_t o_token, int64_t o_head,
+                     float scale, int64_t window, float softcap, void* workspace,
+                     int64_t workspace_bytes, void* stream);
+
+/* Rotary positions: in the first `rot` of x's dim elements the plane i (elements i
+ * and i + rot / 2, or 2i and 2i + 1 with interleaved = 1) is turned by the angle
+ * positions[t] * freqs[i] and multiplied by `scale`; the others are copied.
+ * backward = 1 turns the other way: the gradient of x from that of out.
+ * x, out: bf16 or f32 [tokens, heads, dim], strides for tokens and heads; out may be
+ * x itself.  positions: int32 or int64 (pos_bytes 4, 8); freqs: double [rot / 2].   */
+int ttlh_rope(const void* x, void* out, int dtype, const void* positions, int pos_bytes,
+              const double* freqs, int64_t tokens, int64_t heads, int64_t dim, int64_t rot,
+              int64_t x_token, int64_t x_head, int64_t o_token, int64_t o_head, int interleaved,
+              float scale, int backward, void* stream);
+
 /* ------------------------------------------------------------------------ */
 const char* ttlh_last_error(void);
 int ttlh_version(void);

@@ -1,0 +1,313 @@
+"""Rotary positions and the 8-bit key/value cache without a GPU: what the wrappers
+and the library refuse, the frequencies, and the header's rules for positions and
+scales, compiled for the host."""
+
+import ctypes
+import math
+import os
+import shutil
+import subprocess
+
+import pytest
+import torch
+
+from oracle import kv_cache as R
+from ttlhip import _lib as L
+from ttlhip import kernels as K
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+INT8, E4M3 = torch.int8, torch.float8_e4m3fn
+
+
+def _call(**change):
+    """A valid call's arguments on the CPU, some of them changed."""
+    a = dict(k_cache=torch.zeros(6, 2, 16, 64, dtype=INT8), v_cache=torch.zeros(6, 2, 16, 64, dtype=INT8),
+             k_scale=torch.ones(6, 2), v_scale=torch.ones(6, 2),
+             table=torch.zeros(3, 2, dtype=torch.int32), lengths=torch.ones(3, dtype=torch.int32),
+             starts=torch.tensor([0, 2, 3, 5], dtype=torch.int32))
+    a.update(change)
+    return a
+
+
+X = torch.zeros(5, 2, 64, dtype=torch.bfloat16)
+Q = torch.zeros(5, 6, 64, dtype=torch.bfloat16)
+
+BAD_CACHES = [
+    dict(k_cache=torch.zeros(6, 2, 16, 64)),
+    dict(k_cache=torch.zeros(6, 2, 16, 64, dtype=E4M3)),
+    dict(k_cache=torch.zeros(6, 2, 16, 64, dtype=INT8).transpose(1, 2)),
+    dict(k_cache=torch.zeros(6, 2, 16 * 64, dtype=INT8)),
+    dict(v_cache=torch.zeros(7, 2, 16, 64, dtype=INT8)),
+    dict(k_scale=torch.ones(6, 2, dtype=torch.float64)),
+    dict(v_scale=torch.ones(6, 3)),
+    dict(k_scale=torch.ones(6, 4)[:, ::2]),
+    dict(table=torch.zeros(3, 2, dtype=torch.int64)),
+    dict(table=torch.zeros(3, 4, dtype=torch.int32)[:, ::2]),
+    dict(table=torch.zeros(3, dtype=torch.int32)),
+    dict(lengths=torch.ones(2, dtype=torch.int32)),
+    dict(lengths=torch.ones(3, dtype=torch.int64)),
+    dict(starts=torch.zeros(3, dtype=torch.int32)),
+    dict(starts=torch.zeros(4, dtype=torch.int64)),
+    dict(starts=None),  # 5 tokens, 3 sequences
+]
+
+
+@pytest.mark.parametrize("change", BAD_CACHES)
+def test_bad_caches_are_refused(change):
+    with pytest.raises(ValueError):
+        K.kv_cache_write(X, X, **_call(**change))
+    with pytest.raises(ValueError):
+        K.sdpa_cached(Q, o=Q.clone(), scale=0.1, **_call(**change))
+
+
+@pytest.mark.parametrize("k,v", [
+    (X[0], X[0]), (X, X[:4]), (X, X.float()), (torch.zeros(5, 3, 64), torch.zeros(5, 3, 64)),
+    (torch.zeros(5, 2, 128), torch.zeros(5, 2, 128)), (torch.zeros(5, 2, 128)[..., ::2],) * 2])
+def test_bad_tokens_are_refused(k, v):
+    with pytest.raises(ValueError):
+        K.kv_cache_write(k, v, **_call())
+
+
+def test_half_precision_is_refused():
+    with pytest.raises(TypeError):
+        K.kv_cache_write(X.half(), X.half(), **_call())
+
+
+@pytest.mark.parametrize("q,o", [
+    (Q[0], Q[0]), (Q, Q[:4]), (Q.float(), Q.float()), (Q, Q.float()), (Q[:, :3], Q[:, :3].clone()),
+    (torch.zeros(5, 4, 128, dtype=torch.bfloat16),) * 2,
+    (Q, torch.zeros(5, 1, 64, dtype=torch.bfloat16).expand(5, 6, 64)),
+    (Q, torch.zeros(1, 6, 64, dtype=torch.bfloat16).expand(5, 6, 64)),
+    (torch.zeros(5, 6, 68, dtype=torch.bfloat16)[..., :64], Q),
+    (torch.zeros(5 * 6 * 64 + 1, dtype=torch.bfloat16)[1:].view(5, 6, 64), Q)])
+def test_bad_queries_are_refused(q, o):
+    with pytest.raises(ValueError):
+        K.sdpa_cached(q, o=o, scale=0.1, **_call())
+
+
+def test_device_tensors_only():
+    for f in (lambda: K.kv_cache_write(X, X, **_call()),
+              lambda: K.sdpa_cached(Q, o=Q.clone(), scale=0.1, **_call()),
+              lambda: K.rope(X, torch.zeros(5, dtype=torch.int32), K.rope_freqs(64, device="cpu"), X)):
+        with pytest.raises(RuntimeError, match="no CPU path"):
+            f()
+
+
+POS, FREQS = torch.zeros(5, dtype=torch.int32), torch.ones(32, dtype=torch.float64)
+
+
+@pytest.mark.parametrize("change", [
+    dict(x=X[0]), dict(out=X[:4]), dict(out=X.float()), dict(positions=POS[:4]),
+    dict(positions=POS.float()), dict(positions=torch.zeros(10, dtype=torch.int32)[::2]),
+    dict(freqs=FREQS.float()), dict(freqs=torch.ones(33, dtype=torch.float64)),
+    dict(freqs=torch.ones(64, dtype=torch.float64)[::2]), dict(freqs=FREQS[None]),
+    dict(x=torch.zeros(5, 2, 128, dtype=torch.bfloat16)[..., ::2]),
+    dict(out=torch.zeros(5, 1, 64, dtype=torch.bfloat16).expand(5, 2, 64)),
+    dict(out=X.view(2, 5, 64).transpose(0, 1))])
+def test_bad_rope_calls_are_refused(change):
+    a = dict(x=X, positions=POS, freqs=FREQS, out=torch.zeros_like(X))
+    a.update(change)
+    with pytest.raises(ValueError):
+        K.rope(**a)
+
+
+# --- the C ABI ----------------------------------------------------------------
+
+
+def _c_cache(**change):
+    c = L.KVCache(k=4096, v=8192, k_scale=256, v_scale=512, table=1024, lengths=2048, starts=3000,
+                  table_ld=2, pages=6, width=2, heads=2, seqs=3, tokens=5, page=16, dim=64,
+                  format=0, pad=0)
+    for n, x in change.items():
+        setattr(c, n, x)
+    return ctypes.byref(c)
+
+
+@pytest.mark.parametrize("change,status", [
+    (dict(page=24), L.TTLH_EUNSUPPORTED), (dict(page=256), L.TTLH_EUNSUPPORTED),
+    (dict(dim=96), L.TTLH_EUNSUPPORTED), (dict(format=2), L.TTLH_EINVAL),
+    (dict(heads=0), L.TTLH_EINVAL), (dict(pages=-1), L.TTLH_EINVAL), (dict(seqs=-1), L.TTLH_EINVAL),
+    (dict(table_ld=1), L.TTLH_EINVAL), (dict(starts=None), L.TTLH_EINVAL),
+    (dict(k=None), L.TTLH_EINVAL), (dict(k=4100), L.TTLH_EINVAL), (dict(lengths=None), L.TTLH_EINVAL),
+    (dict(table=None), L.TTLH_EINVAL), (dict(v_scale=None), L.TTLH_EINVAL),
+    (dict(width=2 ** 27), L.TTLH_EINVAL), (dict(width=2 ** 27, table_ld=2 ** 27), L.TTLH_EUNSUPPORTED),
+    (dict(tokens=2 ** 28), L.TTLH_EUNSUPPORTED), (dict(pages=2 ** 31), L.TTLH_EUNSUPPORTED)])
+def test_library_refuses_bad_caches(change, status):
+    lib = L.load()
+    assert lib.ttlh_kv_cache_write(_c_cache(**change), 16, 16, 0, 128, 64, 128, 64, None) == status
+    assert lib.ttlh_last_error()
+    assert lib.ttlh_sdpa_cached(_c_cache(**change), 16, 16, 4, 256, 64, 256, 64, 0.1, 0, 0.0, None, 0,
+                                None) == status
+
+
+def test_library_refuses_bad_calls():
+    lib = L.load()
+    E = L.TTLH_EINVAL
+    assert lib.ttlh_kv_cache_write(None, 16, 16, 0, 128, 64, 128, 64, None) == E
+    assert lib.ttlh_kv_cache_write(_c_cache(), 16, 16, 2, 128, 64, 128, 64, None) == E
+    assert lib.ttlh_kv_cache_write(_c_cache(), None, 16, 0, 128, 64, 128, 64, None) == E
+
+    def attention(q=16, o=16, heads=4, strides=(256, 64, 256, 64), scale=0.1, window=0, cap=0.0):
+        return lib.ttlh_sdpa_cached(_c_cache(), q, o, heads, *strides, scale, window, cap, None, 0, None)
+
+    for bad in (dict(q=None), dict(q=8), dict(o=8), dict(heads=3), dict(heads=0), dict(window=-1),
+                dict(strides=(252, 64, 256, 64)), dict(strides=(256, 64, 256, 4)),
+                dict(scale=math.inf), dict(scale=math.nan), dict(cap=-1.0), dict(cap=math.nan),
+                dict(cap=math.inf)):
+        assert attention(**bad) == E, bad
+
+    def rope(x=16, dtype=0, pos=16, pb=4, freqs=16, sizes=(5, 2, 64, 64), scale=1.0):
+        return lib.ttlh_rope(x, x, dtype, pos, pb, freqs, *sizes, 128, 64, 128, 64, 0, scale, 0, None)
+
+    for bad in (dict(x=None), dict(dtype=3), dict(pos=None), dict(pb=2), dict(freqs=None),
+                dict(sizes=(5, 2, 64, 63)), dict(sizes=(5, 2, 64, 66)), dict(sizes=(-1, 2, 64, 64)),
+                dict(sizes=(5, 2, 0, 0)), dict(scale=math.nan)):
+        assert rope(**bad) == E, bad
+    assert rope(sizes=(5, 2, 4096, 2048)) == L.TTLH_EUNSUPPORTED
+    assert rope(sizes=(2 ** 31, 2, 64, 64)) == L.TTLH_EUNSUPPORTED
+
+
+def test_nothing_to_do_is_no_error():
+    lib = L.load()
+    assert lib.ttlh_rope(None, None, 0, None, 4, None, 0, 2, 64, 64, 0, 0, 0, 0, 0, 1.0, 0, None) == 0
+    empty = _c_cache(tokens=0)
+    assert lib.ttlh_kv_cache_write(empty, None, None, 0, 0, 0, 0, 0, None) == 0
+    assert lib.ttlh_sdpa_cached(empty, None, None, 4, 0, 0, 0, 0, 0.1, 0, 0.0, None, 0, None) == 0
+
+
+# --- frequencies --------------------------------------------------------------
+
+
+def test_rope_freqs():
+    f = K.rope_freqs(8, base=10000.0, device="cpu")
+    assert f.dtype == torch.float64
+    assert torch.allclose(f, torch.tensor([1.0, 0.1, 0.01, 0.001], dtype=torch.float64), rtol=1e-14)
+    assert torch.allclose(K.rope_freqs(8, scaling="linear", factor=4.0, device="cpu"), f / 4, rtol=1e-14)
+    b = K.rope_freqs(8, scaling="base", factor=4.0, device="cpu")
+    assert abs(float(b[0]) - 1) < 1e-14 and abs(float(b[-1]) / float(f[-1]) - 0.25) < 1e-14
+    # turns over 4096: 652, 65, 6.5, 0.65: two kept, one blended, one divided
+    p = K.rope_freqs(8, scaling="parts", factor=4.0, original=4096, device="cpu")
+    assert torch.equal(p[:2], f[:2]) and abs(float(p[3] / f[3]) - 0.25) < 1e-14
+    keep = (4096 * 0.01 / (2 * math.pi) - 1) / 31
+    assert abs(float(p[2]) - 0.01 * (keep + (1 - keep) / 4)) < 1e-16
+
+
+@pytest.mark.parametrize("bad", [dict(rot=3), dict(rot=0), dict(rot=8, base=0.0), dict(rot=8, factor=0.5),
+                                 dict(rot=8, scaling="other"), dict(rot=8, scaling="parts", factor=2.0),
+                                 dict(rot=8, scaling="parts", original=10, fast=1.0, slow=1.0)])
+def test_bad_frequencies_are_refused(bad):
+    with pytest.raises(ValueError):
+        K.rope_freqs(device="cpu", **bad)
+
+
+# --- the header's rules, on the host ------------------------------------------
+
+SOURCE = r"""
+#include "ttlh_kvcache.h"
+extern "C" float scale_for(float a, int f) { return ttlh::scale_for(a, f); }
+extern "C" float joined(float a, float b) { return ttlh::joined_scale(a, b); }
+static ttlh::CacheArgs args(const int32_t* t, int ld, int width, int pages, int shift, const int32_t* starts,
+                            int tokens) {
+  ttlh::CacheArgs c = {};
+  c.table = t; c.table_ld = ld; c.width = width; c.pages = pages; c.shift = shift; c.starts = starts;
+  c.tokens = tokens; c.heads = 8; c.dim = 128;
+  return c;
+}
+extern "C" int page_at(const int32_t* t, int ld, int width, int pages, int shift, int b, int pos) {
+  return ttlh::page_at(args(t, ld, width, pages, shift, nullptr, 0), b, pos);
+}
+extern "C" void tokens_of(const int32_t* s, int tokens, int b, int* out) {
+  ttlh::seq_tokens(args(nullptr, 0, 0, 0, 4, s, tokens), b, out[0], out[1]);
+}
+extern "C" void seen(int width, int len, int n, int i, int window, int* out) {
+  ttlh::seen_by(args(nullptr, 0, width, 0, 4, nullptr, 0), len, n, i, window, out[0], out[1]);
+}
+extern "C" int64_t offset(int page, int head, int slot) {
+  return ttlh::slot_offset(args(nullptr, 0, 0, 0, 7, nullptr, 0), page, head, slot);
+}
+"""
+
+
+@pytest.fixture(scope="module")
+def rules(tmp_path_factory):
+    gxx = shutil.which("g++")
+    if gxx is None:
+        pytest.skip("no g++")
+    d = tmp_path_factory.mktemp("rules")
+    (d / "rules.cpp").write_text(SOURCE)
+    subprocess.run([gxx, "-std=c++17", "-O1", "-shared", "-fPIC", "-I", os.path.join(ROOT, "include"),
+                    "-I", os.path.join(ROOT, "tt-lang_amd", "csrc"), str(d / "rules.cpp"), "-o",
+                    str(d / "rules.so")], check=True)
+    lib = ctypes.CDLL(str(d / "rules.so"))
+    lib.scale_for.restype = lib.joined.restype = ctypes.c_float
+    lib.scale_for.argtypes = [ctypes.c_float, ctypes.c_int]
+    lib.joined.argtypes = [ctypes.c_float, ctypes.c_float]
+    lib.offset.restype = ctypes.c_int64
+    return lib
+
+
+@pytest.mark.parametrize("fmt,dtype", [(0, INT8), (1, E4M3)])
+def test_scales_are_the_smallest_powers_of_two(rules, fmt, dtype):
+    vals = [0.0, 1e-45, 1e-38, 2.0 ** -126, 2.0 ** -120, 1.0, 126.9, 127.0, 127.00001, 254.0, 254.1, 448.0,
+            448.1, 3.4028234e38, 1e-30, 0.3]
+    vals += [float(v) for v in torch.randn(200, generator=torch.Generator().manual_seed(1)).abs()]
+    for a in vals:
+        a = ctypes.c_float(a).value
+        s = rules.scale_for(a, fmt)
+        assert s == R.scale_for(a, dtype), a
+        assert R.TOP[dtype] * s >= a
+    assert math.isnan(rules.scale_for(math.inf, fmt)) and math.isnan(rules.scale_for(math.nan, fmt))
+
+
+def test_joined_scales(rules):
+    nan, inf = math.nan, math.inf
+    assert rules.joined(1.0, 2.0) == 2.0 and rules.joined(2.0, 1.0) == 2.0
+    assert rules.joined(0.0, 1.0) == 1.0 and rules.joined(-1.0, 1.0) == 1.0
+    for a, b in ((nan, 1.0), (1.0, nan), (inf, 1.0)):
+        assert math.isnan(rules.joined(a, b))
+
+
+def test_positions_outside_have_no_page(rules):
+    t = (ctypes.c_int32 * 8)(0, 5, -1, 6, 2, 2 ** 31 - 1, -2 ** 31, 3)
+    at = lambda b, pos: rules.page_at(t, 4, 4, 6, 4, b, pos)  # noqa: E731
+    assert [at(0, p) for p in (0, 15, 16, 31, 32, 48, 63)] == [0, 0, 5, 5, -1, -1, -1]
+    assert [at(1, p) for p in (0, 16, 32, 48)] == [2, -1, -1, 3]
+    for pos in (-1, -2 ** 31, 64, 2 ** 31 - 1):
+        assert at(0, pos) == -1
+    assert rules.page_at(t, 4, 0, 6, 4, 0, 0) == -1
+
+
+def test_tokens_outside_the_packed_rows_do_not_exist(rules):
+    def of(starts, tokens):
+        s, out = (ctypes.c_int32 * len(starts))(*starts), (ctypes.c_int * 2)()
+        res = []
+        for b in range(len(starts) - 1):
+            rules.tokens_of(s, tokens, b, out)
+            res.append((out[0], out[1]))
+        return res
+    assert of([0, 2, 2, 5], 5) == [(0, 2), (2, 0), (2, 3)]
+    for starts in ([-3, 12, 500], [15, 5, 20], [2 ** 31 - 1, -2 ** 31, 7], [30, 31, 32]):
+        for first, n in of(starts, 20):
+            assert 0 <= first <= first + n <= 20
+
+
+def test_what_a_token_sees(rules):
+    def seen(*a):
+        out = (ctypes.c_int * 2)()
+        rules.seen(*a, out)
+        return range(out[0], out[1])
+    big = 2 ** 31 - 1
+    for width in (0, 3, 2 ** 27 - 1):
+        for length in (0, 1, 20, 48, 60, big, -1, -big - 1):
+            for n in (1, 7, 2 ** 28 - 1):
+                for i in {0, n // 2, n - 1}:
+                    for window in (0, 1, 5, big):
+                        end = length - n + i + 1
+                        want = range(max(0, end - window) if window else 0, max(0, end))
+                        want = range(min(want.start, 16 * width), min(want.stop, 16 * width))
+                        got = seen(width, length, n, i, window)
+                        assert list(got[:3]) == list(want[:3]) and len(got) == len(want)
+
+
+def test_offsets_pass_32_bits(rules):
+    assert rules.offset(2 ** 20, 7, 127) == ((2 ** 20 * 8 + 7) * 128 + 127) * 128

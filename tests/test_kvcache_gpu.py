@@ -1,0 +1,641 @@
+"""Rotary positions and the 8-bit key/value cache on the MI355X against float64
+restatements (oracle/kv_cache.py).
+
+Tolerances, derived:
+* rope: a c - b s with c and s one rounding of scale times an fp32 rounding of the
+  exact cosine, two products and a sum: (|a| + |b|) scale 5 * 2^-24, and for bf16 a
+  rounding of the result, 2^-8 of it.
+* kv_cache_write: codes and scales are equal: scales are powers of two, so every
+  quotient is exact and each code one rounding of an exact value.
+* sdpa_cached: p v sums run over bf16 roundings of p (2^-8 each: 2^-8 sum p |v|),
+  the result is rounded to bf16 (2^-8 of it).  Scores are fp32 sums of dim products
+  and a few factors, off by at most (dim + 16) 2^-24 of the sum of |q k| scale (and by
+  2^-21 softcap where capped), which moves p, in numerator and denominator, by twice
+  that; n terms in fp32 sums add (n + 64) 2^-24, exponentials 2^-21.
+"""
+
+import math
+
+import pytest
+import torch
+
+from oracle import kv_cache as R
+from ttlhip import kernels as K
+
+pytestmark = pytest.mark.gpu
+
+INT8, E4M3 = torch.int8, torch.float8_e4m3fn
+BF16, F32 = torch.bfloat16, torch.float32
+
+
+def _gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+# --- rope ---------------------------------------------------------------------
+
+
+def _check_rope(out, x, positions, freqs, interleaved, scale, backward):
+    ref = R.rope(x, positions, freqs, interleaved, scale, backward)
+    r = 2 * freqs.numel()
+    big = x.double().abs()
+    both = big.clone()  # |a| + |b| of an element's plane
+    if interleaved:
+        pair = big[..., 0:r:2] + big[..., 1:r:2]
+        both[..., 0:r:2], both[..., 1:r:2] = pair, pair
+    else:
+        pair = big[..., : r // 2] + big[..., r // 2 : r]
+        both[..., :r] = torch.cat((pair, pair), -1)
+    tol = both * abs(scale) * 5 * 2.0 ** -24
+    tol[..., r:] = 0
+    if out.dtype == BF16:
+        tol = tol + 2.0 ** -8 * ref.abs() * (1 + 2.0 ** -20) + (tol * 2.0 ** -8)
+        tol[..., r:] = 0
+    bad = (out.double() - ref).abs() > tol
+    assert not bad.any(), (int(bad.sum()), float(((out.double() - ref).abs() - tol).max()))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("tokens,heads,dim,rot", [
+    (1, 1, 64, 64), (1, 40, 128, 128), (3, 5, 80, 32), (7, 3, 96, 64), (130, 2, 10, 6),
+    (2, 2, 7, 2), (5, 1, 128, 0), (2, 70, 128, 128), (1, 3, 2048, 1024), (9, 1, 3, 0),
+    (4100, 2, 32, 16)])
+def test_rope(dtype, interleaved, tokens, heads, dim, rot):
+    g = _gen(tokens + heads + dim)
+    x = torch.randn(tokens, heads, dim, generator=g).to(dtype)
+    pos = torch.randint(0, 5000, (tokens,), generator=g, dtype=torch.int32)
+    f = 10000.0 ** (-torch.arange(0, rot, 2, dtype=torch.float64) / max(rot, 1))
+    for backward in (False, True):
+        out = torch.full_like(x, 7.0).cuda()
+        K.rope(x.cuda(), pos.cuda(), f.cuda(), out, interleaved, 1.25, backward)
+        _check_rope(out.cpu(), x, pos, f, interleaved, 1.25, backward)
+
+
+@pytest.mark.parametrize("far", [2 ** 20, 2 ** 24 + 3, 2 ** 31 - 64])
+def test_rope_far_positions_keep_their_angles(far):
+    g = _gen(3)
+    x = torch.randn(64, 2, 128, generator=g)
+    pos = far + torch.arange(64)
+    f = K.rope_freqs(128, device="cpu")
+    out = torch.empty_like(x, device="cuda")
+    K.rope(x.cuda(), pos.cuda(), f.cuda(), out)
+    _check_rope(out.cpu(), x, pos, f, False, 1.0, False)
+    neg = torch.empty_like(x, device="cuda")
+    K.rope(x.cuda(), -pos.cuda(), f.cuda(), neg)
+    _check_rope(neg.cpu(), x, -pos, f, False, 1.0, False)
+
+
+@pytest.mark.parametrize("offset", [0, 1])
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_rope_in_place_in_a_projection(offset, interleaved):
+    """q and k of one buffer in one call, in place; v beside them stays.  offset 1:
+    addresses that vectors cannot have."""
+    g = _gen(5)
+    buf = torch.randn(33, 12 * 64 + 8, generator=g).to(BF16).cuda()
+    qk = buf[:, offset:offset + 8 * 64].unflatten(1, (8, 64))
+    before = buf.clone()
+    pos = torch.arange(33, dtype=torch.int32)
+    f = K.rope_freqs(64, device="cpu")
+    K.rope(qk, pos.cuda(), f.cuda(), qk, interleaved)
+    old = before[:, offset:offset + 512].unflatten(1, (8, 64)).cpu()
+    _check_rope(qk.cpu(), old, pos, f, interleaved, 1.0, False)
+    assert torch.equal(buf[:, offset + 512:], before[:, offset + 512:])
+    assert torch.equal(buf[:, :offset], before[:, :offset])
+
+
+def test_rope_heads_before_tokens():
+    g = _gen(6)
+    x = torch.randn(4, 50, 64, generator=g).to(BF16)  # [heads, tokens, dim]
+    pos = torch.arange(50, dtype=torch.int64) * 7
+    f = K.rope_freqs(64, device="cpu")
+    out = torch.empty_like(x, device="cuda")
+    K.rope(x.cuda().transpose(0, 1), pos.cuda(), f.cuda(), out.transpose(0, 1))
+    _check_rope(out.cpu().transpose(0, 1), x.transpose(0, 1), pos, f, False, 1.0, False)
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_rope_gradient(interleaved):
+    """backward against the formula's gradient (autograd of the float64 form) and
+    against differences of the forward kernel."""
+    g = _gen(7)
+    x, dy = torch.randn(5, 3, 32, generator=g), torch.randn(5, 3, 32, generator=g)
+    pos = torch.tensor([0, 1, 17, 999, 123456], dtype=torch.int32)
+    f = K.rope_freqs(16, device="cpu")
+    dx = torch.empty_like(x, device="cuda")
+    K.rope(dy.cuda(), pos.cuda(), f.cuda(), dx, interleaved, 1.5, backward=True)
+    xd = x.double().requires_grad_()
+    a = pos.double()[:, None] * f
+    c, s = 1.5 * torch.cos(a)[:, None], 1.5 * torch.sin(a)[:, None]
+    u, w = (xd[..., 0:16:2], xd[..., 1:16:2]) if interleaved else (xd[..., :8], xd[..., 8:16])
+    yu, yw = u * c - w * s, w * c + u * s
+    du, dw = (dy[..., 0:16:2], dy[..., 1:16:2]) if interleaved else (dy[..., :8], dy[..., 8:16])
+    ((yu * du).sum() + (yw * dw).sum() + (xd[..., 16:] * dy[..., 16:]).sum()).backward()
+    # |dy| <= 6 here: both elements of a plane, 5 roundings of 2^-24
+    assert float((dx.cpu().double() - xd.grad).abs().max()) <= 2 * 6 * 1.5 * 5 * 2.0 ** -24
+    # the map is linear: differences of step 2 around x = 0 are its columns, exactly
+    # rounded like the outputs (|x| = 1: 1.5 * 5 * 2^-24 each, times 32 of dy)
+    for i in (0, 3, 9, 15, 16, 31):
+        e = torch.zeros_like(x)
+        e[..., i] = 1.0
+        up, down = torch.empty_like(dx), torch.empty_like(dx)
+        K.rope(e.cuda(), pos.cuda(), f.cuda(), up, interleaved, 1.5)
+        K.rope(-e.cuda(), pos.cuda(), f.cuda(), down, interleaved, 1.5)
+        diff = (((up - down) / 2).cpu().double() * dy.double()).sum(-1)
+        assert float((diff - dx[..., i].cpu().double()).abs().max()) <= 32 * 6 * 1.5 * 6 * 2.0 ** -24
+
+
+# --- the cache ----------------------------------------------------------------
+
+
+def _cache(pages, heads, page, dim, dtype, seed):
+    """Pages filled with something: codes of every kind (NaN's too, in e4m3)."""
+    g = _gen(seed)
+    raw = [torch.randint(0, 256, (pages, heads, page, dim), generator=g, dtype=torch.uint8)
+           for _ in range(2)]
+    sc = [torch.exp2(torch.randint(-6, 3, (pages, heads), generator=g).float()) for _ in range(2)]
+    return [raw[0].view(dtype), raw[1].view(dtype), sc[0], sc[1]]
+
+
+def _table(need, width, pages, seed):
+    order = torch.randperm(pages, generator=_gen(seed)).to(torch.int32)
+    t = torch.full((len(need), width), -1, dtype=torch.int32)
+    at = 0
+    for b, n in enumerate(need):
+        t[b, :n] = order[at:at + n]
+        at += n
+    return t
+
+
+def _same(a, b):
+    return torch.equal(a.view(torch.uint8) if a.dtype == E4M3 else a,
+                       b.view(torch.uint8) if b.dtype == E4M3 else b)
+
+
+def _run_write(k, v, cache, table, lengths, starts=None):
+    """The kernel on copies against the oracle on copies; returns the kernel's."""
+    ref, dev = [c.clone() for c in cache], [c.cuda() for c in cache]
+    R.write(k, v, *ref, table, lengths, starts)
+    K.kv_cache_write(k.cuda(), v.cuda(), *dev, table.cuda(), lengths.cuda(),
+                     starts=None if starts is None else starts.cuda())
+    got = [c.cpu() for c in dev]
+    for name, x, y in zip(("k", "v", "k_scale", "v_scale"), got, ref):
+        if x.dtype == F32:
+            assert torch.equal(x.isnan(), y.isnan()), name
+            x, y = x.nan_to_num(), y.nan_to_num()
+        if x.dtype == E4M3:  # -0 and 0 are one value
+            x, y = x.float().nan_to_num(500.0), y.float().nan_to_num(500.0)
+        assert torch.equal(x, y), (name, int((x != y).sum()))
+    return got
+
+
+def _random_call(lens, news, heads, dim, page, dtype, cdtype, seed, one=False):
+    need = [-(-n // page) for n in lens]
+    pages = sum(need) + 2
+    table = _table(need, max(need) + 1, pages, seed)
+    cache = _cache(pages, heads, page, dim, cdtype, seed + 1)
+    g = _gen(seed + 2)
+    t = sum(news)
+    k = (torch.randn(t, heads, dim, generator=g) * torch.exp2(4 * torch.randn(t, heads, 1, generator=g)))
+    v = torch.randn(t, heads, dim, generator=g) * 0.01
+    starts = None if one else torch.tensor([sum(news[:i]) for i in range(len(news) + 1)],
+                                           dtype=torch.int32)
+    return k.to(dtype), v.to(dtype), cache, table, torch.tensor(lens, dtype=torch.int32), starts
+
+
+def _valid_codes(cache, table, lengths, news, page):
+    """Earlier tokens' codes as a write leaves them: no NaN."""
+    if cache[0].dtype != E4M3:
+        return
+    for c in cache[:2]:
+        raw = c.view(torch.uint8)
+        raw[(raw & 0x7f) == 0x7f] = 0x12
+
+
+@pytest.mark.parametrize("cdtype", [INT8, E4M3])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("page,dim", [(16, 64), (16, 128), (32, 128), (64, 64), (64, 128), (128, 128)])
+def test_write_ragged(cdtype, dtype, page, dim):
+    lens, news = [1, 17, 200, 128, 129, 65, 64, 300], [1, 17, 1, 128, 2, 0, 5, 299]
+    call = _random_call(lens, news, 3, dim, page, dtype, cdtype, page + dim)
+    _valid_codes(call[2], call[3], lens, news, page)
+    _run_write(*call)
+
+
+@pytest.mark.parametrize("cdtype", [INT8, E4M3])
+@pytest.mark.parametrize("seqs,heads,dim", [(1, 1, 64), (1, 8, 128), (70, 3, 128), (5, 17, 64)])
+def test_write_one_token_each(cdtype, seqs, heads, dim):
+    lens = [1 + (37 * b) % 150 for b in range(seqs)]
+    call = _random_call(lens, [1] * seqs, heads, dim, 32, BF16, cdtype, seqs, one=True)
+    _valid_codes(call[2], call[3], lens, None, 32)
+    _run_write(*call)
+
+
+@pytest.mark.parametrize("cdtype", [INT8, E4M3])
+def test_write_token_by_token_follows_the_definition(cdtype):
+    """40 calls of one token, magnitudes growing: every growth rounds again."""
+    cache = _cache(4, 2, 16, 64, cdtype, 9)
+    table = torch.tensor([[2, 0, 3]], dtype=torch.int32)
+    g = _gen(10)
+    for i in range(40):
+        k = torch.randn(1, 2, 64, generator=g) * 1.1 ** i
+        v = torch.randn(1, 2, 64, generator=g)
+        cache = _run_write(k, v, cache, table, torch.tensor([i + 1], dtype=torch.int32))
+    # every key is within the last rounding and those before it, each at half the step
+    # of the one before: less than one step of the final scale (int8)
+    if cdtype == INT8:
+        assert float(cache[0][2].float().abs().max()) <= 127
+
+
+@pytest.mark.parametrize("cdtype", [INT8, E4M3])
+@pytest.mark.parametrize("value", [0.0, -0.0, 1e-45, 2.0 ** -126, 127.0, 127.00001, 448.0, 449.0, 254.0,
+                                   3.4028234e38, math.inf, -math.inf, math.nan])
+def test_write_special_values(cdtype, value):
+    cache = _cache(2, 1, 16, 64, cdtype, 11)
+    _valid_codes(cache, None, None, None, 16)
+    k = torch.zeros(2, 1, 64)
+    k[1, 0, 5] = value
+    v = torch.randn(2, 1, 64, generator=_gen(1))
+    table = torch.tensor([[1]], dtype=torch.int32)
+    for length in (2, 5):  # a new page; one that holds tokens
+        _run_write(k, v, cache, table, torch.tensor([length], dtype=torch.int32),
+                   torch.tensor([0, 2], dtype=torch.int32))
+
+
+def test_write_after_nan_stays_nan_until_the_page_begins_anew():
+    cache = _cache(1, 1, 16, 64, INT8, 12)
+    table = torch.zeros(1, 1, dtype=torch.int32)
+    k = torch.full((1, 1, 64), math.nan)
+    one = torch.ones(1, 1, 64)
+    cache = _run_write(k, one, cache, table, torch.tensor([1], dtype=torch.int32))
+    cache = _run_write(one, one, cache, table, torch.tensor([2], dtype=torch.int32))
+    assert math.isnan(cache[2][0, 0])
+    cache = _run_write(one, one, cache, table, torch.tensor([1], dtype=torch.int32))
+    assert float(cache[2][0, 0]) == 2.0 ** -6
+
+
+@pytest.mark.parametrize("lens,starts,table", [
+    ([40, 20], [0, 10, 20], [[-1, 1, 99], [0, -7, 2]]),         # pages that do not exist
+    ([500, 3], [0, 10, 20], [[0, 1, 2], [3, 4, 5]]),            # past the table, before position 0
+    ([-5, 0], [0, 10, 20], [[0, 1, 2], [3, 4, 5]]),             # no tokens
+    ([20, 20], [-3, 12, 500], [[0, 1, 2], [3, 4, 5]]),          # starts outside the packed rows
+    ([20, 20], [15, 5, 20], [[0, 1, 2], [3, 4, 5]]),            # starts that go back
+    ([2 ** 31 - 1, -2 ** 31], [0, 10, 20], [[0, 1, 2], [3, 4, 5]]),
+])
+@pytest.mark.parametrize("cdtype", [INT8, E4M3])
+def test_tables_lengths_and_starts_out_of_range_touch_nothing(cdtype, lens, starts, table):
+    cache = _cache(6, 2, 16, 64, cdtype, 13)
+    _valid_codes(cache, None, None, None, 16)
+    g = _gen(14)
+    k, v = torch.randn(20, 2, 64, generator=g), torch.randn(20, 2, 64, generator=g)
+    t, n, s = (torch.tensor(x, dtype=torch.int32) for x in (table, lens, starts))
+    got = _run_write(k, v, cache, t, n, s)
+    q = torch.randn(20, 4, 64, generator=g).to(BF16)
+    _check_attention(q, got, t, n, s, 0.125)
+
+
+def test_write_strided_views():
+    g = _gen(15)
+    qkv = torch.randn(50, 12, 128, generator=g).to(BF16)
+    lens = torch.tensor([50], dtype=torch.int32)
+    starts = torch.tensor([0, 50], dtype=torch.int32)
+    table = torch.tensor([[1, 0]], dtype=torch.int32)
+    cache = _cache(2, 2, 32, 128, INT8, 16)
+    ref = [c.clone() for c in cache]
+    R.write(qkv[:, 8:10], qkv[:, 10:12], *ref, table, lens, starts)
+    dev, d = [c.cuda() for c in cache], qkv.cuda()
+    wide = torch.full((1, 5), -1, dtype=torch.int32)
+    wide[:, :2] = table
+    K.kv_cache_write(d[:, 8:10], d[:, 10:12], *dev, wide.cuda()[:, :2], lens.cuda(), starts.cuda())
+    for x, y in zip(dev, ref):
+        assert _same(x.cpu(), y)
+    # off every vector's address, heads before tokens
+    flat = torch.randn(1 + 2 * 50 * 128, generator=g)
+    x = flat[1:].view(2, 50, 128).transpose(0, 1)
+    ref, dev = [c.clone() for c in cache], [c.cuda() for c in cache]
+    R.write(x, x, *ref, table, lens, starts)
+    xd = flat.cuda()[1:].view(2, 50, 128).transpose(0, 1)
+    K.kv_cache_write(xd, xd, *dev, table.cuda(), lens.cuda(), starts.cuda())
+    for a, b in zip(dev, ref):
+        assert _same(a.cpu(), b)
+
+
+# --- attention ----------------------------------------------------------------
+
+
+def _tolerance(ref, size, reach, dim, n, softcap):
+    off = (dim + 16) * 2.0 ** -24 * reach + 2.0 ** -21 * softcap
+    share = 2.0 ** -8 + 2 * off + 2 * (n + 64) * 2.0 ** -24 + 2 * 2.0 ** -21
+    return size * share + 2.0 ** -8 * (ref.abs() + size * share) + 1e-37
+
+
+def _check_attention(q, cache, table, lengths, starts, scale, window=0, softcap=0.0, o=None):
+    ref, size, reach = R.attention(q, *cache, table, lengths, scale, starts, window, softcap)
+    out = torch.full_like(q, 7.0).cuda() if o is None else o
+    K.sdpa_cached(q.cuda() if not q.is_cuda else q, *[c.cuda() for c in cache], table.cuda(),
+                  lengths.cuda(), out, scale,
+                  starts=None if starts is None else starts.cuda(), window=window, softcap=softcap)
+    got = out.cpu()
+    n = max([1] + [min(int(x), table.shape[1] * cache[0].shape[2]) for x in lengths])
+    tol = _tolerance(ref, size, reach, q.shape[2], n, softcap)
+    owned = torch.zeros(q.shape[0], dtype=torch.bool)
+    for first, m in R.spans(lengths, starts, q.shape[0]):
+        owned[first:first + m] = True
+    assert (got[~owned] == 7.0).all(), "rows of no sequence"
+    got, ref, tol = got[owned].double(), ref[owned], tol[owned]
+    assert torch.equal(got.isnan(), ref.isnan())
+    err = (got - ref).abs().nan_to_num()
+    assert (err <= tol.nan_to_num(1.0)).all(), (float((err - tol).max()), float(err.max()))
+    return got
+
+
+def _attention_call(lens, news, heads, group, dim, page, cdtype, seed, one=False, loud=1.5):
+    need = [-(-max(n, 0) // page) for n in lens]
+    pages = sum(need) + 2
+    table = _table(need, max(need) + 1, pages, seed)
+    cache = _cache(pages, heads, page, dim, cdtype, seed + 1)
+    # what a write leaves in the tokens' slots; the others keep any code
+    g = _gen(seed + 2)
+    codes = []
+    for c in cache[:2]:
+        x = (torch.randn(c.shape, generator=g) * 40).clamp(-127, 127)
+        x = x.round().to(torch.int8) if cdtype == INT8 else x.to(E4M3)
+        raw = x.view(torch.uint8)
+        keep = torch.zeros(pages, page, dtype=torch.bool)
+        for b, n in enumerate(lens):
+            for j in range(n):
+                keep[table[b, j // page], j % page] = True
+        raw = torch.where(keep[:, None, :, None], raw, c.view(torch.uint8))
+        codes.append(raw.view(cdtype))
+    sc = [torch.exp2(torch.randint(-7, -3, (pages, heads), generator=g).float()) for _ in range(2)]
+    q = (torch.randn(sum(news), heads * group, dim, generator=g) * loud).to(BF16)
+    starts = None if one else torch.tensor([sum(news[:i]) for i in range(len(news) + 1)],
+                                           dtype=torch.int32)
+    return q, codes + sc, table, torch.tensor(lens, dtype=torch.int32), starts
+
+
+@pytest.mark.parametrize("cdtype", [INT8, E4M3])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("page", [16, 32, 64, 128])
+def test_attention_one_token_each(cdtype, dim, page):
+    lens = [1, 2, 15, 16, 17, 31, 33, 64, 65, 127, 130, 200]
+    q, cache, table, n, _ = _attention_call(lens, [1] * len(lens), 2, 4, dim, page, cdtype, 21, True)
+    _check_attention(q, cache, table, n, None, dim ** -0.5)
+
+
+@pytest.mark.parametrize("heads,group", [(1, 1), (1, 2), (3, 3), (2, 7), (1, 8), (1, 16), (2, 17),
+                                         (1, 32), (1, 40), (5, 1)])
+@pytest.mark.parametrize("news", [[1, 1], [2, 3], [9, 1], [40, 33], [0, 5]])
+def test_attention_groups_and_tokens(heads, group, news):
+    lens = [150, 75]
+    q, cache, table, n, starts = _attention_call(lens, news, heads, group, 64, 32, INT8, 22)
+    _check_attention(q, cache, table, n, starts, 0.125)
+
+
+@pytest.mark.parametrize("cdtype", [INT8, E4M3])
+@pytest.mark.parametrize("dim,page", [(64, 16), (128, 16), (128, 64), (64, 128)])
+@pytest.mark.parametrize("lens,news", [
+    ([130, 1, 33], [130, 1, 33]),           # whole prompts
+    ([257], [257]),
+    ([300, 128, 64, 190], [100, 128, 1, 7]),
+    ([513], [65]),
+])
+def test_attention_chunks(cdtype, dim, page, lens, news):
+    q, cache, table, n, starts = _attention_call(lens, news, 2, 2, dim, page, cdtype, 23)
+    _check_attention(q, cache, table, n, starts, dim ** -0.5)
+
+
+@pytest.mark.parametrize("window", [1, 2, 16, 31, 100, 1000, 2 ** 31 - 1, 2 ** 40])
+@pytest.mark.parametrize("news", [[1, 1], [130, 40]])
+def test_attention_window(window, news):
+    q, cache, table, n, starts = _attention_call([300, 55], news, 2, 4, 128, 32, INT8, 24)
+    _check_attention(q, cache, table, n, starts, 0.09, window=window)
+
+
+@pytest.mark.parametrize("softcap", [0.5, 30.0, 1e4])
+@pytest.mark.parametrize("news", [[1, 1], [130, 40]])
+@pytest.mark.parametrize("window", [0, 50])
+def test_attention_softcap(softcap, news, window):
+    q, cache, table, n, starts = _attention_call([300, 55], news, 2, 4, 128, 32, E4M3, 25, loud=4.0)
+    _check_attention(q, cache, table, n, starts, 0.09, window=window, softcap=softcap)
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.09, 1.0])
+@pytest.mark.parametrize("news", [[1, 1], [70, 40]])
+def test_attention_scales(scale, news):
+    q, cache, table, n, starts = _attention_call([300, 55], news, 2, 4, 128, 32, INT8, 26)
+    _check_attention(q, cache, table, n, starts, scale)
+
+
+@pytest.mark.parametrize("news", [[1, 1, 1], [130, 20, 40]])
+def test_attention_missing_pages_and_rows_that_see_nothing(news):
+    q, cache, table, n, starts = _attention_call([300, 55, 90], news, 2, 4, 128, 32, E4M3, 27)
+    table[0, 2] = -1
+    table[0, 5] = 10 ** 6
+    table[1] = -1  # nothing to see: zeros
+    got = _check_attention(q, cache, table, n, starts, 0.09)
+    assert (got[news[0]:news[0] + news[1]] == 0).all()
+    _check_attention(q, cache, table, n, starts, 0.09, window=20)
+
+
+@pytest.mark.parametrize("which", [2, 3])
+@pytest.mark.parametrize("news", [[1, 1], [130, 55]])
+def test_attention_nan_reaches_only_the_tokens_that_see_it(which, news):
+    """A page's NaN scale: the tokens that see any of it, in its head."""
+    q, cache, table, n, starts = _attention_call([300, 55], news, 2, 4, 128, 32, INT8, 28)
+    cache[which][table[0, 7], 1] = math.nan  # positions 224 .. 255
+    cache[which][table[1, 1], 0] = math.nan  # positions 32 .. 54
+    got = _check_attention(q, cache, table, n, starts, 0.09)
+    assert got.isnan().any() and not got.isnan().all()
+    got = _check_attention(q, cache, table, n, starts, 0.09, window=20)
+    if news[0] > 1:
+        assert got.isnan().any() and not got.isnan().all()
+
+
+@pytest.mark.parametrize("news", [[1, 1], [70, 40]])
+def test_attention_of_queries_that_are_not_finite(news):
+    q, cache, table, n, starts = _attention_call([300, 55], news, 1, 4, 64, 32, INT8, 29)
+    q[0, 1, 3] = math.nan
+    q[1, 2, 5] = math.nan
+    got = _check_attention(q, cache, table, n, starts, 0.125)
+    assert int(got.isnan().any(-1).sum()) == 2
+
+
+@pytest.mark.parametrize("news", [[1, 1], [130, 55]])
+def test_attention_large_scores(news):
+    """Scores that differ by thousands: exponentials of 0 beside one of 1."""
+    q, cache, table, n, starts = _attention_call([300, 55], news, 2, 2, 64, 16, INT8, 30, loud=3000.0)
+    ref, size, reach = R.attention(q, *cache, table, n, 0.125, starts)
+    out = torch.empty_like(q, device="cuda")
+    K.sdpa_cached(q.cuda(), *[c.cuda() for c in cache], table.cuda(), n.cuda(), out, 0.125,
+                  starts=starts.cuda())
+    assert torch.isfinite(out).all()
+    tol = _tolerance(ref, size, reach, 64, 300, 0.0)
+    assert ((out.cpu().double() - ref).abs() <= tol).all()
+
+
+def test_attention_strided_views():
+    q, cache, table, n, starts = _attention_call([100, 55], [37, 20], 2, 4, 64, 32, INT8, 31)
+    buf = torch.zeros(57, 20, 64, dtype=BF16, device="cuda")
+    buf[:, 4:12] = q.cuda()
+    o = torch.full((8, 57, 64), 7.0, dtype=BF16, device="cuda").transpose(0, 1)
+    ref = torch.full((57, 8, 64), 7.0, dtype=BF16, device="cuda")
+    dev = [c.cuda() for c in cache]
+    K.sdpa_cached(buf[:, 4:12], *dev, table.cuda(), n.cuda(), o, 0.125, starts=starts.cuda())
+    K.sdpa_cached(q.cuda(), *dev, table.cuda(), n.cuda(), ref, 0.125, starts=starts.cuda())
+    assert torch.equal(o, ref)
+
+
+def test_rows_behind_the_last_sequence_stay():
+    q, cache, table, n, starts = _attention_call([100, 55], [37, 20], 2, 4, 64, 32, INT8, 32)
+    q = torch.cat((q, torch.ones(9, 8, 64, dtype=BF16)))
+    _check_attention(q, cache, table, n, starts, 0.125)
+
+
+def test_empty_calls():
+    cache = [c.cuda() for c in _cache(2, 2, 16, 64, INT8, 33)]
+    none = torch.zeros(0, 4, 64, dtype=BF16, device="cuda")
+    before = [c.clone() for c in cache]
+    for seqs, starts in ((0, None), (0, torch.zeros(1, dtype=torch.int32, device="cuda")),
+                         (3, torch.zeros(4, dtype=torch.int32, device="cuda"))):
+        table = torch.zeros(seqs, 2, dtype=torch.int32, device="cuda")
+        n = torch.ones(seqs, dtype=torch.int32, device="cuda")
+        K.kv_cache_write(none[:, :2], none[:, :2], *cache, table, n, starts=starts)
+        K.sdpa_cached(none, *cache, table, n, torch.empty_like(none), 0.1, starts=starts)
+    K.rope(none, torch.zeros(0, dtype=torch.int32, device="cuda"), K.rope_freqs(64), none)
+    # a table without columns: nothing to write to, nothing to see
+    one = torch.ones(1, 4, 64, dtype=BF16, device="cuda")
+    o = torch.full_like(one, 7.0)
+    table = torch.zeros(1, 0, dtype=torch.int32, device="cuda")
+    n = torch.ones(1, dtype=torch.int32, device="cuda")
+    K.kv_cache_write(one[:, :2], one[:, :2], *cache, table, n)
+    K.sdpa_cached(one, *cache, table, n, o, 0.1)
+    assert (o == 0).all()
+    assert all(_same(a, b) for a, b in zip(cache, before))
+
+
+# --- together -----------------------------------------------------------------
+
+
+def _step(qkv, pos, freqs, cache, table, lengths, o, starts=None, window=0):
+    """One layer's attention of a step: 4 q heads, 2 k heads, 2 v heads of 64."""
+    K.rope(qkv[:, :6], pos, freqs, qkv[:, :6])
+    K.kv_cache_write(qkv[:, 4:6], qkv[:, 6:], *cache, table, lengths, starts=starts)
+    K.sdpa_cached(qkv[:, :4], *cache, table, lengths, o, 0.125, starts=starts, window=window)
+
+
+def _oracle_step(qkv, pos, freqs, cache, table, lengths, starts=None, window=0):
+    qk = R.rope(qkv[:, :6], pos, freqs).to(BF16)
+    R.write(qk[:, 4:6], qkv[:, 6:], *cache, table, lengths, starts)
+    return R.attention(qk[:, :4], *cache, table, lengths, 0.125, starts, window)
+
+
+@pytest.mark.parametrize("cdtype", [INT8, E4M3])
+def test_prompts_then_tokens(cdtype):
+    """Two prompts, then ten tokens each, as a program serves them; the oracle follows
+    with the kernel's rotated values (a rounding of rope may fall either way)."""
+    g = _gen(40)
+    freqs = K.rope_freqs(64, scaling="parts", factor=4.0, original=64, device="cpu")
+    lens = [45, 9]
+    dev = [c.cuda() for c in _cache(16, 2, 16, 64, cdtype, 41)]
+    table = _table([5, 5], 5, 16, 42)
+    ref = [c.cpu().clone() for c in dev]
+    starts = torch.tensor([0, 45, 54], dtype=torch.int32)
+    for step in range(11):
+        if step == 0:
+            pos = torch.cat([torch.arange(n) for n in lens]).to(torch.int32)
+            s = starts
+        else:
+            lens = [n + 1 for n in lens]
+            pos, s = torch.tensor([n - 1 for n in lens], dtype=torch.int32), None
+        n = torch.tensor(lens, dtype=torch.int32)
+        qkv = torch.randn(len(pos), 8, 64, generator=g).to(BF16)
+        d = qkv.cuda()
+        o = torch.full((len(pos), 4, 64), 7.0, dtype=BF16, device="cuda")
+        _step(d, pos.cuda(), freqs.cuda(), dev, table.cuda(), n.cuda(), o,
+              None if s is None else s.cuda())
+        turned = d.cpu()
+        _check_rope(turned[:, :6], qkv[:, :6], pos, freqs, False, 1.0, False)
+        R.write(turned[:, 4:6], turned[:, 6:], *ref, table, n, s)
+        for a, b in zip(dev, ref):
+            assert torch.equal(a.float().cpu().nan_to_num(500.0), b.float().nan_to_num(500.0)), step
+        out, size, reach = R.attention(turned[:, :4], *ref, table, n, 0.125, s)
+        err = (o.cpu().double() - out).abs()
+        assert (err <= _tolerance(out, size, reach, 64, 60, 0.0)).all(), (step, float(err.max()))
+
+
+def test_captured_steps_follow_the_lengths():
+    """Steps captured into two graphs replay on lengths that grow on the device, with
+    eager calls between them, and equal the eager steps bit for bit."""
+    g = _gen(43)
+    seqs, width = 5, 20
+    table = _table([width] * seqs, width, seqs * width, 44).cuda()
+    freqs = K.rope_freqs(64)
+    first = [c.cuda() for c in _cache(seqs * width, 2, 16, 64, INT8, 45)]
+    lens0 = torch.tensor([1, 70, 16, 200, 33], dtype=torch.int32, device="cuda")
+    qkvs = [torch.randn(seqs, 8, 64, generator=g).to(BF16).cuda() for _ in range(12)]
+
+    def eager():
+        cache, lens, outs = [c.clone() for c in first], lens0.clone(), []
+        for x in qkvs:
+            x, o = x.clone(), torch.empty(seqs, 4, 64, dtype=BF16, device="cuda")
+            _step(x, lens - 1, freqs, cache, table, lens, o)
+            outs.append(o)
+            lens += 1
+        return outs, cache
+
+    want, want_cache = eager()
+    cache, lens = [c.clone() for c in first], lens0.clone()
+    x = [torch.empty_like(qkvs[0]) for _ in range(2)]
+    o = [torch.empty(seqs, 4, 64, dtype=BF16, device="cuda") for _ in range(2)]
+    graphs = []
+    saved = [c.clone() for c in cache], lens.clone()
+    for i in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            _step(x[i], lens - 1, freqs, cache, table, lens, o[i])
+            lens.add_(1)
+        graphs.append(graph)
+    for c, s in zip(cache, saved[0]):
+        c.copy_(s)
+    lens.copy_(saved[1])
+    for j, q in enumerate(qkvs):
+        x[j % 2].copy_(q)
+        graphs[j % 2].replay()
+        if j % 3 == 0:
+            again, _ = eager()
+            torch.cuda.synchronize()
+        assert torch.equal(o[j % 2], want[j]), j
+    assert all(_same(a, b) for a, b in zip(cache, want_cache))
+
+
+def test_two_streams_at_once():
+    calls = [_attention_call([400, 333, 90], [1, 1, 1], 2, 4, 128, 32, INT8, 50 + i, True)
+             for i in range(2)]
+    dev = [[q.cuda(), [c.cuda() for c in cache], t.cuda(), n.cuda()] for q, cache, t, n, _ in calls]
+    want = []
+    for q, cache, t, n in dev:
+        o = torch.empty_like(q)
+        K.sdpa_cached(q, *cache, t, n, o, 0.09)
+        want.append(o)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    outs = [[torch.full_like(d[0], 7.0) for _ in range(20)] for d in dev]
+    torch.cuda.synchronize()
+    for j in range(20):
+        for s, (q, cache, t, n), o in zip(streams, dev, outs):
+            K.sdpa_cached(q, *cache, t, n, o[j], 0.09, stream=s)
+    torch.cuda.synchronize()
+    for w, o in zip(want, outs):
+        assert all(torch.equal(w, x) for x in o)
+
+
+def test_same_call_same_bits():
+    q, cache, table, n, starts = _attention_call([1500, 700], [3, 2], 2, 4, 128, 64, INT8, 60)
+    dev = [c.cuda() for c in cache]
+    outs = []
+    for _ in range(5):
+        o = torch.empty_like(q, device="cuda")
+        K.sdpa_cached(q.cuda(), *dev, table.cuda(), n.cuda(), o, 0.09, starts=starts.cuda())
+        outs.append(o)
+    assert all(torch.equal(outs[0], o) for o in outs)

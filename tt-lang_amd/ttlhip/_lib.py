@@ -87,12 +87,27 @@ class RowReduce(C.Structure):
     ]
 
 
+class KVCache(C.Structure):
+    _fields_ = [
+        ("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p),
+        ("table", C.c_void_p), ("lengths", C.c_void_p), ("starts", C.c_void_p),
+        ("table_ld", C.c_int64), ("pages", C.c_int64), ("width", C.c_int64),
+        ("heads", C.c_int64), ("seqs", C.c_int64), ("tokens", C.c_int64),
+        ("page", C.c_int32), ("dim", C.c_int32), ("format", C.c_int32), ("pad", C.c_int32),
+    ]
+
+
+# ttlh_kv_cache formats of codes
+CACHE_INT8, CACHE_E4M3 = 0, 1
+
 # The structs' layouts for struct.pack, which builds a launch's argument arrays
 # in a microsecond where one ctypes object per step takes about one each.
 INSTR_FMT, OPERAND_FMT, ROW_REDUCE_FMT = "3Bxff", "Qii6q", "QQiiQifQiiq"
+KV_CACHE_FMT = "7Q6q4i"
 assert struct.calcsize("=" + INSTR_FMT) == C.sizeof(Instr)
 assert struct.calcsize("=" + OPERAND_FMT) == C.sizeof(Operand)
 assert struct.calcsize("=" + ROW_REDUCE_FMT) == C.sizeof(RowReduce)
+assert struct.calcsize("=" + KV_CACHE_FMT) == C.sizeof(KVCache)
 
 
 @functools.lru_cache(maxsize=128)
@@ -144,6 +159,12 @@ SIGNATURES = {
     "ttlh_matmul_bfp8w_ws": (_int, [_vp, _i64, _vp, _vp, _i64, _i64, _i64, _i64, _vp, _i64, _vp]),
     "ttlh_sdpa_fwd": (_int, [_vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, C.c_float, _int, _vp]),
     "ttlh_sdpa_fwd_form": (_int, [_i64, _i64, _i64, _i64, _int]),
+    "ttlh_kv_cache_write": (_int, [_vp, _vp, _vp, _int, _i64, _i64, _i64, _i64, _vp]),
+    "ttlh_sdpa_cached_workspace_bytes": (_i64, [_vp, _i64]),
+    "ttlh_sdpa_cached": (_int, [_vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, C.c_float, _i64,
+                                C.c_float, _vp, _i64, _vp]),
+    "ttlh_rope": (_int, [_vp, _vp, _int, _vp, _int, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i64,
+                         _i64, _int, C.c_float, _int, _vp]),
     "ttlh_last_error": (C.c_char_p, []),
     "ttlh_version": (_int, []),
 }

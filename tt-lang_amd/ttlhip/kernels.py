@@ -11,6 +11,7 @@ from __future__ import annotations
 
 import ctypes as C
 import functools
+import math
 import struct
 import threading
 from dataclasses import dataclass
@@ -733,3 +734,208 @@ def sdpa_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: torch.Tensor,
     B, H, S, D = q.shape
     L.call("ttlh_sdpa_fwd", q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), B, H, S, D,
            float(scale), int(bool(causal)), L.stream_ptr(stream))
+
+
+# --- serving from an 8-bit key/value cache ------------------------------------
+
+CACHE_FORMATS = {torch.int8: L.CACHE_INT8, torch.float8_e4m3fn: L.CACHE_E4M3}
+_KV_CACHE = struct.Struct("=" + L.KV_CACHE_FMT)
+
+
+def rope_freqs(rot: int, base: float = 10000.0, scaling: Optional[str] = None,
+               factor: float = 1.0, original: int = 0, fast: float = 32.0, slow: float = 1.0,
+               device=None) -> torch.Tensor:
+    """The frequencies of rope(): radians per position of the rot / 2 planes,
+    base^(-2i / rot), in float64 on `device` (default: the GPU where there is one).
+
+    scaling, for contexts `factor` times the `original` one:
+      "linear"  every frequency divided by factor
+      "base"    the base raised so that the slowest plane's frequency is divided by
+                factor and the fastest one's kept
+      "parts"   planes that turn at least `fast` times over the original context are
+                kept, those that turn at most `slow` times divided by factor, those
+                between blended linearly in their number of turns"""
+    if rot <= 0 or rot % 2:
+        raise ValueError(f"rope_freqs: rot must be positive and even, got {rot}")
+    if not base > 0 or not factor >= 1:
+        raise ValueError("rope_freqs: base must be positive and factor at least 1")
+    if device is None:
+        device = "cuda" if torch.cuda.is_available() else "cpu"
+    if scaling == "base" and rot > 2:
+        base = base * factor ** (rot / (rot - 2))
+    f = base ** (-torch.arange(0, rot, 2, dtype=torch.float64) / rot)
+    if scaling == "linear":
+        f = f / factor
+    elif scaling == "parts":
+        if original <= 0 or not fast > slow:
+            raise ValueError("rope_freqs: 'parts' needs the original context, and fast > slow")
+        turns = f * (original / (2 * math.pi))
+        keep = ((turns - slow) / (fast - slow)).clamp(0.0, 1.0)
+        f = f * keep + f / factor * (1 - keep)
+    elif scaling not in (None, "base"):
+        raise ValueError(f"rope_freqs: scaling must be None, 'linear', 'base' or 'parts', got {scaling!r}")
+    return f.to(device)
+
+
+def _check_on_one_device(what: str, tensors, stream) -> None:
+    """All on the device that the launch goes to: the stream's, or the current one."""
+    for t in tensors:
+        if not t.is_cuda:
+            raise RuntimeError(f"{what} takes device (HIP) tensors; there is no CPU path")
+    dev = stream.device.index if stream is not None else torch._C._cuda_getDevice()
+    for t in tensors:
+        if t.get_device() != dev:
+            raise ValueError(f"{what}: a tensor on device {t.get_device()}, the launch on {dev}")
+
+
+def _check_heads(what: str, name: str, t: torch.Tensor, shape=None) -> None:
+    """t is [tokens, heads, dim] with unit stride along dim (any others)."""
+    if t.dim() != 3 or (shape is not None and t.shape != shape):
+        raise ValueError(f"{what}: {name} must be [tokens, heads, dim]"
+                         f"{'' if shape is None else f' = {tuple(shape)}'}, got {tuple(t.shape)}")
+    if t.stride(2) != 1 and t.shape[2] > 1:
+        raise ValueError(f"{what}: {name} must have unit stride along dim")
+
+
+def _head_strides(t: torch.Tensor):
+    """Strides of tokens and heads (0 along a dimension of one)."""
+    a, b, _ = t.stride()
+    return (a if t.shape[0] > 1 else 0, b if t.shape[1] > 1 else 0)
+
+
+def rope(x: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor, out: torch.Tensor,
+         interleaved: bool = False, scale: float = 1.0, backward: bool = False,
+         stream=None) -> None:
+    """Rotary positions: out = x [tokens, heads, dim] with plane i of the first
+    2 len(freqs) elements of each head turned by positions[token] * freqs[i] and
+    multiplied by `scale` (rope_freqs(); the angles in float64), the other
+    elements copied.  Plane i: elements i and i + len(freqs), or 2i and 2i + 1
+    where `interleaved`.  backward: the gradient of x from that of out (the
+    opposite turn).  x and out: bf16 or f32, any strides for tokens and heads
+    (q and k of one projection are turned by one call), and out may be x."""
+    _check_heads("rope", "x", x)
+    _check_heads("rope", "out", out, x.shape)
+    tokens, heads, dim = x.shape
+    if out.dtype != x.dtype:
+        raise ValueError(f"rope: out must be {x.dtype} as x is, got {out.dtype}")
+    if positions.shape != (tokens,) or positions.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"rope: positions must be int32 or int64 [{tokens}], got "
+                         f"{positions.dtype} {tuple(positions.shape)}")
+    if freqs.dim() != 1 or freqs.dtype != torch.float64 or 2 * freqs.shape[0] > dim:
+        raise ValueError(f"rope: freqs must be float64 with at most dim / 2 = {dim // 2} elements, "
+                         f"got {freqs.dtype} {tuple(freqs.shape)}")
+    if not positions.is_contiguous() or not freqs.is_contiguous():
+        raise ValueError("rope: positions and freqs must be contiguous")
+    if (tokens > 1 and out.stride(0) == 0) or (heads > 1 and out.stride(1) == 0):
+        raise ValueError("rope: out must not repeat its elements")
+    if out.data_ptr() == x.data_ptr() and out.stride() != x.stride():
+        raise ValueError("rope: out may be x itself, not another view of its memory")
+    code = L.dtype_code(x.dtype)
+    _check_on_one_device("rope", (x, positions, freqs, out), stream)
+    L.call("ttlh_rope", x.data_ptr(), out.data_ptr(), code, positions.data_ptr(),
+           positions.element_size(), freqs.data_ptr(), tokens, heads, dim, 2 * freqs.shape[0],
+           *_head_strides(x), *_head_strides(out), interleaved, scale, backward,
+           L.stream_ptr(stream))
+
+
+def _kv_cache(what: str, tokens: int, k_cache, v_cache, k_scale, v_scale, table, lengths, starts):
+    """The ttlh_kv_cache of a call with `tokens` packed new tokens."""
+    if k_cache.dim() != 4 or not k_cache.is_contiguous() or not v_cache.is_contiguous():
+        raise ValueError(f"{what}: the caches must be contiguous [pages, heads, page, dim]")
+    fmt = CACHE_FORMATS.get(k_cache.dtype)
+    if fmt is None or v_cache.dtype != k_cache.dtype or v_cache.shape != k_cache.shape:
+        raise ValueError(f"{what}: both caches must be int8 or float8_e4m3fn of one shape, got "
+                         f"{k_cache.dtype} {tuple(k_cache.shape)} and {v_cache.dtype} "
+                         f"{tuple(v_cache.shape)}")
+    pages, heads, page, dim = k_cache.shape
+    for t, n in ((k_scale, "k_scale"), (v_scale, "v_scale")):
+        if t.dtype != torch.float32 or t.shape != (pages, heads) or not t.is_contiguous():
+            raise ValueError(f"{what}: {n} must be contiguous float32 [pages, heads] = "
+                             f"{(pages, heads)}, got {t.dtype} {tuple(t.shape)}")
+    if table.dim() != 2 or table.dtype != torch.int32 or (table.shape[1] > 1 and table.stride(1) != 1):
+        raise ValueError(f"{what}: table must be int32 [sequences, pages] with unit column stride")
+    seqs, width = table.shape
+    if lengths.shape != (seqs,) or lengths.dtype != torch.int32 or not lengths.is_contiguous():
+        raise ValueError(f"{what}: lengths must be contiguous int32 [{seqs}], got {lengths.dtype} "
+                         f"{tuple(lengths.shape)}")
+    if starts is None:
+        if tokens != seqs:
+            raise ValueError(f"{what}: without starts there is one new token for each of the "
+                             f"{seqs} sequences, got {tokens}")
+    elif starts.shape != (seqs + 1,) or starts.dtype != torch.int32 or not starts.is_contiguous():
+        raise ValueError(f"{what}: starts must be contiguous int32 [{seqs + 1}], got "
+                         f"{starts.dtype} {tuple(starts.shape)}")
+    return _KV_CACHE.pack(k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(),
+                          v_scale.data_ptr(), table.data_ptr(), lengths.data_ptr(),
+                          0 if starts is None else starts.data_ptr(), table.stride(0), pages, width,
+                          heads, seqs, tokens, page, dim, fmt, 0)
+
+
+def kv_cache_write(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                   k_scale: torch.Tensor, v_scale: torch.Tensor, table: torch.Tensor,
+                   lengths: torch.Tensor, starts: Optional[torch.Tensor] = None,
+                   stream=None) -> None:
+    """New tokens' keys and values (bf16 or f32 [tokens, heads, dim], any strides
+    for tokens and heads) into a cache of 8-bit codes.
+
+    k_cache, v_cache: int8 or float8_e4m3fn [pages, heads, page, dim], a page of
+    16, 32, 64 or 128 tokens; k_scale, v_scale: float32 [pages, heads]: a value is
+    code * scale.  table: int32 [sequences, n]: the page of each run of `page`
+    positions.  lengths: int32 [sequences], with the new tokens.  starts: int32
+    [sequences + 1], the packed new tokens of each sequence (None: one each).
+
+    The scale of a page and head is the smallest power of two that holds its
+    tokens (ttlh_kv_cache_write says more): earlier tokens of a page whose scale
+    grows are rounded again.  Positions that the table does not name, and pages
+    that the cache does not have, are not written; a page that two sequences
+    write in one call gets either's."""
+    _check_heads("kv_cache_write", "k", k)
+    _check_heads("kv_cache_write", "v", v, k.shape)
+    if v.dtype != k.dtype:
+        raise ValueError(f"kv_cache_write: k and v must have one dtype, got {k.dtype} and {v.dtype}")
+    cache = _kv_cache("kv_cache_write", k.shape[0], k_cache, v_cache, k_scale, v_scale, table,
+                      lengths, starts)
+    if k.shape[1:] != (k_cache.shape[1], k_cache.shape[3]):
+        raise ValueError(f"kv_cache_write: tokens of {tuple(k.shape[1:])}, a cache of "
+                         f"{(k_cache.shape[1], k_cache.shape[3])} (heads, dim)")
+    code = L.dtype_code(k.dtype)
+    tensors = (k, v, k_cache, v_cache, k_scale, v_scale, table, lengths)
+    _check_on_one_device("kv_cache_write", tensors if starts is None else tensors + (starts,), stream)
+    L.call("ttlh_kv_cache_write", cache, k.data_ptr(), v.data_ptr(), code, *_head_strides(k),
+           *_head_strides(v), L.stream_ptr(stream))
+
+
+def sdpa_cached(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                k_scale: torch.Tensor, v_scale: torch.Tensor, table: torch.Tensor,
+                lengths: torch.Tensor, o: torch.Tensor, scale: float,
+                starts: Optional[torch.Tensor] = None, window: int = 0, softcap: float = 0.0,
+                stream=None) -> None:
+    """Attention of new tokens over the cache that kv_cache_write() filled (the
+    new tokens' own keys among them): o = softmax(cap(scale q k^T)) v, a token at
+    position p seeing the positions up to p, or the last `window` of them.
+    softcap: cap(x) = softcap tanh(x / softcap) (0: x).  q, o: bf16 [tokens,
+    q heads, dim], any strides for tokens and heads that are multiples of 8; q heads
+    share the cache's heads in equal groups.  Positions that the table does not
+    name are not seen; a token that sees nothing gets zeros.  Rows of o behind the
+    last sequence's tokens stay as they are."""
+    _check_heads("sdpa_cached", "q", q)
+    _check_heads("sdpa_cached", "o", o, q.shape)
+    if q.dtype != torch.bfloat16 or o.dtype != torch.bfloat16:
+        raise ValueError(f"sdpa_cached: q and o must be bf16, got {q.dtype} and {o.dtype}")
+    tokens, q_heads, dim = q.shape
+    cache = _kv_cache("sdpa_cached", tokens, k_cache, v_cache, k_scale, v_scale, table, lengths,
+                      starts)
+    heads = k_cache.shape[1]
+    if dim != k_cache.shape[3] or heads == 0 or q_heads == 0 or q_heads % heads:
+        raise ValueError(f"sdpa_cached: q of {(q_heads, dim)} (heads, dim) over a cache of "
+                         f"{(heads, k_cache.shape[3])}")
+    if (tokens > 1 and o.stride(0) == 0) or (q_heads > 1 and o.stride(1) == 0):
+        raise ValueError("sdpa_cached: o must not repeat its elements")
+    if (q.data_ptr() | o.data_ptr()) & 15 or any(n & 7 for n in _head_strides(q) + _head_strides(o)):
+        raise ValueError("sdpa_cached: q and o must be 16-byte aligned with strides that are "
+                         "multiples of 8")
+    tensors = (q, k_cache, v_cache, k_scale, v_scale, table, lengths, o)
+    _check_on_one_device("sdpa_cached", tensors if starts is None else tensors + (starts,), stream)
+    sp = L.stream_ptr(stream)
+    L.call("ttlh_sdpa_cached", cache, q.data_ptr(), o.data_ptr(), q_heads, *_head_strides(q),
+           *_head_strides(o), scale, window, softcap, 0, 0, sp)
