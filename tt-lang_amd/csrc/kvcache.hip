@@ -322,7 +322,7 @@ int check_cache(const char* fn, const ttlh_kv_cache* c, CacheArgs* a) {
                    (c->table_ld >= c->width || c->seqs <= 1),
                TTLH_EINVAL, "%s: bad sizes", fn);
   TTLH_REQUIRE(c->pages < (int64_t(1) << 31) && c->heads < 65536 && c->seqs < (int64_t(1) << 24) &&
-                   c->tokens < (int64_t(1) << 28) && c->width * c->page < (int64_t(1) << 31),
+                   c->tokens < (int64_t(1) << 28) && c->width * c->page <= (int64_t(1) << 30),
                TTLH_EUNSUPPORTED, "%s: too many pages, positions, heads, sequences or tokens", fn);
   TTLH_REQUIRE(c->starts || c->tokens == c->seqs, TTLH_EINVAL,
                "%s: without starts there is one token for each sequence", fn);

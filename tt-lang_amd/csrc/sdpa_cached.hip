@@ -1,8 +1,31 @@
-// Attention of new tokens over an 8-bit key/value cache (see ttlhip.h) for gfx950.
-// One wave for each (new token, q head): its positions one after the other, with
-// the running maximum and sum of an online softmax, a lane for each 64th element.
+// Attention of new tokens over an 8-bit key/value cache (see ttlhip.h) for gfx950:
+//   o = softmax(cap(scale q K^T)) V,  fp32 scores, statistics and sums.
+//
+// The q heads that share a cache head, for all new tokens of a sequence, are the
+// rows of one problem: row r is token r / group, head r % group of the group.  The
+// rows go in tiles, and K and V are read once for a tile.  Codes are whole numbers
+// (or e4m3 values) that bf16 holds exactly, so the products run on the codes and the
+// scales multiply what comes out: K's the scores, V's the probabilities before
+// their rounding to bf16 for the second product.  Both kernels compute the
+// transposes S^T = K Q^T and O^T += V^T P^T: a row's scores, its maximum and its part
+// of O then lie in the same lanes, and P^T needs no exchange between the products
+// (the order of the positions inside a product is free).
+//
+//  * cached_rows_kernel: up to 16 MT rows in a tile (answers token by token, drafts):
+//    HBM bound.  Eight waves take turns at 32 positions and meet in LDS at the end;
+//    codes go from memory to registers, no LDS on the way.
+//  * cached_tiles_kernel: tiles of 128 rows (prompts): MFMA bound.  Blocks of 64
+//    positions are decoded once into LDS for four waves of 32 rows.
+//
+// Few tiles with many positions are divided into parts (see Plan), whose results
+// meet in cached_join_kernel in the order of the parts.
+//
+// A page whose K or V scale is not finite makes NaN of what sees it.  A NaN in V's
+// scale is carried by the scores instead (kscale, vscale below): a row that does not
+// see the page has a probability of 0 there, and 0 NaN would be NaN.
 
 #include <cmath>
+#include <type_traits>
 
 #include "ttlh_common.h"
 #include "ttlh_kvcache.h"
@@ -11,65 +34,884 @@
 namespace ttlh {
 namespace {
 
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef short i16x4 __attribute__((ext_vector_type(4)));
+typedef short i16x8 __attribute__((ext_vector_type(8)));
+typedef __attribute__((address_space(3))) i16x4 lds_i16x4;
+
+constexpr float kLog2e = 1.4426950408889634f;
+
 struct CachedArgs {
   CacheArgs c;
   const uint16_t* q;
   uint16_t* o;
   int64_t q_token, q_head, o_token, o_head;
-  int32_t q_heads, group;
-  int32_t window;  // 0: none
-  float scale, softcap;
+  int32_t group;
+  int32_t window;     // 0: none
+  int32_t target;     // parts of all sequences together, for one head, about; 0: undivided
+  int32_t least;      // positions of a part, at least
+  float scale_log2;   // scale log2 e, or 2 scale log2 e / softcap
+  float cap_log2;     // softcap log2 e, or 0
+  float* part_o;      // [slot, head, rows of a tile, dim]
+  float* part_ml;     // [slot, head, rows of a tile, 2]: maximum and sum
 };
 
-struct TokensOf {
-  const CacheArgs& c;
-  __device__ int operator()(int b) const {
-    int first, n;
-    seq_tokens(c, b, first, n);
-    return n;
-  }
+// ---- which part of which tile of which sequence a workgroup has --------------
+//
+// Lengths are on the device, so the division is made there, by every workgroup for
+// itself, from one pass over the sequences: with W the positions of all tiles
+// together, a part has `chunk` = W / target positions (at least `least`), so the
+// parts are alike whatever the lengths are.  There are at most (tiles + target)
+// parts, and at most 2 target of them belong to tiles of several parts, which have
+// `slots` for their results.
+struct Plan {
+  int b, first, n, len;      // the sequence, its new tokens and positions
+  int row0, rows;            // the tile's first row, the sequence's rows
+  int part, parts, slot;     // this part; the slot of the tile's part 0
 };
 
-__device__ __forceinline__ float wave_sum(float x) {
+__device__ __forceinline__ int64_t wave_total(int64_t x) {
 #pragma unroll
   for (int i = 32; i; i >>= 1) x += __shfl_xor(x, i);
   return x;
 }
 
+template <int BM>
+struct Division {
+  const CachedArgs& p;
+  int chunk;
+
+  // tiles of sequence b, and the positions that its rows see between them
+  __device__ __forceinline__ void extent(int b, int& tiles, int& range) const {
+    int first, n, lo, hi, x;
+    seq_tokens(p.c, b, first, n);
+    tiles = (n * p.group + BM - 1) / BM;
+    range = 0;
+    if (n > 0) {
+      seen_by(p.c, p.c.lengths[b], n, 0, p.window, lo, x);
+      seen_by(p.c, p.c.lengths[b], n, n - 1, p.window, x, hi);
+      range = hi > lo ? hi - lo : 0;
+    }
+  }
+  __device__ __forceinline__ int parts_of(int range) const {
+    return range > chunk ? (range - 1) / chunk + 1 : 1;
+  }
+  __device__ __forceinline__ void divide() {
+    chunk = 0x7fffffff;
+    if (p.target == 0) return;
+    const int lane = threadIdx.x & 63;
+    int64_t sum = 0;
+    for (int b = lane; b < p.c.seqs; b += 64) {
+      int tiles, range;
+      extent(b, tiles, range);
+      sum += static_cast<int64_t>(tiles) * range;
+    }
+    sum = wave_total(sum);
+    const int64_t each = (((sum + p.target - 1) / p.target) + 63) & ~int64_t(63);
+    chunk = static_cast<int>(each < p.least ? p.least : each > 0x7fffffc0 ? 0x7fffffc0 : each);
+    chunk = __builtin_amdgcn_readfirstlane(chunk);
+  }
+  // item `item` of the parts (JOIN: of the tiles), or false past the last one
+  template <bool JOIN>
+  __device__ __forceinline__ bool find(int64_t item, Plan& w) const {
+    const int lane = threadIdx.x & 63;
+    int64_t items = 0, slots = 0;
+    for (int b0 = 0; b0 < p.c.seqs; b0 += 64) {
+      int tiles = 0, range = 0;
+      if (b0 + lane < p.c.seqs) extent(b0 + lane, tiles, range);
+      const int parts = parts_of(range);
+      const int64_t mine = JOIN ? tiles : static_cast<int64_t>(tiles) * parts;
+      const int64_t mine_slots = parts > 1 ? static_cast<int64_t>(tiles) * parts : 0;
+      int64_t end = mine, send = mine_slots;
+#pragma unroll
+      for (int i = 1; i < 64; i <<= 1) {
+        const int64_t o = __shfl_up(end, i), so = __shfl_up(send, i);
+        if (lane >= i) {
+          end += o;
+          send += so;
+        }
+      }
+      const unsigned long long past = __ballot(items + end > item);
+      if (past) {
+        const int l = __builtin_amdgcn_readfirstlane(__ffsll(past) - 1);
+        const int local = __builtin_amdgcn_readfirstlane(
+            static_cast<int>(item - items - (__shfl(end, l) - __shfl(mine, l))));
+        w.b = b0 + l;
+        w.parts = __builtin_amdgcn_readlane(parts, l);
+        const int nt = __builtin_amdgcn_readlane(tiles, l);
+        // (the last tile of a prompt sees the most: it goes first)
+        const int tile = JOIN ? nt - 1 - local : nt - 1 - local / w.parts;
+        w.part = JOIN ? 0 : local % w.parts;
+        w.slot = __builtin_amdgcn_readfirstlane(static_cast<int>(
+                     slots + __shfl(send, l) - __shfl(mine_slots, l))) +
+                 (nt - 1 - tile) * w.parts;
+        seq_tokens(p.c, w.b, w.first, w.n);
+        w.len = p.c.lengths[w.b];
+        w.row0 = tile * BM;
+        w.rows = w.n * p.group;
+        // (never more slots than there are, unless lengths change under the call)
+        return w.parts == 1 || w.slot + w.parts <= 2 * p.target;
+      }
+      items += __shfl(end, 63);
+      slots += __shfl(send, 63);
+    }
+    return false;
+  }
+};
+
+// The positions of a part of a tile: those its rows see, [lo, hi) in all parts, of
+// which this part has [begin, end), begin a multiple of ALIGN; and the positions
+// [all_lo, all_hi) that every row sees.
+struct Span {
+  int lo, hi, all_lo, all_hi, begin, end;
+};
+template <int BM, int ALIGN>
+__device__ __forceinline__ Span span_of(const CachedArgs& p, const Plan& w) {
+  Span s;
+  const int i0 = w.row0 / p.group, i1 = (min(w.row0 + BM, w.rows) - 1) / p.group;
+  seen_by(p.c, w.len, w.n, i0, p.window, s.lo, s.all_hi);
+  seen_by(p.c, w.len, w.n, i1, p.window, s.all_lo, s.hi);
+  if (p.c.pages == 0) s.hi = 0;
+  const int from = s.lo & ~(ALIGN - 1);
+  const int units = s.hi > from ? (s.hi - from + ALIGN - 1) / ALIGN : 0;
+  const int per = (units + w.parts - 1) / w.parts;
+  s.begin = from + min(units, w.part * per) * ALIGN;
+  s.end = min(s.hi, from + min(units, (w.part + 1) * per) * ALIGN);
+  return s;
+}
+
+// ---- codes to bf16 -----------------------------------------------------------
+
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+
+// Byte J of w as a signed number, in one instruction.  (As asm: written in C++, the
+// conversions of one dword's bytes become one vector conversion, whose four results
+// then live until the last of them is used, and the registers do not suffice.)
+template <int J>
+__device__ __forceinline__ float int8_of(uint32_t w) {
+  float f;
+  if constexpr (J == 0)
+    asm("v_cvt_f32_i32_sdwa %0, sext(%1) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_0"
+        : "=v"(f) : "v"(w));
+  else if constexpr (J == 1)
+    asm("v_cvt_f32_i32_sdwa %0, sext(%1) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_1"
+        : "=v"(f) : "v"(w));
+  else if constexpr (J == 2)
+    asm("v_cvt_f32_i32_sdwa %0, sext(%1) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_2"
+        : "=v"(f) : "v"(w));
+  else
+    asm("v_cvt_f32_i32_sdwa %0, sext(%1) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_3"
+        : "=v"(f) : "v"(w));
+  return f;
+}
+
+// bytes 2 i, 2 i + 1 of w
+template <int FMT, int I>
+__device__ __forceinline__ uint32_t pair_of(uint32_t w) {
+  if constexpr (FMT == TTLH_CACHE_E4M3)
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, I == 1));
+  else
+    return cvt_pk_bf16x2(int8_of<2 * I>(w), int8_of<2 * I + 1>(w));
+}
+template <int FMT>
+__device__ __forceinline__ u32x4 eight_of(uint32_t a, uint32_t b) {
+  return u32x4{pair_of<FMT, 0>(a), pair_of<FMT, 1>(a), pair_of<FMT, 0>(b), pair_of<FMT, 1>(b)};
+}
+// byte J of a and of b
+template <int FMT, int J>
+__device__ __forceinline__ uint32_t pair_across(uint32_t a, uint32_t b) {
+  if constexpr (FMT == TTLH_CACHE_E4M3) {
+    // one permutation serves two neighbouring J
+    constexpr uint32_t sel = J < 2 ? 0x05010400u : 0x07030602u;
+    return pair_of<FMT, (J & 1)>(__builtin_amdgcn_perm(b, a, sel));
+  } else {
+    return cvt_pk_bf16x2(int8_of<J>(a), int8_of<J>(b));
+  }
+}
+
+__device__ __forceinline__ float uniform(float x, int lane) {
+  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), lane));
+}
+
+// What a wave knows about 64 subtiles of 16 positions, one in a lane: the page (or
+// -1), the scores' factor and V's scale.
+struct Subtiles {
+  int page;
+  float kscale, vscale;
+
+  __device__ __forceinline__ void load(const CachedArgs& p, int b, int h, int pos) {
+    page = page_at(p.c, b, pos);
+    kscale = vscale = 0.0f;
+    if (page >= 0) {
+      const int64_t at = static_cast<int64_t>(page) * p.c.heads + h;
+      kscale = p.c.k_scale[at] * p.scale_log2;
+      vscale = p.c.v_scale[at];
+      if (!(fabsf(vscale) < INFINITY) || !(fabsf(p.c.k_scale[at]) < INFINITY)) {
+        kscale = __int_as_float(0x7fc00000);
+        vscale = 0.0f;
+      }
+    }
+  }
+};
+
+// x (in units of log2) of a raw score: capped where there is a cap, as
+// C tanh(t) = C - 2 C / (1 + e^2t) with e^2t = 2^(raw kscale)
+__device__ __forceinline__ float score(float raw, float kscale, float cap) {
+  const float x = raw * kscale;
+  if (cap == 0.0f) return x;
+  return __builtin_fmaf(-2.0f * cap, __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x)), cap);
+}
+
+__device__ __forceinline__ float xor32_max(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false,
+                                                  false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float xor32_add(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false,
+                                                  false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+__device__ __forceinline__ float xor16_max(float x) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false,
+                                                  false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float xor16_add(float x) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false,
+                                                  false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// ---- few rows ----------------------------------------------------------------
+//
+// A wave's step: 32 positions (two subtiles of 16, each on one page) against 16 MT
+// rows.  Lane (n = lane % 16, g = lane / 16).  S^T: 16x16x32 MFMAs, lane (n, g) has
+// K's row n of a subtile, 16 bytes at 16 g (and at 64 + 16 g), which are two
+// operands; S^T leaves it positions 4 g + i of each subtile for row n of the tile.
+// O^T: operand k = 8 g + 4 s + i is position 16 s + 4 g + i, so those scores are
+// the P^T operand as they stand, and lane (n, g) reads D / 16 bytes at n D / 16 of
+// its 8 positions, byte j of which is the operand of tile j: O^T's row m of tile j
+// is element m D / 16 + j.
+constexpr int kRowWaves = 8;
+constexpr int kStep = 32;
+
+template <int D, int FMT, int MT>
+struct Rows {
+  static constexpr int NK = D / 64;   // 16-byte loads of a K row
+  static constexpr int NC = D / 32;   // K operands of a subtile
+  static constexpr int NV = D / 64;   // dwords of a V load
+  static constexpr int NT = D / 16;   // tiles of O^T
+
+  struct Codes {
+    u32x4 k[2][NK];
+    uint32_t v[2][4][NV];
+  };
+
+  const CachedArgs& p;
+  const Plan& w;
+  const Span& s;
+  int h, n, g;
+  bf16x8 q[MT][NC];
+  f32x4 o[MT][NT];
+  float m[MT], l[MT];
+  int from[MT], end[MT];  // what the lane's rows see
+  Subtiles sub;
+
+  __device__ __forceinline__ void load(Codes& x, int k) const {
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const int page = max(__builtin_amdgcn_readlane(sub.page, (2 * k + t) & 63), 0);
+      const int slot = (s.begin + (k * kRowWaves + wave()) * kStep + 16 * t) & ((1 << p.c.shift) - 1);
+      const int64_t at = slot_offset(p.c, page, h, slot);
+      const uint8_t* kp = p.c.k + at + n * D + 16 * g;
+#pragma unroll
+      for (int i = 0; i < NK; ++i) x.k[t][i] = *reinterpret_cast<const u32x4*>(kp + 64 * i);
+      const uint8_t* vp = p.c.v + at + 4 * g * D + n * (D / 16);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (NV == 2) {
+          const u32x2 v = *reinterpret_cast<const u32x2*>(vp + i * D);
+          x.v[t][i][0] = v[0];
+          x.v[t][i][1] = v[1];
+        } else {
+          x.v[t][i][0] = *reinterpret_cast<const uint32_t*>(vp + i * D);
+        }
+      }
+    }
+  }
+  __device__ __forceinline__ int wave() const {
+    return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  }
+
+  __device__ __forceinline__ void step(Codes& x, int k) {
+    const int pos = s.begin + (k * kRowWaves + wave()) * kStep;
+    float ks[2], vs[2];
+    bool there[2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const int l = (2 * k + t) & 63;
+      ks[t] = uniform(sub.kscale, l);
+      vs[t] = uniform(sub.vscale, l);
+      there[t] = __builtin_amdgcn_readlane(sub.page, l) >= 0;
+    }
+    const bool mask = !there[0] || !there[1] || pos < s.all_lo || pos + kStep > s.all_hi;
+    f32x4 sc[MT][2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+#pragma unroll
+      for (int r = 0; r < MT; ++r) sc[r][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        const u32x4 raw = x.k[t][c >> 1];
+        const bf16x8 kf = __builtin_bit_cast(
+            bf16x8, (c & 1) ? eight_of<FMT>(raw[2], raw[3]) : eight_of<FMT>(raw[0], raw[1]));
+#pragma unroll
+        for (int r = 0; r < MT; ++r)
+          sc[r][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, q[r][c], sc[r][t], 0, 0, 0);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+    if (mask) {
+      // codes that no row sees may be anything: 0 times them has to be 0
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int j = pos + 16 * t + 4 * g + i;
+          const bool seen = there[t] && j >= s.lo && j < s.hi;
+#pragma unroll
+          for (int d = 0; d < NV; ++d) x.v[t][i][d] = seen ? x.v[t][i][d] : 0u;
+        }
+    }
+    bf16x8 pf[MT];
+#pragma unroll
+    for (int r = 0; r < MT; ++r) {
+      float e[8];
+      float mx = -INFINITY;
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) e[4 * t + i] = score(sc[r][t][i], ks[t], p.cap_log2);
+      if (mask) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int j = pos + 16 * t + 4 * g + i;
+            if (!there[t] || j < from[r] || j >= end[r]) e[4 * t + i] = -INFINITY;
+          }
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) mx = fmaxf(mx, e[i]);
+      if (__any(mx > m[r])) {  // (else the maximum stands, and so do the sums)
+        const float to = fmaxf(m[r], xor32_max(xor16_max(mx)));
+        const float alpha = to == m[r] ? 1.0f : __builtin_amdgcn_exp2f(m[r] - to);
+        m[r] = to;
+        l[r] *= alpha;
+#pragma unroll
+        for (int j = 0; j < NT; ++j) o[r][j] *= alpha;
+      }
+      const float mm = m[r] == -INFINITY ? 0.0f : m[r];
+      float sum = 0.0f;
+      u32x4 pk;
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          e[4 * t + i] = __builtin_amdgcn_exp2f(e[4 * t + i] - mm);
+          sum += e[4 * t + i];
+        }
+        pk[2 * t] = cvt_pk_bf16x2(e[4 * t] * vs[t], e[4 * t + 1] * vs[t]);
+        pk[2 * t + 1] = cvt_pk_bf16x2(e[4 * t + 2] * vs[t], e[4 * t + 3] * vs[t]);
+      }
+      l[r] += sum;
+      pf[r] = __builtin_bit_cast(bf16x8, pk);
+    }
+    products(x, pf);
+  }
+
+  template <int J>
+  __device__ __forceinline__ bf16x8 vfrag(const Codes& x) const {
+    u32x4 f;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      f[2 * t] = pair_across<FMT, (J & 3)>(x.v[t][0][J / 4], x.v[t][1][J / 4]);
+      f[2 * t + 1] = pair_across<FMT, (J & 3)>(x.v[t][2][J / 4], x.v[t][3][J / 4]);
+    }
+    return __builtin_bit_cast(bf16x8, f);
+  }
+  template <int J = 0>
+  __device__ __forceinline__ void products(const Codes& x, const bf16x8 (&pf)[MT]) {
+    const bf16x8 vf = vfrag<J>(x);
+#pragma unroll
+    for (int r = 0; r < MT; ++r)
+      o[r][J] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[r], o[r][J], 0, 0, 0);
+    __builtin_amdgcn_sched_barrier(0);
+    if constexpr (J + 1 < NT) products<J + 1>(x, pf);
+  }
+};
+
+template <int D, int FMT, int MT>
+__global__ __launch_bounds__(kRowWaves * 64, 2) void cached_rows_kernel(
+    const CachedArgs p) {
+  constexpr int BM = 16 * MT;
+  constexpr int LD = D + 4;  // LDS row: 16 rows' 16-byte writes spread over the banks
+  __shared__ float part[kRowWaves][16][LD];
+  __shared__ float ml[kRowWaves][16][2];
+
+  Division<BM> div{p};
+  div.divide();
+  const int h = blockIdx.x % p.c.heads;
+  Plan w;
+  if (!div.template find<false>(blockIdx.x / p.c.heads, w)) return;
+  const Span s = span_of<BM, kStep>(p, w);
+  Rows<D, FMT, MT> x{p, w, s, h};
+  const int lane = threadIdx.x & 63, wave = x.wave();
+  x.n = lane & 15;
+  x.g = lane >> 4;
+  // steps of this wave: k * 8 + wave of the part's
+  const int total = s.end > s.begin ? (s.end - s.begin + kStep - 1) / kStep : 0;
+  const int steps = total > wave ? (total - wave - 1) / kRowWaves + 1 : 0;
+  const auto refill = [&](int k) {  // steps k .. k + 31, two subtiles each
+    const int pos = s.begin + ((k + (lane >> 1)) * kRowWaves + wave) * kStep + 16 * (lane & 1);
+    x.sub.load(p, w.b, h, pos >= 0 && pos < s.hi ? pos : -1);
+  };
+  if (steps > 0) refill(0);
+#pragma unroll
+  for (int r = 0; r < MT; ++r) {
+    const int row = min(w.row0 + 16 * r + x.n, w.rows - 1);
+    const int i = row / p.group;
+    const uint16_t* qp = p.q + static_cast<int64_t>(w.first + i) * p.q_token +
+                         static_cast<int64_t>(h * p.group + row - i * p.group) * p.q_head;
+#pragma unroll
+    for (int c = 0; c < D / 32; ++c)
+      x.q[r][c] = *reinterpret_cast<const bf16x8*>(qp + 64 * (c >> 1) + 16 * x.g + 8 * (c & 1));
+    seen_by(p.c, w.len, w.n, i, p.window, x.from[r], x.end[r]);
+    x.m[r] = -INFINITY;
+    x.l[r] = 0.0f;
+#pragma unroll
+    for (int j = 0; j < D / 16; ++j) x.o[r][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  }
+  typename Rows<D, FMT, MT>::Codes a, b;
+  if (steps > 0) x.load(a, 0);
+  for (int k0 = 0; k0 < steps; k0 += 32) {
+    if (k0 > 0) {
+      refill(k0);
+      x.load(a, k0);
+    }
+    const int kn = min(steps, k0 + 32);
+    for (int k = k0; k < kn; ++k) {
+      if (k + 1 < kn) x.load(b, k + 1);
+      x.step(a, k);
+      a = b;
+    }
+  }
+
+  // The waves meet: their maxima, sums and O in LDS, 16 rows at a time; a thread
+  // has four elements of a row.
+  const int64_t slot = (static_cast<int64_t>(w.slot + w.part) * p.c.heads + h) * BM;
+#pragma unroll
+  for (int r = 0; r < MT; ++r) {
+    if (w.row0 + 16 * r >= w.rows) break;  // (uniform)
+    const float l = xor32_add(xor16_add(x.l[r]));
+    if (r) __syncthreads();
+    if (x.g == 0) {
+      ml[wave][x.n][0] = x.m[r];
+      ml[wave][x.n][1] = l;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < D / 16; j += 4)
+        *reinterpret_cast<f32x4*>(&part[wave][x.n][(4 * x.g + i) * (D / 16) + j]) =
+            f32x4{x.o[r][j][i], x.o[r][j + 1][i], x.o[r][j + 2][i], x.o[r][j + 3][i]};
+    __syncthreads();
+    for (int e = threadIdx.x; e < 16 * (D / 4); e += kRowWaves * 64) {
+      const int row = e / (D / 4), d = (e % (D / 4)) * 4;
+      float mt = -INFINITY;
+#pragma unroll
+      for (int v = 0; v < kRowWaves; ++v) mt = fmaxf(mt, ml[v][row][0]);
+      const float mm = mt == -INFINITY ? 0.0f : mt;
+      float lt = 0.0f;
+      f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int v = 0; v < kRowWaves; ++v) {
+        const float f = __builtin_amdgcn_exp2f(ml[v][row][0] - mm);
+        lt += ml[v][row][1] * f;
+        acc += *reinterpret_cast<const f32x4*>(&part[v][row][d]) * f;
+      }
+      const int at = w.row0 + 16 * r + row;
+      if (at >= w.rows) continue;
+      if (w.parts > 1) {
+        *reinterpret_cast<f32x4*>(p.part_o + (slot + 16 * r + row) * D + d) = acc;
+        if (d == 0) {
+          p.part_ml[(slot + 16 * r + row) * 2] = mt;
+          p.part_ml[(slot + 16 * r + row) * 2 + 1] = lt;
+        }
+      } else {
+        const int i = at / p.group;
+        const float inv = lt == 0.0f ? 0.0f : 1.0f / lt;
+        uint16_t* op = p.o + static_cast<int64_t>(w.first + i) * p.o_token +
+                       static_cast<int64_t>(h * p.group + at - i * p.group) * p.o_head + d;
+        *reinterpret_cast<u32x2*>(op) = u32x2{cvt_pk_bf16x2(acc[0] * inv, acc[1] * inv),
+                                              cvt_pk_bf16x2(acc[2] * inv, acc[3] * inv)};
+      }
+    }
+  }
+}
+
+// ---- many rows ---------------------------------------------------------------
+//
+// 128 rows a workgroup, 32 a wave; blocks of 64 positions.  The layouts of the
+// products are those of 32x32x16 MFMAs on K and V in LDS: K row-major, 16-byte chunk
+// c of row r at c ^ (r & 15) (dim 64: c ^ ((r >> 1) & 7)); V row-major, read with
+// ds_read_b64_tr_b16, chunk c of row r at c ^ 4 (r & 3) (dim 64: c ^ 4 ((r >> 1) & 1)).
+// The codes of the next block are on their way to registers while this one
+// computes, and are decoded into the other buffer after it.
+constexpr int kTileRows = 128;
+constexpr int kBlock = 64;
+constexpr int kTileThreads = 256;
+
 template <int D, int FMT>
-__global__ __launch_bounds__(64) void sdpa_cached_simple(const CachedArgs p) {
-  const CacheArgs& c = p.c;
-  int b, i, first, n;
-  if (!find_item(c.seqs, blockIdx.x, TokensOf{c}, b, i)) return;
-  seq_tokens(c, b, first, n);
-  const int hq = blockIdx.y, h = hq / p.group, lane = threadIdx.x;
-  float q[D / 64], o[D / 64], m = -INFINITY, l = 0.0f;
-  const uint16_t* qr = p.q + (first + i) * p.q_token + hq * p.q_head;
-  for (int d = 0; d < D / 64; ++d) {
-    q[d] = bf16_to_f32(qr[d * 64 + lane]);
-    o[d] = 0.0f;
+struct Tiles {
+  static constexpr int ND = D / 32, NDC = D / 16;
+  static constexpr int kChunks = D / 16;                    // 16-byte pieces of codes in a row
+  static constexpr int kLoads = kBlock * kChunks / kTileThreads;  // of a thread, for K and for V
+
+  const CachedArgs& p;
+  const Plan& w;
+  const Span& s;
+  uint16_t (*Ks)[kBlock * D];
+  uint16_t (*Vs)[kBlock * D];
+  int hd, wave, lane, l32, h;
+  int from, end;   // what the lane's row sees
+  bf16x8 qop[NDC];
+  f32x16 o[ND];
+  float m, l;
+  Subtiles sub;    // of blocks kb0 .. kb0 + 15
+  u32x4 kraw[kLoads], vraw[kLoads];
+  int k_frag, v_frag[ND];
+
+  static __device__ __forceinline__ int k_swz(int r) { return D == 128 ? r & 15 : (r >> 1) & 7; }
+  static __device__ __forceinline__ int v_swz(int r) {
+    return D == 128 ? (r & 3) << 2 : ((r >> 1) & 1) << 2;
   }
-  int from, end;
-  seen_by(c, c.lengths[b], n, i, p.window, from, end);
-  for (int j = from; j < end; ++j) {
-    const int page = page_at(c, b, j);
-    if (page < 0) continue;
-    const int64_t at = slot_offset(c, page, h, j & ((1 << c.shift) - 1));
-    const int64_t sc = static_cast<int64_t>(page) * c.heads + h;
-    float s = 0.0f;
-    for (int d = 0; d < D / 64; ++d) s += q[d] * from_code<FMT>(c.k[at + d * 64 + lane]);
-    s = wave_sum(s) * c.k_scale[sc] * p.scale;
-    if (p.softcap > 0.0f) s = p.softcap * tanhf(s / p.softcap);
-    const float mn = fmaxf(m, s), e = expf(s - (mn == -INFINITY ? 0.0f : mn));
-    const float alpha = m == -INFINITY ? 0.0f : expf(m - mn);
-    l = l * alpha + e;
-    for (int d = 0; d < D / 64; ++d)
-      o[d] = o[d] * alpha + e * (from_code<FMT>(c.v[at + d * 64 + lane]) * c.v_scale[sc]);
-    m = mn;
+  // the row and the piece of codes of a thread's load i; the rows of a wave's load
+  // are in one subtile
+  __device__ __forceinline__ int load_row(int i) const {
+    return (static_cast<int>(threadIdx.x) + i * kTileThreads) / kChunks;
   }
-  uint16_t* orow = p.o + (first + i) * p.o_token + hq * p.o_head;
-  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-  for (int d = 0; d < D / 64; ++d) orow[d * 64 + lane] = f32_to_bf16(o[d] * inv);
+  __device__ __forceinline__ int load_sub(int i) const {
+    return (wave * 64 + i * kTileThreads) / kChunks / 16;
+  }
+
+  __device__ __forceinline__ void setup() {
+    k_frag = l32 * D + ((h ^ k_swz(l32)) << 3);
+    const int vr = (lane & 15) >> 2;
+#pragma unroll
+    for (int j = 0; j < ND; ++j) {
+      const int chunk = 4 * j + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+      v_frag[j] = (4 * h + vr) * D + ((chunk ^ v_swz(vr)) << 3) + 4 * (lane & 1);
+    }
+  }
+  __device__ __forceinline__ void refill(int kb) {  // kb a multiple of 16
+    const int pos = s.begin + kb * kBlock + lane * 16;
+    sub.load(p, w.b, hd, pos >= 0 && pos < s.hi ? pos : -1);
+  }
+  __device__ __forceinline__ void load(int kb) {
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const int st = load_sub(i), row = load_row(i);
+      const int page = max(__builtin_amdgcn_readlane(sub.page, (kb & 15) * 4 + st), 0);
+      const int slot = (s.begin + kb * kBlock + 16 * st) & ((1 << p.c.shift) - 1);
+      const int64_t at = slot_offset(p.c, page, hd, slot);
+      const int off = (row - 16 * st) * D + (threadIdx.x % kChunks) * 16;
+      kraw[i] = *reinterpret_cast<const u32x4*>(p.c.k + at + off);
+      vraw[i] = *reinterpret_cast<const u32x4*>(p.c.v + at + off);
+    }
+  }
+  // block kb's codes, decoded, into LDS; those that no row sees as zeros (V)
+  __device__ __forceinline__ void stage(int kb, int buf) {
+    const int pos = s.begin + kb * kBlock;
+    const bool edge = pos < s.lo || pos + kBlock > s.hi ||
+                      __any(lane >> 2 == (kb & 15) && sub.page < 0);
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const int row = load_row(i), c = threadIdx.x % kChunks;
+      if (edge) {
+        const bool there = __builtin_amdgcn_readlane(sub.page, (kb & 15) * 4 + load_sub(i)) >= 0;
+        if (!there || pos + row < s.lo || pos + row >= s.hi) vraw[i] = u32x4{0u, 0u, 0u, 0u};
+      }
+      uint16_t* kd = Ks[buf] + row * D;
+      uint16_t* vd = Vs[buf] + row * D;
+      *reinterpret_cast<u32x4*>(kd + ((2 * c ^ k_swz(row)) << 3)) = eight_of<FMT>(kraw[i][0], kraw[i][1]);
+      *reinterpret_cast<u32x4*>(kd + (((2 * c + 1) ^ k_swz(row)) << 3)) = eight_of<FMT>(kraw[i][2], kraw[i][3]);
+      *reinterpret_cast<u32x4*>(vd + ((2 * c ^ v_swz(row)) << 3)) = eight_of<FMT>(vraw[i][0], vraw[i][1]);
+      *reinterpret_cast<u32x4*>(vd + (((2 * c + 1) ^ v_swz(row)) << 3)) = eight_of<FMT>(vraw[i][2], vraw[i][3]);
+    }
+  }
+  __device__ __forceinline__ i16x4 read_v4(const uint16_t* Vb, int kv, int j) const {
+    return __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(Vb + v_frag[j] + kv * D));
+  }
+  __device__ __forceinline__ void scores(const uint16_t* K_, f32x16 (&sv)[2]) {
+    constexpr int kAhead = 4;
+    const auto frag = [&](int i) {
+      return *reinterpret_cast<const bf16x8*>(K_ + (k_frag ^ ((i % NDC) * 16)) + (i / NDC) * 32 * D);
+    };
+    bf16x8 f[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) f[i] = frag(i);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) sv[t][r] = 0.0f;
+#pragma unroll
+      for (int dc = 0; dc < NDC; ++dc) {
+        const int i = t * NDC + dc;
+        sv[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f[i % kAhead], qop[dc], sv[t], 0, 0, 0);
+        if (i + kAhead < 2 * NDC) f[i % kAhead] = frag(i + kAhead);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+  }
+
+  __device__ __forceinline__ void block(int kb, int buf) {
+    const uint16_t *Kc = Ks[buf], *Vc = Vs[buf];
+    const int pos = s.begin + kb * kBlock;
+    f32x16 cur[2];
+    scores(Kc, cur);
+    // V^T operand i of lane (d = 32 j + l32, h), j = i % ND: positions {16 c + 4 h + u,
+    // 16 c + 4 h + 8 + u}, c = i / ND; the first ones are read under the softmax
+    const auto vfrag = [&](int i) {
+      const i16x4 lo = read_v4(Vc, 16 * (i / ND), i % ND);
+      const i16x4 hi = read_v4(Vc, 16 * (i / ND) + 8, i % ND);
+      const i16x8 f = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+      return __builtin_bit_cast(bf16x8, f);
+    };
+    constexpr int kAhead = 4;
+    bf16x8 vf[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) vf[i] = vfrag(i);
+    __builtin_amdgcn_sched_barrier(0);
+
+    float ks[4], vs[4];
+    bool there[4];
+    bool all = true;
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      const int at = (kb & 15) * 4 + t;
+      ks[t] = uniform(sub.kscale, at);
+      vs[t] = uniform(sub.vscale, at);
+      there[t] = __builtin_amdgcn_readlane(sub.page, at) >= 0;
+      all = all && there[t];
+    }
+    // accumulator r of half t: position 32 t + 8 (r / 4) + 4 h + r % 4, subtile 2 t + r / 8
+    float mx = -INFINITY;
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) cur[t][r] = score(cur[t][r], ks[2 * t + (r >> 3)], p.cap_log2);
+    if (!all || pos < s.all_lo || pos + kBlock > s.all_hi) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int j = pos + 32 * t + 8 * (r >> 2) + 4 * h + (r & 3);
+          if (!there[2 * t + (r >> 3)] || j < from || j >= end) cur[t][r] = -INFINITY;
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) mx = fmaxf(mx, cur[t][r]);
+    if (__any(mx > m)) {
+      const float to = fmaxf(m, xor32_max(mx));
+      const float alpha = to == m ? 1.0f : __builtin_amdgcn_exp2f(m - to);
+      l *= alpha;
+#pragma unroll
+      for (int j = 0; j < ND; ++j) o[j] *= alpha;
+      m = to;
+    }
+    const float mm = m == -INFINITY ? 0.0f : m;
+    float rs = 0.0f;
+    bf16x8 pb[4];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const int t = c >> 1, r0 = 8 * (c & 1);
+      float e[8];
+#pragma unroll
+      for (int r = 0; r < 8; ++r) {
+        e[r] = __builtin_amdgcn_exp2f(cur[t][r0 + r] - mm);
+        rs += e[r];
+      }
+      u32x4 f;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) f[r] = cvt_pk_bf16x2(e[2 * r] * vs[c], e[2 * r + 1] * vs[c]);
+      pb[c] = __builtin_bit_cast(bf16x8, f);
+    }
+    l += rs;  // of this lane's positions: the two halves meet at the end
+#pragma unroll
+    for (int i = 0; i < 4 * ND; ++i) {
+      o[i % ND] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[i % kAhead], pb[i / ND], o[i % ND], 0,
+                                                          0, 0);
+      if (i + kAhead < 4 * ND) vf[i % kAhead] = vfrag(i + kAhead);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+};
+
+template <int D, int FMT>
+__global__ __launch_bounds__(kTileThreads, 2) void cached_tiles_kernel(const CachedArgs p) {
+  __shared__ __attribute__((aligned(256))) uint16_t KV[2][2][kBlock * D];
+  Division<kTileRows> div{p};
+  div.divide();
+  Plan w;
+  if (!div.template find<false>(blockIdx.x / p.c.heads, w)) return;
+  const Span s = span_of<kTileRows, kBlock>(p, w);
+  Tiles<D, FMT> x{p, w, s, KV[0], KV[1]};
+  x.hd = blockIdx.x % p.c.heads;
+  x.lane = threadIdx.x & 63;
+  x.wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  x.l32 = x.lane & 31;
+  x.h = x.lane >> 5;
+  x.setup();
+  x.m = -INFINITY;
+  x.l = 0.0f;
+  const int row = w.row0 + x.wave * 32 + x.l32, qrow = min(row, w.rows - 1);
+  const int i = qrow / p.group;
+  const int64_t head = x.hd * p.group + qrow - i * p.group;
+  seen_by(p.c, w.len, w.n, i, p.window, x.from, x.end);
+  const int nb = s.end > s.begin ? (s.end - s.begin + kBlock - 1) / kBlock : 0;
+  if (nb > 0) {
+    x.refill(0);
+    x.load(0);
+  }
+  const uint16_t* qp = p.q + static_cast<int64_t>(w.first + i) * p.q_token + head * p.q_head;
+#pragma unroll
+  for (int dc = 0; dc < D / 16; ++dc)
+    x.qop[dc] = *reinterpret_cast<const bf16x8*>(qp + dc * 16 + 8 * x.h);
+#pragma unroll
+  for (int j = 0; j < D / 32; ++j)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) x.o[j][r] = 0.0f;
+  // the positions that some row of this wave sees
+  const int i_lo = min(w.row0 + x.wave * 32, w.rows - 1) / p.group;
+  const int i_hi = min(w.row0 + x.wave * 32 + 31, w.rows - 1) / p.group;
+  int wave_lo, wave_hi, unused;
+  seen_by(p.c, w.len, w.n, i_lo, p.window, wave_lo, unused);
+  seen_by(p.c, w.len, w.n, i_hi, p.window, unused, wave_hi);
+  if (w.row0 + x.wave * 32 >= w.rows) wave_hi = 0;
+  if (nb > 0) x.stage(0, 0);
+  __syncthreads();
+  for (int kb = 0; kb < nb; ++kb) {
+    // (sub holds what block kb's scores need; the next block's is loaded early
+    // only within the same sixteen)
+    const bool more = kb + 1 < nb, ahead = more && ((kb + 1) & 15) != 0;
+    if (ahead) x.load(kb + 1);
+    const int pos = s.begin + kb * kBlock;
+    if (pos < wave_hi && pos + kBlock > wave_lo) x.block(kb, kb & 1);
+    if (more && !ahead) {
+      x.refill(kb + 1);
+      x.load(kb + 1);
+    }
+    if (more) x.stage(kb + 1, (kb + 1) & 1);
+    __syncthreads();
+  }
+  if (row >= w.rows) return;
+  const float lt = xor32_add(x.l);
+  if (w.parts > 1) {
+    const int64_t at = (static_cast<int64_t>(w.slot + w.part) * p.c.heads + x.hd) * kTileRows +
+                       (row - w.row0);
+#pragma unroll
+    for (int j = 0; j < D / 32; ++j)
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        *reinterpret_cast<f32x4*>(p.part_o + at * D + 32 * j + 8 * u + 4 * x.h) =
+            f32x4{x.o[j][4 * u], x.o[j][4 * u + 1], x.o[j][4 * u + 2], x.o[j][4 * u + 3]};
+    if (x.h == 0) {
+      p.part_ml[at * 2] = x.m;
+      p.part_ml[at * 2 + 1] = lt;
+    }
+    return;
+  }
+  const float inv = lt == 0.0f ? 0.0f : 1.0f / lt;
+  uint16_t* op = p.o + static_cast<int64_t>(w.first + i) * p.o_token + head * p.o_head;
+#pragma unroll
+  for (int j = 0; j < D / 32; ++j)
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      *reinterpret_cast<u32x2*>(op + 32 * j + 8 * u + 4 * x.h) =
+          u32x2{cvt_pk_bf16x2(x.o[j][4 * u] * inv, x.o[j][4 * u + 1] * inv),
+                cvt_pk_bf16x2(x.o[j][4 * u + 2] * inv, x.o[j][4 * u + 3] * inv)};
+}
+
+// The parts of a tile, in their order; a thread has four elements of a row.
+template <int D, int BM>
+__global__ __launch_bounds__(256) void cached_join_kernel(const CachedArgs p) {
+  Division<BM> div{p};
+  div.divide();
+  Plan w;
+  if (!div.template find<true>(blockIdx.x / p.c.heads, w) || w.parts == 1) return;
+  const int h = blockIdx.x % p.c.heads;
+  const int n = min(BM, w.rows - w.row0);
+  for (int e = threadIdx.x; e < n * (D / 4); e += 256) {
+    const int row = e / (D / 4), d = (e % (D / 4)) * 4;
+    const int64_t step = static_cast<int64_t>(p.c.heads) * BM;
+    const int64_t at = (static_cast<int64_t>(w.slot) * p.c.heads + h) * BM + row;
+    float mt = -INFINITY;
+    for (int i = 0; i < w.parts; ++i) mt = fmaxf(mt, p.part_ml[(at + i * step) * 2]);
+    const float mm = mt == -INFINITY ? 0.0f : mt;
+    float lt = 0.0f;
+    f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int i = 0; i < w.parts; ++i) {
+      const float f = __builtin_amdgcn_exp2f(p.part_ml[(at + i * step) * 2] - mm);
+      lt += p.part_ml[(at + i * step) * 2 + 1] * f;
+      acc += *reinterpret_cast<const f32x4*>(p.part_o + (at + i * step) * D + d) * f;
+    }
+    const int i = (w.row0 + row) / p.group;
+    const float inv = lt == 0.0f ? 0.0f : 1.0f / lt;
+    uint16_t* op = p.o + static_cast<int64_t>(w.first + i) * p.o_token +
+                   static_cast<int64_t>(h * p.group + w.row0 + row - i * p.group) * p.o_head + d;
+    *reinterpret_cast<u32x2*>(op) = u32x2{cvt_pk_bf16x2(acc[0] * inv, acc[1] * inv),
+                                          cvt_pk_bf16x2(acc[2] * inv, acc[3] * inv)};
+  }
+}
+
+// ---- the choice --------------------------------------------------------------
+
+// Rows of a tile and about how many parts, by the sizes that the host knows.
+struct Choice {
+  int bm;
+  int64_t tiles;   // at most
+  int32_t target, least;
+};
+Choice choose(const ttlh_kv_cache* c, int64_t q_heads) {
+  Choice x;
+  const int64_t group = q_heads / c->heads;
+  // rows of a sequence: on average, half as many again where they may differ
+  const int64_t rows = c->tokens * group;
+  const int64_t some = (c->starts ? rows + rows / 2 : rows) / (c->seqs > 0 ? c->seqs : 1);
+  x.bm = some <= 16 ? 16 : some <= 32 ? 32 : some <= 48 ? 48 : kTileRows;
+  x.tiles = (c->starts ? rows / x.bm + c->seqs : c->seqs * ((group + x.bm - 1) / x.bm));
+  const int64_t places = x.bm == kTileRows ? 512 : 1024;  // workgroups that fill the chip
+  x.least = 256;
+  const int64_t positions = c->width * c->page;
+  // (undivided where the tiles that there are for certain fill it, or no sequence
+  // can be longer than one part)
+  const int64_t certain = c->starts ? rows / x.bm : x.tiles;
+  x.target = certain * c->heads >= places || positions <= x.least
+                 ? 0
+                 : static_cast<int32_t>((places + c->heads - 1) / c->heads);
+  return x;
+}
+
+int64_t workspace_bytes(const ttlh_kv_cache* c, const Choice& x) {
+  return 2 * int64_t(x.target) * c->heads * x.bm * (c->dim + 2) * 4;
 }
 
 }  // namespace
@@ -78,19 +920,25 @@ __global__ __launch_bounds__(64) void sdpa_cached_simple(const CachedArgs p) {
 using namespace ttlh;
 
 extern "C" int64_t ttlh_sdpa_cached_workspace_bytes(const ttlh_kv_cache* cache, int64_t q_heads) {
-  return 0;
+  CacheArgs a;
+  if (check_cache("ttlh_sdpa_cached_workspace_bytes", cache, &a) != TTLH_OK || q_heads <= 0 ||
+      q_heads % cache->heads)
+    return 0;
+  return workspace_bytes(cache, choose(cache, q_heads));
 }
 
 extern "C" int ttlh_sdpa_cached(const ttlh_kv_cache* cache, const void* Q, void* O, int64_t q_heads,
                                 int64_t q_token, int64_t q_head, int64_t o_token, int64_t o_head,
                                 float scale, int64_t window, float softcap, void* workspace,
-                                int64_t workspace_bytes, void* stream) {
+                                int64_t workspace_size, void* stream) {
   clear_error();
   CachedArgs a;
   const int st = check_cache("ttlh_sdpa_cached", cache, &a.c);
   if (st != TTLH_OK) return st;
-  TTLH_REQUIRE(q_heads > 0 && q_heads % cache->heads == 0 && q_heads < 65536, TTLH_EINVAL,
+  TTLH_REQUIRE(q_heads > 0 && q_heads % cache->heads == 0, TTLH_EINVAL,
                "ttlh_sdpa_cached: q heads must be a multiple of the cache's");
+  TTLH_REQUIRE(q_heads < 65536 && cache->tokens * q_heads < (int64_t(1) << 31), TTLH_EUNSUPPORTED,
+               "ttlh_sdpa_cached: too many q heads or tokens");
   TTLH_REQUIRE(std::isfinite(scale), TTLH_EINVAL, "ttlh_sdpa_cached: scale must be finite");
   TTLH_REQUIRE(softcap >= 0.0f && std::isfinite(softcap), TTLH_EINVAL,
                "ttlh_sdpa_cached: softcap must be finite and not negative");
@@ -100,24 +948,53 @@ extern "C" int ttlh_sdpa_cached(const ttlh_kv_cache* cache, const void* Q, void*
   TTLH_REQUIRE(((reinterpret_cast<uintptr_t>(Q) | reinterpret_cast<uintptr_t>(O)) & 15) == 0 &&
                    ((q_token | q_head | o_token | o_head) & 7) == 0,
                TTLH_EINVAL, "ttlh_sdpa_cached: Q and O must be 16-byte aligned, strides multiples of 8");
+  const Choice x = choose(cache, q_heads);
+  const int64_t need = workspace_bytes(cache, x);
+  TTLH_REQUIRE(need == 0 || (workspace && workspace_size >= need &&
+                             (reinterpret_cast<uintptr_t>(workspace) & 15) == 0),
+               TTLH_EINVAL, "ttlh_sdpa_cached: the workspace must have %lld bytes, 16-byte aligned",
+               static_cast<long long>(need));
   a.q = static_cast<const uint16_t*>(Q);
   a.o = static_cast<uint16_t*>(O);
   a.q_token = q_token;
   a.q_head = q_head;
   a.o_token = o_token;
   a.o_head = o_head;
-  a.q_heads = static_cast<int32_t>(q_heads);
   a.group = static_cast<int32_t>(q_heads / cache->heads);
   a.window = static_cast<int32_t>(window < (int64_t(1) << 31) ? window : 0);
-  a.scale = scale;
-  a.softcap = softcap;
-  const dim3 grid(static_cast<uint32_t>(cache->tokens), static_cast<uint32_t>(q_heads));
+  a.target = x.target;
+  a.least = x.least;
+  a.scale_log2 = softcap > 0.0f ? scale / softcap * 2.0f * kLog2e : scale * kLog2e;
+  a.cap_log2 = softcap * kLog2e;
+  a.part_o = static_cast<float*>(workspace);
+  a.part_ml = a.part_o + 2 * int64_t(x.target) * cache->heads * x.bm * cache->dim;
+  const int64_t items = (x.tiles + x.target) * cache->heads;
+  TTLH_REQUIRE(items < (int64_t(1) << 31), TTLH_EUNSUPPORTED, "ttlh_sdpa_cached: too many tiles");
+  const dim3 grid(static_cast<uint32_t>(items));
+  const dim3 joins(static_cast<uint32_t>(x.tiles * cache->heads));
   hipStream_t s = static_cast<hipStream_t>(stream);
-  const auto run = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(64), 0, s, a); };
-  const bool int8 = cache->format == TTLH_CACHE_INT8;
+  const auto run = [&](auto kernel, int threads, auto join) {
+    hipLaunchKernelGGL(kernel, grid, dim3(threads), 0, s, a);
+    if (x.target) hipLaunchKernelGGL(join, joins, dim3(256), 0, s, a);
+  };
+  const auto pick = [&](auto dim, auto fmt) {
+    constexpr int D = decltype(dim)::value, F = decltype(fmt)::value;
+    if (x.bm == 16)
+      run(cached_rows_kernel<D, F, 1>, 64 * kRowWaves, cached_join_kernel<D, 16>);
+    else if (x.bm == 32)
+      run(cached_rows_kernel<D, F, 2>, 64 * kRowWaves, cached_join_kernel<D, 32>);
+    else if (x.bm == 48)
+      run(cached_rows_kernel<D, F, 3>, 64 * kRowWaves, cached_join_kernel<D, 48>);
+    else
+      run(cached_tiles_kernel<D, F>, kTileThreads, cached_join_kernel<D, kTileRows>);
+  };
+  const std::integral_constant<int, 64> d64;
+  const std::integral_constant<int, 128> d128;
+  const std::integral_constant<int, TTLH_CACHE_INT8> i8;
+  const std::integral_constant<int, TTLH_CACHE_E4M3> f8;
   if (cache->dim == 128)
-    int8 ? run(sdpa_cached_simple<128, TTLH_CACHE_INT8>) : run(sdpa_cached_simple<128, TTLH_CACHE_E4M3>);
+    cache->format == TTLH_CACHE_INT8 ? pick(d128, i8) : pick(d128, f8);
   else
-    int8 ? run(sdpa_cached_simple<64, TTLH_CACHE_INT8>) : run(sdpa_cached_simple<64, TTLH_CACHE_E4M3>);
-  return check_launch("sdpa_cached_simple");
+    cache->format == TTLH_CACHE_INT8 ? pick(d64, i8) : pick(d64, f8);
+  return check_launch("ttlh_sdpa_cached");
 }

@@ -72,6 +72,17 @@ def _workspace(device: torch.device, stream, nbytes: int,
     return ws
 
 
+def _workspace_or_graphs(device: torch.device, stream, nbytes: int, sp: int) -> torch.Tensor:
+    """The cached workspace; under capture memory of the graph's own, which no
+    eager call, no other graph and no later, larger workspace has to do with."""
+    if not torch.cuda.is_current_stream_capturing():
+        return _workspace(device, stream, nbytes, sp)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    if stream is not None:
+        ws.record_stream(stream)
+    return ws
+
+
 # The matmul's scratch (partial sums of products that divide K among several
 # workgroups, and their counters): a fixed 4 MiB per (device, stream), zeroed
 # once and left to the library; the oldest goes back to the allocator when a
@@ -937,5 +948,7 @@ def sdpa_cached(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
     tensors = (q, k_cache, v_cache, k_scale, v_scale, table, lengths, o)
     _check_on_one_device("sdpa_cached", tensors if starts is None else tensors + (starts,), stream)
     sp = L.stream_ptr(stream)
+    nbytes = L.load().ttlh_sdpa_cached_workspace_bytes(cache, q_heads)
+    ws = _workspace_or_graphs(q.device, stream, nbytes, sp) if nbytes else None
     L.call("ttlh_sdpa_cached", cache, q.data_ptr(), o.data_ptr(), q_heads, *_head_strides(q),
-           *_head_strides(o), scale, window, softcap, 0, 0, sp)
+           *_head_strides(o), scale, window, softcap, 0 if ws is None else ws.data_ptr(), nbytes, sp)
