@@ -8,9 +8,17 @@
 // off, which fp32 cannot hold from position 2^10 on, so a workgroup computes the
 // angles of its tokens in fp64, once for all heads, into LDS.
 //
-// kv_cache_write: a workgroup for each (page that gets tokens, head, K or V).
+// kv_cache_write: reads the tokens once and writes a byte for each value; HBM bound
+// for prompts, latency bound for a token each.
+//  * kv_write_kernel: a workgroup for each page that gets tokens and head, K and V.
+//    The values stay in registers between the search for the largest one and their
+//    rounding.
+//  * kv_write_one_kernel (no starts: a token for each sequence): a thread for each
+//    eight values, so that a page's head is a group of 8 or 16 lanes that needs no
+//    barrier; earlier codes are touched where a scale grows.
 
 #include <cmath>
+#include <type_traits>
 
 #include "ttlh_common.h"
 #include "ttlh_kvcache.h"
@@ -169,6 +177,7 @@ struct WriteArgs {
   CacheArgs c;
   const void* x[2];
   int64_t token[2], head[2];
+  bool vec;  // 16-byte loads
 };
 
 // pages that sequence b's new tokens reach
@@ -184,54 +193,164 @@ struct PagesOf {
   }
 };
 
-template <typename T, int FMT>
+// Eight neighbouring values.
+template <typename T>
+struct Eight {
+  u32x4 w[sizeof(T) / 2];
+  // vec: 16-byte loads; else element by element
+  __device__ __forceinline__ void load(const T* x, bool vec) {
+    if (vec) {
+#pragma unroll
+      for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i)
+        w[i] = reinterpret_cast<const u32x4*>(x)[i];
+    } else if constexpr (sizeof(T) == 2) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[0][i] = x[2 * i] | static_cast<uint32_t>(x[2 * i + 1]) << 16;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) w[i / 4][i % 4] = __float_as_uint(x[i]);
+    }
+  }
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) w[i] = u32x4{0u, 0u, 0u, 0u};
+  }
+  __device__ __forceinline__ uint32_t bits(int i) const {  // of value i as fp32
+    if constexpr (sizeof(T) == 2)
+      return (i & 1) ? w[0][i / 2] & 0xffff0000u : w[0][i / 2] << 16;
+    else
+      return w[i / 4][i % 4];
+  }
+  // the largest magnitude by its bits: infinities and NaN are larger than any number
+  __device__ __forceinline__ uint32_t largest() const {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = max(m, bits(i) & 0x7fffffffu);
+    return m;
+  }
+  // the codes of value * inv (zeros where inv is NaN)
+  template <int FMT>
+  __device__ __forceinline__ uint2 codes(float inv) const {
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = inv == inv ? __uint_as_float(bits(i)) * inv : 0.0f;
+    return uint2{four_codes<FMT>(v[0], v[1], v[2], v[3]), four_codes<FMT>(v[4], v[5], v[6], v[7])};
+  }
+};
+
+// codes whose scale grows: times `down` = old / new scale, and rounded again
+template <int FMT>
+__device__ __forceinline__ uint2 scaled_down(uint2 c, float down) {
+  float v[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    v[i] = from_code<FMT>(static_cast<uint8_t>((i < 4 ? c.x : c.y) >> (8 * (i & 3)))) * down;
+  return uint2{four_codes<FMT>(v[0], v[1], v[2], v[3]), four_codes<FMT>(v[4], v[5], v[6], v[7])};
+}
+
+// SWEEPS: rounds of 256 threads with eight values each that cover a page's head.
+template <typename T, int FMT, int D, int SWEEPS>
 __global__ __launch_bounds__(256) void kv_write_kernel(const WriteArgs p) {
+  constexpr int kPer = D / 8;              // threads of a token
+  constexpr int kTokens = 256 / kPer;      // tokens of a sweep
   const CacheArgs& c = p.c;
   int b, j;
   if (!find_item(c.seqs, blockIdx.x, PagesOf{c}, b, j)) return;
-  const int h = blockIdx.y, which = blockIdx.z;
+  const int h = blockIdx.y;
   int first, n;
   seq_tokens(c, b, first, n);
-  const int len = c.lengths[b], begin = len - n;  // (len >= 1 here)
-  const int slot_page = (max(begin, 0) >> c.shift) + j;
-  const int page0 = slot_page << c.shift;
+  const int len = c.lengths[b];  // (>= 1 here)
+  const int64_t begin = static_cast<int64_t>(len) - n;
+  const int page0 = (static_cast<int>(begin > 0 ? begin >> c.shift : 0) + j) << c.shift;
   const int page = page_at(c, b, page0);
   if (page < 0) return;
-  const int lo = max(begin, page0) - page0;  // slots lo .. hi - 1 get tokens
-  const int hi = min(len, page0 + (1 << c.shift)) - page0;
-  const bool earlier = begin > page0;
-  const T* x = static_cast<const T*>(p.x[which]) + h * p.head[which] +
-               static_cast<int64_t>(first + page0 - begin) * p.token[which];
-  uint8_t* codes = (which ? c.v : c.k) + slot_offset(c, page, h, 0);
-  float* scale = (which ? c.v_scale : c.k_scale) + static_cast<int64_t>(page) * c.heads + h;
-
-  // the largest magnitude, by its bits: infinity and NaN are the largest ones
-  uint32_t big = 0;
-  for (int i = threadIdx.x + lo * c.dim; i < hi * c.dim; i += 256) {
-    const int s = i / c.dim;
-    big = max(big, __float_as_uint(to_f32(x[s * p.token[which] + i - s * c.dim])) & 0x7fffffffu);
+  const int lo = begin > page0 ? static_cast<int>(begin) - page0 : 0;  // slots lo .. hi - 1
+  const int hi = min(len - page0, 1 << c.shift);
+  const int t0 = threadIdx.x / kPer, e = (threadIdx.x % kPer) * 8;
+  Eight<T> x[2][SWEEPS];
+  uint32_t big[2] = {0, 0};
+#pragma unroll
+  for (int i = 0; i < SWEEPS; ++i) {
+    const int t = t0 + i * kTokens;
+#pragma unroll
+    for (int z = 0; z < 2; ++z)
+      if (t >= lo && t < hi)
+        x[z][i].load(static_cast<const T*>(p.x[z]) + (first + page0 - begin + t) * p.token[z] +
+                         h * p.head[z] + e, p.vec);
+      else
+        x[z][i].clear();
   }
-  __shared__ uint32_t part[4];
-  big = wave_max(big);
-  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = big;
+#pragma unroll
+  for (int z = 0; z < 2; ++z) {
+#pragma unroll
+    for (int i = 0; i < SWEEPS; ++i) big[z] = max(big[z], x[z][i].largest());
+    big[z] = wave_max(big[z]);
+  }
+  __shared__ uint32_t part[2][4];
+  if ((threadIdx.x & 63) == 0) {
+    part[0][threadIdx.x >> 6] = big[0];
+    part[1][threadIdx.x >> 6] = big[1];
+  }
   __syncthreads();
-  big = max(max(part[0], part[1]), max(part[2], part[3]));
+#pragma unroll
+  for (int z = 0; z < 2; ++z) {
+    float* scale = (z ? c.v_scale : c.k_scale) + static_cast<int64_t>(page) * c.heads + h;
+    uint8_t* codes = (z ? c.v : c.k) + slot_offset(c, page, h, 0) + e;
+    const uint32_t m = max(max(part[z][0], part[z][1]), max(part[z][2], part[z][3]));
+    float s = scale_for(__uint_as_float(m), FMT);
+    if (lo > 0) {  // earlier tokens
+      const float old = *scale;
+      s = joined_scale(old, s);
+      if (s > old)
+        for (int t = t0; t < lo; t += kTokens) {
+          uint2* at = reinterpret_cast<uint2*>(codes + t * D);
+          *at = scaled_down<FMT>(*at, old / s);
+        }
+    }
+    const float inv = 1.0f / s;
+#pragma unroll
+    for (int i = 0; i < SWEEPS; ++i) {
+      const int t = t0 + i * kTokens;
+      if (t >= lo && t < hi) *reinterpret_cast<uint2*>(codes + t * D) = x[z][i].template codes<FMT>(inv);
+    }
+    if (lo > 0) __syncthreads();  // (uniform) every thread has read the old scale
+    if (threadIdx.x == 0) *scale = s;
+  }
+}
+
+template <typename T, int FMT, int D>
+__global__ __launch_bounds__(256) void kv_write_one_kernel(const WriteArgs p) {
+  constexpr int kPer = D / 8;
+  const CacheArgs& c = p.c;
+  const int b = blockIdx.x;
+  const int unit = blockIdx.y * (256 / kPer) + threadIdx.x / kPer;  // (head, K or V)
+  const int h = unit >> 1, z = unit & 1, e = (threadIdx.x % kPer) * 8;
+  const int pos = c.lengths[b] - 1, page = page_at(c, b, c.lengths[b] > 0 ? pos : -1);
+  if (page < 0 || h >= c.heads) return;
+  const int slot = pos & ((1 << c.shift) - 1);
+  float* scale = (z ? c.v_scale : c.k_scale) + static_cast<int64_t>(page) * c.heads + h;
+  uint8_t* codes = (z ? c.v : c.k) + slot_offset(c, page, h, 0) + e;
+  Eight<T> x;
+  x.load(static_cast<const T*>(z ? p.x[1] : p.x[0]) + b * (z ? p.token[1] : p.token[0]) +
+             h * (z ? p.head[1] : p.head[0]) + e, p.vec);
   const float old = *scale;
-  float s = scale_for(__uint_as_float(big), FMT);
-  if (earlier) s = joined_scale(old, s);
-  if (earlier && s > old) {
-    const float down = old / s;
-    for (int i = threadIdx.x; i < lo * c.dim; i += 256)
-      codes[i] = to_code<FMT>(from_code<FMT>(codes[i]) * down);
+  uint32_t m = x.largest();
+#pragma unroll
+  for (int i = kPer / 2; i; i >>= 1)
+    m = max(m, static_cast<uint32_t>(__shfl_xor(static_cast<int>(m), i)));
+  float s = scale_for(__uint_as_float(m), FMT);
+  if (slot > 0) {
+    s = joined_scale(old, s);
+    if (s > old)
+      for (int t = 0; t < slot; ++t) {
+        uint2* at = reinterpret_cast<uint2*>(codes + t * D);
+        *at = scaled_down<FMT>(*at, old / s);
+      }
   }
-  const float inv = 1.0f / s;
-  for (int i = threadIdx.x + lo * c.dim; i < hi * c.dim; i += 256) {
-    const int r = i / c.dim;
-    const float v = to_f32(x[r * p.token[which] + i - r * c.dim]) * inv;
-    codes[i] = to_code<FMT>(inv == inv ? v : 0.0f);
-  }
-  __syncthreads();  // every thread has read the old scale
-  if (threadIdx.x == 0) *scale = s;
+  *reinterpret_cast<uint2*>(codes + slot * D) = x.template codes<FMT>(1.0f / s);
+  // (the group's lanes have all read the old scale: they run in one wave, and the
+  // exchanges above need its value from no one)
+  if (e == 0 && !(slot > 0 && s == old)) *scale = s;
 }
 
 }  // namespace
@@ -292,8 +411,7 @@ extern "C" int ttlh_rope(const void* x, void* out, int dtype, const void* positi
     a.tpb >>= 1;
   a.by_units = static_cast<uint32_t>(((uint64_t(1) << 32) + a.units - 1) / a.units);
   a.by_heads = static_cast<uint32_t>(((uint64_t(1) << 32) + a.hpb - 1) / a.hpb);
-  TTLH_REQUIRE(static_cast<int64_t>(a.tpb) * a.hpb * a.units < 131072, TTLH_EUNSUPPORTED,
-               "ttlh_rope: too many elements in a head");
+  TTLH_REQUIRE((heads + a.hpb - 1) / a.hpb < 65536, TTLH_EUNSUPPORTED, "ttlh_rope: too many heads");
   const dim3 grid(static_cast<uint32_t>((tokens + a.tpb - 1) / a.tpb),
                   static_cast<uint32_t>((heads + a.hpb - 1) / a.hpb));
   hipStream_t s = static_cast<hipStream_t>(stream);
@@ -369,15 +487,44 @@ extern "C" int ttlh_kv_cache_write(const ttlh_kv_cache* cache, const void* k, co
   a.token[1] = v_token;
   a.head[0] = k_head;
   a.head[1] = v_head;
-  // n tokens reach at most (n - 2) / page + 2 pages
-  const int64_t items = cache->starts ? cache->tokens / cache->page + 2 * cache->seqs : cache->seqs;
-  const dim3 grid(static_cast<uint32_t>(items), static_cast<uint32_t>(cache->heads), 2);
+  const int wide = dtype == TTLH_BF16 ? 8 : 4;
+  a.vec = (k_token | k_head | v_token | v_head) % wide == 0 &&
+          ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15) == 0;
   hipStream_t s = static_cast<hipStream_t>(stream);
-  const auto run = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(256), 0, s, a); };
+  const auto pick = [&](auto value, auto fmt, auto dim) {
+    typedef decltype(value) T;
+    constexpr int F = decltype(fmt)::value, D = decltype(dim)::value;
+    if (!cache->starts) {
+      const dim3 grid(static_cast<uint32_t>(cache->seqs),
+                      static_cast<uint32_t>((2 * cache->heads * (D / 8) + 255) / 256));
+      hipLaunchKernelGGL((kv_write_one_kernel<T, F, D>), grid, dim3(256), 0, s, a);
+      return;
+    }
+    // n tokens reach at most (n - 2) / page + 2 pages
+    const dim3 grid(static_cast<uint32_t>(cache->tokens / cache->page + 2 * cache->seqs),
+                    static_cast<uint32_t>(cache->heads));
+    const auto run = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(256), 0, s, a); };
+    const int sweeps = cache->page * D / 2048;
+    if (sweeps <= 1)
+      run(kv_write_kernel<T, F, D, 1>);
+    else if (sweeps == 2)
+      run(kv_write_kernel<T, F, D, 2>);
+    else if (sweeps == 4)
+      run(kv_write_kernel<T, F, D, 4>);
+    else if constexpr (D == 128)
+      run(kv_write_kernel<T, F, D, 8>);
+  };
+  const std::integral_constant<int, TTLH_CACHE_INT8> i8;
+  const std::integral_constant<int, TTLH_CACHE_E4M3> f8;
+  const std::integral_constant<int, 64> d64;
+  const std::integral_constant<int, 128> d128;
+  const auto dims = [&](auto value, auto fmt) {
+    cache->dim == 128 ? pick(value, fmt, d128) : pick(value, fmt, d64);
+  };
   const bool int8 = cache->format == TTLH_CACHE_INT8;
   if (dtype == TTLH_BF16)
-    int8 ? run(kv_write_kernel<uint16_t, TTLH_CACHE_INT8>) : run(kv_write_kernel<uint16_t, TTLH_CACHE_E4M3>);
+    int8 ? dims(uint16_t(), i8) : dims(uint16_t(), f8);
   else
-    int8 ? run(kv_write_kernel<float, TTLH_CACHE_INT8>) : run(kv_write_kernel<float, TTLH_CACHE_E4M3>);
+    int8 ? dims(float(), i8) : dims(float(), f8);
   return check_launch("kv_write_kernel");
 }

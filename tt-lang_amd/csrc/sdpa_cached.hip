@@ -82,30 +82,29 @@ template <int BM>
 struct Division {
   const CachedArgs& p;
   int chunk;
+  int tiles, range;  // of sequence threadIdx.x % 64, where there are no more than 64
 
   // tiles of sequence b, and the positions that its rows see between them
-  __device__ __forceinline__ void extent(int b, int& tiles, int& range) const {
+  __device__ __forceinline__ void extent(int b) {
+    tiles = range = 0;
+    if (b >= p.c.seqs) return;
     int first, n, lo, hi, x;
     seq_tokens(p.c, b, first, n);
+    if (n == 0) return;
+    const int len = p.c.lengths[b];
     tiles = (n * p.group + BM - 1) / BM;
-    range = 0;
-    if (n > 0) {
-      seen_by(p.c, p.c.lengths[b], n, 0, p.window, lo, x);
-      seen_by(p.c, p.c.lengths[b], n, n - 1, p.window, x, hi);
-      range = hi > lo ? hi - lo : 0;
-    }
-  }
-  __device__ __forceinline__ int parts_of(int range) const {
-    return range > chunk ? (range - 1) / chunk + 1 : 1;
+    seen_by(p.c, len, n, 0, p.window, lo, x);
+    seen_by(p.c, len, n, n - 1, p.window, x, hi);
+    range = hi > lo ? hi - lo : 0;
   }
   __device__ __forceinline__ void divide() {
+    const int lane = threadIdx.x & 63;
+    extent(lane);
     chunk = 0x7fffffff;
     if (p.target == 0) return;
-    const int lane = threadIdx.x & 63;
-    int64_t sum = 0;
-    for (int b = lane; b < p.c.seqs; b += 64) {
-      int tiles, range;
-      extent(b, tiles, range);
+    int64_t sum = static_cast<int64_t>(tiles) * range;
+    for (int b = lane + 64; b < p.c.seqs; b += 64) {
+      extent(b);
       sum += static_cast<int64_t>(tiles) * range;
     }
     sum = wave_total(sum);
@@ -115,13 +114,12 @@ struct Division {
   }
   // item `item` of the parts (JOIN: of the tiles), or false past the last one
   template <bool JOIN>
-  __device__ __forceinline__ bool find(int64_t item, Plan& w) const {
+  __device__ __forceinline__ bool find(int64_t item, Plan& w) {
     const int lane = threadIdx.x & 63;
     int64_t items = 0, slots = 0;
     for (int b0 = 0; b0 < p.c.seqs; b0 += 64) {
-      int tiles = 0, range = 0;
-      if (b0 + lane < p.c.seqs) extent(b0 + lane, tiles, range);
-      const int parts = parts_of(range);
+      if (p.c.seqs > 64) extent(b0 + lane);
+      const int parts = range > chunk ? (range - 1) / chunk + 1 : 1;
       const int64_t mine = JOIN ? tiles : static_cast<int64_t>(tiles) * parts;
       const int64_t mine_slots = parts > 1 ? static_cast<int64_t>(tiles) * parts : 0;
       int64_t end = mine, send = mine_slots;
@@ -151,8 +149,9 @@ struct Division {
         w.len = p.c.lengths[w.b];
         w.row0 = tile * BM;
         w.rows = w.n * p.group;
-        // (never more slots than there are, unless lengths change under the call)
-        return w.parts == 1 || w.slot + w.parts <= 2 * p.target;
+        // (never more slots than there are, nor a tile without rows, unless lengths
+        // or starts change under the call)
+        return (w.parts == 1 || w.slot + w.parts <= 2 * p.target) && w.row0 < w.rows;
       }
       items += __shfl(end, 63);
       slots += __shfl(send, 63);
@@ -257,11 +256,8 @@ struct Subtiles {
   }
 };
 
-// x (in units of log2) of a raw score: capped where there is a cap, as
-// C tanh(t) = C - 2 C / (1 + e^2t) with e^2t = 2^(raw kscale)
-__device__ __forceinline__ float score(float raw, float kscale, float cap) {
-  const float x = raw * kscale;
-  if (cap == 0.0f) return x;
+// C tanh(t) = C - 2 C / (1 + e^2t), from x = 2 t log2 e
+__device__ __forceinline__ float capped(float x, float cap) {
   return __builtin_fmaf(-2.0f * cap, __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x)), cap);
 }
 
@@ -315,30 +311,42 @@ struct Rows {
   const Plan& w;
   const Span& s;
   int h, n, g;
-  bf16x8 q[MT][NC];
+  // Q^T operands: with three row tiles in LDS, an operand's 64 lanes side by side
+  // (in registers, 44 of them would spill)
+  static constexpr bool kQinLds = MT > 2 && D == 128;
+  bf16x8 q[kQinLds ? 1 : MT][kQinLds ? 1 : NC];
+  const bf16x8* q_lds;
   f32x4 o[MT][NT];
   float m[MT], l[MT];
-  int from[MT], end[MT];  // what the lane's rows see
+  uint32_t k_off, v_off;  // the lane's bytes in a subtile
   Subtiles sub;
 
-  __device__ __forceinline__ void load(Codes& x, int k) const {
+  // step k's subtile t: its first byte in the cache (of page 0 where it has none)
+  __device__ __forceinline__ int64_t subtile_at(int k, int t) const {
+    const int page = max(__builtin_amdgcn_readlane(sub.page, (2 * k + t) & 63), 0);
+    const int slot = (s.begin + (k * kRowWaves + wave()) * kStep + 16 * t) & ((1 << p.c.shift) - 1);
+    return slot_offset(p.c, page, h, slot);
+  }
+  __device__ __forceinline__ void load_k(Codes& x, int k) const {
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      const int page = max(__builtin_amdgcn_readlane(sub.page, (2 * k + t) & 63), 0);
-      const int slot = (s.begin + (k * kRowWaves + wave()) * kStep + 16 * t) & ((1 << p.c.shift) - 1);
-      const int64_t at = slot_offset(p.c, page, h, slot);
-      const uint8_t* kp = p.c.k + at + n * D + 16 * g;
+      const uint8_t* kp = p.c.k + subtile_at(k, t);
 #pragma unroll
-      for (int i = 0; i < NK; ++i) x.k[t][i] = *reinterpret_cast<const u32x4*>(kp + 64 * i);
-      const uint8_t* vp = p.c.v + at + 4 * g * D + n * (D / 16);
+      for (int i = 0; i < NK; ++i) x.k[t][i] = *reinterpret_cast<const u32x4*>(kp + 64 * i + k_off);
+    }
+  }
+  __device__ __forceinline__ void load_v(Codes& x, int k) const {
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const uint8_t* vp = p.c.v + subtile_at(k, t);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         if constexpr (NV == 2) {
-          const u32x2 v = *reinterpret_cast<const u32x2*>(vp + i * D);
+          const u32x2 v = *reinterpret_cast<const u32x2*>(vp + i * D + v_off);
           x.v[t][i][0] = v[0];
           x.v[t][i][1] = v[1];
         } else {
-          x.v[t][i][0] = *reinterpret_cast<const uint32_t*>(vp + i * D);
+          x.v[t][i][0] = *reinterpret_cast<const uint32_t*>(vp + i * D + v_off);
         }
       }
     }
@@ -347,7 +355,8 @@ struct Rows {
     return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   }
 
-  __device__ __forceinline__ void step(Codes& x, int k) {
+  // step k; the codes of step k + 2, if `more`, follow it into the same registers
+  __device__ __forceinline__ void step(Codes& x, int k, bool more) {
     const int pos = s.begin + (k * kRowWaves + wave()) * kStep;
     float ks[2], vs[2];
     bool there[2];
@@ -361,20 +370,28 @@ struct Rows {
     const bool mask = !there[0] || !there[1] || pos < s.all_lo || pos + kStep > s.all_hi;
     f32x4 sc[MT][2];
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
+    for (int r = 0; r < MT; ++r)
 #pragma unroll
-      for (int r = 0; r < MT; ++r) sc[r][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      for (int t = 0; t < 2; ++t) sc[r][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-      for (int c = 0; c < NC; ++c) {
+    for (int c = 0; c < NC; ++c) {
+      bf16x8 kf[2];
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
         const u32x4 raw = x.k[t][c >> 1];
-        const bf16x8 kf = __builtin_bit_cast(
+        kf[t] = __builtin_bit_cast(
             bf16x8, (c & 1) ? eight_of<FMT>(raw[2], raw[3]) : eight_of<FMT>(raw[0], raw[1]));
-#pragma unroll
-        for (int r = 0; r < MT; ++r)
-          sc[r][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, q[r][c], sc[r][t], 0, 0, 0);
-        __builtin_amdgcn_sched_barrier(0);
       }
+#pragma unroll
+      for (int r = 0; r < MT; ++r) {
+        const bf16x8 qf = kQinLds ? q_lds[(r * NC + c) * 64] : q[kQinLds ? 0 : r][kQinLds ? 0 : c];
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+          sc[r][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[t], qf, sc[r][t], 0, 0, 0);
+      }
+      __builtin_amdgcn_sched_barrier(0);
     }
+    if (more) load_k(x, k + 2);
     if (mask) {
       // codes that no row sees may be anything: 0 times them has to be 0
 #pragma unroll
@@ -395,14 +412,20 @@ struct Rows {
 #pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) e[4 * t + i] = score(sc[r][t][i], ks[t], p.cap_log2);
+        for (int i = 0; i < 4; ++i) e[4 * t + i] = sc[r][t][i] * ks[t];
+      if (p.cap_log2 != 0.0f) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) e[i] = capped(e[i], p.cap_log2);
+      }
       if (mask) {
+        int from, end;
+        seen_by(p.c, w.len, w.n, min(w.row0 + 16 * r + n, w.rows - 1) / p.group, p.window, from, end);
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const int j = pos + 16 * t + 4 * g + i;
-            if (!there[t] || j < from[r] || j >= end[r]) e[4 * t + i] = -INFINITY;
+            if (!there[t] || j < from || j >= end) e[4 * t + i] = -INFINITY;
           }
       }
 #pragma unroll
@@ -432,6 +455,7 @@ struct Rows {
       pf[r] = __builtin_bit_cast(bf16x8, pk);
     }
     products(x, pf);
+    if (more) load_v(x, k + 2);
   }
 
   template <int J>
@@ -469,10 +493,14 @@ __global__ __launch_bounds__(kRowWaves * 64, 2) void cached_rows_kernel(
   Plan w;
   if (!div.template find<false>(blockIdx.x / p.c.heads, w)) return;
   const Span s = span_of<BM, kStep>(p, w);
-  Rows<D, FMT, MT> x{p, w, s, h};
+  typedef Rows<D, FMT, MT> R;
+  R x{p, w, s, h};
+  __shared__ bf16x8 q_lds[R::kQinLds ? MT * (D / 32) * 64 : 1];
   const int lane = threadIdx.x & 63, wave = x.wave();
   x.n = lane & 15;
   x.g = lane >> 4;
+  x.k_off = x.n * D + 16 * x.g;
+  x.v_off = 4 * x.g * D + x.n * (D / 16);
   // steps of this wave: k * 8 + wave of the part's
   const int total = s.end > s.begin ? (s.end - s.begin + kStep - 1) / kStep : 0;
   const int steps = total > wave ? (total - wave - 1) / kRowWaves + 1 : 0;
@@ -488,26 +516,36 @@ __global__ __launch_bounds__(kRowWaves * 64, 2) void cached_rows_kernel(
     const uint16_t* qp = p.q + static_cast<int64_t>(w.first + i) * p.q_token +
                          static_cast<int64_t>(h * p.group + row - i * p.group) * p.q_head;
 #pragma unroll
-    for (int c = 0; c < D / 32; ++c)
-      x.q[r][c] = *reinterpret_cast<const bf16x8*>(qp + 64 * (c >> 1) + 16 * x.g + 8 * (c & 1));
-    seen_by(p.c, w.len, w.n, i, p.window, x.from[r], x.end[r]);
+    for (int c = 0; c < D / 32; ++c) {
+      const bf16x8 qf = *reinterpret_cast<const bf16x8*>(qp + 64 * (c >> 1) + 16 * x.g + 8 * (c & 1));
+      if constexpr (R::kQinLds) {
+        if (wave == (r * (D / 32) + c) % kRowWaves) q_lds[(r * (D / 32) + c) * 64 + lane] = qf;
+      } else {
+        x.q[r][c] = qf;
+      }
+    }
     x.m[r] = -INFINITY;
     x.l[r] = 0.0f;
 #pragma unroll
     for (int j = 0; j < D / 16; ++j) x.o[r][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   }
-  typename Rows<D, FMT, MT>::Codes a, b;
-  if (steps > 0) x.load(a, 0);
+  if constexpr (R::kQinLds) {
+    x.q_lds = q_lds + lane;
+    __syncthreads();
+  }
+  typename R::Codes a, b;
   for (int k0 = 0; k0 < steps; k0 += 32) {
-    if (k0 > 0) {
-      refill(k0);
-      x.load(a, k0);
-    }
+    if (k0 > 0) refill(k0);
     const int kn = min(steps, k0 + 32);
-    for (int k = k0; k < kn; ++k) {
-      if (k + 1 < kn) x.load(b, k + 1);
-      x.step(a, k);
-      a = b;
+    x.load_k(a, k0);
+    x.load_v(a, k0);
+    if (k0 + 1 < kn) {
+      x.load_k(b, k0 + 1);
+      x.load_v(b, k0 + 1);
+    }
+    for (int k = k0; k < kn; k += 2) {
+      x.step(a, k, k + 2 < kn);
+      if (k + 1 < kn) x.step(b, k + 1, k + 3 < kn);
     }
   }
 
@@ -715,7 +753,13 @@ struct Tiles {
 #pragma unroll
     for (int t = 0; t < 2; ++t)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) cur[t][r] = score(cur[t][r], ks[2 * t + (r >> 3)], p.cap_log2);
+      for (int r = 0; r < 16; ++r) cur[t][r] *= ks[2 * t + (r >> 3)];
+    if (p.cap_log2 != 0.0f) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) cur[t][r] = capped(cur[t][r], p.cap_log2);
+    }
     if (!all || pos < s.all_lo || pos + kBlock > s.all_hi) {
 #pragma unroll
       for (int t = 0; t < 2; ++t)
@@ -850,36 +894,77 @@ __global__ __launch_bounds__(kTileThreads, 2) void cached_tiles_kernel(const Cac
                 cvt_pk_bf16x2(x.o[j][4 * u + 2] * inv, x.o[j][4 * u + 3] * inv)};
 }
 
-// The parts of a tile, in their order; a thread has four elements of a row.
+// The parts of a tile: the rows of a workgroup (blockIdx.y counts them) by four
+// waves, wave v taking parts v, v + 4, .., and the waves' results in their order:
+// the same sum whenever the parts are the same.  A lane has four elements of a row.
 template <int D, int BM>
 __global__ __launch_bounds__(256) void cached_join_kernel(const CachedArgs p) {
+  constexpr int kRows = 256 / D;  // 64 lanes, D / 4 a row
+  __shared__ f32x4 acc_s[4][64];
+  __shared__ float m_s[4][64], l_s[4][64];
   Division<BM> div{p};
   div.divide();
   Plan w;
   if (!div.template find<true>(blockIdx.x / p.c.heads, w) || w.parts == 1) return;
-  const int h = blockIdx.x % p.c.heads;
-  const int n = min(BM, w.rows - w.row0);
-  for (int e = threadIdx.x; e < n * (D / 4); e += 256) {
-    const int row = e / (D / 4), d = (e % (D / 4)) * 4;
-    const int64_t step = static_cast<int64_t>(p.c.heads) * BM;
-    const int64_t at = (static_cast<int64_t>(w.slot) * p.c.heads + h) * BM + row;
-    float mt = -INFINITY;
-    for (int i = 0; i < w.parts; ++i) mt = fmaxf(mt, p.part_ml[(at + i * step) * 2]);
-    const float mm = mt == -INFINITY ? 0.0f : mt;
-    float lt = 0.0f;
-    f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int i = 0; i < w.parts; ++i) {
-      const float f = __builtin_amdgcn_exp2f(p.part_ml[(at + i * step) * 2] - mm);
-      lt += p.part_ml[(at + i * step) * 2 + 1] * f;
-      acc += *reinterpret_cast<const f32x4*>(p.part_o + (at + i * step) * D + d) * f;
+  const int h = blockIdx.x % p.c.heads, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int row = blockIdx.y * kRows + lane / (D / 4), d = (lane % (D / 4)) * 4;
+  if (w.row0 + static_cast<int>(blockIdx.y) * kRows >= w.rows) return;  // (uniform)
+  const bool mine = w.row0 + row < w.rows;
+  const int64_t step = static_cast<int64_t>(p.c.heads) * BM;
+  const int64_t at = (static_cast<int64_t>(w.slot) * p.c.heads + h) * BM + (mine ? row : 0);
+  float m = -INFINITY, l = 0.0f;
+  f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+  constexpr int kAhead = 4;
+  for (int i0 = wave; i0 < w.parts; i0 += 4 * kAhead) {
+    float pm[kAhead], pl[kAhead];
+    f32x4 po[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const bool there = i0 + 4 * i < w.parts;
+      const int64_t r = at + (there ? i0 + 4 * i : i0) * step;
+      pm[i] = there ? p.part_ml[r * 2] : -INFINITY;
+      pl[i] = p.part_ml[r * 2 + 1];
+      po[i] = *reinterpret_cast<const f32x4*>(p.part_o + r * D + d);
     }
-    const int i = (w.row0 + row) / p.group;
-    const float inv = lt == 0.0f ? 0.0f : 1.0f / lt;
-    uint16_t* op = p.o + static_cast<int64_t>(w.first + i) * p.o_token +
-                   static_cast<int64_t>(h * p.group + w.row0 + row - i * p.group) * p.o_head + d;
-    *reinterpret_cast<u32x2*>(op) = u32x2{cvt_pk_bf16x2(acc[0] * inv, acc[1] * inv),
-                                          cvt_pk_bf16x2(acc[2] * inv, acc[3] * inv)};
+    float to = m;
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) to = fmaxf(to, pm[i]);
+    const float mm = to == -INFINITY ? 0.0f : to, f = __builtin_amdgcn_exp2f(m - mm);
+    l *= f;
+    acc *= f;
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const float e = __builtin_amdgcn_exp2f(pm[i] - mm);
+      if (i0 + 4 * i < w.parts) {
+        l += pl[i] * e;
+        acc += po[i] * e;
+      }
+    }
+    m = to;
   }
+  m_s[wave][lane] = m;
+  l_s[wave][lane] = l;
+  acc_s[wave][lane] = acc;
+  __syncthreads();
+  if (wave != 0 || !mine) return;
+  float mt = -INFINITY;
+#pragma unroll
+  for (int v = 0; v < 4; ++v) mt = fmaxf(mt, m_s[v][lane]);
+  const float mm = mt == -INFINITY ? 0.0f : mt;
+  float lt = 0.0f;
+  acc = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+  for (int v = 0; v < 4; ++v) {
+    const float f = __builtin_amdgcn_exp2f(m_s[v][lane] - mm);
+    lt += l_s[v][lane] * f;
+    acc += acc_s[v][lane] * f;
+  }
+  const int i = (w.row0 + row) / p.group;
+  const float inv = lt == 0.0f ? 0.0f : 1.0f / lt;
+  uint16_t* op = p.o + static_cast<int64_t>(w.first + i) * p.o_token +
+                 static_cast<int64_t>(h * p.group + w.row0 + row - i * p.group) * p.o_head + d;
+  *reinterpret_cast<u32x2*>(op) = u32x2{cvt_pk_bf16x2(acc[0] * inv, acc[1] * inv),
+                                        cvt_pk_bf16x2(acc[2] * inv, acc[3] * inv)};
 }
 
 // ---- the choice --------------------------------------------------------------
@@ -971,7 +1056,11 @@ extern "C" int ttlh_sdpa_cached(const ttlh_kv_cache* cache, const void* Q, void*
   const int64_t items = (x.tiles + x.target) * cache->heads;
   TTLH_REQUIRE(items < (int64_t(1) << 31), TTLH_EUNSUPPORTED, "ttlh_sdpa_cached: too many tiles");
   const dim3 grid(static_cast<uint32_t>(items));
-  const dim3 joins(static_cast<uint32_t>(x.tiles * cache->heads));
+  // (rows of a tile: without starts no more than the group)
+  const int64_t rows = !cache->starts && a.group < x.bm ? a.group : x.bm;
+  const int per = 256 / cache->dim;
+  const dim3 joins(static_cast<uint32_t>(x.tiles * cache->heads),
+                   static_cast<uint32_t>((rows + per - 1) / per));
   hipStream_t s = static_cast<hipStream_t>(stream);
   const auto run = [&](auto kernel, int threads, auto join) {
     hipLaunchKernelGGL(kernel, grid, dim3(threads), 0, s, a);

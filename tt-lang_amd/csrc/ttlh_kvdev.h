@@ -22,13 +22,16 @@ __device__ __forceinline__ uint16_t from_f32<uint16_t>(float x) {
   return static_cast<uint16_t>(cvt_pk_bf16x2(x, x));
 }
 
-// one code <-> its value; values are at most the largest code
+// values, at most the largest code in magnitude, rounded to four codes
 template <int FMT>
-__device__ __forceinline__ uint8_t to_code(float x) {
-  if constexpr (FMT == TTLH_CACHE_INT8)
-    return static_cast<uint8_t>(static_cast<int>(rintf(x)));
-  else
-    return static_cast<uint8_t>(__builtin_amdgcn_cvt_pk_fp8_f32(x, x, 0, false));
+__device__ __forceinline__ uint32_t four_codes(float a, float b, float c, float d) {
+  if constexpr (FMT == TTLH_CACHE_INT8) {
+    const int i = static_cast<int>(rintf(a)), j = static_cast<int>(rintf(b));
+    const int k = static_cast<int>(rintf(c)), l = static_cast<int>(rintf(d));
+    return (i & 255) | (j & 255) << 8 | (k & 255) << 16 | static_cast<uint32_t>(l) << 24;
+  } else {
+    return __builtin_amdgcn_cvt_pk_fp8_f32(c, d, __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false), true);
+  }
 }
 template <int FMT>
 __device__ __forceinline__ float from_code(uint8_t c) {
