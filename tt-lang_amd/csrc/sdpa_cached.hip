@@ -12,7 +12,7 @@
 // (the order of the positions inside a product is free).
 //
 //  * cached_rows_kernel: up to 16 MT rows in a tile (answers token by token, drafts):
-//    HBM bound.  Eight waves take turns at 32 positions and meet in LDS at the end;
+//    HBM bound.  Four waves take turns at 32 positions and meet in LDS at the end;
 //    codes go from memory to registers, no LDS on the way.
 //  * cached_tiles_kernel: tiles of 128 rows (prompts): MFMA bound.  Blocks of 64
 //    positions are decoded once into LDS for four waves of 32 rows.
@@ -72,12 +72,6 @@ struct Plan {
   int part, parts, slot;     // this part; the slot of the tile's part 0
 };
 
-__device__ __forceinline__ int64_t wave_total(int64_t x) {
-#pragma unroll
-  for (int i = 32; i; i >>= 1) x += __shfl_xor(x, i);
-  return x;
-}
-
 template <int BM>
 struct Division {
   const CachedArgs& p;
@@ -102,59 +96,48 @@ struct Division {
     extent(lane);
     chunk = 0x7fffffff;
     if (p.target == 0) return;
-    int64_t sum = static_cast<int64_t>(tiles) * range;
+    // (in fp32: off by less than one part in 2 target, and the same in every wave)
+    float sum = static_cast<float>(tiles) * range;
     for (int b = lane + 64; b < p.c.seqs; b += 64) {
       extent(b);
-      sum += static_cast<int64_t>(tiles) * range;
+      sum += static_cast<float>(tiles) * range;
     }
-    sum = wave_total(sum);
-    const int64_t each = (((sum + p.target - 1) / p.target) + 63) & ~int64_t(63);
-    chunk = static_cast<int>(each < p.least ? p.least : each > 0x7fffffc0 ? 0x7fffffc0 : each);
+    const float each = fminf(wave_total(sum) / p.target, 1073741824.0f);
+    chunk = max((static_cast<int>(each) + 64) & ~63, p.least);
     chunk = __builtin_amdgcn_readfirstlane(chunk);
+    if (p.c.seqs > 64) tiles = range = 0;
   }
   // item `item` of the parts (JOIN: of the tiles), or false past the last one
   template <bool JOIN>
-  __device__ __forceinline__ bool find(int64_t item, Plan& w) {
+  __device__ __forceinline__ bool find(int item, Plan& w) {
     const int lane = threadIdx.x & 63;
-    int64_t items = 0, slots = 0;
+    int items = 0, slots = 0;
     for (int b0 = 0; b0 < p.c.seqs; b0 += 64) {
       if (p.c.seqs > 64) extent(b0 + lane);
       const int parts = range > chunk ? (range - 1) / chunk + 1 : 1;
-      const int64_t mine = JOIN ? tiles : static_cast<int64_t>(tiles) * parts;
-      const int64_t mine_slots = parts > 1 ? static_cast<int64_t>(tiles) * parts : 0;
-      int64_t end = mine, send = mine_slots;
-#pragma unroll
-      for (int i = 1; i < 64; i <<= 1) {
-        const int64_t o = __shfl_up(end, i), so = __shfl_up(send, i);
-        if (lane >= i) {
-          end += o;
-          send += so;
-        }
-      }
+      const int mine = JOIN ? tiles : tiles * parts, mine_slots = parts > 1 ? tiles * parts : 0;
+      const int end = prefix_sum(mine), send = prefix_sum(mine_slots);
       const unsigned long long past = __ballot(items + end > item);
       if (past) {
         const int l = __builtin_amdgcn_readfirstlane(__ffsll(past) - 1);
-        const int local = __builtin_amdgcn_readfirstlane(
-            static_cast<int>(item - items - (__shfl(end, l) - __shfl(mine, l))));
+        const auto at = [&](int x) { return __builtin_amdgcn_readlane(x, l); };
+        const int local = item - items - (at(end) - at(mine)), nt = at(tiles);
         w.b = b0 + l;
-        w.parts = __builtin_amdgcn_readlane(parts, l);
-        const int nt = __builtin_amdgcn_readlane(tiles, l);
+        w.parts = at(parts);
         // (the last tile of a prompt sees the most: it goes first)
-        const int tile = JOIN ? nt - 1 - local : nt - 1 - local / w.parts;
-        w.part = JOIN ? 0 : local % w.parts;
-        w.slot = __builtin_amdgcn_readfirstlane(static_cast<int>(
-                     slots + __shfl(send, l) - __shfl(mine_slots, l))) +
-                 (nt - 1 - tile) * w.parts;
+        const int before = JOIN ? local : local / w.parts, tile = nt - 1 - before;
+        w.part = JOIN ? 0 : local - before * w.parts;
+        w.slot = slots + at(send) - at(mine_slots) + before * w.parts;
         seq_tokens(p.c, w.b, w.first, w.n);
         w.len = p.c.lengths[w.b];
         w.row0 = tile * BM;
         w.rows = w.n * p.group;
-        // (never more slots than there are, nor a tile without rows, unless lengths
-        // or starts change under the call)
-        return (w.parts == 1 || w.slot + w.parts <= 2 * p.target) && w.row0 < w.rows;
+        // (always, unless starts overlap, or they or lengths change under the call)
+        return (w.parts == 1 || (w.slot >= 0 && w.slot + w.parts <= 2 * p.target)) &&
+               w.row0 >= 0 && w.row0 < w.rows;
       }
-      items += __shfl(end, 63);
-      slots += __shfl(send, 63);
+      items += __builtin_amdgcn_readlane(end, 63);
+      slots += __builtin_amdgcn_readlane(send, 63);
     }
     return false;
   }
@@ -241,18 +224,17 @@ struct Subtiles {
   int page;
   float kscale, vscale;
 
+  // (the scales are only asked for: finish() waits for them)
   __device__ __forceinline__ void load(const CachedArgs& p, int b, int h, int pos) {
     page = page_at(p.c, b, pos);
-    kscale = vscale = 0.0f;
-    if (page >= 0) {
-      const int64_t at = static_cast<int64_t>(page) * p.c.heads + h;
-      kscale = p.c.k_scale[at] * p.scale_log2;
-      vscale = p.c.v_scale[at];
-      if (!(fabsf(vscale) < INFINITY) || !(fabsf(p.c.k_scale[at]) < INFINITY)) {
-        kscale = __int_as_float(0x7fc00000);
-        vscale = 0.0f;
-      }
-    }
+    const int64_t at = static_cast<int64_t>(max(page, 0)) * p.c.heads + h;
+    kscale = p.c.k_scale[at];
+    vscale = p.c.v_scale[at];
+  }
+  __device__ __forceinline__ void finish(float scale) {
+    const bool fine = fabsf(kscale) < INFINITY && fabsf(vscale) < INFINITY;
+    kscale = fine ? kscale * scale : __int_as_float(0x7fc00000);
+    vscale = fine ? vscale : 0.0f;
   }
 };
 
@@ -292,7 +274,7 @@ __device__ __forceinline__ float xor16_add(float x) {
 // the P^T operand as they stand, and lane (n, g) reads D / 16 bytes at n D / 16 of
 // its 8 positions, byte j of which is the operand of tile j: O^T's row m of tile j
 // is element m D / 16 + j.
-constexpr int kRowWaves = 8;
+constexpr int kRowWaves = 4;
 constexpr int kStep = 32;
 
 template <int D, int FMT, int MT>
@@ -480,12 +462,14 @@ struct Rows {
 };
 
 template <int D, int FMT, int MT>
-__global__ __launch_bounds__(kRowWaves * 64, 2) void cached_rows_kernel(
+__global__ __launch_bounds__(kRowWaves * 64, MT == 1 ? 3 : 2) void cached_rows_kernel(
     const CachedArgs p) {
   constexpr int BM = 16 * MT;
   constexpr int LD = D + 4;  // LDS row: 16 rows' 16-byte writes spread over the banks
+  typedef Rows<D, FMT, MT> R;
+  __shared__ bf16x8 q_lds[R::kQinLds ? MT * (D / 32) * 64 : 1];
   __shared__ float part[kRowWaves][16][LD];
-  __shared__ float ml[kRowWaves][16][2];
+  __shared__ float ml[kRowWaves][BM][2];
 
   Division<BM> div{p};
   div.divide();
@@ -493,22 +477,29 @@ __global__ __launch_bounds__(kRowWaves * 64, 2) void cached_rows_kernel(
   Plan w;
   if (!div.template find<false>(blockIdx.x / p.c.heads, w)) return;
   const Span s = span_of<BM, kStep>(p, w);
-  typedef Rows<D, FMT, MT> R;
   R x{p, w, s, h};
-  __shared__ bf16x8 q_lds[R::kQinLds ? MT * (D / 32) * 64 : 1];
   const int lane = threadIdx.x & 63, wave = x.wave();
   x.n = lane & 15;
   x.g = lane >> 4;
   x.k_off = x.n * D + 16 * x.g;
   x.v_off = 4 * x.g * D + x.n * (D / 16);
-  // steps of this wave: k * 8 + wave of the part's
+  // steps of this wave: k * 4 + wave of the part's
   const int total = s.end > s.begin ? (s.end - s.begin + kStep - 1) / kStep : 0;
   const int steps = total > wave ? (total - wave - 1) / kRowWaves + 1 : 0;
+  typename R::Codes a, b;
+  int kn;
   const auto refill = [&](int k) {  // steps k .. k + 31, two subtiles each
     const int pos = s.begin + ((k + (lane >> 1)) * kRowWaves + wave) * kStep + 16 * (lane & 1);
-    x.sub.load(p, w.b, h, pos >= 0 && pos < s.hi ? pos : -1);
+    x.sub.load(p, w.b, h, pos < s.hi ? pos : -1);
+    kn = min(steps, k + 32);
+    x.load_k(a, k);
+    x.load_v(a, k);
+    if (k + 1 < kn) {
+      x.load_k(b, k + 1);
+      x.load_v(b, k + 1);
+    }
+    x.sub.finish(p.scale_log2);
   };
-  if (steps > 0) refill(0);
 #pragma unroll
   for (int r = 0; r < MT; ++r) {
     const int row = min(w.row0 + 16 * r + x.n, w.rows - 1);
@@ -529,64 +520,64 @@ __global__ __launch_bounds__(kRowWaves * 64, 2) void cached_rows_kernel(
 #pragma unroll
     for (int j = 0; j < D / 16; ++j) x.o[r][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   }
+  if (steps > 0) refill(0);
   if constexpr (R::kQinLds) {
     x.q_lds = q_lds + lane;
     __syncthreads();
   }
-  typename R::Codes a, b;
   for (int k0 = 0; k0 < steps; k0 += 32) {
     if (k0 > 0) refill(k0);
-    const int kn = min(steps, k0 + 32);
-    x.load_k(a, k0);
-    x.load_v(a, k0);
-    if (k0 + 1 < kn) {
-      x.load_k(b, k0 + 1);
-      x.load_v(b, k0 + 1);
-    }
     for (int k = k0; k < kn; k += 2) {
       x.step(a, k, k + 2 < kn);
       if (k + 1 < kn) x.step(b, k + 1, k + 3 < kn);
     }
   }
 
-  // The waves meet: their maxima, sums and O in LDS, 16 rows at a time; a thread
-  // has four elements of a row.
+  // The waves meet: first their maxima, by which each scales its sums and O; then
+  // O in LDS, 16 rows at a time, a thread adding four elements of a row in the
+  // order of the waves.
+  const int rows = min(BM, w.rows - w.row0);
+#pragma unroll
+  for (int r = 0; r < MT; ++r) {
+    x.l[r] = xor32_add(xor16_add(x.l[r]));
+    if (x.g == 0) ml[wave][16 * r + x.n][0] = x.m[r];
+  }
+  __syncthreads();
   const int64_t slot = (static_cast<int64_t>(w.slot + w.part) * p.c.heads + h) * BM;
 #pragma unroll
   for (int r = 0; r < MT; ++r) {
-    if (w.row0 + 16 * r >= w.rows) break;  // (uniform)
-    const float l = xor32_add(xor16_add(x.l[r]));
-    if (r) __syncthreads();
-    if (x.g == 0) {
-      ml[wave][x.n][0] = x.m[r];
-      ml[wave][x.n][1] = l;
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int j = 0; j < D / 16; j += 4)
-        *reinterpret_cast<f32x4*>(&part[wave][x.n][(4 * x.g + i) * (D / 16) + j]) =
-            f32x4{x.o[r][j][i], x.o[r][j + 1][i], x.o[r][j + 2][i], x.o[r][j + 3][i]};
-    __syncthreads();
-    for (int e = threadIdx.x; e < 16 * (D / 4); e += kRowWaves * 64) {
-      const int row = e / (D / 4), d = (e % (D / 4)) * 4;
+    if (16 * r >= rows) break;  // (uniform)
+    if (16 * r + x.n < rows) {
       float mt = -INFINITY;
 #pragma unroll
-      for (int v = 0; v < kRowWaves; ++v) mt = fmaxf(mt, ml[v][row][0]);
-      const float mm = mt == -INFINITY ? 0.0f : mt;
+      for (int v = 0; v < kRowWaves; ++v) mt = fmaxf(mt, ml[v][16 * r + x.n][0]);
+      const float f = __builtin_amdgcn_exp2f(x.m[r] - (mt == -INFINITY ? 0.0f : mt));
+      if (x.g == 0) ml[wave][16 * r + x.n][1] = x.l[r] * f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < D / 16; j += 4)
+          *reinterpret_cast<f32x4*>(&part[wave][x.n][(4 * x.g + i) * (D / 16) + j]) =
+              f32x4{x.o[r][j][i] * f, x.o[r][j + 1][i] * f, x.o[r][j + 2][i] * f,
+                    x.o[r][j + 3][i] * f};
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < min(16, rows - 16 * r) * (D / 4); e += kRowWaves * 64) {
+      const int row = e / (D / 4), d = (e % (D / 4)) * 4;
       float lt = 0.0f;
       f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
       for (int v = 0; v < kRowWaves; ++v) {
-        const float f = __builtin_amdgcn_exp2f(ml[v][row][0] - mm);
-        lt += ml[v][row][1] * f;
-        acc += *reinterpret_cast<const f32x4*>(&part[v][row][d]) * f;
+        lt += ml[v][16 * r + row][1];
+        acc += *reinterpret_cast<const f32x4*>(&part[v][row][d]);
       }
       const int at = w.row0 + 16 * r + row;
-      if (at >= w.rows) continue;
       if (w.parts > 1) {
         *reinterpret_cast<f32x4*>(p.part_o + (slot + 16 * r + row) * D + d) = acc;
         if (d == 0) {
+          float mt = -INFINITY;
+#pragma unroll
+          for (int v = 0; v < kRowWaves; ++v) mt = fmaxf(mt, ml[v][16 * r + row][0]);
           p.part_ml[(slot + 16 * r + row) * 2] = mt;
           p.part_ml[(slot + 16 * r + row) * 2 + 1] = lt;
         }
@@ -599,6 +590,7 @@ __global__ __launch_bounds__(kRowWaves * 64, 2) void cached_rows_kernel(
                                               cvt_pk_bf16x2(acc[2] * inv, acc[3] * inv)};
       }
     }
+    if (16 * (r + 1) < rows) __syncthreads();
   }
 }
 
@@ -631,6 +623,7 @@ struct Tiles {
   f32x16 o[ND];
   float m, l;
   Subtiles sub;    // of blocks kb0 .. kb0 + 15
+  uint64_t paged, plain;  // subtiles with a page; with scales in the ordinary range
   u32x4 kraw[kLoads], vraw[kLoads];
   int k_frag, v_frag[ND];
 
@@ -658,7 +651,12 @@ struct Tiles {
   }
   __device__ __forceinline__ void refill(int kb) {  // kb a multiple of 16
     const int pos = s.begin + kb * kBlock + lane * 16;
-    sub.load(p, w.b, hd, pos >= 0 && pos < s.hi ? pos : -1);
+    sub.load(p, w.b, hd, pos < s.hi ? pos : -1);
+  }
+  __device__ __forceinline__ void finish() {
+    sub.finish(p.scale_log2);
+    paged = __ballot(sub.page >= 0);
+    plain = __ballot(sub.kscale > 0.0f && sub.vscale > 0x1p-60f && sub.vscale < 0x1p60f);
   }
   __device__ __forceinline__ void load(int kb) {
 #pragma unroll
@@ -667,7 +665,7 @@ struct Tiles {
       const int page = max(__builtin_amdgcn_readlane(sub.page, (kb & 15) * 4 + st), 0);
       const int slot = (s.begin + kb * kBlock + 16 * st) & ((1 << p.c.shift) - 1);
       const int64_t at = slot_offset(p.c, page, hd, slot);
-      const int off = (row - 16 * st) * D + (threadIdx.x % kChunks) * 16;
+      const uint32_t off = (row - 16 * st) * D + (threadIdx.x % kChunks) * 16;
       kraw[i] = *reinterpret_cast<const u32x4*>(p.c.k + at + off);
       vraw[i] = *reinterpret_cast<const u32x4*>(p.c.v + at + off);
     }
@@ -675,21 +673,24 @@ struct Tiles {
   // block kb's codes, decoded, into LDS; those that no row sees as zeros (V)
   __device__ __forceinline__ void stage(int kb, int buf) {
     const int pos = s.begin + kb * kBlock;
-    const bool edge = pos < s.lo || pos + kBlock > s.hi ||
-                      __any(lane >> 2 == (kb & 15) && sub.page < 0);
+    const int there = (paged >> ((kb & 15) * 4)) & 15;
+    const bool edge = pos < s.lo || pos + kBlock > s.hi || there != 15;
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
       const int row = load_row(i), c = threadIdx.x % kChunks;
       if (edge) {
-        const bool there = __builtin_amdgcn_readlane(sub.page, (kb & 15) * 4 + load_sub(i)) >= 0;
-        if (!there || pos + row < s.lo || pos + row >= s.hi) vraw[i] = u32x4{0u, 0u, 0u, 0u};
+        if (!((there >> load_sub(i)) & 1) || pos + row < s.lo || pos + row >= s.hi) vraw[i] = u32x4{0u, 0u, 0u, 0u};
       }
       uint16_t* kd = Ks[buf] + row * D;
       uint16_t* vd = Vs[buf] + row * D;
+      // (every second row's V goes odd chunk first: with both even, two rows' writes
+      // would meet in the same banks)
+      const int odd = D == 128 ? row & 1 : (row >> 1) & 1;
+      const u32x4 v = odd ? u32x4{vraw[i][2], vraw[i][3], vraw[i][0], vraw[i][1]} : vraw[i];
       *reinterpret_cast<u32x4*>(kd + ((2 * c ^ k_swz(row)) << 3)) = eight_of<FMT>(kraw[i][0], kraw[i][1]);
       *reinterpret_cast<u32x4*>(kd + (((2 * c + 1) ^ k_swz(row)) << 3)) = eight_of<FMT>(kraw[i][2], kraw[i][3]);
-      *reinterpret_cast<u32x4*>(vd + ((2 * c ^ v_swz(row)) << 3)) = eight_of<FMT>(vraw[i][0], vraw[i][1]);
-      *reinterpret_cast<u32x4*>(vd + (((2 * c + 1) ^ v_swz(row)) << 3)) = eight_of<FMT>(vraw[i][2], vraw[i][3]);
+      *reinterpret_cast<u32x4*>(vd + (((2 * c + odd) ^ v_swz(row)) << 3)) = eight_of<FMT>(v[0], v[1]);
+      *reinterpret_cast<u32x4*>(vd + (((2 * c + 1 - odd) ^ v_swz(row)) << 3)) = eight_of<FMT>(v[2], v[3]);
     }
   }
   __device__ __forceinline__ i16x4 read_v4(const uint16_t* Vb, int kv, int j) const {
@@ -738,41 +739,59 @@ struct Tiles {
     __builtin_amdgcn_sched_barrier(0);
 
     float ks[4], vs[4];
-    bool there[4];
-    bool all = true;
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
-      const int at = (kb & 15) * 4 + t;
-      ks[t] = uniform(sub.kscale, at);
-      vs[t] = uniform(sub.vscale, at);
-      there[t] = __builtin_amdgcn_readlane(sub.page, at) >= 0;
-      all = all && there[t];
+      ks[t] = uniform(sub.kscale, (kb & 15) * 4 + t);
+      vs[t] = uniform(sub.vscale, (kb & 15) * 4 + t);
     }
     // accumulator r of half t: position 32 t + 8 (r / 4) + 4 h + r % 4, subtile 2 t + r / 8
-    float mx = -INFINITY;
-#pragma unroll
-    for (int t = 0; t < 2; ++t)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) cur[t][r] *= ks[2 * t + (r >> 3)];
-    if (p.cap_log2 != 0.0f) {
+    const int there = (paged >> ((kb & 15) * 4)) & 15;
+    const bool mask = there != 15 || pos < s.all_lo || pos + kBlock > s.all_hi;
+    const bool quick = ((plain >> ((kb & 15) * 4)) & 15) == 15;
+    const float cap = p.cap_log2;
+    // With scales in the ordinary range (quick) K's go into the exponents'
+    // multiplications and V's into their additions, 3 instructions for a score in
+    // place of 5:  p vs = 2^(x f + b).  x: the raw score; where it is capped,
+    // u = 1 / (1 + e^2t) of C tanh t = C - 2 C u, the largest where u is least.
+    if (!quick || cap != 0.0f) {
+      asm volatile("");  // a branch: not 32 multiplications by one
 #pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) cur[t][r] = capped(cur[t][r], p.cap_log2);
+        for (int r = 0; r < 16; ++r) cur[t][r] *= ks[2 * t + (r >> 3)];
     }
-    if (!all || pos < s.all_lo || pos + kBlock > s.all_hi) {
+    if (cap != 0.0f) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          cur[t][r] = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(cur[t][r]));
+    }
+    if (mask) {
+      const float with = cap != 0.0f ? INFINITY : -INFINITY;
 #pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           const int j = pos + 32 * t + 8 * (r >> 2) + 4 * h + (r & 3);
-          if (!there[2 * t + (r >> 3)] || j < from || j >= end) cur[t][r] = -INFINITY;
+          if (!((there >> (2 * t + (r >> 3))) & 1) || j < from || j >= end) cur[t][r] = with;
         }
     }
+    float f[4];
+    float mx = -INFINITY;
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
+    for (int c = 0; c < 4; ++c) {
+      f[c] = cap != 0.0f ? -2.0f * cap : quick ? ks[c] : 1.0f;
+      float x = cur[c >> 1][8 * (c & 1)];
+      if (cap != 0.0f) {
 #pragma unroll
-      for (int r = 0; r < 16; ++r) mx = fmaxf(mx, cur[t][r]);
+        for (int r = 1; r < 8; ++r) x = fminf(x, cur[c >> 1][8 * (c & 1) + r]);
+      } else {
+#pragma unroll
+        for (int r = 1; r < 8; ++r) x = fmaxf(x, cur[c >> 1][8 * (c & 1) + r]);
+      }
+      mx = fmaxf(mx, __builtin_fmaf(x, f[c], cap));
+    }
     if (__any(mx > m)) {
       const float to = fmaxf(m, xor32_max(mx));
       const float alpha = to == m ? 1.0f : __builtin_amdgcn_exp2f(m - to);
@@ -781,22 +800,40 @@ struct Tiles {
       for (int j = 0; j < ND; ++j) o[j] *= alpha;
       m = to;
     }
-    const float mm = m == -INFINITY ? 0.0f : m;
-    float rs = 0.0f;
+    const float b = cap - (m == -INFINITY ? 0.0f : m);
     bf16x8 pb[4];
+    float rs = 0.0f;
+    if (quick) {
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      const int t = c >> 1, r0 = 8 * (c & 1);
-      float e[8];
+      for (int c = 0; c < 4; ++c) {
+        const float bc = b + __builtin_amdgcn_logf(vs[c]);
+        float sum = 0.0f;
+        u32x4 w;
 #pragma unroll
-      for (int r = 0; r < 8; ++r) {
-        e[r] = __builtin_amdgcn_exp2f(cur[t][r0 + r] - mm);
-        rs += e[r];
+        for (int r = 0; r < 4; ++r) {
+          const int i = 8 * (c & 1) + 2 * r;
+          const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(cur[c >> 1][i], f[c], bc));
+          const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(cur[c >> 1][i + 1], f[c], bc));
+          sum += e0 + e1;
+          w[r] = cvt_pk_bf16x2(e0, e1);
+        }
+        rs = __builtin_fmaf(sum, __builtin_amdgcn_rcpf(vs[c]), rs);
+        pb[c] = __builtin_bit_cast(bf16x8, w);
       }
-      u32x4 f;
+    } else {
 #pragma unroll
-      for (int r = 0; r < 4; ++r) f[r] = cvt_pk_bf16x2(e[2 * r] * vs[c], e[2 * r + 1] * vs[c]);
-      pb[c] = __builtin_bit_cast(bf16x8, f);
+      for (int c = 0; c < 4; ++c) {
+        u32x4 w;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int i = 8 * (c & 1) + 2 * r;
+          const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(cur[c >> 1][i], f[c], b));
+          const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(cur[c >> 1][i + 1], f[c], b));
+          rs += e0 + e1;
+          w[r] = cvt_pk_bf16x2(e0 * vs[c], e1 * vs[c]);
+        }
+        pb[c] = __builtin_bit_cast(bf16x8, w);
+      }
     }
     l += rs;  // of this lane's positions: the two halves meet at the end
 #pragma unroll
@@ -834,6 +871,7 @@ __global__ __launch_bounds__(kTileThreads, 2) void cached_tiles_kernel(const Cac
   if (nb > 0) {
     x.refill(0);
     x.load(0);
+    x.finish();
   }
   const uint16_t* qp = p.q + static_cast<int64_t>(w.first + i) * p.q_token + head * p.q_head;
 #pragma unroll
@@ -862,6 +900,7 @@ __global__ __launch_bounds__(kTileThreads, 2) void cached_tiles_kernel(const Cac
     if (more && !ahead) {
       x.refill(kb + 1);
       x.load(kb + 1);
+      x.finish();
     }
     if (more) x.stage(kb + 1, (kb + 1) & 1);
     __syncthreads();
@@ -983,13 +1022,15 @@ Choice choose(const ttlh_kv_cache* c, int64_t q_heads) {
   const int64_t some = (c->starts ? rows + rows / 2 : rows) / (c->seqs > 0 ? c->seqs : 1);
   x.bm = some <= 16 ? 16 : some <= 32 ? 32 : some <= 48 ? 48 : kTileRows;
   x.tiles = (c->starts ? rows / x.bm + c->seqs : c->seqs * ((group + x.bm - 1) / x.bm));
-  const int64_t places = x.bm == kTileRows ? 512 : 1024;  // workgroups that fill the chip
-  x.least = 256;
-  const int64_t positions = c->width * c->page;
-  // (undivided where the tiles that there are for certain fill it, or no sequence
-  // can be longer than one part)
-  const int64_t certain = c->starts ? rows / x.bm : x.tiles;
-  x.target = certain * c->heads >= places || positions <= x.least
+  // Parts that fill the chip, twice over where a CU holds three workgroups (16 rows:
+  // 32 answers of up to 8192 positions 78 us with 768 parts, 74 with 1536; 48 rows:
+  // 92 us with 768, 97 with 1024, 105 with 512).  A part's start and end cost about as
+  // much as 512 positions; where there are two workgroups for each CU undivided, parts of
+  // fewer than 2048 do not pay (768 tiles of 1024 positions: 25 us, halved 31).
+  const int64_t places = x.bm == 16 ? 1536 : x.bm == kTileRows ? 512 : 768;
+  const int64_t certain = (c->starts ? rows / x.bm : x.tiles) * c->heads;
+  x.least = certain >= 512 ? 2048 : 512;
+  x.target = certain >= places || c->width * c->page <= x.least
                  ? 0
                  : static_cast<int32_t>((places + c->heads - 1) / c->heads);
   return x;
