@@ -20,9 +20,9 @@
 // Few tiles with many positions are divided into parts (see Plan), whose results
 // meet in cached_join_kernel in the order of the parts.
 //
-// A page whose K or V scale is not finite makes NaN of what sees it.  A NaN in V's
-// scale is carried by the scores instead (kscale, vscale below): a row that does not
-// see the page has a probability of 0 there, and 0 NaN would be NaN.
+// A page whose K or V scale is negative or not finite makes NaN of what sees it.  A NaN
+// in V's scale is carried by the scores instead (Subtiles::finish): a row that does
+// not see the page has a probability of 0 there, and 0 NaN would be NaN.
 
 #include <cmath>
 #include <type_traits>
@@ -52,7 +52,8 @@ struct CachedArgs {
   int32_t window;     // 0: none
   int32_t target;     // parts of all sequences together, for one head, about; 0: undivided
   int32_t least;      // positions of a part, at least
-  float scale_log2;   // scale log2 e, or 2 scale log2 e / softcap
+  float scale_log2;   // |scale| log2 e, or 2 |scale| log2 e / softcap
+  uint32_t flip;      // sign bits of two bf16, if the scale is negative: Q's change
   float cap_log2;     // softcap log2 e, or 0
   float* part_o;      // [slot, head, rows of a tile, dim]
   float* part_ml;     // [slot, head, rows of a tile, 2]: maximum and sum
@@ -106,6 +107,47 @@ struct Division {
     chunk = max((static_cast<int>(each) + 64) & ~63, p.least);
     chunk = __builtin_amdgcn_readfirstlane(chunk);
     if (p.c.seqs > 64) tiles = range = 0;
+  }
+  // Tile `item` of all, those that see the most positions first (by 64 of them): with
+  // prompts of several lengths the last workgroups to start are then the shortest.
+  // For undivided tiles of up to 64 sequences, without a window.
+  __device__ __forceinline__ bool find_longest(int item, Plan& w) {
+    const int lane = threadIdx.x & 63;
+    int first = 0, n = 0, len = 0;
+    if (lane < p.c.seqs) {
+      seq_tokens(p.c, lane, first, n);
+      len = p.c.lengths[lane];
+    }
+    // tiles whose last row sees at least 64 level positions
+    const auto count = [&](int level) {
+      if (level == 0) return tiles;
+      const int64_t y = int64_t(level) * 64 - 1 - (int64_t(len) - n);  // needs token y or a later one
+      if (level * 64 > capacity(p.c) || y >= n) return 0;
+      return y <= 0 ? tiles : tiles - static_cast<int>(y * p.group / BM);
+    };
+    const auto total = [&](int x) { return __builtin_amdgcn_readlane(prefix_sum(x), 63); };
+    int lo = 0, hi = (capacity(p.c) >> 6) + 1;  // total(count(lo)) > item >= total(count(hi))
+    if (total(tiles) <= item) return false;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (total(count(mid)) > item)
+        lo = mid;
+      else
+        hi = mid;
+    }
+    const int with = count(lo), more = count(hi), mine = with - more;
+    const int left = item - total(more), end = prefix_sum(mine);
+    const int l = __builtin_amdgcn_readfirstlane(__ffsll(__ballot(end > left)) - 1) & 63;
+    const auto at = [&](int x) { return __builtin_amdgcn_readlane(x, l); };
+    w.b = l;
+    w.first = at(first);
+    w.n = at(n);
+    w.len = at(len);
+    w.row0 = (at(tiles) - at(with) + left - (at(end) - at(mine))) * BM;
+    w.rows = w.n * p.group;
+    w.part = w.slot = 0;
+    w.parts = 1;
+    return w.row0 >= 0 && w.row0 < w.rows;
   }
   // item `item` of the parts (JOIN: of the tiles), or false past the last one
   template <bool JOIN>
@@ -218,23 +260,33 @@ __device__ __forceinline__ float uniform(float x, int lane) {
   return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), lane));
 }
 
+__device__ __forceinline__ bf16x8 query(const CachedArgs& p, const uint16_t* at) {
+  u32x4 v = *reinterpret_cast<const u32x4*>(at);
+  v ^= p.flip;
+  return __builtin_bit_cast(bf16x8, v);
+}
+
 // What a wave knows about 64 subtiles of 16 positions, one in a lane: the page (or
 // -1), the scores' factor and V's scale.
 struct Subtiles {
   int page;
   float kscale, vscale;
 
-  // (the scales are only asked for: finish() waits for them)
-  __device__ __forceinline__ void load(const CachedArgs& p, int b, int h, int pos) {
-    page = page_at(p.c, b, pos);
+  // In three steps, so that a wave with other work need not wait for a load: the
+  // table's entry, the scales of its page, the factors.
+  __device__ __forceinline__ void ask_page(const CachedArgs& p, int b, int pos) {
+    page = pos >= 0 && pos < capacity(p.c) ? p.c.table[b * p.c.table_ld + (pos >> p.c.shift)] : -1;
+  }
+  __device__ __forceinline__ void ask_scales(const CachedArgs& p, int h) {
+    if (page < 0 || page >= p.c.pages) page = -1;
     const int64_t at = static_cast<int64_t>(max(page, 0)) * p.c.heads + h;
     kscale = p.c.k_scale[at];
     vscale = p.c.v_scale[at];
   }
   __device__ __forceinline__ void finish(float scale) {
-    const bool fine = fabsf(kscale) < INFINITY && fabsf(vscale) < INFINITY;
+    const bool fine = kscale >= 0.0f && kscale < INFINITY && vscale >= 0.0f && vscale < INFINITY;
     kscale = fine ? kscale * scale : __int_as_float(0x7fc00000);
-    vscale = fine ? vscale : 0.0f;
+    vscale = fine ? fmaxf(vscale, 0x1p-126f) : 1.0f;
   }
 };
 
@@ -490,7 +542,8 @@ __global__ __launch_bounds__(kRowWaves * 64, MT == 1 ? 3 : 2) void cached_rows_k
   int kn;
   const auto refill = [&](int k) {  // steps k .. k + 31, two subtiles each
     const int pos = s.begin + ((k + (lane >> 1)) * kRowWaves + wave) * kStep + 16 * (lane & 1);
-    x.sub.load(p, w.b, h, pos < s.hi ? pos : -1);
+    x.sub.ask_page(p, w.b, pos < s.hi ? pos : -1);
+    x.sub.ask_scales(p, h);
     kn = min(steps, k + 32);
     x.load_k(a, k);
     x.load_v(a, k);
@@ -508,7 +561,7 @@ __global__ __launch_bounds__(kRowWaves * 64, MT == 1 ? 3 : 2) void cached_rows_k
                          static_cast<int64_t>(h * p.group + row - i * p.group) * p.q_head;
 #pragma unroll
     for (int c = 0; c < D / 32; ++c) {
-      const bf16x8 qf = *reinterpret_cast<const bf16x8*>(qp + 64 * (c >> 1) + 16 * x.g + 8 * (c & 1));
+      const bf16x8 qf = query(p, qp + 64 * (c >> 1) + 16 * x.g + 8 * (c & 1));
       if constexpr (R::kQinLds) {
         if (wave == (r * (D / 32) + c) % kRowWaves) q_lds[(r * (D / 32) + c) * 64 + lane] = qf;
       } else {
@@ -596,21 +649,37 @@ __global__ __launch_bounds__(kRowWaves * 64, MT == 1 ? 3 : 2) void cached_rows_k
 
 // ---- many rows ---------------------------------------------------------------
 //
-// 128 rows a workgroup, 32 a wave; blocks of 64 positions.  The layouts of the
-// products are those of 32x32x16 MFMAs on K and V in LDS: K row-major, 16-byte chunk
-// c of row r at c ^ (r & 15) (dim 64: c ^ ((r >> 1) & 7)); V row-major, read with
-// ds_read_b64_tr_b16, chunk c of row r at c ^ 4 (r & 3) (dim 64: c ^ 4 ((r >> 1) & 1)).
-// The codes of the next block are on their way to registers while this one
-// computes, and are decoded into the other buffer after it.
+// 128 rows a workgroup, 32 a wave; blocks of 64 positions in 32x32x16 MFMAs, K and V
+// decoded to bf16 in LDS: K row-major, 16-byte chunk c of row r at c ^ (r & 15) (dim
+// 64: c ^ ((r >> 1) & 7)); V row-major, read with ds_read_b64_tr_b16, chunk c of row r
+// at c ^ 4 (r & 3) (dim 64: c ^ 4 ((r >> 1) & 1)).  Two buffers of each.
+//
+// A block has 32 MFMAs and, for each, about ten other vector instructions (for 32
+// rows of 64 scores three each and the decoding), so these are laid between the
+// MFMAs, which run meanwhile; two workgroups share a CU.  In order, with half t the
+// block's positions 32 t .. 32 t + 31:
+//     S of half 0            | the next block's K codes are decoded into LDS
+//     S of half 1            | softmax of half 0
+//     O += V P of half 0     | softmax of half 1
+//     O += V P of half 1     | the next block's V codes are decoded into LDS
+// The running maximum m moves only where a lane's sum shows that it lags (or where
+// there is none yet): p is at most 2^8 then, which bf16 and fp32 hold as well as 1,
+// and half a block needs no maximum before its exponentials.
+// (Softmax, decoding and products one after the other took 700 us for 2048 new
+// tokens at 18000, 32 / 8 heads of 128.)
 constexpr int kTileRows = 128;
 constexpr int kBlock = 64;
 constexpr int kTileThreads = 256;
 
-template <int D, int FMT>
+template <int D, int FMT, bool CAP>
 struct Tiles {
   static constexpr int ND = D / 32, NDC = D / 16;
-  static constexpr int kChunks = D / 16;                    // 16-byte pieces of codes in a row
-  static constexpr int kLoads = kBlock * kChunks / kTileThreads;  // of a thread, for K and for V
+  static constexpr int kChunks = D / 8;                           // of eight codes in a row
+  static constexpr int kSweep = kTileThreads / kChunks;           // rows of one load of all threads
+  static constexpr int kUnits = kBlock / kSweep;                  // loads of a thread, for K and for V
+  static constexpr int kProducts = 2 * NDC + 4 * ND;              // MFMAs of a block
+  static constexpr int kAhead = 4;                                // operands read ahead
+  static constexpr float kFar = 256.0f;
 
   const CachedArgs& p;
   const Plan& w;
@@ -621,23 +690,21 @@ struct Tiles {
   int from, end;   // what the lane's row sees
   bf16x8 qop[NDC];
   f32x16 o[ND];
-  float m, l;
-  Subtiles sub;    // of blocks kb0 .. kb0 + 15
-  uint64_t paged, plain;  // subtiles with a page; with scales in the ordinary range
-  u32x4 kraw[kLoads], vraw[kLoads];
-  int k_frag, v_frag[ND];
+  f32x16 cur[2];   // scores of the two halves
+  bf16x8 f[kAhead];
+  u32x4 pw[4];     // P of the block's subtiles as bf16
+  float m, l, rs, part;  // rs, part: sums of p over half a block, over a subtile
+  Subtiles sub;    // of the sixteen blocks of the one that computes
+  Subtiles next;   // of the next sixteen, from the middle of these on
+  float lv, iv;    // sub's log2 and reciprocal of V's scales
+  uint64_t paged, broken; // sub's subtiles with a page; with a scale that makes NaN
+  u32x2 kraw[kUnits], vraw[kUnits];
+  int k_frag, v_frag[ND], k_to, v_to;
+  uint32_t unit_off;
 
   static __device__ __forceinline__ int k_swz(int r) { return D == 128 ? r & 15 : (r >> 1) & 7; }
   static __device__ __forceinline__ int v_swz(int r) {
     return D == 128 ? (r & 3) << 2 : ((r >> 1) & 1) << 2;
-  }
-  // the row and the piece of codes of a thread's load i; the rows of a wave's load
-  // are in one subtile
-  __device__ __forceinline__ int load_row(int i) const {
-    return (static_cast<int>(threadIdx.x) + i * kTileThreads) / kChunks;
-  }
-  __device__ __forceinline__ int load_sub(int i) const {
-    return (wave * 64 + i * kTileThreads) / kChunks / 16;
   }
 
   __device__ __forceinline__ void setup() {
@@ -648,239 +715,334 @@ struct Tiles {
       const int chunk = 4 * j + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
       v_frag[j] = (4 * h + vr) * D + ((chunk ^ v_swz(vr)) << 3) + 4 * (lane & 1);
     }
+    // the thread's chunk: row `row` of each sweep; 16 (or 8) lanes write a whole row
+    const int row = threadIdx.x / kChunks, c = threadIdx.x % kChunks;
+    k_to = row * D + ((c ^ k_swz(row)) << 3);
+    v_to = row * D + ((c ^ v_swz(row)) << 3);
+    unit_off = (row & 15) * D + c * 8;
+    m = -INFINITY;
+    l = 0.0f;
+#pragma unroll
+    for (int j = 0; j < ND; ++j)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) o[j][r] = 0.0f;
   }
-  __device__ __forceinline__ void refill(int kb) {  // kb a multiple of 16
+
+  // ---- codes ----
+  // the subtile of the thread's unit i (the rows of a wave's load are in one)
+  __device__ __forceinline__ int unit_sub(int i) const {
+    return D == 128 ? i : 2 * i + (wave >> 1);
+  }
+  __device__ __forceinline__ void ask_page(Subtiles& x, int kb) const {  // kb a multiple of 16
     const int pos = s.begin + kb * kBlock + lane * 16;
-    sub.load(p, w.b, hd, pos < s.hi ? pos : -1);
+    x.ask_page(p, w.b, pos < s.hi ? pos : -1);
   }
   __device__ __forceinline__ void finish() {
-    sub.finish(p.scale_log2);
+    broken = __ballot(!(sub.kscale < INFINITY));
+    if (!(sub.kscale < INFINITY)) sub.kscale = 1.0f;  // (hide() makes the NaN)
+    sub.kscale = fmaxf(sub.kscale, 0x1p-126f);        // (0 times -inf would be NaN)
+    const bool far = far_scale(sub.vscale);           // (restage_v() multiplies)
+    lv = far ? 0.0f : __builtin_amdgcn_logf(sub.vscale);
+    iv = far ? 1.0f : __builtin_amdgcn_rcpf(sub.vscale);
     paged = __ballot(sub.page >= 0);
-    plain = __ballot(sub.kscale > 0.0f && sub.vscale > 0x1p-60f && sub.vscale < 0x1p60f);
   }
-  __device__ __forceinline__ void load(int kb) {
+  // V scales so small or large that p times them leaves the exponents' range go into
+  // V itself.
+  static __device__ __forceinline__ bool far_scale(float v) { return v < 0x1p-60f || v > 0x1p60f; }
+  __device__ __forceinline__ void restage_v(int kb) {
+    const bool later = (kb & 15) == 0 && kb > 0;
+    float scale = later ? next.vscale : sub.vscale;
+    const int at = (kb & 15) * 4;
+    if (__builtin_expect(((__ballot(far_scale(scale)) >> at) & 15) == 0, 1)) return;
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i) {
-      const int st = load_sub(i), row = load_row(i);
-      const int page = max(__builtin_amdgcn_readlane(sub.page, (kb & 15) * 4 + st), 0);
+    for (int i = 0; i < kUnits; ++i) {
+      const float f = uniform(scale, at + unit_sub(i));
+      if (!far_scale(f)) continue;
+      u32x4 v = eight_of<FMT>(vraw[i][0], vraw[i][1]);
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        v[j] = cvt_pk_bf16x2(__uint_as_float(v[j] << 16) * f, __uint_as_float(v[j] & 0xffff0000u) * f);
+      *reinterpret_cast<u32x4*>(Vs[kb & 1] + v_to + i * kSweep * D) = v;
+    }
+  }
+  // block kb's codes into registers, AHEAD blocks before it computes
+  template <int AHEAD>
+  __device__ __forceinline__ void load(const uint8_t* codes, u32x2 (&raw)[kUnits], int kb) const {
+    const bool later = (kb & 15) < AHEAD && kb >= 16;
+#pragma unroll
+    for (int i = 0; i < kUnits; ++i) {
+      const int st = unit_sub(i), at = (kb & 15) * 4 + st;
+      const int here = __builtin_amdgcn_readlane(sub.page, at);
+      const int there = __builtin_amdgcn_readlane(next.page, at);
+      const int page = max(later ? there : here, 0);
       const int slot = (s.begin + kb * kBlock + 16 * st) & ((1 << p.c.shift) - 1);
-      const int64_t at = slot_offset(p.c, page, hd, slot);
-      const uint32_t off = (row - 16 * st) * D + (threadIdx.x % kChunks) * 16;
-      kraw[i] = *reinterpret_cast<const u32x4*>(p.c.k + at + off);
-      vraw[i] = *reinterpret_cast<const u32x4*>(p.c.v + at + off);
+      raw[i] = *reinterpret_cast<const u32x2*>(codes + slot_offset(p.c, page, hd, slot) + unit_off);
     }
   }
-  // block kb's codes, decoded, into LDS; those that no row sees as zeros (V)
-  __device__ __forceinline__ void stage(int kb, int buf) {
-    const int pos = s.begin + kb * kBlock;
-    const int there = (paged >> ((kb & 15) * 4)) & 15;
-    const bool edge = pos < s.lo || pos + kBlock > s.hi || there != 15;
-#pragma unroll
-    for (int i = 0; i < kLoads; ++i) {
-      const int row = load_row(i), c = threadIdx.x % kChunks;
-      if (edge) {
-        if (!((there >> load_sub(i)) & 1) || pos + row < s.lo || pos + row >= s.hi) vraw[i] = u32x4{0u, 0u, 0u, 0u};
-      }
-      uint16_t* kd = Ks[buf] + row * D;
-      uint16_t* vd = Vs[buf] + row * D;
-      // (every second row's V goes odd chunk first: with both even, two rows' writes
-      // would meet in the same banks)
-      const int odd = D == 128 ? row & 1 : (row >> 1) & 1;
-      const u32x4 v = odd ? u32x4{vraw[i][2], vraw[i][3], vraw[i][0], vraw[i][1]} : vraw[i];
-      *reinterpret_cast<u32x4*>(kd + ((2 * c ^ k_swz(row)) << 3)) = eight_of<FMT>(kraw[i][0], kraw[i][1]);
-      *reinterpret_cast<u32x4*>(kd + (((2 * c + 1) ^ k_swz(row)) << 3)) = eight_of<FMT>(kraw[i][2], kraw[i][3]);
-      *reinterpret_cast<u32x4*>(vd + (((2 * c + odd) ^ v_swz(row)) << 3)) = eight_of<FMT>(v[0], v[1]);
-      *reinterpret_cast<u32x4*>(vd + (((2 * c + 1 - odd) ^ v_swz(row)) << 3)) = eight_of<FMT>(v[2], v[3]);
-    }
+  template <int I>
+  __device__ __forceinline__ void stage(uint16_t* to, const u32x2 (&raw)[kUnits]) const {
+    *reinterpret_cast<u32x4*>(to + I * kSweep * D) = eight_of<FMT>(raw[I][0], raw[I][1]);
   }
-  __device__ __forceinline__ i16x4 read_v4(const uint16_t* Vb, int kv, int j) const {
-    return __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(Vb + v_frag[j] + kv * D));
+  template <int I = 0>
+  __device__ __forceinline__ void stage_all(int buf) {
+    stage<I>(Ks[buf] + k_to, kraw);
+    stage<I>(Vs[buf] + v_to, vraw);
+    if constexpr (I + 1 < kUnits) stage_all<I + 1>(buf);
   }
-  __device__ __forceinline__ void scores(const uint16_t* K_, f32x16 (&sv)[2]) {
-    constexpr int kAhead = 4;
-    const auto frag = [&](int i) {
-      return *reinterpret_cast<const bf16x8*>(K_ + (k_frag ^ ((i % NDC) * 16)) + (i / NDC) * 32 * D);
-    };
-    bf16x8 f[kAhead];
+  // bits: the subtiles of block kb (this one or the next) that have a page
+  __device__ __forceinline__ int pages_of(int kb) const {
+    const uint64_t all = (kb & 15) == 0 && kb > 0 ? __ballot(next.page >= 0) : paged;
+    return (all >> ((kb & 15) * 4)) & 15;
+  }
+  // V codes of block kb that no row sees may be anything, and 0 times them has to be 0
+  __device__ __forceinline__ void clear_unseen(int kb) {
+    const int pos = s.begin + kb * kBlock, pages = pages_of(kb);
+    if (pos >= s.lo && pos + kBlock <= s.hi && pages == 15) return;
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i) f[i] = frag(i);
-    __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-#pragma unroll
-      for (int r = 0; r < 16; ++r) sv[t][r] = 0.0f;
-#pragma unroll
-      for (int dc = 0; dc < NDC; ++dc) {
-        const int i = t * NDC + dc;
-        sv[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f[i % kAhead], qop[dc], sv[t], 0, 0, 0);
-        if (i + kAhead < 2 * NDC) f[i % kAhead] = frag(i + kAhead);
-        __builtin_amdgcn_sched_barrier(0);
-      }
+    for (int i = 0; i < kUnits; ++i) {
+      const int j = pos + i * kSweep + static_cast<int>(threadIdx.x) / kChunks;
+      if (!((pages >> unit_sub(i)) & 1) || j < s.lo || j >= s.hi) vraw[i] = u32x2{0u, 0u};
     }
   }
 
-  __device__ __forceinline__ void block(int kb, int buf) {
-    const uint16_t *Kc = Ks[buf], *Vc = Vs[buf];
-    const int pos = s.begin + kb * kBlock;
-    f32x16 cur[2];
-    scores(Kc, cur);
-    // V^T operand i of lane (d = 32 j + l32, h), j = i % ND: positions {16 c + 4 h + u,
-    // 16 c + 4 h + 8 + u}, c = i / ND; the first ones are read under the softmax
-    const auto vfrag = [&](int i) {
-      const i16x4 lo = read_v4(Vc, 16 * (i / ND), i % ND);
-      const i16x4 hi = read_v4(Vc, 16 * (i / ND) + 8, i % ND);
-      const i16x8 f = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-      return __builtin_bit_cast(bf16x8, f);
-    };
-    constexpr int kAhead = 4;
-    bf16x8 vf[kAhead];
-#pragma unroll
-    for (int i = 0; i < kAhead; ++i) vf[i] = vfrag(i);
-    __builtin_amdgcn_sched_barrier(0);
-
-    float ks[4], vs[4];
-#pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      ks[t] = uniform(sub.kscale, (kb & 15) * 4 + t);
-      vs[t] = uniform(sub.vscale, (kb & 15) * 4 + t);
+  // ---- products ----
+  // MFMA operand i of a block: K's, then V's: V^T operand i of lane (d = 32 j + l32,
+  // h), j = i % ND, has positions {16 c + 4 h + u, 16 c + 4 h + 8 + u}, c = i / ND
+  template <int I>
+  __device__ __forceinline__ void read(const uint16_t* Kc, const uint16_t* Vc) {
+    if constexpr (I < 2 * NDC) {
+      f[I % kAhead] = *reinterpret_cast<const bf16x8*>(Kc + (k_frag ^ ((I % NDC) * 16)) +
+                                                       (I / NDC) * 32 * D);
+    } else if constexpr (I < kProducts) {
+      constexpr int i = I - 2 * NDC;
+      const uint16_t* at = Vc + v_frag[i % ND] + 16 * (i / ND) * D;
+      const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)at);
+      const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(at + 8 * D));
+      const i16x8 x = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+      f[I % kAhead] = __builtin_bit_cast(bf16x8, x);
     }
-    // accumulator r of half t: position 32 t + 8 (r / 4) + 4 h + r % 4, subtile 2 t + r / 8
-    const int there = (paged >> ((kb & 15) * 4)) & 15;
-    const bool mask = there != 15 || pos < s.all_lo || pos + kBlock > s.all_hi;
-    const bool quick = ((plain >> ((kb & 15) * 4)) & 15) == 15;
-    const float cap = p.cap_log2;
-    // With scales in the ordinary range (quick) K's go into the exponents'
-    // multiplications and V's into their additions, 3 instructions for a score in
-    // place of 5:  p vs = 2^(x f + b).  x: the raw score; where it is capped,
-    // u = 1 / (1 + e^2t) of C tanh t = C - 2 C u, the largest where u is least.
-    if (!quick || cap != 0.0f) {
-      asm volatile("");  // a branch: not 32 multiplications by one
+  }
+  template <int I>
+  __device__ __forceinline__ void product(const uint16_t* Kc, const uint16_t* Vc) {
+    if constexpr (I < 2 * NDC) {
+      constexpr int t = I / NDC;
+      if constexpr (I % NDC == 0) {
 #pragma unroll
-      for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) cur[t][r] *= ks[2 * t + (r >> 3)];
-    }
-    if (cap != 0.0f) {
-#pragma unroll
-      for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int r = 0; r < 16; ++r)
-          cur[t][r] = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(cur[t][r]));
-    }
-    if (mask) {
-      const float with = cap != 0.0f ? INFINITY : -INFINITY;
-#pragma unroll
-      for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int j = pos + 32 * t + 8 * (r >> 2) + 4 * h + (r & 3);
-          if (!((there >> (2 * t + (r >> 3))) & 1) || j < from || j >= end) cur[t][r] = with;
-        }
-    }
-    float f[4];
-    float mx = -INFINITY;
-#pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      f[c] = cap != 0.0f ? -2.0f * cap : quick ? ks[c] : 1.0f;
-      float x = cur[c >> 1][8 * (c & 1)];
-      if (cap != 0.0f) {
-#pragma unroll
-        for (int r = 1; r < 8; ++r) x = fminf(x, cur[c >> 1][8 * (c & 1) + r]);
-      } else {
-#pragma unroll
-        for (int r = 1; r < 8; ++r) x = fmaxf(x, cur[c >> 1][8 * (c & 1) + r]);
+        for (int r = 0; r < 16; ++r) cur[t][r] = 0.0f;
       }
-      mx = fmaxf(mx, __builtin_fmaf(x, f[c], cap));
+      cur[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f[I % kAhead], qop[I % NDC], cur[t], 0, 0, 0);
+    } else {
+      constexpr int i = I - 2 * NDC;
+      o[i % ND] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f[I % kAhead],
+                                                          __builtin_bit_cast(bf16x8, pw[i / ND]),
+                                                          o[i % ND], 0, 0, 0);
     }
-    if (__any(mx > m)) {
+    read<I + kAhead>(Kc, Vc);
+  }
+
+  // ---- softmax ----
+  // Of a block's subtile c: the scores' factor, log2 and reciprocal of V's scale.
+  struct Factors {
+    float ks[4], lv[4], iv[4];
+    int there, bad, pos;  // bits: subtiles with a page; with a scale that makes NaN
+    bool edge;            // some row does not see all of it, or some scale is bad
+  };
+  static __device__ __forceinline__ float nan_value() { return __int_as_float(0x7fc00000); }
+  // Half T of an edge block: scores that are not seen, and those of bad pages.
+  // (Where scores are capped, C tanh t = C - 2 C u with u = 1 / (1 + e^2t), it takes
+  // the u that pair() left: u = inf is not seen.)
+  template <int T>
+  __device__ __forceinline__ void hide(const Factors& k) {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const int c = 2 * T + (r >> 3), j = k.pos + 32 * T + 8 * (r >> 2) + 4 * h + (r & 3);
+      if ((k.bad >> c) & 1) cur[T][r] = nan_value();
+      if (!((k.there >> c) & 1) || j < from || j >= end) cur[T][r] = CAP ? INFINITY : -INFINITY;
+    }
+  }
+  // p times V's scale = 2^(x f + b) of scores 2 Q, 2 Q + 1 of half T: the K scale in f
+  // (or, capped, in x) and V's in b.  (Accumulator r: position 32 T + 8 (r / 4) + 4 h +
+  // r % 4 of the block, subtile 2 T + r / 8.)
+  template <int T, int Q>
+  __device__ __forceinline__ void pair(const Factors& k, float base) {
+    constexpr int c = 2 * T + Q / 4;
+    const float f = CAP ? -2.0f * p.cap_log2 : k.ks[c], b = base + k.lv[c];
+    float e[2];
+#pragma unroll
+    for (int z = 0; z < 2; ++z) {
+      float x = cur[T][2 * Q + z];
+      if constexpr (CAP) {
+        x = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x * k.ks[c]));
+        cur[T][2 * Q + z] = x;
+      }
+      e[z] = __builtin_amdgcn_exp2f(__builtin_fmaf(x, f, b));
+    }
+    sum<T, Q>(k, e[0] + e[1]);
+    pw[c][Q % 4] = cvt_pk_bf16x2(e[0], e[1]);
+  }
+  // (a subtile's pairs first, then times its 1 / V scale)
+  template <int T, int Q>
+  __device__ __forceinline__ void sum(const Factors& k, float x) {
+    constexpr int c = 2 * T + Q / 4;
+    part = Q % 4 == 0 ? x : part + x;
+    if constexpr (Q % 4 == 3) rs = Q == 3 ? part * k.iv[c] : __builtin_fmaf(part, k.iv[c], rs);
+  }
+  __device__ __forceinline__ float base() const {
+    return (CAP ? p.cap_log2 : 0.0f) - (m == -INFINITY ? 0.0f : m);
+  }
+  // The same for the whole of half T from what pair() left in cur.  (As asm, like the
+  // products' rescaling below: in C++ a second set of P lives across the branch.)
+  template <int T, int Q = 0>
+  __device__ __forceinline__ void again(const Factors& k, float base) {
+    constexpr int c = 2 * T + Q / 4;
+    const float f = CAP ? -2.0f * p.cap_log2 : k.ks[c], b = base + k.lv[c];
+    float e0, e1;
+    asm volatile(
+        "v_fma_f32 %1, %3, %5, %6\n\t"
+        "v_fma_f32 %2, %4, %5, %6\n\t"
+        "v_exp_f32 %1, %1\n\t"
+        "v_exp_f32 %2, %2\n\t"
+        "s_nop 1\n\t"
+        "v_cvt_pk_bf16_f32 %0, %1, %2"
+        : "+v"(pw[c][Q % 4]), "=&v"(e0), "=&v"(e1)
+        : "v"(cur[T][2 * Q]), "v"(cur[T][2 * Q + 1]), "v"(f), "v"(b));
+    sum<T, Q>(k, e0 + e1);
+    if constexpr (Q < 7) again<T, Q + 1>(k, base);
+  }
+  template <int T>
+  __device__ __forceinline__ void settle(const Factors& k) {
+    if ((CAP && k.edge) || __any(rs > kFar || m == -INFINITY)) {
+      if (CAP && k.edge) hide<T>(k);
+      float mx = -INFINITY;
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        float x = cur[T][8 * c];
+#pragma unroll
+        for (int r = 1; r < 8; ++r)
+          x = CAP ? fminf(x, cur[T][8 * c + r]) : fmaxf(x, cur[T][8 * c + r]);
+        const float f = CAP ? -2.0f * p.cap_log2 : k.ks[2 * T + c];
+        mx = fmaxf(mx, __builtin_fmaf(x, f, CAP ? p.cap_log2 : 0.0f));
+      }
       const float to = fmaxf(m, xor32_max(mx));
       const float alpha = to == m ? 1.0f : __builtin_amdgcn_exp2f(m - to);
       l *= alpha;
+      // (as asm: written in C++, the compiler keeps a second O across the branch, and
+      // spills.  It does not see the asm read the MFMAs' results and write their
+      // operands, so the wait states are explicit.)
+      asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 7");
 #pragma unroll
-      for (int j = 0; j < ND; ++j) o[j] *= alpha;
+      for (int j = 0; j < ND; ++j)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) asm volatile("v_mul_f32 %0, %1, %0" : "+v"(o[j][r]) : "v"(alpha));
       m = to;
+      again<T>(k, base());
+      asm volatile("s_nop 7");
     }
-    const float b = cap - (m == -INFINITY ? 0.0f : m);
-    bf16x8 pb[4];
-    float rs = 0.0f;
-    if (quick) {
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        const float bc = b + __builtin_amdgcn_logf(vs[c]);
-        float sum = 0.0f;
-        u32x4 w;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int i = 8 * (c & 1) + 2 * r;
-          const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(cur[c >> 1][i], f[c], bc));
-          const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(cur[c >> 1][i + 1], f[c], bc));
-          sum += e0 + e1;
-          w[r] = cvt_pk_bf16x2(e0, e1);
-        }
-        rs = __builtin_fmaf(sum, __builtin_amdgcn_rcpf(vs[c]), rs);
-        pb[c] = __builtin_bit_cast(bf16x8, w);
-      }
-    } else {
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        u32x4 w;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int i = 8 * (c & 1) + 2 * r;
-          const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(cur[c >> 1][i], f[c], b));
-          const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(cur[c >> 1][i + 1], f[c], b));
-          rs += e0 + e1;
-          w[r] = cvt_pk_bf16x2(e0 * vs[c], e1 * vs[c]);
-        }
-        pb[c] = __builtin_bit_cast(bf16x8, w);
-      }
+    l += rs;  // of this lane's positions: the two halves of a row meet at the end
+  }
+
+  // MFMA I and what is laid behind it
+  template <int I = 0>
+  __device__ __forceinline__ void chain(const Factors& k, float b, int kb, int nb) {
+    const int buf = kb & 1;
+    constexpr int kPairs = 8 / NDC;  // of a half behind each MFMA
+    product<I>(Ks[buf], Vs[buf]);
+    constexpr int g = I / NDC, i = I % NDC;  // (a half's products are NDC MFMAs too)
+    if constexpr (g == 0 && (i & 1)) stage<i / 2>(Ks[buf ^ 1] + k_to, kraw);
+    if constexpr (g == 1 || g == 2) {
+      pair<g - 1, kPairs * i>(k, b);
+      if constexpr (kPairs == 2) pair<g - 1, kPairs * i + 1>(k, b);
     }
-    l += rs;  // of this lane's positions: the two halves meet at the end
+    if constexpr (g == 3 && (i & 1)) stage<i / 2>(Vs[buf ^ 1] + v_to, vraw);
+    __builtin_amdgcn_sched_barrier(0);
+    if constexpr (g == 0 && i == NDC - 1) {
+      if (kb + 2 < nb) load<2>(p.c.k, kraw, kb + 2);
+      if (!CAP && k.edge) hide<0>(k);
+    }
+    if constexpr (g == 1 && i == NDC - 1) {
+      settle<0>(k);
+      b = base();
+      if (!CAP && k.edge) hide<1>(k);
+    }
+    if constexpr (g == 2 && i == NDC - 1) {
+      settle<1>(k);
+      clear_unseen(kb + 1);
+    }
+    if constexpr (I + 1 < kProducts) chain<I + 1>(k, b, kb, nb);
+  }
+
+  // Block kb; the next one's codes (in registers) go to the other LDS buffers, and
+  // those of the one after it follow into the registers.
+  __device__ __forceinline__ void block(int kb, int nb) {
+    const uint16_t *Kc = Ks[kb & 1], *Vc = Vs[kb & 1];
+    read<0>(Kc, Vc);
+    read<1>(Kc, Vc);
+    read<2>(Kc, Vc);
+    read<3>(Kc, Vc);
+    __builtin_amdgcn_sched_barrier(0);
+    Factors k;
+    const int at = (kb & 15) * 4;
+    k.pos = s.begin + kb * kBlock;
+    k.there = (paged >> at) & 15;
+    k.bad = (broken >> at) & 15;
 #pragma unroll
-    for (int i = 0; i < 4 * ND; ++i) {
-      o[i % ND] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[i % kAhead], pb[i / ND], o[i % ND], 0,
-                                                          0, 0);
-      if (i + kAhead < 4 * ND) vf[i % kAhead] = vfrag(i + kAhead);
-      __builtin_amdgcn_sched_barrier(0);
+    for (int t = 0; t < 4; ++t) {
+      k.ks[t] = uniform(sub.kscale, at + t);
+      k.lv[t] = uniform(lv, at + t);
+      k.iv[t] = uniform(iv, at + t);
+    }
+    k.edge = k.there != 15 || k.bad != 0 || k.pos < s.all_lo || k.pos + kBlock > s.all_hi;
+    chain(k, base(), kb, nb);
+    restage_v(kb + 1);
+    if (kb + 2 < nb) load<2>(p.c.v, vraw, kb + 2);
+  }
+  // the same without the block itself
+  __device__ __forceinline__ void skip(int kb, int nb) {
+    clear_unseen(kb + 1);
+    stage_all((kb & 1) ^ 1);
+    restage_v(kb + 1);
+    if (kb + 2 < nb) {
+      load<2>(p.c.k, kraw, kb + 2);
+      load<2>(p.c.v, vraw, kb + 2);
     }
   }
 };
 
-template <int D, int FMT>
-__global__ __launch_bounds__(kTileThreads, 2) void cached_tiles_kernel(const CachedArgs p) {
+template <int D, int FMT, bool CAP>
+__global__ __launch_bounds__(kTileThreads, D == 64 ? 3 : 2) void cached_tiles_kernel(
+    const CachedArgs p) {
   __shared__ __attribute__((aligned(256))) uint16_t KV[2][2][kBlock * D];
   Division<kTileRows> div{p};
   div.divide();
   Plan w;
-  if (!div.template find<false>(blockIdx.x / p.c.heads, w)) return;
+  const int item = blockIdx.x / p.c.heads;
+  const bool sorted = p.target == 0 && p.window == 0 && p.c.seqs > 1 && p.c.seqs <= 64;
+  if (!(sorted ? div.find_longest(item, w) : div.template find<false>(item, w))) return;
   const Span s = span_of<kTileRows, kBlock>(p, w);
-  Tiles<D, FMT> x{p, w, s, KV[0], KV[1]};
+  Tiles<D, FMT, CAP> x{p, w, s, KV[0], KV[1]};
   x.hd = blockIdx.x % p.c.heads;
   x.lane = threadIdx.x & 63;
   x.wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   x.l32 = x.lane & 31;
   x.h = x.lane >> 5;
   x.setup();
-  x.m = -INFINITY;
-  x.l = 0.0f;
+  const int nb = s.end > s.begin ? (s.end - s.begin + kBlock - 1) / kBlock : 0;
+  if (nb > 0) {
+    x.ask_page(x.sub, 0);
+    x.sub.ask_scales(p, x.hd);
+    x.template load<0>(p.c.k, x.kraw, 0);
+    x.template load<0>(p.c.v, x.vraw, 0);
+    x.sub.finish(p.scale_log2);
+    x.next = x.sub;
+  }
   const int row = w.row0 + x.wave * 32 + x.l32, qrow = min(row, w.rows - 1);
   const int i = qrow / p.group;
   const int64_t head = x.hd * p.group + qrow - i * p.group;
   seen_by(p.c, w.len, w.n, i, p.window, x.from, x.end);
-  const int nb = s.end > s.begin ? (s.end - s.begin + kBlock - 1) / kBlock : 0;
-  if (nb > 0) {
-    x.refill(0);
-    x.load(0);
-    x.finish();
-  }
   const uint16_t* qp = p.q + static_cast<int64_t>(w.first + i) * p.q_token + head * p.q_head;
 #pragma unroll
   for (int dc = 0; dc < D / 16; ++dc)
-    x.qop[dc] = *reinterpret_cast<const bf16x8*>(qp + dc * 16 + 8 * x.h);
-#pragma unroll
-  for (int j = 0; j < D / 32; ++j)
-#pragma unroll
-    for (int r = 0; r < 16; ++r) x.o[j][r] = 0.0f;
+    x.qop[dc] = query(p, qp + dc * 16 + 8 * x.h);
   // the positions that some row of this wave sees
   const int i_lo = min(w.row0 + x.wave * 32, w.rows - 1) / p.group;
   const int i_hi = min(w.row0 + x.wave * 32 + 31, w.rows - 1) / p.group;
@@ -888,21 +1050,30 @@ __global__ __launch_bounds__(kTileThreads, 2) void cached_tiles_kernel(const Cac
   seen_by(p.c, w.len, w.n, i_lo, p.window, wave_lo, unused);
   seen_by(p.c, w.len, w.n, i_hi, p.window, unused, wave_hi);
   if (w.row0 + x.wave * 32 >= w.rows) wave_hi = 0;
-  if (nb > 0) x.stage(0, 0);
+  if (nb > 0) {
+    x.finish();
+    x.clear_unseen(0);
+    x.stage_all(0);
+    x.restage_v(0);
+    if (nb > 1) {
+      x.template load<0>(p.c.k, x.kraw, 1);
+      x.template load<0>(p.c.v, x.vraw, 1);
+    }
+  }
   __syncthreads();
   for (int kb = 0; kb < nb; ++kb) {
-    // (sub holds what block kb's scores need; the next block's is loaded early
-    // only within the same sixteen)
-    const bool more = kb + 1 < nb, ahead = more && ((kb + 1) & 15) != 0;
-    if (ahead) x.load(kb + 1);
-    const int pos = s.begin + kb * kBlock;
-    if (pos < wave_hi && pos + kBlock > wave_lo) x.block(kb, kb & 1);
-    if (more && !ahead) {
-      x.refill(kb + 1);
-      x.load(kb + 1);
+    if ((kb & 15) == 0 && kb > 0) {
+      x.sub = x.next;
       x.finish();
     }
-    if (more) x.stage(kb + 1, (kb + 1) & 1);
+    if ((kb & 15) == 8 && kb + 8 < nb) x.ask_page(x.next, kb + 8);
+    if ((kb & 15) == 10 && kb + 6 < nb) x.next.ask_scales(p, x.hd);
+    if ((kb & 15) == 12 && kb + 4 < nb) x.next.finish(p.scale_log2);
+    const int pos = s.begin + kb * kBlock;
+    if (pos < wave_hi && pos + kBlock > wave_lo)
+      x.block(kb, nb);
+    else
+      x.skip(kb, nb);
     __syncthreads();
   }
   if (row >= w.rows) return;
@@ -1066,8 +1237,9 @@ extern "C" int ttlh_sdpa_cached(const ttlh_kv_cache* cache, const void* Q, void*
   TTLH_REQUIRE(q_heads < 65536 && cache->tokens * q_heads < (int64_t(1) << 31), TTLH_EUNSUPPORTED,
                "ttlh_sdpa_cached: too many q heads or tokens");
   TTLH_REQUIRE(std::isfinite(scale), TTLH_EINVAL, "ttlh_sdpa_cached: scale must be finite");
-  TTLH_REQUIRE(softcap >= 0.0f && std::isfinite(softcap), TTLH_EINVAL,
-               "ttlh_sdpa_cached: softcap must be finite and not negative");
+  TTLH_REQUIRE(softcap == 0.0f || (softcap >= 0x1p-16f && softcap <= 0x1p16f), TTLH_EINVAL,
+               "ttlh_sdpa_cached: softcap must be 0 or from 2^-16 to 2^16");
+  TTLH_REQUIRE(std::fabs(scale) <= 1e30f, TTLH_EINVAL, "ttlh_sdpa_cached: scale is at most 1e30");
   TTLH_REQUIRE(window >= 0, TTLH_EINVAL, "ttlh_sdpa_cached: window must not be negative");
   if (cache->seqs == 0 || cache->tokens == 0) return TTLH_OK;
   TTLH_REQUIRE(Q && O, TTLH_EINVAL, "ttlh_sdpa_cached: null pointer");
@@ -1090,7 +1262,8 @@ extern "C" int ttlh_sdpa_cached(const ttlh_kv_cache* cache, const void* Q, void*
   a.window = static_cast<int32_t>(window < (int64_t(1) << 31) ? window : 0);
   a.target = x.target;
   a.least = x.least;
-  a.scale_log2 = softcap > 0.0f ? scale / softcap * 2.0f * kLog2e : scale * kLog2e;
+  a.scale_log2 = std::fabs(softcap > 0.0f ? scale / softcap * 2.0f * kLog2e : scale * kLog2e);
+  a.flip = scale < 0.0f ? 0x80008000u : 0u;
   a.cap_log2 = softcap * kLog2e;
   a.part_o = static_cast<float*>(workspace);
   a.part_ml = a.part_o + 2 * int64_t(x.target) * cache->heads * x.bm * cache->dim;
@@ -1115,8 +1288,10 @@ extern "C" int ttlh_sdpa_cached(const ttlh_kv_cache* cache, const void* Q, void*
       run(cached_rows_kernel<D, F, 2>, 64 * kRowWaves, cached_join_kernel<D, 32>);
     else if (x.bm == 48)
       run(cached_rows_kernel<D, F, 3>, 64 * kRowWaves, cached_join_kernel<D, 48>);
+    else if (softcap > 0.0f)
+      run(cached_tiles_kernel<D, F, true>, kTileThreads, cached_join_kernel<D, kTileRows>);
     else
-      run(cached_tiles_kernel<D, F>, kTileThreads, cached_join_kernel<D, kTileRows>);
+      run(cached_tiles_kernel<D, F, false>, kTileThreads, cached_join_kernel<D, kTileRows>);
   };
   const std::integral_constant<int, 64> d64;
   const std::integral_constant<int, 128> d128;

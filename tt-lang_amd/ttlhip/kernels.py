@@ -924,10 +924,11 @@ def sdpa_cached(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
     """Attention of new tokens over the cache that kv_cache_write() filled (the
     new tokens' own keys among them): o = softmax(cap(scale q k^T)) v, a token at
     position p seeing the positions up to p, or the last `window` of them.
-    softcap: cap(x) = softcap tanh(x / softcap) (0: x).  q, o: bf16 [tokens,
+    softcap: cap(x) = softcap tanh(x / softcap), from 2^-16 to 2^16 (0: x).  q, o: bf16 [tokens,
     q heads, dim], any strides for tokens and heads that are multiples of 8; q heads
     share the cache's heads in equal groups.  Positions that the table does not
-    name are not seen; a token that sees nothing gets zeros.  Rows of o behind the
+    name are not seen; a token that sees nothing gets zeros, one that sees a page
+    with a negative or non-finite scale NaN.  Rows of o behind the
     last sequence's tokens stay as they are."""
     _check_heads("sdpa_cached", "q", q)
     _check_heads("sdpa_cached", "o", o, q.shape)
