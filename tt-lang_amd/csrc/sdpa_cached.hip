@@ -242,6 +242,29 @@ __device__ __forceinline__ uint32_t pair_of(uint32_t w) {
 }
 template <int FMT>
 __device__ __forceinline__ u32x4 eight_of(uint32_t a, uint32_t b) {
+  if constexpr (FMT == TTLH_CACHE_INT8) {
+    // (one block: between separate ones the compiler leaves wait states that these
+    // instructions, which write whole registers, do not need)
+    u32x4 w;
+    uint32_t t[4];
+    asm("v_cvt_f32_i32_sdwa %0, sext(%8) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_0\n\t"
+        "v_cvt_f32_i32_sdwa %4, sext(%8) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_1\n\t"
+        "v_cvt_f32_i32_sdwa %1, sext(%8) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_2\n\t"
+        "v_cvt_f32_i32_sdwa %5, sext(%8) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_3\n\t"
+        "v_cvt_f32_i32_sdwa %2, sext(%9) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_0\n\t"
+        "v_cvt_f32_i32_sdwa %6, sext(%9) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_1\n\t"
+        "v_cvt_f32_i32_sdwa %3, sext(%9) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_2\n\t"
+        "v_cvt_f32_i32_sdwa %7, sext(%9) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_3\n\t"
+        "v_cvt_pk_bf16_f32 %0, %0, %4\n\t"
+        "v_cvt_pk_bf16_f32 %1, %1, %5\n\t"
+        "v_cvt_pk_bf16_f32 %2, %2, %6\n\t"
+        "v_cvt_pk_bf16_f32 %3, %3, %7\n\t"
+        "s_nop 0"
+        : "=&v"(w[0]), "=&v"(w[1]), "=&v"(w[2]), "=&v"(w[3]), "=&v"(t[0]), "=&v"(t[1]), "=&v"(t[2]),
+          "=&v"(t[3])
+        : "v"(a), "v"(b));
+    return w;
+  }
   return u32x4{pair_of<FMT, 0>(a), pair_of<FMT, 1>(a), pair_of<FMT, 0>(b), pair_of<FMT, 1>(b)};
 }
 // byte J of a and of b
@@ -267,9 +290,11 @@ __device__ __forceinline__ bf16x8 query(const CachedArgs& p, const uint16_t* at)
 }
 
 // What a wave knows about 64 subtiles of 16 positions, one in a lane: the page (or
-// -1), the scores' factor and V's scale.
+// -1), where the codes are, counted in subtiles (page 0's where there is no page), the
+// scores' factor and V's scale.
 struct Subtiles {
   int page;
+  uint32_t unit;
   float kscale, vscale;
 
   // In three steps, so that a wave with other work need not wait for a load: the
@@ -277,9 +302,10 @@ struct Subtiles {
   __device__ __forceinline__ void ask_page(const CachedArgs& p, int b, int pos) {
     page = pos >= 0 && pos < capacity(p.c) ? p.c.table[b * p.c.table_ld + (pos >> p.c.shift)] : -1;
   }
-  __device__ __forceinline__ void ask_scales(const CachedArgs& p, int h) {
+  __device__ __forceinline__ void ask_scales(const CachedArgs& p, int h, int pos) {
     if (page < 0 || page >= p.c.pages) page = -1;
     const int64_t at = static_cast<int64_t>(max(page, 0)) * p.c.heads + h;
+    unit = static_cast<uint32_t>(at << (p.c.shift - 4)) + ((pos & ((1 << p.c.shift) - 1)) >> 4);
     kscale = p.c.k_scale[at];
     vscale = p.c.v_scale[at];
   }
@@ -355,11 +381,10 @@ struct Rows {
   uint32_t k_off, v_off;  // the lane's bytes in a subtile
   Subtiles sub;
 
-  // step k's subtile t: its first byte in the cache (of page 0 where it has none)
+  // step k's subtile t: its first byte in the cache
   __device__ __forceinline__ int64_t subtile_at(int k, int t) const {
-    const int page = max(__builtin_amdgcn_readlane(sub.page, (2 * k + t) & 63), 0);
-    const int slot = (s.begin + (k * kRowWaves + wave()) * kStep + 16 * t) & ((1 << p.c.shift) - 1);
-    return slot_offset(p.c, page, h, slot);
+    return static_cast<int64_t>(static_cast<uint32_t>(
+               __builtin_amdgcn_readlane(sub.unit, (2 * k + t) & 63))) * (16 * D);
   }
   __device__ __forceinline__ void load_k(Codes& x, int k) const {
 #pragma unroll
@@ -543,7 +568,7 @@ __global__ __launch_bounds__(kRowWaves * 64, MT == 1 ? 3 : 2) void cached_rows_k
   const auto refill = [&](int k) {  // steps k .. k + 31, two subtiles each
     const int pos = s.begin + ((k + (lane >> 1)) * kRowWaves + wave) * kStep + 16 * (lane & 1);
     x.sub.ask_page(p, w.b, pos < s.hi ? pos : -1);
-    x.sub.ask_scales(p, h);
+    x.sub.ask_scales(p, h, pos);
     kn = min(steps, k + 32);
     x.load_k(a, k);
     x.load_v(a, k);
@@ -699,6 +724,7 @@ struct Tiles {
   float lv, iv;    // sub's log2 and reciprocal of V's scales
   uint64_t paged, broken; // sub's subtiles with a page; with a scale that makes NaN
   u32x2 kraw[kUnits], vraw[kUnits];
+  uint32_t load_unit;  // sub.unit, or next.unit, of the block whose codes are loaded
   int k_frag, v_frag[ND], k_to, v_to;
   uint32_t unit_off;
 
@@ -737,6 +763,9 @@ struct Tiles {
     const int pos = s.begin + kb * kBlock + lane * 16;
     x.ask_page(p, w.b, pos < s.hi ? pos : -1);
   }
+  __device__ __forceinline__ void ask_scales(Subtiles& x, int kb) const {
+    x.ask_scales(p, hd, s.begin + kb * kBlock + lane * 16);
+  }
   __device__ __forceinline__ void finish() {
     broken = __ballot(!(sub.kscale < INFINITY));
     if (!(sub.kscale < INFINITY)) sub.kscale = 1.0f;  // (hide() makes the NaN)
@@ -765,18 +794,12 @@ struct Tiles {
       *reinterpret_cast<u32x4*>(Vs[kb & 1] + v_to + i * kSweep * D) = v;
     }
   }
-  // block kb's codes into registers, AHEAD blocks before it computes
-  template <int AHEAD>
+  // block kb's codes into registers
   __device__ __forceinline__ void load(const uint8_t* codes, u32x2 (&raw)[kUnits], int kb) const {
-    const bool later = (kb & 15) < AHEAD && kb >= 16;
 #pragma unroll
     for (int i = 0; i < kUnits; ++i) {
-      const int st = unit_sub(i), at = (kb & 15) * 4 + st;
-      const int here = __builtin_amdgcn_readlane(sub.page, at);
-      const int there = __builtin_amdgcn_readlane(next.page, at);
-      const int page = max(later ? there : here, 0);
-      const int slot = (s.begin + kb * kBlock + 16 * st) & ((1 << p.c.shift) - 1);
-      raw[i] = *reinterpret_cast<const u32x2*>(codes + slot_offset(p.c, page, hd, slot) + unit_off);
+      const uint32_t u = __builtin_amdgcn_readlane(load_unit, (kb & 15) * 4 + unit_sub(i));
+      raw[i] = *reinterpret_cast<const u32x2*>(codes + static_cast<uint64_t>(u) * (16 * D) + unit_off);
     }
   }
   template <int I>
@@ -941,10 +964,9 @@ struct Tiles {
     l += rs;  // of this lane's positions: the two halves of a row meet at the end
   }
 
-  // MFMA I and what is laid behind it
-  template <int I = 0>
+  // MFMA I and what is laid behind it; buf: kb & 1
+  template <int buf, int I = 0>
   __device__ __forceinline__ void chain(const Factors& k, float b, int kb, int nb) {
-    const int buf = kb & 1;
     constexpr int kPairs = 8 / NDC;  // of a half behind each MFMA
     product<I>(Ks[buf], Vs[buf]);
     constexpr int g = I / NDC, i = I % NDC;  // (a half's products are NDC MFMAs too)
@@ -956,7 +978,7 @@ struct Tiles {
     if constexpr (g == 3 && (i & 1)) stage<i / 2>(Vs[buf ^ 1] + v_to, vraw);
     __builtin_amdgcn_sched_barrier(0);
     if constexpr (g == 0 && i == NDC - 1) {
-      if (kb + 2 < nb) load<2>(p.c.k, kraw, kb + 2);
+      if (kb + 2 < nb) load(p.c.k, kraw, kb + 2);
       if (!CAP && k.edge) hide<0>(k);
     }
     if constexpr (g == 1 && i == NDC - 1) {
@@ -968,13 +990,14 @@ struct Tiles {
       settle<1>(k);
       clear_unseen(kb + 1);
     }
-    if constexpr (I + 1 < kProducts) chain<I + 1>(k, b, kb, nb);
+    if constexpr (I + 1 < kProducts) chain<buf, I + 1>(k, b, kb, nb);
   }
 
   // Block kb; the next one's codes (in registers) go to the other LDS buffers, and
   // those of the one after it follow into the registers.
+  template <int buf>
   __device__ __forceinline__ void block(int kb, int nb) {
-    const uint16_t *Kc = Ks[kb & 1], *Vc = Vs[kb & 1];
+    const uint16_t *Kc = Ks[buf], *Vc = Vs[buf];
     read<0>(Kc, Vc);
     read<1>(Kc, Vc);
     read<2>(Kc, Vc);
@@ -992,9 +1015,9 @@ struct Tiles {
       k.iv[t] = uniform(iv, at + t);
     }
     k.edge = k.there != 15 || k.bad != 0 || k.pos < s.all_lo || k.pos + kBlock > s.all_hi;
-    chain(k, base(), kb, nb);
+    chain<buf>(k, base(), kb, nb);
     restage_v(kb + 1);
-    if (kb + 2 < nb) load<2>(p.c.v, vraw, kb + 2);
+    if (kb + 2 < nb) load(p.c.v, vraw, kb + 2);
   }
   // the same without the block itself
   __device__ __forceinline__ void skip(int kb, int nb) {
@@ -1002,8 +1025,8 @@ struct Tiles {
     stage_all((kb & 1) ^ 1);
     restage_v(kb + 1);
     if (kb + 2 < nb) {
-      load<2>(p.c.k, kraw, kb + 2);
-      load<2>(p.c.v, vraw, kb + 2);
+      load(p.c.k, kraw, kb + 2);
+      load(p.c.v, vraw, kb + 2);
     }
   }
 };
@@ -1029,9 +1052,10 @@ __global__ __launch_bounds__(kTileThreads, D == 64 ? 3 : 2) void cached_tiles_ke
   const int nb = s.end > s.begin ? (s.end - s.begin + kBlock - 1) / kBlock : 0;
   if (nb > 0) {
     x.ask_page(x.sub, 0);
-    x.sub.ask_scales(p, x.hd);
-    x.template load<0>(p.c.k, x.kraw, 0);
-    x.template load<0>(p.c.v, x.vraw, 0);
+    x.ask_scales(x.sub, 0);
+    x.load_unit = x.sub.unit;
+    x.load(p.c.k, x.kraw, 0);
+    x.load(p.c.v, x.vraw, 0);
     x.sub.finish(p.scale_log2);
     x.next = x.sub;
   }
@@ -1056,25 +1080,30 @@ __global__ __launch_bounds__(kTileThreads, D == 64 ? 3 : 2) void cached_tiles_ke
     x.stage_all(0);
     x.restage_v(0);
     if (nb > 1) {
-      x.template load<0>(p.c.k, x.kraw, 1);
-      x.template load<0>(p.c.v, x.vraw, 1);
+      x.load(p.c.k, x.kraw, 1);
+      x.load(p.c.v, x.vraw, 1);
     }
   }
   __syncthreads();
-  for (int kb = 0; kb < nb; ++kb) {
+  const auto step = [&](int kb, auto buf) {
+    const int pos = s.begin + kb * kBlock;
+    if (pos < wave_hi && pos + kBlock > wave_lo)
+      x.template block<decltype(buf)::value>(kb, nb);
+    else
+      x.skip(kb, nb);
+    __syncthreads();
+  };
+  for (int kb = 0; kb < nb; kb += 2) {
     if ((kb & 15) == 0 && kb > 0) {
       x.sub = x.next;
       x.finish();
     }
     if ((kb & 15) == 8 && kb + 8 < nb) x.ask_page(x.next, kb + 8);
-    if ((kb & 15) == 10 && kb + 6 < nb) x.next.ask_scales(p, x.hd);
+    if ((kb & 15) == 10 && kb + 6 < nb) x.ask_scales(x.next, kb + 6);
     if ((kb & 15) == 12 && kb + 4 < nb) x.next.finish(p.scale_log2);
-    const int pos = s.begin + kb * kBlock;
-    if (pos < wave_hi && pos + kBlock > wave_lo)
-      x.block(kb, nb);
-    else
-      x.skip(kb, nb);
-    __syncthreads();
+    if ((kb & 15) == 14) x.load_unit = x.next.unit;
+    step(kb, std::integral_constant<int, 0>());
+    if (kb + 1 < nb) step(kb + 1, std::integral_constant<int, 1>());
   }
   if (row >= w.rows) return;
   const float lt = xor32_add(x.l);
