@@ -723,6 +723,7 @@ struct Tiles {
   Subtiles next;   // of the next sixteen, from the middle of these on
   float lv, iv;    // sub's log2 and reciprocal of V's scales
   uint64_t paged, broken; // sub's subtiles with a page; with a scale that makes NaN
+  uint64_t special;       // its subtiles that some row does not see, or with such scales
   u32x2 kraw[kUnits], vraw[kUnits];
   uint32_t load_unit;  // sub.unit, or next.unit, of the block whose codes are loaded
   int k_frag, v_frag[ND], k_to, v_to;
@@ -766,7 +767,7 @@ struct Tiles {
   __device__ __forceinline__ void ask_scales(Subtiles& x, int kb) const {
     x.ask_scales(p, hd, s.begin + kb * kBlock + lane * 16);
   }
-  __device__ __forceinline__ void finish() {
+  __device__ __forceinline__ void finish(int kb) {  // kb a multiple of 16
     broken = __ballot(!(sub.kscale < INFINITY));
     if (!(sub.kscale < INFINITY)) sub.kscale = 1.0f;  // (hide() makes the NaN)
     sub.kscale = fmaxf(sub.kscale, 0x1p-126f);        // (0 times -inf would be NaN)
@@ -774,33 +775,47 @@ struct Tiles {
     lv = far ? 0.0f : __builtin_amdgcn_logf(sub.vscale);
     iv = far ? 1.0f : __builtin_amdgcn_rcpf(sub.vscale);
     paged = __ballot(sub.page >= 0);
+    const int pos = s.begin + (kb * 4 + lane) * 16;
+    special = __ballot(sub.page < 0 || far || pos < s.all_lo || pos + 16 > s.all_hi) | broken;
   }
+  // whether block kb of the sixteen has such a subtile (the first of the next sixteen
+  // is not known yet: it may)
+  __device__ __forceinline__ bool is_special(int kb) const { return (special >> ((kb & 15) * 4)) & 15; }
+  __device__ __forceinline__ bool may_be_special(int kb) const { return (kb & 15) == 0 || is_special(kb); }
   // V scales so small or large that p times them leaves the exponents' range go into
   // V itself.
   static __device__ __forceinline__ bool far_scale(float v) { return v < 0x1p-60f || v > 0x1p60f; }
-  __device__ __forceinline__ void restage_v(int kb) {
+  __device__ __forceinline__ void restage_v(int kb) const {
     const bool later = (kb & 15) == 0 && kb > 0;
-    float scale = later ? next.vscale : sub.vscale;
+    const float scale = later ? next.vscale : sub.vscale;
+    const uint32_t unit = later ? next.unit : sub.unit;
     const int at = (kb & 15) * 4;
-    if (__builtin_expect(((__ballot(far_scale(scale)) >> at) & 15) == 0, 1)) return;
-#pragma unroll
+    if (((__ballot(far_scale(scale)) >> at) & 15) == 0) return;
     for (int i = 0; i < kUnits; ++i) {
       const float f = uniform(scale, at + unit_sub(i));
-      if (!far_scale(f)) continue;
-      u32x4 v = eight_of<FMT>(vraw[i][0], vraw[i][1]);
+      const int j = s.begin + kb * kBlock + i * kSweep + static_cast<int>(threadIdx.x) / kChunks;
+      if (!far_scale(f) || j < s.lo || j >= s.hi) continue;
+      const uint32_t u = __builtin_amdgcn_readlane(unit, at + unit_sub(i));
+      const u32x2 raw = *reinterpret_cast<const u32x2*>(p.c.v + static_cast<uint64_t>(u) * (16 * D) +
+                                                        unit_off);
+      u32x4 v = eight_of<FMT>(raw[0], raw[1]);
 #pragma unroll
       for (int j = 0; j < 4; ++j)
         v[j] = cvt_pk_bf16x2(__uint_as_float(v[j] << 16) * f, __uint_as_float(v[j] & 0xffff0000u) * f);
       *reinterpret_cast<u32x4*>(Vs[kb & 1] + v_to + i * kSweep * D) = v;
     }
   }
-  // block kb's codes into registers
+  // unit I of block kb's codes into registers (any lane's load_unit is in the cache)
+  template <int I>
   __device__ __forceinline__ void load(const uint8_t* codes, u32x2 (&raw)[kUnits], int kb) const {
-#pragma unroll
-    for (int i = 0; i < kUnits; ++i) {
-      const uint32_t u = __builtin_amdgcn_readlane(load_unit, (kb & 15) * 4 + unit_sub(i));
-      raw[i] = *reinterpret_cast<const u32x2*>(codes + static_cast<uint64_t>(u) * (16 * D) + unit_off);
-    }
+    const uint32_t u = __builtin_amdgcn_readlane(load_unit, (kb & 15) * 4 + unit_sub(I));
+    raw[I] = *reinterpret_cast<const u32x2*>(codes + static_cast<uint64_t>(u) * (16 * D) + unit_off);
+  }
+  template <int I = 0>
+  __device__ __forceinline__ void load_all(int kb) {
+    load<I>(p.c.k, kraw, kb);
+    load<I>(p.c.v, vraw, kb);
+    if constexpr (I + 1 < kUnits) load_all<I + 1>(kb);
   }
   template <int I>
   __device__ __forceinline__ void stage(uint16_t* to, const u32x2 (&raw)[kUnits]) const {
@@ -964,21 +979,34 @@ struct Tiles {
     l += rs;  // of this lane's positions: the two halves of a row meet at the end
   }
 
-  // MFMA I and what is laid behind it; buf: kb & 1
+  // MFMA I and what is laid behind it; buf: kb & 1.  (A half's products are NDC MFMAs
+  // too.  The first pair waits for the second MFMA: the scores of the half before it
+  // are not there yet.)
+  template <int Q, int N, int T>
+  __device__ __forceinline__ void pairs(const Factors& k, float b) {
+    if constexpr (N > 0) {
+      pair<T, Q>(k, b);
+      pairs<Q + 1, N - 1, T>(k, b);
+    }
+  }
   template <int buf, int I = 0>
   __device__ __forceinline__ void chain(const Factors& k, float b, int kb, int nb) {
-    constexpr int kPairs = 8 / NDC;  // of a half behind each MFMA
     product<I>(Ks[buf], Vs[buf]);
-    constexpr int g = I / NDC, i = I % NDC;  // (a half's products are NDC MFMAs too)
+    __builtin_amdgcn_sched_barrier(0);
+    constexpr int g = I / NDC, i = I % NDC;
     if constexpr (g == 0 && (i & 1)) stage<i / 2>(Ks[buf ^ 1] + k_to, kraw);
+    if constexpr (g == 0 && !(i & 1) && i > 0) load<i / 2 - 1>(p.c.k, kraw, kb + 2);
+    if constexpr (g == 1 && i == 0) load<kUnits - 1>(p.c.k, kraw, kb + 2);
     if constexpr (g == 1 || g == 2) {
-      pair<g - 1, kPairs * i>(k, b);
-      if constexpr (kPairs == 2) pair<g - 1, kPairs * i + 1>(k, b);
+      constexpr int kDone[5] = {0, 0, 2, 5, 8};  // (dim 64) pairs before MFMA i
+      constexpr int from = D == 128 ? (i ? i - 1 : 0) : kDone[i % 4];
+      constexpr int to = i == NDC - 1 ? 8 : D == 128 ? i : kDone[i % 4 + 1];
+      pairs<from, to - from, g - 1>(k, b);
     }
     if constexpr (g == 3 && (i & 1)) stage<i / 2>(Vs[buf ^ 1] + v_to, vraw);
+    if constexpr (g == 3 && !(i & 1) && i > 0) load<i / 2 - 1>(p.c.v, vraw, kb + 2);
     __builtin_amdgcn_sched_barrier(0);
     if constexpr (g == 0 && i == NDC - 1) {
-      if (kb + 2 < nb) load(p.c.k, kraw, kb + 2);
       if (!CAP && k.edge) hide<0>(k);
     }
     if constexpr (g == 1 && i == NDC - 1) {
@@ -988,7 +1016,7 @@ struct Tiles {
     }
     if constexpr (g == 2 && i == NDC - 1) {
       settle<1>(k);
-      clear_unseen(kb + 1);
+      if (may_be_special(kb + 1)) clear_unseen(kb + 1);
     }
     if constexpr (I + 1 < kProducts) chain<buf, I + 1>(k, b, kb, nb);
   }
@@ -1014,25 +1042,22 @@ struct Tiles {
       k.lv[t] = uniform(lv, at + t);
       k.iv[t] = uniform(iv, at + t);
     }
-    k.edge = k.there != 15 || k.bad != 0 || k.pos < s.all_lo || k.pos + kBlock > s.all_hi;
+    k.edge = is_special(kb);
     chain<buf>(k, base(), kb, nb);
-    restage_v(kb + 1);
-    if (kb + 2 < nb) load(p.c.v, vraw, kb + 2);
+    load<kUnits - 1>(p.c.v, vraw, kb + 2);
+    if (may_be_special(kb + 1)) restage_v(kb + 1);
   }
   // the same without the block itself
   __device__ __forceinline__ void skip(int kb, int nb) {
     clear_unseen(kb + 1);
     stage_all((kb & 1) ^ 1);
     restage_v(kb + 1);
-    if (kb + 2 < nb) {
-      load(p.c.k, kraw, kb + 2);
-      load(p.c.v, vraw, kb + 2);
-    }
+    load_all(kb + 2);
   }
 };
 
 template <int D, int FMT, bool CAP>
-__global__ __launch_bounds__(kTileThreads, D == 64 ? 3 : 2) void cached_tiles_kernel(
+__global__ __launch_bounds__(kTileThreads, D == 64 && !CAP ? 3 : 2) void cached_tiles_kernel(
     const CachedArgs p) {
   __shared__ __attribute__((aligned(256))) uint16_t KV[2][2][kBlock * D];
   Division<kTileRows> div{p};
@@ -1054,8 +1079,7 @@ __global__ __launch_bounds__(kTileThreads, D == 64 ? 3 : 2) void cached_tiles_ke
     x.ask_page(x.sub, 0);
     x.ask_scales(x.sub, 0);
     x.load_unit = x.sub.unit;
-    x.load(p.c.k, x.kraw, 0);
-    x.load(p.c.v, x.vraw, 0);
+    x.load_all(0);
     x.sub.finish(p.scale_log2);
     x.next = x.sub;
   }
@@ -1075,14 +1099,11 @@ __global__ __launch_bounds__(kTileThreads, D == 64 ? 3 : 2) void cached_tiles_ke
   seen_by(p.c, w.len, w.n, i_hi, p.window, unused, wave_hi);
   if (w.row0 + x.wave * 32 >= w.rows) wave_hi = 0;
   if (nb > 0) {
-    x.finish();
+    x.finish(0);
     x.clear_unseen(0);
     x.stage_all(0);
     x.restage_v(0);
-    if (nb > 1) {
-      x.load(p.c.k, x.kraw, 1);
-      x.load(p.c.v, x.vraw, 1);
-    }
+    x.load_all(1);
   }
   __syncthreads();
   const auto step = [&](int kb, auto buf) {
@@ -1096,7 +1117,7 @@ __global__ __launch_bounds__(kTileThreads, D == 64 ? 3 : 2) void cached_tiles_ke
   for (int kb = 0; kb < nb; kb += 2) {
     if ((kb & 15) == 0 && kb > 0) {
       x.sub = x.next;
-      x.finish();
+      x.finish(kb);
     }
     if ((kb & 15) == 8 && kb + 8 < nb) x.ask_page(x.next, kb + 8);
     if ((kb & 15) == 10 && kb + 6 < nb) x.ask_scales(x.next, kb + 6);
