@@ -12,7 +12,7 @@
 // (the order of the positions inside a product is free).
 //
 //  * cached_rows_kernel: up to 16 MT rows in a tile (answers token by token, drafts):
-//    HBM bound.  Four waves take turns at 32 positions and meet in LDS at the end;
+//    HBM bound.  Four waves (eight, where there are few workgroups) take turns at 32 positions and meet in LDS at the end;
 //    codes go from memory to registers, no LDS on the way.
 //  * cached_tiles_kernel: tiles of 128 rows (prompts): MFMA bound.  Blocks of 64
 //    positions are decoded once into LDS for four waves of 32 rows.
@@ -63,10 +63,10 @@ struct CachedArgs {
 //
 // Lengths are on the device, so the division is made there, by every workgroup for
 // itself, from one pass over the sequences: with W the positions of all tiles
-// together, a part has `chunk` = W / target positions (at least `least`), so the
-// parts are alike whatever the lengths are.  There are at most (tiles + target)
-// parts, and at most 2 target of them belong to tiles of several parts, which have
-// `slots` for their results.
+// together, a part has `chunk` = W / (target - tiles / 2) positions (at least `least`),
+// so the parts are alike whatever the lengths are, and there are about as many as
+// the chip has places.  There are at most (tiles + target) parts, and at most 2 target
+// of them belong to tiles of several parts, which have `slots` for their results.
 struct Plan {
   int b, first, n, len;      // the sequence, its new tokens and positions
   int row0, rows;            // the tile's first row, the sequence's rows
@@ -98,12 +98,16 @@ struct Division {
     chunk = 0x7fffffff;
     if (p.target == 0) return;
     // (in fp32: off by less than one part in 2 target, and the same in every wave)
-    float sum = static_cast<float>(tiles) * range;
+    float sum = static_cast<float>(tiles) * range, all = tiles;
     for (int b = lane + 64; b < p.c.seqs; b += 64) {
       extent(b);
       sum += static_cast<float>(tiles) * range;
+      all += tiles;
     }
-    const float each = fminf(wave_total(sum) / p.target, 1073741824.0f);
+    all = wave_total(all);
+    // (a tile's last part is half a part too many on average: so many places are left)
+    const float parts = fmaxf(p.target - 0.5f * all, 0.5f * p.target);
+    const float each = fminf(wave_total(sum) / parts, 1073741824.0f);
     chunk = max((static_cast<int>(each) + 64) & ~63, p.least);
     chunk = __builtin_amdgcn_readfirstlane(chunk);
     if (p.c.seqs > 64) tiles = range = 0;
@@ -352,11 +356,16 @@ __device__ __forceinline__ float xor16_add(float x) {
 // the P^T operand as they stand, and lane (n, g) reads D / 16 bytes at n D / 16 of
 // its 8 positions, byte j of which is the operand of tile j: O^T's row m of tile j
 // is element m D / 16 + j.
-constexpr int kRowWaves = 4;
 constexpr int kStep = 32;
 
-template <int D, int FMT, int MT>
+// workgroups of W waves on a CU, by their registers
+constexpr int rows_per_cu(int dim, int mt, int w) {
+  return w == 8 ? 1 : dim == 128 ? (mt == 1 ? 3 : 2) : (mt == 1 ? 4 : mt == 2 ? 3 : 2);
+}
+
+template <int D, int FMT, int MT, int W>
 struct Rows {
+  static constexpr int kRowWaves = W;
   static constexpr int NK = D / 64;   // 16-byte loads of a K row
   static constexpr int NC = D / 32;   // K operands of a subtile
   static constexpr int NV = D / 64;   // dwords of a V load
@@ -538,12 +547,13 @@ struct Rows {
   }
 };
 
-template <int D, int FMT, int MT>
-__global__ __launch_bounds__(kRowWaves * 64, MT == 1 ? 3 : 2) void cached_rows_kernel(
+template <int D, int FMT, int MT, int W>
+__global__ __launch_bounds__(W * 64, rows_per_cu(D, MT, W) * W / 4) void cached_rows_kernel(
     const CachedArgs p) {
+  constexpr int kRowWaves = W;
   constexpr int BM = 16 * MT;
   constexpr int LD = D + 4;  // LDS row: 16 rows' 16-byte writes spread over the banks
-  typedef Rows<D, FMT, MT> R;
+  typedef Rows<D, FMT, MT, W> R;
   __shared__ bf16x8 q_lds[R::kQinLds ? MT * (D / 32) * 64 : 1];
   __shared__ float part[kRowWaves][16][LD];
   __shared__ float ml[kRowWaves][BM][2];
@@ -560,7 +570,7 @@ __global__ __launch_bounds__(kRowWaves * 64, MT == 1 ? 3 : 2) void cached_rows_k
   x.g = lane >> 4;
   x.k_off = x.n * D + 16 * x.g;
   x.v_off = 4 * x.g * D + x.n * (D / 16);
-  // steps of this wave: k * 4 + wave of the part's
+  // steps of this wave: k * W + wave of the part's
   const int total = s.end > s.begin ? (s.end - s.begin + kStep - 1) / kStep : 0;
   const int steps = total > wave ? (total - wave - 1) / kRowWaves + 1 : 0;
   typename R::Codes a, b;
@@ -1123,6 +1133,16 @@ __global__ __launch_bounds__(kTileThreads, D == 64 && !CAP ? 3 : 2) void cached_
     if ((kb & 15) == 10 && kb + 6 < nb) x.ask_scales(x.next, kb + 6);
     if ((kb & 15) == 12 && kb + 4 < nb) x.next.finish(p.scale_log2);
     if ((kb & 15) == 14) x.load_unit = x.next.unit;
+    // Of two waves on a SIMD the older one goes first all the time, and where all
+    // workgroups run at once its CU is half empty when it has ended: so the two (as far
+    // as their numbers tell them) go first in turns (612 -> 595 us for 512 workgroups).
+    // Where others wait for a place, the older ones are the longer ones.
+    if (gridDim.x <= 768) {
+      if (((blockIdx.x >> 8) ^ (kb >> 1)) & 1)
+        __builtin_amdgcn_s_setprio(1);
+      else
+        __builtin_amdgcn_s_setprio(0);
+    }
     step(kb, std::integral_constant<int, 0>());
     if (kb + 1 < nb) step(kb + 1, std::integral_constant<int, 1>());
   }
@@ -1231,7 +1251,7 @@ __global__ __launch_bounds__(256) void cached_join_kernel(const CachedArgs p) {
 
 // Rows of a tile and about how many parts, by the sizes that the host knows.
 struct Choice {
-  int bm;
+  int bm, waves;
   int64_t tiles;   // at most
   int32_t target, least;
 };
@@ -1243,13 +1263,17 @@ Choice choose(const ttlh_kv_cache* c, int64_t q_heads) {
   const int64_t some = (c->starts ? rows + rows / 2 : rows) / (c->seqs > 0 ? c->seqs : 1);
   x.bm = some <= 16 ? 16 : some <= 32 ? 32 : some <= 48 ? 48 : kTileRows;
   x.tiles = (c->starts ? rows / x.bm + c->seqs : c->seqs * ((group + x.bm - 1) / x.bm));
-  // Parts that fill the chip, twice over where a CU holds three workgroups (16 rows:
-  // 32 answers of up to 8192 positions 78 us with 768 parts, 74 with 1536; 48 rows:
-  // 92 us with 768, 97 with 1024, 105 with 512).  A part's start and end cost about as
-  // much as 512 positions; where there are two workgroups for each CU undivided, parts of
-  // fewer than 2048 do not pay (768 tiles of 1024 positions: 25 us, halved 31).
-  const int64_t places = x.bm == 16 ? 1536 : x.bm == kTileRows ? 512 : 768;
   const int64_t certain = (c->starts ? rows / x.bm : x.tiles) * c->heads;
+  // With few tiles twice the waves, half the steps of each: 8 tiles of 65536 positions
+  // 37.0 -> 33.6 us, of 262144 106 -> 101 (but 128 tiles of 4096 23.5 -> 31.4).
+  x.waves = x.bm == 16 && x.tiles * c->heads <= 32 ? 8 : 4;
+  // As many parts as the chip has places (32 answers of up to 8192 positions 72 us;
+  // with twice as many parts 74, with a few too many 79; drafts 82, 97, 105).  A part's
+  // start and end cost about as much as 512 positions; where there are two workgroups
+  // for each CU undivided, parts of fewer than 2048 do not pay (768 tiles of 1024
+  // positions: 25 us, halved 31).
+  const int64_t places =
+      256 * (x.bm == kTileRows ? 2 : rows_per_cu(c->dim, x.bm / 16, x.waves));
   x.least = certain >= 512 ? 2048 : 512;
   x.target = certain >= places || c->width * c->page <= x.least
                  ? 0
@@ -1332,12 +1356,14 @@ extern "C" int ttlh_sdpa_cached(const ttlh_kv_cache* cache, const void* Q, void*
   };
   const auto pick = [&](auto dim, auto fmt) {
     constexpr int D = decltype(dim)::value, F = decltype(fmt)::value;
-    if (x.bm == 16)
-      run(cached_rows_kernel<D, F, 1>, 64 * kRowWaves, cached_join_kernel<D, 16>);
+    if (x.bm == 16 && x.waves == 8)
+      run(cached_rows_kernel<D, F, 1, 8>, 512, cached_join_kernel<D, 16>);
+    else if (x.bm == 16)
+      run(cached_rows_kernel<D, F, 1, 4>, 256, cached_join_kernel<D, 16>);
     else if (x.bm == 32)
-      run(cached_rows_kernel<D, F, 2>, 64 * kRowWaves, cached_join_kernel<D, 32>);
+      run(cached_rows_kernel<D, F, 2, 4>, 256, cached_join_kernel<D, 32>);
     else if (x.bm == 48)
-      run(cached_rows_kernel<D, F, 3>, 64 * kRowWaves, cached_join_kernel<D, 48>);
+      run(cached_rows_kernel<D, F, 3, 4>, 256, cached_join_kernel<D, 48>);
     else if (softcap > 0.0f)
       run(cached_tiles_kernel<D, F, true>, kTileThreads, cached_join_kernel<D, kTileRows>);
     else

@@ -790,28 +790,35 @@ def rope_freqs(rot: int, base: float = 10000.0, scaling: Optional[str] = None,
 
 def _check_on_one_device(what: str, tensors, stream) -> None:
     """All on the device that the launch goes to: the stream's, or the current one."""
+    if stream is not None:
+        dev = stream.device.index
+    else:
+        dev = torch._C._cuda_getDevice() if tensors[0].is_cuda else -2
     for t in tensors:
-        if not t.is_cuda:
-            raise RuntimeError(f"{what} takes device (HIP) tensors; there is no CPU path")
-    dev = stream.device.index if stream is not None else torch._C._cuda_getDevice()
-    for t in tensors:
-        if t.get_device() != dev:
-            raise ValueError(f"{what}: a tensor on device {t.get_device()}, the launch on {dev}")
+        d = t.get_device()
+        if d != dev:
+            if d < 0:
+                raise RuntimeError(f"{what} takes device (HIP) tensors; there is no CPU path")
+            raise ValueError(f"{what}: a tensor on device {d}, the launch on {dev}")
 
 
-def _check_heads(what: str, name: str, t: torch.Tensor, shape=None) -> None:
-    """t is [tokens, heads, dim] with unit stride along dim (any others)."""
-    if t.dim() != 3 or (shape is not None and t.shape != shape):
+def _heads(what: str, name: str, t: torch.Tensor, shape=None):
+    """(shape, stride of tokens, stride of heads) of t, [tokens, heads, dim] with unit
+    stride along dim and any others (0 along a dimension of one)."""
+    s = t.shape
+    if len(s) != 3 or (shape is not None and s != shape):
         raise ValueError(f"{what}: {name} must be [tokens, heads, dim]"
-                         f"{'' if shape is None else f' = {tuple(shape)}'}, got {tuple(t.shape)}")
-    if t.stride(2) != 1 and t.shape[2] > 1:
+                         f"{'' if shape is None else f' = {tuple(shape)}'}, got {tuple(s)}")
+    a, b, c = t.stride()
+    tokens, heads, dim = s
+    if c != 1 and dim > 1:
         raise ValueError(f"{what}: {name} must have unit stride along dim")
+    return s, a if tokens > 1 else 0, b if heads > 1 else 0
 
 
-def _head_strides(t: torch.Tensor):
-    """Strides of tokens and heads (0 along a dimension of one)."""
-    a, b, _ = t.stride()
-    return (a if t.shape[0] > 1 else 0, b if t.shape[1] > 1 else 0)
+def _check_distinct(what: str, name: str, shape, token: int, head: int) -> None:
+    if (token == 0 and shape[0] > 1) or (head == 0 and shape[1] > 1):
+        raise ValueError(f"{what}: {name} must not repeat its elements")
 
 
 def rope(x: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor, out: torch.Tensor,
@@ -824,62 +831,66 @@ def rope(x: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor, out: tor
     where `interleaved`.  backward: the gradient of x from that of out (the
     opposite turn).  x and out: bf16 or f32, any strides for tokens and heads
     (q and k of one projection are turned by one call), and out may be x."""
-    _check_heads("rope", "x", x)
-    _check_heads("rope", "out", out, x.shape)
-    tokens, heads, dim = x.shape
+    shape, xt, xh = _heads("rope", "x", x)
+    _, ot, oh = _heads("rope", "out", out, shape)
+    tokens, heads, dim = shape
+    planes = freqs.shape[0] if freqs.dim() == 1 else dim
     if out.dtype != x.dtype:
         raise ValueError(f"rope: out must be {x.dtype} as x is, got {out.dtype}")
     if positions.shape != (tokens,) or positions.dtype not in (torch.int32, torch.int64):
         raise ValueError(f"rope: positions must be int32 or int64 [{tokens}], got "
                          f"{positions.dtype} {tuple(positions.shape)}")
-    if freqs.dim() != 1 or freqs.dtype != torch.float64 or 2 * freqs.shape[0] > dim:
+    if 2 * planes > dim or freqs.dtype != torch.float64 or freqs.dim() != 1:
         raise ValueError(f"rope: freqs must be float64 with at most dim / 2 = {dim // 2} elements, "
                          f"got {freqs.dtype} {tuple(freqs.shape)}")
     if not positions.is_contiguous() or not freqs.is_contiguous():
         raise ValueError("rope: positions and freqs must be contiguous")
-    if (tokens > 1 and out.stride(0) == 0) or (heads > 1 and out.stride(1) == 0):
-        raise ValueError("rope: out must not repeat its elements")
-    if out.data_ptr() == x.data_ptr() and out.stride() != x.stride():
+    _check_distinct("rope", "out", shape, ot, oh)
+    xp, op = x.data_ptr(), out.data_ptr()
+    if op == xp and (ot != xt or oh != xh):
         raise ValueError("rope: out may be x itself, not another view of its memory")
     code = L.dtype_code(x.dtype)
     _check_on_one_device("rope", (x, positions, freqs, out), stream)
-    L.call("ttlh_rope", x.data_ptr(), out.data_ptr(), code, positions.data_ptr(),
-           positions.element_size(), freqs.data_ptr(), tokens, heads, dim, 2 * freqs.shape[0],
-           *_head_strides(x), *_head_strides(out), interleaved, scale, backward,
-           L.stream_ptr(stream))
+    L.call("ttlh_rope", xp, op, code, positions.data_ptr(), positions.element_size(),
+           freqs.data_ptr(), tokens, heads, dim, 2 * planes, xt, xh, ot, oh, interleaved, scale,
+           backward, L.stream_ptr(stream))
 
 
 def _kv_cache(what: str, tokens: int, k_cache, v_cache, k_scale, v_scale, table, lengths, starts):
-    """The ttlh_kv_cache of a call with `tokens` packed new tokens."""
-    if k_cache.dim() != 4 or not k_cache.is_contiguous() or not v_cache.is_contiguous():
+    """(heads, dim, ttlh_kv_cache) of a call with `tokens` packed new tokens."""
+    shape, dtype = k_cache.shape, k_cache.dtype
+    if len(shape) != 4 or not k_cache.is_contiguous() or not v_cache.is_contiguous():
         raise ValueError(f"{what}: the caches must be contiguous [pages, heads, page, dim]")
-    fmt = CACHE_FORMATS.get(k_cache.dtype)
-    if fmt is None or v_cache.dtype != k_cache.dtype or v_cache.shape != k_cache.shape:
+    fmt = CACHE_FORMATS.get(dtype)
+    if fmt is None or v_cache.dtype != dtype or v_cache.shape != shape:
         raise ValueError(f"{what}: both caches must be int8 or float8_e4m3fn of one shape, got "
-                         f"{k_cache.dtype} {tuple(k_cache.shape)} and {v_cache.dtype} "
-                         f"{tuple(v_cache.shape)}")
-    pages, heads, page, dim = k_cache.shape
+                         f"{dtype} {tuple(shape)} and {v_cache.dtype} {tuple(v_cache.shape)}")
+    pages, heads, page, dim = shape
     for t, n in ((k_scale, "k_scale"), (v_scale, "v_scale")):
         if t.dtype != torch.float32 or t.shape != (pages, heads) or not t.is_contiguous():
             raise ValueError(f"{what}: {n} must be contiguous float32 [pages, heads] = "
                              f"{(pages, heads)}, got {t.dtype} {tuple(t.shape)}")
-    if table.dim() != 2 or table.dtype != torch.int32 or (table.shape[1] > 1 and table.stride(1) != 1):
-        raise ValueError(f"{what}: table must be int32 [sequences, pages] with unit column stride")
+    if table.dtype != torch.int32 or table.dim() != 2:
+        raise ValueError(f"{what}: table must be int32 [sequences, pages], got {table.dtype} "
+                         f"{tuple(table.shape)}")
     seqs, width = table.shape
-    if lengths.shape != (seqs,) or lengths.dtype != torch.int32 or not lengths.is_contiguous():
+    ld, one = table.stride()
+    if one != 1 and width > 1:
+        raise ValueError(f"{what}: table must have unit column stride")
+    if lengths.dtype != torch.int32 or lengths.shape != (seqs,) or not lengths.is_contiguous():
         raise ValueError(f"{what}: lengths must be contiguous int32 [{seqs}], got {lengths.dtype} "
                          f"{tuple(lengths.shape)}")
     if starts is None:
         if tokens != seqs:
             raise ValueError(f"{what}: without starts there is one new token for each of the "
                              f"{seqs} sequences, got {tokens}")
-    elif starts.shape != (seqs + 1,) or starts.dtype != torch.int32 or not starts.is_contiguous():
+    elif starts.dtype != torch.int32 or starts.shape != (seqs + 1,) or not starts.is_contiguous():
         raise ValueError(f"{what}: starts must be contiguous int32 [{seqs + 1}], got "
                          f"{starts.dtype} {tuple(starts.shape)}")
-    return _KV_CACHE.pack(k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(),
-                          v_scale.data_ptr(), table.data_ptr(), lengths.data_ptr(),
-                          0 if starts is None else starts.data_ptr(), table.stride(0), pages, width,
-                          heads, seqs, tokens, page, dim, fmt, 0)
+    return heads, dim, _KV_CACHE.pack(
+        k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
+        table.data_ptr(), lengths.data_ptr(), 0 if starts is None else starts.data_ptr(),
+        ld if seqs > 1 else width, pages, width, heads, seqs, tokens, page, dim, fmt, 0)
 
 
 def kv_cache_write(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -900,20 +911,20 @@ def kv_cache_write(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_ca
     grows are rounded again.  Positions that the table does not name, and pages
     that the cache does not have, are not written; a page that two sequences
     write in one call gets either's."""
-    _check_heads("kv_cache_write", "k", k)
-    _check_heads("kv_cache_write", "v", v, k.shape)
+    shape, kt, kh = _heads("kv_cache_write", "k", k)
+    _, vt, vh = _heads("kv_cache_write", "v", v, shape)
     if v.dtype != k.dtype:
         raise ValueError(f"kv_cache_write: k and v must have one dtype, got {k.dtype} and {v.dtype}")
-    cache = _kv_cache("kv_cache_write", k.shape[0], k_cache, v_cache, k_scale, v_scale, table,
-                      lengths, starts)
-    if k.shape[1:] != (k_cache.shape[1], k_cache.shape[3]):
-        raise ValueError(f"kv_cache_write: tokens of {tuple(k.shape[1:])}, a cache of "
-                         f"{(k_cache.shape[1], k_cache.shape[3])} (heads, dim)")
+    tokens, heads, dim = shape
+    ch, cd, cache = _kv_cache("kv_cache_write", tokens, k_cache, v_cache, k_scale, v_scale, table,
+                              lengths, starts)
+    if heads != ch or dim != cd:
+        raise ValueError(f"kv_cache_write: tokens of {(heads, dim)}, a cache of {(ch, cd)} (heads, dim)")
     code = L.dtype_code(k.dtype)
     tensors = (k, v, k_cache, v_cache, k_scale, v_scale, table, lengths)
     _check_on_one_device("kv_cache_write", tensors if starts is None else tensors + (starts,), stream)
-    L.call("ttlh_kv_cache_write", cache, k.data_ptr(), v.data_ptr(), code, *_head_strides(k),
-           *_head_strides(v), L.stream_ptr(stream))
+    L.call("ttlh_kv_cache_write", cache, k.data_ptr(), v.data_ptr(), code, kt, kh, vt, vh,
+           L.stream_ptr(stream))
 
 
 def sdpa_cached(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -930,26 +941,25 @@ def sdpa_cached(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
     name are not seen; a token that sees nothing gets zeros, one that sees a page
     with a negative or non-finite scale NaN.  Rows of o behind the
     last sequence's tokens stay as they are."""
-    _check_heads("sdpa_cached", "q", q)
-    _check_heads("sdpa_cached", "o", o, q.shape)
+    shape, qt, qh = _heads("sdpa_cached", "q", q)
+    _, ot, oh = _heads("sdpa_cached", "o", o, shape)
     if q.dtype != torch.bfloat16 or o.dtype != torch.bfloat16:
         raise ValueError(f"sdpa_cached: q and o must be bf16, got {q.dtype} and {o.dtype}")
-    tokens, q_heads, dim = q.shape
-    cache = _kv_cache("sdpa_cached", tokens, k_cache, v_cache, k_scale, v_scale, table, lengths,
-                      starts)
-    heads = k_cache.shape[1]
-    if dim != k_cache.shape[3] or heads == 0 or q_heads == 0 or q_heads % heads:
+    tokens, q_heads, dim = shape
+    heads, cd, cache = _kv_cache("sdpa_cached", tokens, k_cache, v_cache, k_scale, v_scale, table,
+                                 lengths, starts)
+    if dim != cd or heads == 0 or q_heads == 0 or q_heads % heads:
         raise ValueError(f"sdpa_cached: q of {(q_heads, dim)} (heads, dim) over a cache of "
-                         f"{(heads, k_cache.shape[3])}")
-    if (tokens > 1 and o.stride(0) == 0) or (q_heads > 1 and o.stride(1) == 0):
-        raise ValueError("sdpa_cached: o must not repeat its elements")
-    if (q.data_ptr() | o.data_ptr()) & 15 or any(n & 7 for n in _head_strides(q) + _head_strides(o)):
+                         f"{(heads, cd)}")
+    _check_distinct("sdpa_cached", "o", shape, ot, oh)
+    qp, op = q.data_ptr(), o.data_ptr()
+    if (qp | op) & 15 or (qt | qh | ot | oh) & 7:
         raise ValueError("sdpa_cached: q and o must be 16-byte aligned with strides that are "
                          "multiples of 8")
     tensors = (q, k_cache, v_cache, k_scale, v_scale, table, lengths, o)
     _check_on_one_device("sdpa_cached", tensors if starts is None else tensors + (starts,), stream)
     sp = L.stream_ptr(stream)
     nbytes = L.load().ttlh_sdpa_cached_workspace_bytes(cache, q_heads)
-    ws = _workspace_or_graphs(q.device, stream, nbytes, sp) if nbytes else None
-    L.call("ttlh_sdpa_cached", cache, q.data_ptr(), o.data_ptr(), q_heads, *_head_strides(q),
-           *_head_strides(o), scale, window, softcap, 0 if ws is None else ws.data_ptr(), nbytes, sp)
+    ws = _workspace_or_graphs(q.device, stream, nbytes, sp).data_ptr() if nbytes else 0
+    L.call("ttlh_sdpa_cached", cache, qp, op, q_heads, qt, qh, ot, oh, scale, window, softcap, ws,
+           nbytes, sp)
