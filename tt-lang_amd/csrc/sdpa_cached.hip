@@ -12,7 +12,7 @@
 // (the order of the positions inside a product is free).
 //
 //  * cached_rows_kernel: up to 16 MT rows in a tile (answers token by token, drafts):
-//    HBM bound.  Four waves (eight, where there are few workgroups) take turns at 32 positions and meet in LDS at the end;
+//    HBM bound.  Four waves take turns at 32 positions and meet in LDS at the end;
 //    codes go from memory to registers, no LDS on the way.
 //  * cached_tiles_kernel: tiles of 128 rows (prompts): MFMA bound.  Blocks of 64
 //    positions are decoded once into LDS for four waves of 32 rows.
@@ -356,16 +356,16 @@ __device__ __forceinline__ float xor16_add(float x) {
 // the P^T operand as they stand, and lane (n, g) reads D / 16 bytes at n D / 16 of
 // its 8 positions, byte j of which is the operand of tile j: O^T's row m of tile j
 // is element m D / 16 + j.
+constexpr int kRowWaves = 4;
 constexpr int kStep = 32;
 
-// workgroups of W waves on a CU, by their registers
-constexpr int rows_per_cu(int dim, int mt, int w) {
-  return w == 8 ? 1 : dim == 128 ? (mt == 1 ? 3 : 2) : (mt == 1 ? 4 : mt == 2 ? 3 : 2);
+// workgroups on a CU, by their registers
+constexpr int rows_per_cu(int dim, int mt) {
+  return dim == 128 ? (mt == 1 ? 3 : 2) : (mt == 1 ? 4 : mt == 2 ? 3 : 2);
 }
 
-template <int D, int FMT, int MT, int W>
+template <int D, int FMT, int MT>
 struct Rows {
-  static constexpr int kRowWaves = W;
   static constexpr int NK = D / 64;   // 16-byte loads of a K row
   static constexpr int NC = D / 32;   // K operands of a subtile
   static constexpr int NV = D / 64;   // dwords of a V load
@@ -547,13 +547,12 @@ struct Rows {
   }
 };
 
-template <int D, int FMT, int MT, int W>
-__global__ __launch_bounds__(W * 64, rows_per_cu(D, MT, W) * W / 4) void cached_rows_kernel(
+template <int D, int FMT, int MT>
+__global__ __launch_bounds__(kRowWaves * 64, rows_per_cu(D, MT)) void cached_rows_kernel(
     const CachedArgs p) {
-  constexpr int kRowWaves = W;
   constexpr int BM = 16 * MT;
   constexpr int LD = D + 4;  // LDS row: 16 rows' 16-byte writes spread over the banks
-  typedef Rows<D, FMT, MT, W> R;
+  typedef Rows<D, FMT, MT> R;
   __shared__ bf16x8 q_lds[R::kQinLds ? MT * (D / 32) * 64 : 1];
   __shared__ float part[kRowWaves][16][LD];
   __shared__ float ml[kRowWaves][BM][2];
@@ -570,7 +569,7 @@ __global__ __launch_bounds__(W * 64, rows_per_cu(D, MT, W) * W / 4) void cached_
   x.g = lane >> 4;
   x.k_off = x.n * D + 16 * x.g;
   x.v_off = 4 * x.g * D + x.n * (D / 16);
-  // steps of this wave: k * W + wave of the part's
+  // steps of this wave: k * 4 + wave of the part's
   const int total = s.end > s.begin ? (s.end - s.begin + kStep - 1) / kStep : 0;
   const int steps = total > wave ? (total - wave - 1) / kRowWaves + 1 : 0;
   typename R::Codes a, b;
@@ -1251,11 +1250,11 @@ __global__ __launch_bounds__(256) void cached_join_kernel(const CachedArgs p) {
 
 // Rows of a tile and about how many parts, by the sizes that the host knows.
 struct Choice {
-  int bm, waves;
+  int bm;
   int64_t tiles;   // at most
   int32_t target, least;
 };
-Choice choose(const ttlh_kv_cache* c, int64_t q_heads) {
+Choice choose(const ttlh_kv_cache* c, int64_t q_heads, int64_t window) {
   Choice x;
   const int64_t group = q_heads / c->heads;
   // rows of a sequence: on average, half as many again where they may differ
@@ -1264,18 +1263,17 @@ Choice choose(const ttlh_kv_cache* c, int64_t q_heads) {
   x.bm = some <= 16 ? 16 : some <= 32 ? 32 : some <= 48 ? 48 : kTileRows;
   x.tiles = (c->starts ? rows / x.bm + c->seqs : c->seqs * ((group + x.bm - 1) / x.bm));
   const int64_t certain = (c->starts ? rows / x.bm : x.tiles) * c->heads;
-  // With few tiles twice the waves, half the steps of each: 8 tiles of 65536 positions
-  // 37.0 -> 33.6 us, of 262144 106 -> 101 (but 128 tiles of 4096 23.5 -> 31.4).
-  x.waves = x.bm == 16 && x.tiles * c->heads <= 32 ? 8 : 4;
   // As many parts as the chip has places (32 answers of up to 8192 positions 72 us;
   // with twice as many parts 74, with a few too many 79; drafts 82, 97, 105).  A part's
   // start and end cost about as much as 512 positions; where there are two workgroups
   // for each CU undivided, parts of fewer than 2048 do not pay (768 tiles of 1024
   // positions: 25 us, halved 31).
   const int64_t places =
-      256 * (x.bm == kTileRows ? 2 : rows_per_cu(c->dim, x.bm / 16, x.waves));
+      256 * (x.bm == kTileRows ? 2 : rows_per_cu(c->dim, x.bm / 16));
   x.least = certain >= 512 ? 2048 : 512;
-  x.target = certain >= places || c->width * c->page <= x.least
+  const int64_t most = c->width * c->page;  // positions that a sequence's tokens see
+  const int64_t positions = window > 0 && window + c->tokens < most ? window + c->tokens : most;
+  x.target = certain >= places || positions <= x.least
                  ? 0
                  : static_cast<int32_t>((places + c->heads - 1) / c->heads);
   return x;
@@ -1295,7 +1293,7 @@ extern "C" int64_t ttlh_sdpa_cached_workspace_bytes(const ttlh_kv_cache* cache, 
   if (check_cache("ttlh_sdpa_cached_workspace_bytes", cache, &a) != TTLH_OK || q_heads <= 0 ||
       q_heads % cache->heads)
     return 0;
-  return workspace_bytes(cache, choose(cache, q_heads));
+  return workspace_bytes(cache, choose(cache, q_heads, 0));  // (no less than with a window)
 }
 
 extern "C" int ttlh_sdpa_cached(const ttlh_kv_cache* cache, const void* Q, void* O, int64_t q_heads,
@@ -1320,7 +1318,7 @@ extern "C" int ttlh_sdpa_cached(const ttlh_kv_cache* cache, const void* Q, void*
   TTLH_REQUIRE(((reinterpret_cast<uintptr_t>(Q) | reinterpret_cast<uintptr_t>(O)) & 15) == 0 &&
                    ((q_token | q_head | o_token | o_head) & 7) == 0,
                TTLH_EINVAL, "ttlh_sdpa_cached: Q and O must be 16-byte aligned, strides multiples of 8");
-  const Choice x = choose(cache, q_heads);
+  const Choice x = choose(cache, q_heads, window);
   const int64_t need = workspace_bytes(cache, x);
   TTLH_REQUIRE(need == 0 || (workspace && workspace_size >= need &&
                              (reinterpret_cast<uintptr_t>(workspace) & 15) == 0),
@@ -1356,14 +1354,12 @@ extern "C" int ttlh_sdpa_cached(const ttlh_kv_cache* cache, const void* Q, void*
   };
   const auto pick = [&](auto dim, auto fmt) {
     constexpr int D = decltype(dim)::value, F = decltype(fmt)::value;
-    if (x.bm == 16 && x.waves == 8)
-      run(cached_rows_kernel<D, F, 1, 8>, 512, cached_join_kernel<D, 16>);
-    else if (x.bm == 16)
-      run(cached_rows_kernel<D, F, 1, 4>, 256, cached_join_kernel<D, 16>);
+    if (x.bm == 16)
+      run(cached_rows_kernel<D, F, 1>, 64 * kRowWaves, cached_join_kernel<D, 16>);
     else if (x.bm == 32)
-      run(cached_rows_kernel<D, F, 2, 4>, 256, cached_join_kernel<D, 32>);
+      run(cached_rows_kernel<D, F, 2>, 64 * kRowWaves, cached_join_kernel<D, 32>);
     else if (x.bm == 48)
-      run(cached_rows_kernel<D, F, 3, 4>, 256, cached_join_kernel<D, 48>);
+      run(cached_rows_kernel<D, F, 3>, 64 * kRowWaves, cached_join_kernel<D, 48>);
     else if (softcap > 0.0f)
       run(cached_tiles_kernel<D, F, true>, kTileThreads, cached_join_kernel<D, kTileRows>);
     else
