@@ -93,6 +93,39 @@ def test_device_tensors_only():
             f()
 
 
+class _On:
+    """A tensor of another device, as far as the check looks at it."""
+
+    is_cuda = True
+
+    def __init__(self, device):
+        self.device = device
+
+    def get_device(self):
+        return self.device
+
+
+def test_tensors_of_other_devices_are_refused(monkeypatch):
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: 0, raising=False)
+    K._check_on_one_device("f", (_On(0), _On(0)), None)
+    for tensors in ((_On(1), _On(1)), (_On(0), _On(1))):
+        with pytest.raises(ValueError, match="device 1"):
+            K._check_on_one_device("f", tensors, None)
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        K._check_on_one_device("f", (_On(0), X), None)
+    stream = type("S", (), {"device": torch.device("cuda", 1)})()
+    K._check_on_one_device("f", (_On(1), _On(1)), stream)
+    with pytest.raises(ValueError, match="device 0, the launch on 1"):
+        K._check_on_one_device("f", (_On(0),), stream)
+
+
+def test_one_cache_for_k_and_v_is_refused():
+    a = _call()
+    a["v_cache"] = a["k_cache"]
+    with pytest.raises(ValueError, match="one memory"):
+        K.kv_cache_write(X, X, **a)
+
+
 POS, FREQS = torch.zeros(5, dtype=torch.int32), torch.ones(32, dtype=torch.float64)
 
 
@@ -144,6 +177,14 @@ def test_library_refuses_bad_caches(change, status):
 def test_library_refuses_bad_calls():
     lib = L.load()
     E = L.TTLH_EINVAL
+    # a workspace that is not there, too small or off its alignment
+    long = _c_cache(width=200, table_ld=200)
+    need = lib.ttlh_sdpa_cached_workspace_bytes(long, 4)
+    assert need > 0
+    for ws, size in ((None, need), (4096, need - 1), (4104, need)):
+        assert lib.ttlh_sdpa_cached(long, 16, 16, 4, 256, 64, 256, 64, 0.1, 0, 0.0, ws, size, None) == E
+    assert b"workspace" in lib.ttlh_last_error()
+    assert lib.ttlh_sdpa_cached_workspace_bytes(_c_cache(), 4) == 0
     assert lib.ttlh_kv_cache_write(None, 16, 16, 0, 128, 64, 128, 64, None) == E
     assert lib.ttlh_kv_cache_write(_c_cache(), 16, 16, 2, 128, 64, 128, 64, None) == E
     assert lib.ttlh_kv_cache_write(_c_cache(), None, 16, 0, 128, 64, 128, 64, None) == E
@@ -154,7 +195,7 @@ def test_library_refuses_bad_calls():
     for bad in (dict(q=None), dict(q=8), dict(o=8), dict(heads=3), dict(heads=0), dict(window=-1),
                 dict(strides=(252, 64, 256, 64)), dict(strides=(256, 64, 256, 4)),
                 dict(scale=math.inf), dict(scale=math.nan), dict(cap=-1.0), dict(cap=math.nan),
-                dict(cap=math.inf)):
+                dict(cap=math.inf), dict(cap=1e-6), dict(cap=1e6), dict(scale=1e31)):
         assert attention(**bad) == E, bad
 
     def rope(x=16, dtype=0, pos=16, pb=4, freqs=16, sizes=(5, 2, 64, 64), scale=1.0):

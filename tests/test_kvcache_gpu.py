@@ -145,7 +145,7 @@ def test_rope_gradient(interleaved):
         assert float((diff - dx[..., i].cpu().double()).abs().max()) <= 32 * 6 * 1.5 * 6 * 2.0 ** -24
 
 
-# --- the cache ----------------------------------------------------------------
+# --- the cache: writes ----------------------------------------------------------------
 
 
 def _cache(pages, heads, page, dim, dtype, seed):
@@ -309,7 +309,15 @@ def test_write_strided_views():
     K.kv_cache_write(d[:, 8:10], d[:, 10:12], *dev, wide.cuda()[:, :2], lens.cuda(), starts.cuda())
     for x, y in zip(dev, ref):
         assert _same(x.cpu(), y)
-    # off every vector's address, heads before tokens
+    # off every vector's address: bf16 one element on, f32 with heads before tokens
+    odd = torch.randn(50, 4 * 128 + 3, generator=g).to(BF16)
+    ref, dev = [c.clone() for c in cache], [c.cuda() for c in cache]
+    kv = odd[:, 1:513].unflatten(1, (4, 128))
+    R.write(kv[:, :2], kv[:, 2:], *ref, table, lens, starts)
+    kv = odd.cuda()[:, 1:513].unflatten(1, (4, 128))
+    K.kv_cache_write(kv[:, :2], kv[:, 2:], *dev, table.cuda(), lens.cuda(), starts.cuda())
+    for a, b in zip(dev, ref):
+        assert _same(a.cpu(), b)
     flat = torch.randn(1 + 2 * 50 * 128, generator=g)
     x = flat[1:].view(2, 50, 128).transpose(0, 1)
     ref, dev = [c.clone() for c in cache], [c.cuda() for c in cache]
@@ -326,7 +334,8 @@ def test_write_strided_views():
 def _tolerance(ref, size, reach, dim, n, softcap):
     off = (dim + 16) * 2.0 ** -24 * reach + 2.0 ** -21 * softcap
     share = 2.0 ** -8 + 2 * off + 2 * (n + 64) * 2.0 ** -24 + 2 * 2.0 ** -21
-    return size * share + 2.0 ** -8 * (ref.abs() + size * share) + 1e-37
+    # (and p v is below fp32's ordinary range where V is below 2^-118)
+    return size * share + 2.0 ** -8 * (ref.abs() + size * share) + 2.0 ** -118
 
 
 def _check_attention(q, cache, table, lengths, starts, scale, window=0, softcap=0.0, o=None):
@@ -514,6 +523,151 @@ def test_empty_calls():
     assert all(_same(a, b) for a, b in zip(cache, before))
 
 
+# --- long sequences, many of them, divided ones -------------------------------
+
+
+def _check_heads(q, cache, table, n, starts, scale, heads, window=0, softcap=0.0):
+    """The whole call; the cache heads `heads` of it against the oracle."""
+    group = q.shape[1] // cache[0].shape[1]
+    out = torch.full_like(q, 7.0).cuda()
+    K.sdpa_cached(q.cuda(), *[c.cuda() for c in cache], table.cuda(), n.cuda(), out, scale,
+                  starts=None if starts is None else starts.cuda(), window=window, softcap=softcap)
+    out = out.cpu()
+    for h in heads:
+        part = [c[:, h:h + 1] for c in cache]
+        qs = slice(h * group, (h + 1) * group)
+        ref, size, reach = R.attention(q[:, qs], *part, table, n, scale, starts, window, softcap)
+        tol = _tolerance(ref, size, reach, q.shape[2], int(n.max()), softcap)
+        got = out[:, qs].double()
+        assert torch.equal(got.isnan(), ref.isnan()), h
+        err = (got - ref).abs().nan_to_num()
+        assert (err <= tol.nan_to_num(1.0)).all(), (h, float((err - tol).max()))
+    return out
+
+
+@pytest.mark.parametrize("cdtype", [INT8, E4M3])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("group,news", [(4, [1, 1, 1]), (9, [2, 3, 1]), (16, [2, 2, 2]), (3, [40, 11, 90])])
+def test_attention_divided_into_parts(cdtype, dim, group, news):
+    """Every tile size with sequences of several parts, of one and of none."""
+    lens = [4001, 90, 1777]
+    q, cache, table, n, starts = _attention_call(lens, news, 2, group, dim, 64, cdtype, 70)
+    _check_attention(q, cache, table, n, starts, dim ** -0.5)
+    _check_attention(q, cache, table, n, starts, dim ** -0.5, window=1500, softcap=20.0)
+
+
+@pytest.mark.parametrize("page", [16, 64, 128])
+@pytest.mark.parametrize("dim,cdtype", [(64, INT8), (128, E4M3)])
+@pytest.mark.parametrize("softcap", [0.0, 10.0])
+def test_attention_long_undivided_tiles(page, dim, cdtype, softcap):
+    """Tiles that walk more than 2 x 16 blocks, some pages missing and some NaN where
+    the sixteens meet."""
+    q, cache, table, n, starts = _attention_call([2300, 1100], [260, 130], 128, 2, dim, page, cdtype, 71)
+    _check_heads(q, cache, table, n, starts, dim ** -0.5, (0, 127), softcap=softcap)
+    table[0, 1024 // page] = -1
+    table[0, 2047 // page] = 10 ** 7
+    cache[2][table[1, 1023 // page], 0] = math.nan
+    out = _check_heads(q, cache, table, n, starts, dim ** -0.5, (0, 127), softcap=softcap)
+    # (of head 0's, those from the bad page's first position on)
+    sees = torch.arange(970, 1100) >= 1023 // page * page
+    assert torch.equal(out[260:, :2].isnan().all(-1).all(-1), sees)
+    assert not out[260:, 2:].isnan().any()
+
+
+def test_attention_rows_of_more_than_4096_positions():
+    """One part of a wave's more than 32 steps."""
+    q, cache, table, n, _ = _attention_call([17000], [1], 256, 1, 64, 128, INT8, 72, True)
+    _check_heads(q, cache, table, n, None, 0.125, (0, 100, 255))
+
+
+@pytest.mark.parametrize("one", [True, False])
+@pytest.mark.parametrize("group", [2, 30])
+def test_attention_of_150_sequences(one, group):
+    g = _gen(73)
+    lens = [int(x) for x in torch.randint(1, 90, (150,), generator=g)]
+    lens[3], lens[80], lens[149] = 2000, 1300, 700
+    news = [1] * 150 if one else [min(n, int(x)) for n, x in zip(lens, torch.randint(0, 4, (150,), generator=g))]
+    q, cache, table, n, starts = _attention_call(lens, news, 1, group, 64, 32, INT8, 74, one)
+    _check_attention(q, cache, table, n, starts, 0.125)
+
+
+def test_write_of_150_sequences():
+    lens = [1 + (37 * b) % 150 for b in range(150)]
+    news = [min(n, b % 5) for b, n in enumerate(lens)]
+    call = _random_call(lens, news, 2, 64, 16, BF16, INT8, 75)
+    _run_write(*call)
+
+
+@pytest.mark.parametrize("news", [[1, 1], [130, 55]])
+@pytest.mark.parametrize("cdtype", [INT8, E4M3])
+def test_attention_extreme_scales(news, cdtype):
+    """V scales down to those of pages of zeros and up to 2^80, K scales of zero and
+    2^-126; a negative scale is NaN."""
+    q, cache, table, n, starts = _attention_call([300, 55], news, 2, 4, 64, 16, cdtype, 76)
+    ks, vs = cache[2], cache[3]
+    vs[table[0, 1], 0], vs[table[0, 2], 0], vs[table[0, 3], 1] = 2.0 ** -126, 2.0 ** -100, 2.0 ** 80
+    vs[table[1, 0], 1], vs[table[1, 1], 1], vs[table[1, 2], 1] = 2.0 ** -90, 2.0 ** -80, 2.0 ** -85
+    ks[table[0, 4], 0], ks[table[0, 5], 0] = 0.0, 2.0 ** -126
+    _check_attention(q, cache, table, n, starts, 0.125)
+    zero = vs.clone()
+    zero[table[0, 6]] = 0.0
+    _check_attention(q, [*cache[:3], zero], table, n, starts, 0.125)
+    for i in (2, 3):
+        bad = [c.clone() for c in cache]
+        bad[i][table[0, 4], 1] = -1.0
+        o = torch.empty_like(q, device="cuda")
+        K.sdpa_cached(q.cuda(), *[c.cuda() for c in bad], table.cuda(), n.cuda(), o, 0.125,
+                      starts=starts.cuda())
+        pos = [n[0] - news[0] + i for i in range(news[0])]
+        sees = torch.tensor([p >= 64 for p in pos])
+        assert torch.equal(o[:news[0], 4:].isnan().all(-1).all(-1).cpu(), sees)
+        assert not o[:, :4].isnan().any() and not o[news[0]:].isnan().any()
+
+
+@pytest.mark.parametrize("news", [[1, 1], [130, 55]])
+def test_attention_into_its_queries(news):
+    q, cache, table, n, starts = _attention_call([900, 555], news, 2, 4, 128, 32, INT8, 77)
+    dev = [c.cuda() for c in cache]
+    o, x = torch.empty_like(q, device="cuda"), q.cuda()
+    K.sdpa_cached(x, *dev, table.cuda(), n.cuda(), o, 0.09, starts=starts.cuda())
+    K.sdpa_cached(x, *dev, table.cuda(), n.cuda(), x, 0.09, starts=starts.cuda())
+    assert torch.equal(o, x)
+
+
+def test_caches_past_32_bits():
+    """Codes more than 4 GiB into a cache."""
+    heads, page, dim = 8, 128, 128
+    pages = (5 << 30) // (heads * page * dim)
+    k, v = (torch.zeros(pages, heads, page, dim, dtype=INT8, device="cuda") for _ in range(2))
+    ks, vs = (torch.zeros(pages, heads, device="cuda") for _ in range(2))
+    table = torch.tensor([[pages - 1, 3], [pages - 2, pages - 3]], dtype=torch.int32)
+    lens, starts = torch.tensor([200, 250], dtype=torch.int32), torch.tensor([0, 200, 450], dtype=torch.int32)
+    g = _gen(78)
+    x = [torch.randn(450, heads, dim, generator=g).to(BF16) for _ in range(2)]
+    K.kv_cache_write(x[0].cuda(), x[1].cuda(), k, v, ks, vs, table.cuda(), lens.cuda(), starts.cuda())
+    at = [3, pages - 3, pages - 2, pages - 1]
+    small = [c[at].cpu() for c in (k, v, ks, vs)]
+    local = torch.tensor([[3, 0], [2, 1]], dtype=torch.int32)
+    ref = [torch.zeros_like(c) for c in small]
+    R.write(*x, *ref, local, lens, starts)
+    assert all(_same(a, b) for a, b in zip(small, ref))
+    for news in ([1, 1], [60, 50]):
+        st = torch.tensor([0, news[0], sum(news)], dtype=torch.int32)
+        q = torch.randn(sum(news), heads, dim, generator=g).to(BF16)
+        o = torch.empty_like(q, device="cuda")
+        K.sdpa_cached(q.cuda(), k, v, ks, vs, table.cuda(), lens.cuda(), o, 0.09, starts=st.cuda())
+        out, size, reach = R.attention(q, *ref, local, lens, 0.09, st)
+        assert ((o.cpu().double() - out).abs() <= _tolerance(out, size, reach, dim, 250, 0.0)).all()
+
+
+def test_long_and_short_sequences_in_one_call():
+    """A prompt of many tiles beside single tokens far into their sequences: the tiles fill
+    the chip, the long sequences are divided all the same."""
+    lens, news = [700, 9000, 400, 5000], [700, 1, 1, 1]
+    q, cache, table, n, starts = _attention_call(lens, news, 64, 2, 64, 64, INT8, 79)
+    _check_heads(q, cache, table, n, starts, 0.125, (0, 63))
+
+
 # --- together -----------------------------------------------------------------
 
 
@@ -609,8 +763,48 @@ def test_captured_steps_follow_the_lengths():
     assert all(_same(a, b) for a, b in zip(cache, want_cache))
 
 
+@pytest.mark.parametrize("tokens", [1, 40])
+def test_captured_parts_grow_with_the_lengths(tokens):
+    """Divided attention in two graphs, each with its own workspace, replayed in turns while
+    eager calls with other, larger workspaces run between: as many parts as the
+    lengths of each replay ask for, and the eager call's bits."""
+    seqs, width = 3, 130
+    q, cache, table, n, starts = _attention_call([2000, 1000, 400], [tokens] * seqs, 2, 4, 64, 16, INT8, 80)
+    table = torch.cat((table, table[:, :width - table.shape[1]]), 1) if table.shape[1] < width else table
+    dev, table, n = [c.cuda() for c in cache], table.cuda(), n.cuda()
+    starts = None if tokens == 1 else starts.cuda()
+    qs = [q.cuda(), q.flip(0).contiguous().cuda()]
+    lens = torch.full((seqs,), 60, dtype=torch.int32, device="cuda")
+    outs = [torch.empty_like(x) for x in qs]
+    big, bcache, btable, bn, bstarts = _attention_call([3000, 900], [90, 70], 2, 8, 128, 64, INT8, 81)
+    bdev = [big.cuda(), *[c.cuda() for c in bcache], btable.cuda(), bn.cuda()]
+
+    def eager(i, n):
+        o = torch.empty_like(qs[i])
+        K.sdpa_cached(qs[i], *dev, table, n, o, 0.125, starts=starts)
+        return o
+
+    eager(0, lens)
+    graphs = []
+    for i in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            K.sdpa_cached(qs[i], *dev, table, lens, outs[i], 0.125, starts=starts)
+        graphs.append(graph)
+    for j in range(8):
+        now = (n * (j + 1) // 8).clamp(min=tokens)
+        lens.copy_(now)
+        graphs[0].replay()
+        graphs[1].replay()
+        o = torch.empty_like(bdev[0])
+        K.sdpa_cached(*bdev, o, 0.09, starts=bstarts.cuda())
+        for i in range(2):
+            assert torch.equal(outs[i], eager(i, now)), (j, i)
+        torch.cuda.synchronize()
+
+
 def test_two_streams_at_once():
-    calls = [_attention_call([400, 333, 90], [1, 1, 1], 2, 4, 128, 32, INT8, 50 + i, True)
+    calls = [_attention_call([4000, 1333, 90], [1, 1, 1], 2, 4, 128, 32, INT8, 50 + i, True)
              for i in range(2)]
     dev = [[q.cuda(), [c.cuda() for c in cache], t.cuda(), n.cuda()] for q, cache, t, n, _ in calls]
     want = []

@@ -114,7 +114,7 @@ struct Division {
   }
   // Tile `item` of all, those that see the most positions first (by 64 of them): with
   // prompts of several lengths the last workgroups to start are then the shortest.
-  // For undivided tiles of up to 64 sequences, without a window.
+  // For up to 64 sequences, none divided, without a window.
   __device__ __forceinline__ bool find_longest(int item, Plan& w) {
     const int lane = threadIdx.x & 63;
     int first = 0, n = 0, len = 0;
@@ -153,7 +153,8 @@ struct Division {
     w.parts = 1;
     return w.row0 >= 0 && w.row0 < w.rows;
   }
-  // item `item` of the parts (JOIN: of the tiles), or false past the last one
+  // item `item` of the parts (JOIN: of the tiles of several parts), or false past the
+  // last one
   template <bool JOIN>
   __device__ __forceinline__ bool find(int item, Plan& w) {
     const int lane = threadIdx.x & 63;
@@ -161,7 +162,8 @@ struct Division {
     for (int b0 = 0; b0 < p.c.seqs; b0 += 64) {
       if (p.c.seqs > 64) extent(b0 + lane);
       const int parts = range > chunk ? (range - 1) / chunk + 1 : 1;
-      const int mine = JOIN ? tiles : tiles * parts, mine_slots = parts > 1 ? tiles * parts : 0;
+      const int mine_slots = parts > 1 ? tiles * parts : 0;
+      const int mine = !JOIN ? tiles * parts : parts > 1 ? tiles : 0;
       const int end = prefix_sum(mine), send = prefix_sum(mine_slots);
       const unsigned long long past = __ballot(items + end > item);
       if (past) {
@@ -1073,7 +1075,8 @@ __global__ __launch_bounds__(kTileThreads, D == 64 && !CAP ? 3 : 2) void cached_
   div.divide();
   Plan w;
   const int item = blockIdx.x / p.c.heads;
-  const bool sorted = p.target == 0 && p.window == 0 && p.c.seqs > 1 && p.c.seqs <= 64;
+  const bool sorted = p.window == 0 && p.c.seqs > 1 && p.c.seqs <= 64 &&
+                      !__any(div.range > div.chunk);
   if (!(sorted ? div.find_longest(item, w) : div.template find<false>(item, w))) return;
   const Span s = span_of<kTileRows, kBlock>(p, w);
   Tiles<D, FMT, CAP> x{p, w, s, KV[0], KV[1]};
@@ -1173,9 +1176,10 @@ __global__ __launch_bounds__(kTileThreads, D == 64 && !CAP ? 3 : 2) void cached_
                 cvt_pk_bf16x2(x.o[j][4 * u + 2] * inv, x.o[j][4 * u + 3] * inv)};
 }
 
-// The parts of a tile: the rows of a workgroup (blockIdx.y counts them) by four
-// waves, wave v taking parts v, v + 4, .., and the waves' results in their order:
-// the same sum whenever the parts are the same.  A lane has four elements of a row.
+// The parts of a tile, kRows rows at a time (blockIdx.y has every gridDim.y-th of them)
+// by four waves, wave v taking parts v, v + 4, .., and the waves' results in their
+// order: the same sum whenever the parts are the same.  A lane has four elements of
+// a row.
 template <int D, int BM>
 __global__ __launch_bounds__(256) void cached_join_kernel(const CachedArgs p) {
   constexpr int kRows = 256 / D;  // 64 lanes, D / 4 a row
@@ -1184,66 +1188,70 @@ __global__ __launch_bounds__(256) void cached_join_kernel(const CachedArgs p) {
   Division<BM> div{p};
   div.divide();
   Plan w;
-  if (!div.template find<true>(blockIdx.x / p.c.heads, w) || w.parts == 1) return;
+  if (!div.template find<true>(blockIdx.x / p.c.heads, w)) return;
   const int h = blockIdx.x % p.c.heads, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int row = blockIdx.y * kRows + lane / (D / 4), d = (lane % (D / 4)) * 4;
-  if (w.row0 + static_cast<int>(blockIdx.y) * kRows >= w.rows) return;  // (uniform)
-  const bool mine = w.row0 + row < w.rows;
-  const int64_t step = static_cast<int64_t>(p.c.heads) * BM;
-  const int64_t at = (static_cast<int64_t>(w.slot) * p.c.heads + h) * BM + (mine ? row : 0);
-  float m = -INFINITY, l = 0.0f;
-  f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
-  constexpr int kAhead = 4;
-  for (int i0 = wave; i0 < w.parts; i0 += 4 * kAhead) {
-    float pm[kAhead], pl[kAhead];
-    f32x4 po[kAhead];
+  const int rows = min(BM, w.rows - w.row0);
+  for (int r0 = blockIdx.y * kRows; r0 < rows; r0 += gridDim.y * kRows) {
+    const int row = r0 + lane / (D / 4), d = (lane % (D / 4)) * 4;
+    const bool mine = row < rows;
+    const int64_t step = static_cast<int64_t>(p.c.heads) * BM;
+    const int64_t at = (static_cast<int64_t>(w.slot) * p.c.heads + h) * BM + (mine ? row : 0);
+    float m = -INFINITY, l = 0.0f;
+    f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+    constexpr int kAhead = 4;
+    for (int i0 = wave; i0 < w.parts; i0 += 4 * kAhead) {
+      float pm[kAhead], pl[kAhead];
+      f32x4 po[kAhead];
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i) {
-      const bool there = i0 + 4 * i < w.parts;
-      const int64_t r = at + (there ? i0 + 4 * i : i0) * step;
-      pm[i] = there ? p.part_ml[r * 2] : -INFINITY;
-      pl[i] = p.part_ml[r * 2 + 1];
-      po[i] = *reinterpret_cast<const f32x4*>(p.part_o + r * D + d);
-    }
-    float to = m;
-#pragma unroll
-    for (int i = 0; i < kAhead; ++i) to = fmaxf(to, pm[i]);
-    const float mm = to == -INFINITY ? 0.0f : to, f = __builtin_amdgcn_exp2f(m - mm);
-    l *= f;
-    acc *= f;
-#pragma unroll
-    for (int i = 0; i < kAhead; ++i) {
-      const float e = __builtin_amdgcn_exp2f(pm[i] - mm);
-      if (i0 + 4 * i < w.parts) {
-        l += pl[i] * e;
-        acc += po[i] * e;
+      for (int i = 0; i < kAhead; ++i) {
+        const bool there = i0 + 4 * i < w.parts;
+        const int64_t r = at + (there ? i0 + 4 * i : i0) * step;
+        pm[i] = there ? p.part_ml[r * 2] : -INFINITY;
+        pl[i] = p.part_ml[r * 2 + 1];
+        po[i] = *reinterpret_cast<const f32x4*>(p.part_o + r * D + d);
       }
+      float to = m;
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) to = fmaxf(to, pm[i]);
+      const float mm = to == -INFINITY ? 0.0f : to, f = __builtin_amdgcn_exp2f(m - mm);
+      l *= f;
+      acc *= f;
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        const float e = __builtin_amdgcn_exp2f(pm[i] - mm);
+        if (i0 + 4 * i < w.parts) {
+          l += pl[i] * e;
+          acc += po[i] * e;
+        }
+      }
+      m = to;
     }
-    m = to;
-  }
-  m_s[wave][lane] = m;
-  l_s[wave][lane] = l;
-  acc_s[wave][lane] = acc;
-  __syncthreads();
-  if (wave != 0 || !mine) return;
-  float mt = -INFINITY;
+    m_s[wave][lane] = m;
+    l_s[wave][lane] = l;
+    acc_s[wave][lane] = acc;
+    __syncthreads();
+    if (wave == 0 && mine) {
+      float mt = -INFINITY;
 #pragma unroll
-  for (int v = 0; v < 4; ++v) mt = fmaxf(mt, m_s[v][lane]);
-  const float mm = mt == -INFINITY ? 0.0f : mt;
-  float lt = 0.0f;
-  acc = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      for (int v = 0; v < 4; ++v) mt = fmaxf(mt, m_s[v][lane]);
+      const float mm = mt == -INFINITY ? 0.0f : mt;
+      float lt = 0.0f;
+      acc = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-  for (int v = 0; v < 4; ++v) {
-    const float f = __builtin_amdgcn_exp2f(m_s[v][lane] - mm);
-    lt += l_s[v][lane] * f;
-    acc += acc_s[v][lane] * f;
+      for (int v = 0; v < 4; ++v) {
+        const float f = __builtin_amdgcn_exp2f(m_s[v][lane] - mm);
+        lt += l_s[v][lane] * f;
+        acc += acc_s[v][lane] * f;
+      }
+      const int i = (w.row0 + row) / p.group;
+      const float inv = lt == 0.0f ? 0.0f : 1.0f / lt;
+      uint16_t* op = p.o + static_cast<int64_t>(w.first + i) * p.o_token +
+                     static_cast<int64_t>(h * p.group + w.row0 + row - i * p.group) * p.o_head + d;
+      *reinterpret_cast<u32x2*>(op) = u32x2{cvt_pk_bf16x2(acc[0] * inv, acc[1] * inv),
+                                            cvt_pk_bf16x2(acc[2] * inv, acc[3] * inv)};
+    }
+    __syncthreads();  // the next rows' results go over these
   }
-  const int i = (w.row0 + row) / p.group;
-  const float inv = lt == 0.0f ? 0.0f : 1.0f / lt;
-  uint16_t* op = p.o + static_cast<int64_t>(w.first + i) * p.o_token +
-                 static_cast<int64_t>(h * p.group + w.row0 + row - i * p.group) * p.o_head + d;
-  *reinterpret_cast<u32x2*>(op) = u32x2{cvt_pk_bf16x2(acc[0] * inv, acc[1] * inv),
-                                        cvt_pk_bf16x2(acc[2] * inv, acc[3] * inv)};
 }
 
 // ---- the choice --------------------------------------------------------------
@@ -1267,15 +1275,13 @@ Choice choose(const ttlh_kv_cache* c, int64_t q_heads, int64_t window) {
   // with twice as many parts 74, with a few too many 79; drafts 82, 97, 105).  A part's
   // start and end cost about as much as 512 positions; where there are two workgroups
   // for each CU undivided, parts of fewer than 2048 do not pay (768 tiles of 1024
-  // positions: 25 us, halved 31).
-  const int64_t places =
-      256 * (x.bm == kTileRows ? 2 : rows_per_cu(c->dim, x.bm / 16));
-  x.least = certain >= 512 ? 2048 : 512;
+  // positions: 25 us, halved 31), and where the tiles fill all places only those of
+  // much longer sequences than the others are divided.
+  const int64_t places = 256 * (x.bm == kTileRows ? 2 : rows_per_cu(c->dim, x.bm / 16));
+  x.least = certain >= places ? 4096 : certain >= 512 ? 2048 : 512;
   const int64_t most = c->width * c->page;  // positions that a sequence's tokens see
   const int64_t positions = window > 0 && window + c->tokens < most ? window + c->tokens : most;
-  x.target = certain >= places || positions <= x.least
-                 ? 0
-                 : static_cast<int32_t>((places + c->heads - 1) / c->heads);
+  x.target = positions <= x.least ? 0 : static_cast<int32_t>((places + c->heads - 1) / c->heads);
   return x;
 }
 
@@ -1342,11 +1348,12 @@ extern "C" int ttlh_sdpa_cached(const ttlh_kv_cache* cache, const void* Q, void*
   const int64_t items = (x.tiles + x.target) * cache->heads;
   TTLH_REQUIRE(items < (int64_t(1) << 31), TTLH_EUNSUPPORTED, "ttlh_sdpa_cached: too many tiles");
   const dim3 grid(static_cast<uint32_t>(items));
-  // (rows of a tile: without starts no more than the group)
+  // (at most target tiles of several parts; rows of a tile: without starts no more than
+  // the group)
   const int64_t rows = !cache->starts && a.group < x.bm ? a.group : x.bm;
-  const int per = 256 / cache->dim;
-  const dim3 joins(static_cast<uint32_t>(x.tiles * cache->heads),
-                   static_cast<uint32_t>((rows + per - 1) / per));
+  const int64_t rounds = (rows * cache->dim + 255) / 256;
+  const dim3 joins(static_cast<uint32_t>(x.target * cache->heads),
+                   static_cast<uint32_t>(rounds < 16 ? rounds : 16));
   hipStream_t s = static_cast<hipStream_t>(stream);
   const auto run = [&](auto kernel, int threads, auto join) {
     hipLaunchKernelGGL(kernel, grid, dim3(threads), 0, s, a);

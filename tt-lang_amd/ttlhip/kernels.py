@@ -920,6 +920,8 @@ def kv_cache_write(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_ca
                               lengths, starts)
     if heads != ch or dim != cd:
         raise ValueError(f"kv_cache_write: tokens of {(heads, dim)}, a cache of {(ch, cd)} (heads, dim)")
+    if k_cache.data_ptr() == v_cache.data_ptr() and tokens:
+        raise ValueError("kv_cache_write: k_cache and v_cache are one memory")
     code = L.dtype_code(k.dtype)
     tensors = (k, v, k_cache, v_cache, k_scale, v_scale, table, lengths)
     _check_on_one_device("kv_cache_write", tensors if starts is None else tensors + (starts,), stream)
@@ -935,12 +937,14 @@ def sdpa_cached(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
     """Attention of new tokens over the cache that kv_cache_write() filled (the
     new tokens' own keys among them): o = softmax(cap(scale q k^T)) v, a token at
     position p seeing the positions up to p, or the last `window` of them.
-    softcap: cap(x) = softcap tanh(x / softcap), from 2^-16 to 2^16 (0: x).  q, o: bf16 [tokens,
-    q heads, dim], any strides for tokens and heads that are multiples of 8; q heads
-    share the cache's heads in equal groups.  Positions that the table does not
-    name are not seen; a token that sees nothing gets zeros, one that sees a page
-    with a negative or non-finite scale NaN.  Rows of o behind the
-    last sequence's tokens stay as they are."""
+    softcap: cap(x) = softcap tanh(x / softcap), from 2^-16 to 2^16 (0: x).
+
+    q, o: bf16 [tokens, q heads, dim], any strides for tokens and heads that are
+    multiples of 8; o may be q.  q heads share the cache's heads in equal groups; the
+    other arguments are those of kv_cache_write().  Positions that the table does not
+    name are not seen.  A token that sees nothing gets zeros, one that sees a page
+    with a negative or non-finite scale NaN.  Rows of o behind the last sequence's
+    tokens stay as they are."""
     shape, qt, qh = _heads("sdpa_cached", "q", q)
     _, ot, oh = _heads("sdpa_cached", "o", o, shape)
     if q.dtype != torch.bfloat16 or o.dtype != torch.bfloat16:
