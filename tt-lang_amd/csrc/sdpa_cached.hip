@@ -77,16 +77,17 @@ template <int BM>
 struct Division {
   const CachedArgs& p;
   int chunk;
-  int tiles, range;  // of sequence threadIdx.x % 64, where there are no more than 64
+  // Of sequence threadIdx.x % 64, where there are no more than 64: its new tokens and
+  // positions, its tiles, the positions that its rows see between them.
+  int first, n, len, tiles, range;
 
-  // tiles of sequence b, and the positions that its rows see between them
   __device__ __forceinline__ void extent(int b) {
-    tiles = range = 0;
+    first = n = len = tiles = range = 0;
     if (b >= p.c.seqs) return;
-    int first, n, lo, hi, x;
     seq_tokens(p.c, b, first, n);
+    len = p.c.lengths[b];
     if (n == 0) return;
-    const int len = p.c.lengths[b];
+    int lo, hi, x;
     tiles = (n * p.group + BM - 1) / BM;
     seen_by(p.c, len, n, 0, p.window, lo, x);
     seen_by(p.c, len, n, n - 1, p.window, x, hi);
@@ -116,12 +117,6 @@ struct Division {
   // prompts of several lengths the last workgroups to start are then the shortest.
   // For up to 64 sequences, none divided, without a window.
   __device__ __forceinline__ bool find_longest(int item, Plan& w) {
-    const int lane = threadIdx.x & 63;
-    int first = 0, n = 0, len = 0;
-    if (lane < p.c.seqs) {
-      seq_tokens(p.c, lane, first, n);
-      len = p.c.lengths[lane];
-    }
     // tiles whose last row sees at least 64 level positions
     const auto count = [&](int level) {
       if (level == 0) return tiles;
@@ -176,11 +171,12 @@ struct Division {
         const int before = JOIN ? local : local / w.parts, tile = nt - 1 - before;
         w.part = JOIN ? 0 : local - before * w.parts;
         w.slot = slots + at(send) - at(mine_slots) + before * w.parts;
-        seq_tokens(p.c, w.b, w.first, w.n);
-        w.len = p.c.lengths[w.b];
+        w.first = at(first);
+        w.n = at(n);
+        w.len = at(len);
         w.row0 = tile * BM;
         w.rows = w.n * p.group;
-        // (always, unless starts overlap, or they or lengths change under the call)
+        // (always, unless starts overlap)
         return (w.parts == 1 || (w.slot >= 0 && w.slot + w.parts <= 2 * p.target)) &&
                w.row0 >= 0 && w.row0 < w.rows;
       }
@@ -1348,12 +1344,12 @@ extern "C" int ttlh_sdpa_cached(const ttlh_kv_cache* cache, const void* Q, void*
   const int64_t items = (x.tiles + x.target) * cache->heads;
   TTLH_REQUIRE(items < (int64_t(1) << 31), TTLH_EUNSUPPORTED, "ttlh_sdpa_cached: too many tiles");
   const dim3 grid(static_cast<uint32_t>(items));
-  // (at most target tiles of several parts; rows of a tile: without starts no more than
-  // the group)
+  // (at most target tiles have several parts; rows of a tile: without starts no more
+  // than the group.  Most workgroups of the join find nothing to do: few of them.)
   const int64_t rows = !cache->starts && a.group < x.bm ? a.group : x.bm;
   const int64_t rounds = (rows * cache->dim + 255) / 256;
-  const dim3 joins(static_cast<uint32_t>(x.target * cache->heads),
-                   static_cast<uint32_t>(rounds < 16 ? rounds : 16));
+  const dim3 joins(static_cast<uint32_t>((x.tiles < x.target ? x.tiles : x.target) * cache->heads),
+                   static_cast<uint32_t>(rounds < 8 ? rounds : 8));
   hipStream_t s = static_cast<hipStream_t>(stream);
   const auto run = [&](auto kernel, int threads, auto join) {
     hipLaunchKernelGGL(kernel, grid, dim3(threads), 0, s, a);
