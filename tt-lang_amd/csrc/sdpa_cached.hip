@@ -13,9 +13,14 @@
 //
 //  * cached_rows_kernel: up to 16 MT rows in a tile (answers token by token, drafts):
 //    HBM bound.  Four waves take turns at 32 positions and meet in LDS at the end;
-//    codes go from memory to registers, no LDS on the way.
-//  * cached_tiles_kernel: tiles of 128 rows (prompts): MFMA bound.  Blocks of 64
-//    positions are decoded once into LDS for four waves of 32 rows.
+//    codes go from memory to registers, no LDS on the way.  One new token each, 8 x 128
+//    heads, joined: 16 sequences of up to 65537 positions 239 us (5.7 TB/s), 32 of up
+//    to 8192 72 us (4.8 TB/s), one of 501 9.4 us (the latency of its dependent reads).
+//  * cached_tiles_kernel: tiles of 128 rows (prompts): bound by the vector ALU, which
+//    works for the softmax and the decoding between MFMAs.  Blocks of 64 positions
+//    are decoded once into LDS for four waves of 32 rows.  2048 new tokens at 18000,
+//    32 / 8 heads of 128: 612 us, 930 TFLOP/s; four prompts of up to 2049 tokens, 32 / 8
+//    heads of 64 and capped scores (two more transcendentals for each): 101 us.
 //
 // Few tiles with many positions are divided into parts (see Plan), whose results
 // meet in cached_join_kernel in the order of the parts.
@@ -52,6 +57,7 @@ struct CachedArgs {
   int32_t window;     // 0: none
   int32_t target;     // parts of all sequences together, for one head, about; 0: undivided
   int32_t least;      // positions of a part, at least
+  int32_t turns;      // 1: the workgroups with tiles are few enough to run at once
   float scale_log2;   // |scale| log2 e, or 2 |scale| log2 e / softcap
   uint32_t flip;      // sign bits of two bf16, if the scale is negative: Q's change
   float cap_log2;     // softcap log2 e, or 0
@@ -1133,9 +1139,9 @@ __global__ __launch_bounds__(kTileThreads, D == 64 && !CAP ? 3 : 2) void cached_
     if ((kb & 15) == 14) x.load_unit = x.next.unit;
     // Of two waves on a SIMD the older one goes first all the time, and where all
     // workgroups run at once its CU is half empty when it has ended: so the two (as far
-    // as their numbers tell them) go first in turns (612 -> 595 us for 512 workgroups).
+    // as their numbers tell them) go first in turns (628 -> 612 us for 512 workgroups).
     // Where others wait for a place, the older ones are the longer ones.
-    if (gridDim.x <= 768) {
+    if (p.turns) {
       if (((blockIdx.x >> 8) ^ (kb >> 1)) & 1)
         __builtin_amdgcn_s_setprio(1);
       else
@@ -1268,7 +1274,7 @@ Choice choose(const ttlh_kv_cache* c, int64_t q_heads, int64_t window) {
   x.tiles = (c->starts ? rows / x.bm + c->seqs : c->seqs * ((group + x.bm - 1) / x.bm));
   const int64_t certain = (c->starts ? rows / x.bm : x.tiles) * c->heads;
   // As many parts as the chip has places (32 answers of up to 8192 positions 72 us;
-  // with twice as many parts 74, with a few too many 79; drafts 82, 97, 105).  A part's
+  // with half as many 83, a tenth more 78, twice as many 72; 16 drafts 80, 99, 103, 86).  A part's
   // start and end cost about as much as 512 positions; where there are two workgroups
   // for each CU undivided, parts of fewer than 2048 do not pay (768 tiles of 1024
   // positions: 25 us, halved 31), and where the tiles fill all places only those of
@@ -1336,6 +1342,7 @@ extern "C" int ttlh_sdpa_cached(const ttlh_kv_cache* cache, const void* Q, void*
   a.window = static_cast<int32_t>(window < (int64_t(1) << 31) ? window : 0);
   a.target = x.target;
   a.least = x.least;
+  a.turns = x.tiles * cache->heads <= 768;
   a.scale_log2 = std::fabs(softcap > 0.0f ? scale / softcap * 2.0f * kLog2e : scale * kLog2e);
   a.flip = scale < 0.0f ? 0x80008000u : 0u;
   a.cap_log2 = softcap * kLog2e;
