@@ -556,6 +556,17 @@ def test_attention_divided_into_parts(cdtype, dim, group, news):
     _check_attention(q, cache, table, n, starts, dim ** -0.5, window=1500, softcap=20.0)
 
 
+@pytest.mark.parametrize("dim,cdtype", [(64, E4M3), (128, INT8)])
+@pytest.mark.parametrize("group,news", [(2, [1] * 6), (8, [20, 9, 1, 3, 0, 2]), (8, [40, 24, 9]),
+                                        (8, [100, 60, 9, 0, 0, 70])])
+def test_attention_parts_that_fill_the_chip(dim, cdtype, group, news):
+    """More parts than places, were they as short as parts may be: their lengths come from
+    all sequences', for few tiles, for half as many as there are places, and for more."""
+    lens = [9000, 5000, 1503, 700, 0, 4100][:len(news)]
+    q, cache, table, n, starts = _attention_call(lens, news, 64, group, dim, 64, cdtype, 77)
+    _check_heads(q, cache, table, n, starts, dim ** -0.5, (0, 63))
+
+
 @pytest.mark.parametrize("page", [16, 64, 128])
 @pytest.mark.parametrize("dim,cdtype", [(64, INT8), (128, E4M3)])
 @pytest.mark.parametrize("softcap", [0.0, 10.0])

@@ -63,15 +63,17 @@ struct CachedArgs {
   float cap_log2;     // softcap log2 e, or 0
   float* part_o;      // [slot, head, rows of a tile, dim]
   float* part_ml;     // [slot, head, rows of a tile, 2]: maximum and sum
+  int32_t* chunk;     // Division::chunk, for the join
 };
 
 // ---- which part of which tile of which sequence a workgroup has --------------
 //
 // Lengths are on the device, so the division is made there, by every workgroup for
 // itself, from one pass over the sequences: with W the positions of all tiles
-// together, a part has `chunk` = W / (target - tiles / 2) positions (at least `least`),
-// so the parts are alike whatever the lengths are, and there are about as many as
-// the chip has places.  There are at most (tiles + target) parts, and at most 2 target
+// together, a part has the fewest positions (at least `least`) with which there are no
+// more than `target` parts, as many as the chip has places (for more than 64 sequences,
+// or more tiles than that, W / (target - tiles / 2)), so the parts are alike whatever
+// the lengths are.  There are at most (tiles + target) parts, and at most 2 target
 // of them belong to tiles of several parts, which have `slots` for their results.
 struct Plan {
   int b, first, n, len;      // the sequence, its new tokens and positions
@@ -111,12 +113,54 @@ struct Division {
       sum += static_cast<float>(tiles) * range;
       all += tiles;
     }
+    // (for up to 64 sequences: the parts of `least` positions)
+    const float least = p.least;
+    const float few = wave_total(tiles * fmaxf(ceilf(range * __builtin_amdgcn_rcpf(least)), 1.0f));
     all = wave_total(all);
-    // (a tile's last part is half a part too many on average: so many places are left)
-    const float parts = fmaxf(p.target - 0.5f * all, 0.5f * p.target);
-    const float each = fminf(wave_total(sum) / parts, 1073741824.0f);
-    chunk = max((static_cast<int>(each) + 64) & ~63, p.least);
+    sum = wave_total(sum);
+    float each;
+    if (p.c.seqs > 64 || all > p.target) {
+      // (a tile's last part is half a part too many on average: so many places are left)
+      each = sum / fmaxf(p.target - 0.5f * all, 0.5f * p.target);
+    } else {
+      each = few <= p.target ? least : fill(sum, all, p.target);
+      // Tiles of 128 rows have two workgroups on a CU, which take 1.7 times as long
+      // then: where twice the parts are not that much shorter, one each.
+      if (BM == 128 && 2 * all <= p.target && 2 * few > p.target) {
+        const float alone = fill(sum, all, 0.5f * p.target);
+        if (alone < 1.7f * each) each = alone;
+      }
+    }
+    chunk = max((static_cast<int>(fminf(each, 1073741824.0f)) + 63) & ~63, p.least);
     chunk = __builtin_amdgcn_readfirstlane(chunk);
+    if (blockIdx.x == 0 && threadIdx.x == 0) *p.chunk = chunk;
+    if (p.c.seqs > 64) tiles = range = 0;
+  }
+  // The positions of a part: with W = sum positions in `all` tiles, W / (target - all x)
+  // for the first x of these with which there are no more than `target` parts (1 has
+  // no more: a tile's last part is less than one part too many).  (The totals are
+  // independent, so that their latencies overlap: searched one after the other, the
+  // start of each workgroup took 0.5 us longer.)
+  __device__ __forceinline__ float fill(float sum, float all, float target) const {
+    const float w = __builtin_amdgcn_rcpf(fmaxf(sum, 1.0f));
+    float inv[3], parts[3];
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+      inv[i] = (target - 0.25f * (i + 1) * all) * w;
+      parts[i] = tiles * fmaxf(ceilf(range * inv[i] - 0x1p-10f), 1.0f);
+    }
+#pragma unroll
+    for (int i = 0; i < 3; ++i) parts[i] = wave_total(parts[i]);
+    float best = (target - all) * w;
+#pragma unroll
+    for (int i = 2; i >= 0; --i)
+      if (parts[i] <= target) best = inv[i];
+    return __builtin_amdgcn_rcpf(fmaxf(best, 0x1p-30f));
+  }
+  // the same division again (JOIN)
+  __device__ __forceinline__ void divided(int chunk_) {
+    extent(threadIdx.x & 63);
+    chunk = chunk_;
     if (p.c.seqs > 64) tiles = range = 0;
   }
   // Tile `item` of all, those that see the most positions first (by 64 of them): with
@@ -1188,7 +1232,7 @@ __global__ __launch_bounds__(256) void cached_join_kernel(const CachedArgs p) {
   __shared__ f32x4 acc_s[4][64];
   __shared__ float m_s[4][64], l_s[4][64];
   Division<BM> div{p};
-  div.divide();
+  div.divided(__builtin_amdgcn_readfirstlane(*p.chunk));
   Plan w;
   if (!div.template find<true>(blockIdx.x / p.c.heads, w)) return;
   const int h = blockIdx.x % p.c.heads, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -1288,7 +1332,7 @@ Choice choose(const ttlh_kv_cache* c, int64_t q_heads, int64_t window) {
 }
 
 int64_t workspace_bytes(const ttlh_kv_cache* c, const Choice& x) {
-  return 2 * int64_t(x.target) * c->heads * x.bm * (c->dim + 2) * 4;
+  return x.target == 0 ? 0 : 2 * int64_t(x.target) * c->heads * x.bm * (c->dim + 2) * 4 + 16;
 }
 
 }  // namespace
@@ -1348,6 +1392,7 @@ extern "C" int ttlh_sdpa_cached(const ttlh_kv_cache* cache, const void* Q, void*
   a.cap_log2 = softcap * kLog2e;
   a.part_o = static_cast<float*>(workspace);
   a.part_ml = a.part_o + 2 * int64_t(x.target) * cache->heads * x.bm * cache->dim;
+  a.chunk = reinterpret_cast<int32_t*>(a.part_ml + 2 * int64_t(x.target) * cache->heads * x.bm * 2);
   const int64_t items = (x.tiles + x.target) * cache->heads;
   TTLH_REQUIRE(items < (int64_t(1) << 31), TTLH_EUNSUPPORTED, "ttlh_sdpa_cached: too many tiles");
   const dim3 grid(static_cast<uint32_t>(items));
