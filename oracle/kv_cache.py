@@ -95,6 +95,12 @@ def write(k, v, k_cache, v_cache, k_scale, v_scale, table, lengths, starts=None)
                             row / s if math.isfinite(s) else torch.zeros_like(row), codes.dtype)
 
 
+def sound(scale):
+    """A page's scale; one that is negative or not finite makes NaN of the page."""
+    s = scale.double()
+    return torch.where((s >= 0) & s.isfinite(), s, torch.full_like(s, math.nan))
+
+
 def attention(q, k_cache, v_cache, k_scale, v_scale, table, lengths, scale, starts=None,
               window=0, softcap=0.0):
     """(o, size, reach): o float64, NaN in rows of no sequence; per element the sum
@@ -112,8 +118,8 @@ def attention(q, k_cache, v_cache, k_scale, v_scale, table, lengths, scale, star
         pg = torch.tensor([a[1] for a in at], dtype=torch.long)
         slot = torch.tensor([a[2] for a in at], dtype=torch.long)
         for h in range(heads):
-            ks = k_cache[pg, h, slot].double() * k_scale[pg, h].double()[:, None]
-            vs = v_cache[pg, h, slot].double() * v_scale[pg, h].double()[:, None]
+            ks = k_cache[pg, h, slot].double() * sound(k_scale[pg, h])[:, None]
+            vs = v_cache[pg, h, slot].double() * sound(v_scale[pg, h])[:, None]
             for i in range(n):
                 p = int(lengths[b]) - n + i
                 sees = (pos <= p) & ((pos > p - window) if window else (pos >= 0))

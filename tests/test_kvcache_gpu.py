@@ -585,6 +585,50 @@ def test_attention_long_undivided_tiles(page, dim, cdtype, softcap):
     assert not out[260:, 2:].isnan().any()
 
 
+def _check_tokens(q, cache, table, n, starts, scale, heads, tokens, window=0, softcap=0.0):
+    """The whole call; tokens (sequence, new token) of the cache heads `heads` against the
+    oracle, each as the one new token of a sequence that ends with it."""
+    group = q.shape[1] // cache[0].shape[1]
+    out = torch.full_like(q, 7.0).cuda()
+    K.sdpa_cached(q.cuda(), *[c.cuda() for c in cache], table.cuda(), n.cuda(), out, scale,
+                  starts=starts.cuda(), window=window, softcap=softcap)
+    out = out.cpu()
+    assert not (out == 7.0).all(-1).any()
+    for b, i in tokens:
+        t, news = int(starts[b]) + i, int(starts[b + 1] - starts[b])
+        m = n[b:b + 1] - (news - 1 - i)
+        for h in heads:
+            part = [c[:, h:h + 1] for c in cache]
+            qs = slice(h * group, (h + 1) * group)
+            ref, size, reach = R.attention(q[t:t + 1, qs], *part, table[b:b + 1], m, scale, None,
+                                           window, softcap)
+            tol = _tolerance(ref, size, reach, q.shape[2], int(m[0]), softcap)
+            got = out[t:t + 1, qs].double()
+            assert torch.equal(got.isnan(), ref.isnan()), (b, i, h)
+            err = (got - ref).abs().nan_to_num()
+            assert (err <= tol.nan_to_num(1.0)).all(), (b, i, h, float((err - tol).max()))
+
+
+@pytest.mark.parametrize("cdtype", [INT8, E4M3])
+@pytest.mark.parametrize("window,softcap", [(0, 0.0), (3900, 0.0), (0, 20.0)])
+@pytest.mark.parametrize("heads,group,lens,news", [
+    (64, 8, [4097], [201]),         # one chunk, its tiles alike
+    (16, 8, [4100, 2000], [601, 500]),
+    (8, 32, [33000], [49])])        # and divided into parts
+def test_attention_tiles_of_256_rows(cdtype, window, softcap, heads, group, lens, news):
+    """Calls whose rows go in tiles of eight waves, some pages missing, some bad, some with
+    scales that V's codes are multiplied by."""
+    q, cache, table, n, starts = _attention_call(lens, news, heads, group, 128, 32, cdtype, 78)
+    tokens = [(b, i) for b, m in enumerate(news) for i in (0, 7, 8, 31, 32, m - 1)]
+    _check_tokens(q, cache, table, n, starts, 0.09, (0, heads - 1), tokens, window, softcap)
+    last = lens[0] - news[0]
+    table[0, 5], table[0, 1024 // 32] = -1, 10 ** 7
+    cache[3][table[0, 70], 0], cache[3][table[0, 71], 0] = 2.0 ** -110, 2.0 ** 70
+    cache[2][table[0, (last + 8) // 32], 0] = math.nan
+    cache[3][table[0, (last + 8) // 32], heads - 1] = math.inf
+    _check_tokens(q, cache, table, n, starts, 0.09, (0, heads - 1), tokens, window, softcap)
+
+
 def test_attention_rows_of_more_than_4096_positions():
     """One part of a wave's more than 32 steps."""
     q, cache, table, n, _ = _attention_call([17000], [1], 256, 1, 64, 128, INT8, 72, True)

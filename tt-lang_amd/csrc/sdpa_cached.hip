@@ -16,10 +16,10 @@
 //    codes go from memory to registers, no LDS on the way.  One new token each, 8 x 128
 //    heads, joined: 16 sequences of up to 65537 positions 239 us (5.7 TB/s), 32 of up
 //    to 8192 72 us (4.8 TB/s), one of 501 9.4 us (the latency of its dependent reads).
-//  * cached_tiles_kernel: tiles of 128 rows (prompts): bound by the vector ALU, which
-//    works for the softmax and the decoding between MFMAs.  Blocks of 64 positions
-//    are decoded once into LDS for four waves of 32 rows.  2048 new tokens at 18000,
-//    32 / 8 heads of 128: 612 us, 930 TFLOP/s; four prompts of up to 2049 tokens, 32 / 8
+//  * cached_tiles_kernel: tiles of 128 or 256 rows (prompts): bound by the vector ALU,
+//    which works for the softmax and the decoding between MFMAs.  Blocks of 64 positions
+//    are decoded once into LDS for four or eight waves of 32 rows.  2048 new tokens at
+//    18000, 32 / 8 heads of 128: 570 us, 1.0 PFLOP/s; four prompts of up to 2049 tokens, 32 / 8
 //    heads of 64 and capped scores (two more transcendentals for each): 101 us.
 //
 // Few tiles with many positions are divided into parts (see Plan), whose results
@@ -731,14 +731,14 @@ __global__ __launch_bounds__(kRowWaves * 64, rows_per_cu(D, MT)) void cached_row
 
 // ---- many rows ---------------------------------------------------------------
 //
-// 128 rows a workgroup, 32 a wave; blocks of 64 positions in 32x32x16 MFMAs, K and V
+// 32 rows a wave; blocks of 64 positions in 32x32x16 MFMAs, K and V
 // decoded to bf16 in LDS: K row-major, 16-byte chunk c of row r at c ^ (r & 15) (dim
 // 64: c ^ ((r >> 1) & 7)); V row-major, read with ds_read_b64_tr_b16, chunk c of row r
 // at c ^ 4 (r & 3) (dim 64: c ^ 4 ((r >> 1) & 1)).  Two buffers of each.
 //
-// A block has 32 MFMAs and, for each, about ten other vector instructions (for 32
+// A block has 32 MFMAs and, for each, about eight other vector instructions (for 32
 // rows of 64 scores three each and the decoding), so these are laid between the
-// MFMAs, which run meanwhile; two workgroups share a CU.  In order, with half t the
+// MFMAs, which run meanwhile; two waves share a SIMD.  In order, with half t the
 // block's positions 32 t .. 32 t + 31:
 //     S of half 0            | the next block's K codes are decoded into LDS
 //     S of half 1            | softmax of half 0
@@ -749,16 +749,18 @@ __global__ __launch_bounds__(kRowWaves * 64, rows_per_cu(D, MT)) void cached_row
 // and half a block needs no maximum before its exponentials.
 // (Softmax, decoding and products one after the other took 700 us for 2048 new
 // tokens at 18000, 32 / 8 heads of 128.)
-constexpr int kTileRows = 128;
+//
+// NW waves: four, two workgroups on a CU, or (dim 128) eight, which share the decoding,
+// and one (see choose()).
 constexpr int kBlock = 64;
-constexpr int kTileThreads = 256;
 
-template <int D, int FMT, bool CAP>
+template <int D, int FMT, bool CAP, int NW>
 struct Tiles {
   static constexpr int ND = D / 32, NDC = D / 16;
   static constexpr int kChunks = D / 8;                           // of eight codes in a row
-  static constexpr int kSweep = kTileThreads / kChunks;           // rows of one load of all threads
+  static constexpr int kSweep = NW * 64 / kChunks;                // rows of one load of all threads
   static constexpr int kUnits = kBlock / kSweep;                  // loads of a thread, for K and for V
+  static_assert(kUnits >= 1 && kUnits <= NDC / 2, "each unit is staged behind an MFMA of its own");
   static constexpr int kProducts = 2 * NDC + 4 * ND;              // MFMAs of a block
   static constexpr int kAhead = 4;                                // operands read ahead
   static constexpr float kFar = 256.0f;
@@ -813,9 +815,9 @@ struct Tiles {
   }
 
   // ---- codes ----
-  // the subtile of the thread's unit i (the rows of a wave's load are in one)
+  // the subtile of the thread's unit i (the 64 / kChunks rows of a wave's load are in one)
   __device__ __forceinline__ int unit_sub(int i) const {
-    return D == 128 ? i : 2 * i + (wave >> 1);
+    return (kSweep / 16) * i + wave / (16 * kChunks / 64);
   }
   __device__ __forceinline__ void ask_page(Subtiles& x, int kb) const {  // kb a multiple of 16
     const int pos = s.begin + kb * kBlock + lane * 16;
@@ -1051,8 +1053,8 @@ struct Tiles {
     product<I>(Ks[buf], Vs[buf]);
     __builtin_amdgcn_sched_barrier(0);
     constexpr int g = I / NDC, i = I % NDC;
-    if constexpr (g == 0 && (i & 1)) stage<i / 2>(Ks[buf ^ 1] + k_to, kraw);
-    if constexpr (g == 0 && !(i & 1) && i > 0) load<i / 2 - 1>(p.c.k, kraw, kb + 2);
+    if constexpr (g == 0 && (i & 1) && i / 2 < kUnits) stage<i / 2>(Ks[buf ^ 1] + k_to, kraw);
+    if constexpr (g == 0 && !(i & 1) && i > 0 && i / 2 < kUnits) load<i / 2 - 1>(p.c.k, kraw, kb + 2);
     if constexpr (g == 1 && i == 0) load<kUnits - 1>(p.c.k, kraw, kb + 2);
     if constexpr (g == 1 || g == 2) {
       constexpr int kDone[5] = {0, 0, 2, 5, 8};  // (dim 64) pairs before MFMA i
@@ -1060,8 +1062,8 @@ struct Tiles {
       constexpr int to = i == NDC - 1 ? 8 : D == 128 ? i : kDone[i % 4 + 1];
       pairs<from, to - from, g - 1>(k, b);
     }
-    if constexpr (g == 3 && (i & 1)) stage<i / 2>(Vs[buf ^ 1] + v_to, vraw);
-    if constexpr (g == 3 && !(i & 1) && i > 0) load<i / 2 - 1>(p.c.v, vraw, kb + 2);
+    if constexpr (g == 3 && (i & 1) && i / 2 < kUnits) stage<i / 2>(Vs[buf ^ 1] + v_to, vraw);
+    if constexpr (g == 3 && !(i & 1) && i > 0 && i / 2 < kUnits) load<i / 2 - 1>(p.c.v, vraw, kb + 2);
     __builtin_amdgcn_sched_barrier(0);
     if constexpr (g == 0 && i == NDC - 1) {
       if (!CAP && k.edge) hide<0>(k);
@@ -1113,19 +1115,20 @@ struct Tiles {
   }
 };
 
-template <int D, int FMT, bool CAP>
-__global__ __launch_bounds__(kTileThreads, D == 64 && !CAP ? 3 : 2) void cached_tiles_kernel(
+template <int D, int FMT, bool CAP, int NW>
+__global__ __launch_bounds__(NW * 64, D == 64 && !CAP ? 3 : 2) void cached_tiles_kernel(
     const CachedArgs p) {
+  constexpr int kRows = 32 * NW;
   __shared__ __attribute__((aligned(256))) uint16_t KV[2][2][kBlock * D];
-  Division<kTileRows> div{p};
+  Division<kRows> div{p};
   div.divide();
   Plan w;
   const int item = blockIdx.x / p.c.heads;
   const bool sorted = p.window == 0 && p.c.seqs > 1 && p.c.seqs <= 64 &&
                       !__any(div.range > div.chunk);
   if (!(sorted ? div.find_longest(item, w) : div.template find<false>(item, w))) return;
-  const Span s = span_of<kTileRows, kBlock>(p, w);
-  Tiles<D, FMT, CAP> x{p, w, s, KV[0], KV[1]};
+  const Span s = span_of<kRows, kBlock>(p, w);
+  Tiles<D, FMT, CAP, NW> x{p, w, s, KV[0], KV[1]};
   x.hd = blockIdx.x % p.c.heads;
   x.lane = threadIdx.x & 63;
   x.wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -1197,7 +1200,7 @@ __global__ __launch_bounds__(kTileThreads, D == 64 && !CAP ? 3 : 2) void cached_
   if (row >= w.rows) return;
   const float lt = xor32_add(x.l);
   if (w.parts > 1) {
-    const int64_t at = (static_cast<int64_t>(w.slot + w.part) * p.c.heads + x.hd) * kTileRows +
+    const int64_t at = (static_cast<int64_t>(w.slot + w.part) * p.c.heads + x.hd) * kRows +
                        (row - w.row0);
 #pragma unroll
     for (int j = 0; j < D / 32; ++j)
@@ -1314,7 +1317,18 @@ Choice choose(const ttlh_kv_cache* c, int64_t q_heads, int64_t window) {
   // rows of a sequence: on average, half as many again where they may differ
   const int64_t rows = c->tokens * group;
   const int64_t some = (c->starts ? rows + rows / 2 : rows) / (c->seqs > 0 ? c->seqs : 1);
-  x.bm = some <= 16 ? 16 : some <= 32 ? 32 : some <= 48 ? 48 : kTileRows;
+  x.bm = some <= 16 ? 16 : some <= 32 ? 32 : some <= 48 ? 48 : 128;
+  const int64_t most = c->width * c->page;  // positions that a sequence's tokens see
+  // Eight waves of 32 rows decode a block once in place of twice, but their workgroup is
+  // alone on its CU: its start and end are in nobody's shadow, and what it has less
+  // to do than others is lost.  So they have dim 128 (dim 64: 389 us as four, 400 as
+  // eight), long walks, and two rounds of tiles (4096 new tokens at 8192, 32 / 8 heads:
+  // 430 -> 400 us; in one round, 8 sequences of 256 at 8192 lose, 234 -> 248) or one
+  // chunk, whose tiles are alike (2048 at 18000 605 -> 570, 256 at 65536 307 -> 291).
+  const int64_t wide = (c->starts ? rows / 256 : 0) * c->heads;
+  const int64_t walk = window > 0 && window + 256 < most ? window + 256 : most;  // a tile's
+  const bool alike = c->seqs == 1 && 4 * c->tokens <= walk && wide * walk >= 1500000;
+  if (c->dim == 128 && rows >= 1024 * c->seqs && walk >= 4000 && (wide >= 512 || alike)) x.bm = 256;
   x.tiles = (c->starts ? rows / x.bm + c->seqs : c->seqs * ((group + x.bm - 1) / x.bm));
   const int64_t certain = (c->starts ? rows / x.bm : x.tiles) * c->heads;
   // As many parts as the chip has places (32 answers of up to 8192 positions 72 us;
@@ -1323,9 +1337,8 @@ Choice choose(const ttlh_kv_cache* c, int64_t q_heads, int64_t window) {
   // for each CU undivided, parts of fewer than 2048 do not pay (768 tiles of 1024
   // positions: 25 us, halved 31), and where the tiles fill all places only those of
   // much longer sequences than the others are divided.
-  const int64_t places = 256 * (x.bm == kTileRows ? 2 : rows_per_cu(c->dim, x.bm / 16));
+  const int64_t places = 256 * (x.bm == 256 ? 1 : x.bm == 128 ? 2 : rows_per_cu(c->dim, x.bm / 16));
   x.least = certain >= places ? 4096 : certain >= 512 ? 2048 : 512;
-  const int64_t most = c->width * c->page;  // positions that a sequence's tokens see
   const int64_t positions = window > 0 && window + c->tokens < most ? window + c->tokens : most;
   x.target = positions <= x.least ? 0 : static_cast<int32_t>((places + c->heads - 1) / c->heads);
   return x;
@@ -1386,7 +1399,7 @@ extern "C" int ttlh_sdpa_cached(const ttlh_kv_cache* cache, const void* Q, void*
   a.window = static_cast<int32_t>(window < (int64_t(1) << 31) ? window : 0);
   a.target = x.target;
   a.least = x.least;
-  a.turns = x.tiles * cache->heads <= 768;
+  a.turns = x.bm == 128 && x.tiles * cache->heads <= 768;
   a.scale_log2 = std::fabs(softcap > 0.0f ? scale / softcap * 2.0f * kLog2e : scale * kLog2e);
   a.flip = scale < 0.0f ? 0x80008000u : 0u;
   a.cap_log2 = softcap * kLog2e;
@@ -1415,10 +1428,14 @@ extern "C" int ttlh_sdpa_cached(const ttlh_kv_cache* cache, const void* Q, void*
       run(cached_rows_kernel<D, F, 2>, 64 * kRowWaves, cached_join_kernel<D, 32>);
     else if (x.bm == 48)
       run(cached_rows_kernel<D, F, 3>, 64 * kRowWaves, cached_join_kernel<D, 48>);
-    else if (softcap > 0.0f)
-      run(cached_tiles_kernel<D, F, true>, kTileThreads, cached_join_kernel<D, kTileRows>);
-    else
-      run(cached_tiles_kernel<D, F, false>, kTileThreads, cached_join_kernel<D, kTileRows>);
+    else if constexpr (D == 128) {
+      if (x.bm == 256)
+        softcap > 0.0f ? run(cached_tiles_kernel<D, F, true, 8>, 512, cached_join_kernel<D, 256>)
+                       : run(cached_tiles_kernel<D, F, false, 8>, 512, cached_join_kernel<D, 256>);
+    }
+    if (x.bm == 128)
+      softcap > 0.0f ? run(cached_tiles_kernel<D, F, true, 4>, 256, cached_join_kernel<D, 128>)
+                     : run(cached_tiles_kernel<D, F, false, 4>, 256, cached_join_kernel<D, 128>);
   };
   const std::integral_constant<int, 64> d64;
   const std::integral_constant<int, 128> d128;
