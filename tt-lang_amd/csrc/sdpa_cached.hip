@@ -1332,15 +1332,21 @@ Choice choose(const ttlh_kv_cache* c, int64_t q_heads, int64_t window) {
   x.tiles = (c->starts ? rows / x.bm + c->seqs : c->seqs * ((group + x.bm - 1) / x.bm));
   const int64_t certain = (c->starts ? rows / x.bm : x.tiles) * c->heads;
   // As many parts as the chip has places (32 answers of up to 8192 positions 72 us;
-  // with half as many 83, a tenth more 78, twice as many 72; 16 drafts 80, 99, 103, 86).  A part's
-  // start and end cost about as much as 512 positions; where there are two workgroups
+  // with half as many 83, a tenth more 78, twice as many 72; 16 drafts 80, 99, 103, 86).
+  // A part's start and end cost about as much as 512 positions; where there are two workgroups
   // for each CU undivided, parts of fewer than 2048 do not pay (768 tiles of 1024
   // positions: 25 us, halved 31), and where the tiles fill all places only those of
   // much longer sequences than the others are divided.
   const int64_t places = 256 * (x.bm == 256 ? 1 : x.bm == 128 ? 2 : rows_per_cu(c->dim, x.bm / 16));
   x.least = certain >= places ? 4096 : certain >= 512 ? 2048 : 512;
   const int64_t positions = window > 0 && window + c->tokens < most ? window + c->tokens : most;
-  x.target = positions <= x.least ? 0 : static_cast<int32_t>((places + c->heads - 1) / c->heads);
+  // The join costs a launch: one token of up to 896 positions 12.3 us, in two parts 12.9
+  // (1024: 13.2, 12.7; dim 64, 1280: 11.5, 12.2); 32 tokens of 640 24.4 and 24.9, of 768
+  // 27.0 and 26.4.
+  const int64_t alone = x.bm > 16 ? 704 : c->dim == 64 ? 1280 : 960;
+  x.target = positions <= (x.least > 512 ? x.least : alone)
+                 ? 0
+                 : static_cast<int32_t>((places + c->heads - 1) / c->heads);
   return x;
 }
 
@@ -1358,7 +1364,10 @@ extern "C" int64_t ttlh_sdpa_cached_workspace_bytes(const ttlh_kv_cache* cache, 
   if (check_cache("ttlh_sdpa_cached_workspace_bytes", cache, &a) != TTLH_OK || q_heads <= 0 ||
       q_heads % cache->heads)
     return 0;
-  return workspace_bytes(cache, choose(cache, q_heads, 0));  // (no less than with a window)
+  // No less than with a window: that only lowers the positions, and what it may change
+  // the tiles to, 128 rows in place of 256, has twice the places, half the rows, and
+  // where 256 rows have a `least` of 4096 the same one.
+  return workspace_bytes(cache, choose(cache, q_heads, 0));
 }
 
 extern "C" int ttlh_sdpa_cached(const ttlh_kv_cache* cache, const void* Q, void* O, int64_t q_heads,
