@@ -888,3 +888,40 @@ def test_same_call_same_bits():
         K.sdpa_cached(q.cuda(), *dev, table.cuda(), n.cuda(), o, 0.09, starts=starts.cuda())
         outs.append(o)
     assert all(torch.equal(outs[0], o) for o in outs)
+
+
+# --- pages that are not there, values at the ends of the range ---------------------------
+
+
+def _free_page_0(cache, table):
+    """The same call with a page 0 that no sequence has."""
+    free = next(p for p in range(cache[0].shape[0]) if p > 0 and not (table == p).any())
+    for c in cache:
+        raw = c.view(torch.uint8) if c.dtype == E4M3 else c
+        raw[free] = raw[0]
+    table[table == 0] = free
+
+
+@pytest.mark.parametrize("scale0", [0.0, 2.0 ** 70, 2.0 ** -3])
+@pytest.mark.parametrize("softcap", [0.0, 20.0])
+@pytest.mark.parametrize("dim,heads,group,lens,news,holes", [
+    (64, 2, 4, [300, 155], [130, 40], (0, 3, 8)),        # tiles of 128 rows
+    (128, 2, 4, [300, 155], [130, 40], (0, 3, 8)),
+    (128, 64, 8, [4097], [201], (0, 5, 31, 32, 64)),     # tiles of 256 rows
+    (128, 2, 4, [300, 155], [1, 1], (0, 3, 8))])         # few rows
+def test_attention_missing_pages_beside_a_page_0_of_nan_codes(dim, heads, group, lens, news, holes,
+                                                              softcap, scale0):
+    """What is not in the table is not there, whatever is in page 0: here codes that are NaN
+    under a scale that was never written, or one so large that V is multiplied by it."""
+    q, cache, table, n, starts = _attention_call(lens, news, heads, group, dim, 32, E4M3, 82)
+    _free_page_0(cache, table)
+    for c in cache[:2]:
+        c.view(torch.uint8)[0] = 0x7f
+    cache[2][0], cache[3][0] = scale0, scale0
+    for i, p in enumerate(holes):
+        table[0, p] = -1 if i % 2 else 10 ** 6
+    if heads == 2:
+        _check_attention(q, cache, table, n, starts, 0.09, softcap=softcap)
+    else:
+        tokens = [(0, i) for i in (0, 31, 32, 200)]
+        _check_tokens(q, cache, table, n, starts, 0.09, (0, heads - 1), tokens, 0, softcap)

@@ -364,7 +364,9 @@ struct Subtiles {
   __device__ __forceinline__ void finish(float scale) {
     const bool fine = kscale >= 0.0f && kscale < INFINITY && vscale >= 0.0f && vscale < INFINITY;
     kscale = fine ? kscale * scale : __int_as_float(0x7fc00000);
-    vscale = fine ? fmaxf(vscale, 0x1p-126f) : 1.0f;
+    // (page 0's scale says nothing where there is no page: restage_v() would put page
+    // 0's codes, which may be NaN, where clear_unseen() put zeros)
+    vscale = fine && page >= 0 ? fmaxf(vscale, 0x1p-126f) : 1.0f;
   }
 };
 
