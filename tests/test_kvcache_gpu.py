@@ -925,3 +925,37 @@ def test_attention_missing_pages_beside_a_page_0_of_nan_codes(dim, heads, group,
     else:
         tokens = [(0, i) for i in (0, 31, 32, 200)]
         _check_tokens(q, cache, table, n, starts, 0.09, (0, heads - 1), tokens, 0, softcap)
+
+
+@pytest.mark.parametrize("cdtype", [INT8, E4M3])
+@pytest.mark.parametrize("dim,heads,group,length,tokens", [
+    (64, 2, 4, 300, 130), (128, 2, 4, 300, 130), (128, 64, 8, 4117, 201), (64, 2, 4, 300, 2)])
+def test_attention_of_tokens_before_the_largest_value(dim, heads, group, length, tokens, cdtype):
+    """V's last token holds bf16's largest value, whose code times its scale is 2^128: the
+    tokens before it do not see it, in tiles of 128 and 256 rows and in those of few rows."""
+    pages = -(-length // 32)
+    g = _gen(83)
+    cache = [torch.zeros(pages, heads, 32, dim, dtype=cdtype) for _ in range(2)]
+    cache += [torch.zeros(pages, heads) for _ in range(2)]
+    k, v = (torch.randn(length, heads, dim, generator=g).to(BF16) for _ in range(2))
+    v[-1] = torch.finfo(BF16).max
+    table = torch.randperm(pages, generator=g).to(torch.int32)[None]
+    n = torch.tensor([length], dtype=torch.int32)
+    dev = [c.cuda() for c in cache]
+    K.kv_cache_write(k.cuda(), v.cuda(), *dev, table.cuda(), n.cuda(),
+                     torch.tensor([0, length], dtype=torch.int32).cuda())
+    cache = [c.cpu() for c in dev]
+    last = cache[0][table[0, -1].long(), 0, (length - 1) % 32], cache[1][table[0, -1].long(), 0, (length - 1) % 32]
+    assert float(last[1].float()[0]) * float(cache[3][table[0, -1].long(), 0]) == 2.0 ** 128
+    q = torch.randn(tokens, heads * group, dim, generator=g).to(BF16)
+    starts = torch.tensor([0, tokens], dtype=torch.int32)
+    o = torch.full_like(q, 7.0).cuda()
+    K.sdpa_cached(q.cuda(), *dev, table.cuda(), n.cuda(), o, 0.09, starts=starts.cuda())
+    o = o.cpu()
+    for i in {0, tokens // 2, tokens - 2}:
+        for h in (0, heads - 1):
+            qs = slice(h * group, (h + 1) * group)
+            ref, size, reach = R.attention(q[i:i + 1, qs], *[c[:, h:h + 1] for c in cache], table,
+                                           n - (tokens - 1 - i), 0.09)
+            err = (o[i:i + 1, qs].double() - ref).abs()
+            assert (err <= _tolerance(ref, size, reach, dim, length, 0.0)).all(), (i, h, float(err.max()))

@@ -832,9 +832,10 @@ struct Tiles {
     broken = __ballot(!(sub.kscale < INFINITY));
     if (!(sub.kscale < INFINITY)) sub.kscale = 1.0f;  // (hide() makes the NaN)
     sub.kscale = fmaxf(sub.kscale, 0x1p-126f);        // (0 times -inf would be NaN)
-    const bool far = far_scale(sub.vscale);           // (restage_v() multiplies)
-    lv = far ? 0.0f : __builtin_amdgcn_logf(sub.vscale);
-    iv = far ? 1.0f : __builtin_amdgcn_rcpf(sub.vscale);
+    const bool far = far_scale(sub.vscale);           // (restage_v() multiplies by the rest)
+    const float by_p = far ? near_part(sub.vscale) : sub.vscale;
+    lv = __builtin_amdgcn_logf(by_p);
+    iv = __builtin_amdgcn_rcpf(by_p);
     paged = __ballot(sub.page >= 0);
     const int pos = s.begin + (kb * 4 + lane) * 16;
     special = __ballot(sub.page < 0 || far || pos < s.all_lo || pos + 16 > s.all_hi) | broken;
@@ -843,9 +844,12 @@ struct Tiles {
   // is not known yet: it may)
   __device__ __forceinline__ bool is_special(int kb) const { return (special >> ((kb & 15) * 4)) & 15; }
   __device__ __forceinline__ bool may_be_special(int kb) const { return (kb & 15) == 0 || is_special(kb); }
-  // V scales so small or large that p times them leaves the exponents' range go into
-  // V itself.
+  // Of V scales so small or large that p times them leaves the exponents' range, the
+  // power of two 2^-60 or 2^60 goes to p and the rest into V itself: a code times the rest
+  // is at most 448 * 2^68, where a code times the scale could be infinite, which makes NaN
+  // of the rows that do not see it (0 times infinity).
   static __device__ __forceinline__ bool far_scale(float v) { return v < 0x1p-60f || v > 0x1p60f; }
+  static __device__ __forceinline__ float near_part(float v) { return v < 1.0f ? 0x1p-60f : 0x1p60f; }
   __device__ __forceinline__ void restage_v(int kb) const {
     const bool later = (kb & 15) == 0 && kb > 0;
     const float scale = later ? next.vscale : sub.vscale;
@@ -853,9 +857,10 @@ struct Tiles {
     const int at = (kb & 15) * 4;
     if (((__ballot(far_scale(scale)) >> at) & 15) == 0) return;
     for (int i = 0; i < kUnits; ++i) {
-      const float f = uniform(scale, at + unit_sub(i));
+      float f = uniform(scale, at + unit_sub(i));
       const int j = s.begin + kb * kBlock + i * kSweep + static_cast<int>(threadIdx.x) / kChunks;
       if (!far_scale(f) || j < s.lo || j >= s.hi) continue;
+      f *= f < 1.0f ? 0x1p60f : 0x1p-60f;
       const uint32_t u = __builtin_amdgcn_readlane(unit, at + unit_sub(i));
       const u32x2 raw = *reinterpret_cast<const u32x2*>(p.c.v + static_cast<uint64_t>(u) * (16 * D) +
                                                         unit_off);
