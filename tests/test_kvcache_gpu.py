@@ -959,3 +959,24 @@ def test_attention_of_tokens_before_the_largest_value(dim, heads, group, length,
                                            n - (tokens - 1 - i), 0.09)
             err = (o[i:i + 1, qs].double() - ref).abs()
             assert (err <= _tolerance(ref, size, reach, dim, length, 0.0)).all(), (i, h, float(err.max()))
+
+
+@pytest.mark.parametrize("dim,group,length", [
+    (64, 4, 524900), (64, 4, 525100), (128, 4, 393800), (128, 16, 442980), (64, 4, 524800)])
+def test_attention_parts_of_one_long_sequence(dim, group, length):
+    """One cache head and a sequence whose parts are a little longer than a multiple of 64
+    when shared out evenly: the last positions, which weigh the most, are in some part."""
+    page = 128
+    pages = -(-length // page)
+    g = _gen(84)
+    cache = [torch.randint(-40, 41, (pages, 1, page, dim), generator=g, dtype=torch.int8) for _ in range(2)]
+    cache += [torch.full((pages, 1), 2.0 ** -5) for _ in range(2)]
+    last = length - 1
+    table = torch.randperm(pages, generator=g).to(torch.int32)[None]
+    for j in range(last - 9, last + 1):
+        cache[0][table[0, j // page].long(), 0, j % page] = 40
+        cache[1][table[0, j // page].long(), 0, j % page] = 100
+    q = torch.ones(1, group, dim).to(BF16)
+    n = torch.tensor([length], dtype=torch.int32)
+    got = _check_attention(q, cache, table, n, None, dim ** -0.5 * (128 / dim) ** 0.5 * 2)
+    assert (got > 2.5).all()  # (most of the weight is on V = 100 / 32)

@@ -131,7 +131,9 @@ struct Division {
         if (alone < 1.7f * each) each = alone;
       }
     }
-    chunk = max((static_cast<int>(fminf(each, 1073741824.0f)) + 63) & ~63, p.least);
+    // (up: of a length below `each`, such as a multiple of 64 that it is a fraction above,
+    // one sequence can have more parts than there are workgroups)
+    chunk = max((static_cast<int>(ceilf(fminf(each, 1073741824.0f))) + 63) & ~63, p.least);
     chunk = __builtin_amdgcn_readfirstlane(chunk);
     if (blockIdx.x == 0 && threadIdx.x == 0) *p.chunk = chunk;
     if (p.c.seqs > 64) tiles = range = 0;
