@@ -7,6 +7,9 @@ import math
 import os
 import shutil
 import subprocess
+import threading
+import time
+import weakref
 
 import pytest
 import torch
@@ -353,3 +356,81 @@ def test_what_a_token_sees(rules):
 
 def test_offsets_pass_32_bits(rules):
     assert rules.offset(2 ** 20, 7, 127) == ((2 ** 20 * 8 + 7) * 128 + 127) * 128
+
+
+# --- workspaces, on the host ------------------------------------------------------
+
+
+class _Library:
+    """Stands for the library where a call needs a workspace: notes where each launch's is
+    and whether its memory is alive, and lets other threads run while it launches."""
+
+    def __init__(self, monkeypatch):
+        self.alive, self.inside, self.overlaps, self.dead = {}, {}, [], []
+        empty = torch.empty
+
+        def noted(*a, **k):
+            t = empty(*a, **k)
+            self.alive[t.data_ptr()] = t.numel()
+            weakref.finalize(t, self.alive.pop, t.data_ptr(), None)
+            return t
+
+        monkeypatch.setattr(K.torch, "empty", noted)
+        monkeypatch.setattr(K.L, "call", self.call)
+        monkeypatch.setattr(K.L, "stream_ptr", lambda stream=None: 1234)
+        monkeypatch.setattr(K, "_check_on_one_device", lambda *a: None)
+        monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+        K.release_workspaces()
+
+    def call(self, fn, *args):
+        assert fn == "ttlh_sdpa_cached"
+        ws, nbytes = args[-3], args[-2]
+        if ws in self.inside:
+            self.overlaps.append(ws)
+        self.inside[ws] = True
+        time.sleep(0.002)
+        if self.alive.get(ws, 0) < nbytes:
+            self.dead.append(ws)
+        self.inside.pop(ws, None)
+
+
+def _long_call(width):
+    return _call(table=torch.zeros(3, width, dtype=torch.int32))
+
+
+def test_threads_take_turns_at_a_streams_workspace(monkeypatch):
+    """A call has two launches: nobody else's on the same memory may come between them, and
+    the memory lives until they are done, also where another thread asks for more of it or
+    gives the workspaces back."""
+    lib = _Library(monkeypatch)
+    errors = []
+
+    def work(i):
+        try:
+            for j in range(12):
+                q = torch.zeros(5, 2 * (1 + (i + j) % 4), 64, dtype=torch.bfloat16)
+                K.sdpa_cached(q, o=q.clone(), scale=0.1, **_long_call(200))
+                if i == 0 and j % 4 == 3:
+                    K.release_workspaces()
+        except Exception as e:  # noqa: BLE001
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    K.release_workspaces()
+    assert not errors and not lib.overlaps and not lib.dead
+
+
+def test_other_streams_do_not_wait(monkeypatch):
+    """The workspaces of two streams are two."""
+    lib = _Library(monkeypatch)
+    seen = []
+    monkeypatch.setattr(K.L, "call", lambda fn, *a: seen.append(a[-3]))
+    for sp in (1, 2, 1):
+        monkeypatch.setattr(K.L, "stream_ptr", lambda stream=None, sp=sp: sp)
+        K.sdpa_cached(Q, o=Q.clone(), scale=0.1, **_long_call(200))
+    assert seen[0] == seen[2] != seen[1] and not lib.overlaps
+    K.release_workspaces()

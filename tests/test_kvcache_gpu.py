@@ -15,11 +15,14 @@ Tolerances, derived:
 """
 
 import math
+import threading
+import time
 
 import pytest
 import torch
 
 from oracle import kv_cache as R
+from ttlhip import expr as X
 from ttlhip import kernels as K
 
 pytestmark = pytest.mark.gpu
@@ -980,3 +983,45 @@ def test_attention_parts_of_one_long_sequence(dim, group, length):
     n = torch.tensor([length], dtype=torch.int32)
     got = _check_attention(q, cache, table, n, None, dim ** -0.5 * (128 / dim) ** 0.5 * 2)
     assert (got > 2.5).all()  # (most of the weight is on V = 100 / 32)
+
+
+def test_two_threads_on_one_stream():
+    """Divided calls and column sums of two threads on one stream, some with larger
+    workspaces than others, while a third gives the workspaces back: the bits of calls by
+    themselves."""
+    calls = [_attention_call([4000, 1333, 90], [1, 1, 1], 2, 4, 128, 32, INT8, 89, True),
+             _attention_call([3000, 2333, 190], [1, 1, 1], 8, 8, 64, 32, E4M3, 90, True)]
+    dev = [[q.cuda(), *[c.cuda() for c in cache], t.cuda(), n.cuda()] for q, cache, t, n, _ in calls]
+    rows = torch.randn(4096, 512, generator=_gen(91)).cuda()
+    prog = X.compile_expr(X.Leaf(0, F32))
+
+    def once(i):
+        o = torch.empty_like(dev[i][0])
+        s = torch.empty(1, 512, device="cuda")
+        K.sdpa_cached(*dev[i], o, 0.09)
+        K.reduce(prog, [K.OperandMap(rows)], "sum", [0], s, (0, 0, 4096, 512))
+        return o, s
+
+    want = [once(i) for i in range(2)]
+    torch.cuda.synchronize()
+    got, errors = [[], []], []
+
+    def work(i):
+        try:
+            for _ in range(60):
+                got[i].append(once(i))
+        except Exception as e:  # noqa: BLE001
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    while any(t.is_alive() for t in threads):
+        K.release_workspaces()
+        time.sleep(0.001)
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not errors
+    for w, g in zip(want, got):
+        assert len(g) == 60 and all(torch.equal(a, b) for x in g for a, b in zip(w, x))

@@ -49,38 +49,53 @@ def _check_device(t: torch.Tensor, what: str) -> None:
 # per (device, stream), grown to the largest size asked for and then kept.
 # Taking a fresh one from torch's caching allocator on every call costs about
 # 10 us of host time (4096^2 column sums: 35 -> 25 us of host enqueue per
-# call, against 17 us of kernels).  Calls on one stream run in stream
-# order, so they share that stream's buffer safely; calls on different
+# call, against 17 us of kernels).  Calls on one stream share its buffer: the
+# kernels run in stream order, and a call's launches follow each other without
+# another's between them, because the buffer's lock is held from the lookup to
+# the last launch (ctypes lets other threads run meanwhile).  Calls on different
 # streams get different buffers.  A HIP graph captured over such a call
 # keeps the buffer's address: replaying it while eager calls run on the
 # same buffer from another stream races, as with any shared buffer.
+class _Workspace:
+    __slots__ = ("lock", "memory")
+
+    def __init__(self):
+        self.lock = threading.RLock()  # (a finalizer may call from inside an allocation)
+        self.memory = None
+
+
 _WORKSPACES: dict = {}
 
 
-def _workspace(device: torch.device, stream, nbytes: int,
-               sp: Optional[int] = None) -> torch.Tensor:
-    key = (device.index, L.stream_ptr(stream) if sp is None else sp)
-    ws = _WORKSPACES.get(key)
-    if ws is None or ws.numel() < nbytes:
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
-        if stream is not None:
-            # allocated on the current stream, used on `stream`: keep the
-            # block from being handed out again before that stream's work
-            # on it has finished once this buffer is replaced
-            ws.record_stream(stream)
-        _WORKSPACES[key] = ws
-    return ws
+def _with_workspace(device: torch.device, stream, nbytes: int, sp: int, launch) -> None:
+    """launch(address) with `nbytes` of the workspace of the stream (pointer `sp`)."""
+    key = (device.index, sp)
+    slot = _WORKSPACES.get(key)
+    if slot is None:
+        slot = _WORKSPACES.setdefault(key, _Workspace())
+    with slot.lock:
+        ws = slot.memory
+        if ws is None or ws.numel() < nbytes:
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+            if stream is not None:
+                # allocated on the current stream, used on `stream`: keep the
+                # block from being handed out again before that stream's work
+                # on it has finished once this buffer is replaced
+                ws.record_stream(stream)
+            slot.memory = ws
+        launch(ws.data_ptr())
 
 
-def _workspace_or_graphs(device: torch.device, stream, nbytes: int, sp: int) -> torch.Tensor:
-    """The cached workspace; under capture memory of the graph's own, which no
-    eager call, no other graph and no later, larger workspace has to do with."""
+def _with_workspace_or_graphs(device: torch.device, stream, nbytes: int, sp: int, launch) -> None:
+    """The same; under capture with memory of the graph's own, which no eager
+    call, no other graph and no later, larger workspace has to do with."""
     if not torch.cuda.is_current_stream_capturing():
-        return _workspace(device, stream, nbytes, sp)
+        _with_workspace(device, stream, nbytes, sp, launch)
+        return
     ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
     if stream is not None:
         ws.record_stream(stream)
-    return ws
+    launch(ws.data_ptr())
 
 
 # The matmul's scratch (partial sums of products that divide K among several
@@ -344,11 +359,16 @@ def reduce(prog: StackProgram, operands: Sequence[Optional[OperandMap]], kind: s
         return
     stp = L.stream_ptr(stream)
     ws_bytes = _reduce_workspace_bytes(dbits, h, w)
-    ws = _workspace(out.device, stream, ws_bytes, stp) if ws_bytes else None
-    L.call("ttlh_reduce", instrs, ops, n, kcode,
-           dbits, sp, sdt, float(scale), optr, L.dtype_code(out.dtype), out.stride(0),
-           int(bool(out_pad)), y0, x0, h, w, ws.data_ptr() if ws is not None else 0, ws_bytes,
-           stp)
+
+    def launch(ws: int) -> None:
+        L.call("ttlh_reduce", instrs, ops, n, kcode,
+               dbits, sp, sdt, float(scale), optr, L.dtype_code(out.dtype), out.stride(0),
+               int(bool(out_pad)), y0, x0, h, w, ws, ws_bytes, stp)
+
+    if ws_bytes:
+        _with_workspace(out.device, stream, ws_bytes, stp, launch)
+    else:
+        launch(0)
 
 
 @dataclass
@@ -668,9 +688,10 @@ def matmul_bfp8w(a: torch.Tensor, bq: torch.Tensor, c: torch.Tensor, stream=None
         L.check("ttlh_matmul_scratch", _matmul_packed(a, bq, L.TTLH_BFP8, c, M, N, K, stream))
         return
     nbytes = int(L.load().ttlh_matmul_bfp8w_workspace_bytes(M, N, K))
-    ws = _workspace(c.device, stream, nbytes)
-    L.call("ttlh_matmul_bfp8w_ws", a.data_ptr(), a.stride(0), bq.data_ptr(), c.data_ptr(),
-           c.stride(0), M, N, K, ws.data_ptr(), nbytes, L.stream_ptr(stream))
+    sp = L.stream_ptr(stream)
+    _with_workspace(c.device, stream, nbytes, sp, lambda ws: L.call(
+        "ttlh_matmul_bfp8w_ws", a.data_ptr(), a.stride(0), bq.data_ptr(), c.data_ptr(),
+        c.stride(0), M, N, K, ws, nbytes, sp))
 
 
 def bfp4_tiles_bytes(rows: int, cols: int) -> int:
@@ -730,9 +751,10 @@ def matmul_bfp4w(a: torch.Tensor, bq: torch.Tensor, c: torch.Tensor, stream=None
         if status != L.TTLH_EUNSUPPORTED:
             L.check("ttlh_matmul_scratch", status)
             return
-    ws = _workspace(c.device, stream, K * N * 2)
-    L.call("ttlh_matmul_bfp4w_ws", a.data_ptr(), a.stride(0), bq.data_ptr(), c.data_ptr(),
-           c.stride(0), M, N, K, ws.data_ptr(), K * N * 2, L.stream_ptr(stream))
+    sp = L.stream_ptr(stream)
+    _with_workspace(c.device, stream, K * N * 2, sp, lambda ws: L.call(
+        "ttlh_matmul_bfp4w_ws", a.data_ptr(), a.stride(0), bq.data_ptr(), c.data_ptr(),
+        c.stride(0), M, N, K, ws, K * N * 2, sp))
 
 
 def sdpa_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: torch.Tensor, scale: float,
@@ -964,6 +986,12 @@ def sdpa_cached(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
     _check_on_one_device("sdpa_cached", tensors if starts is None else tensors + (starts,), stream)
     sp = L.stream_ptr(stream)
     nbytes = L.load().ttlh_sdpa_cached_workspace_bytes(cache, q_heads)
-    ws = _workspace_or_graphs(q.device, stream, nbytes, sp).data_ptr() if nbytes else 0
-    L.call("ttlh_sdpa_cached", cache, qp, op, q_heads, qt, qh, ot, oh, scale, window, softcap, ws,
-           nbytes, sp)
+
+    def launch(ws: int) -> None:
+        L.call("ttlh_sdpa_cached", cache, qp, op, q_heads, qt, qh, ot, oh, scale, window, softcap,
+               ws, nbytes, sp)
+
+    if nbytes:
+        _with_workspace_or_graphs(q.device, stream, nbytes, sp, launch)
+    else:
+        launch(0)
