@@ -2,6 +2,7 @@
 and the library refuse, the frequencies, and the header's rules for positions and
 scales, compiled for the host."""
 
+import contextlib
 import ctypes
 import math
 import os
@@ -433,4 +434,59 @@ def test_other_streams_do_not_wait(monkeypatch):
         monkeypatch.setattr(K.L, "stream_ptr", lambda stream=None, sp=sp: sp)
         K.sdpa_cached(Q, o=Q.clone(), scale=0.1, **_long_call(200))
     assert seen[0] == seen[2] != seen[1] and not lib.overlaps
+    K.release_workspaces()
+
+
+class _Stream:
+    device = torch.device("cuda", 0)
+    cuda_stream = 77
+
+
+def _current(monkeypatch, pointers, capturing=()):
+    """The current stream is pointers[-1] (a list that torch.cuda.stream() pushes to);
+    streams in `capturing` are being captured."""
+
+    @contextlib.contextmanager
+    def stream(s):
+        pointers.append(s.cuda_stream)
+        yield
+        pointers.pop()
+
+    monkeypatch.setattr(torch.cuda, "stream", stream)
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: None, raising=False)
+    monkeypatch.setattr(K.L, "stream_ptr", lambda s=None: pointers[-1] if s is None else s.cuda_stream)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: pointers[-1] in capturing)
+
+
+@pytest.mark.parametrize("captured", [None, 5, 77])
+def test_workspaces_come_from_the_launch_stream(monkeypatch, captured):
+    """Memory for stream 77 is asked for on stream 77, and it is 77's capture that counts:
+    captured calls have memory of their own, which a later eager call does not get."""
+    lib = _Library(monkeypatch)
+    streams = [5]
+    capturing = {captured}
+    _current(monkeypatch, streams, capturing)
+    asked, used = [], []
+    empty = torch.empty  # (the library's)
+    monkeypatch.setattr(K.torch, "empty", lambda *a, **k: (asked.append(streams[-1]), empty(*a, **k))[1])
+    kept = []
+
+    def call(fn, *a):
+        assert lib.alive.get(a[-3], 0) >= a[-2]
+        used.append(a[-3])
+        kept.append(empty(a[-2], dtype=torch.uint8))  # (nothing else gets this address)
+
+    monkeypatch.setattr(K.L, "call", call)
+    q, o = Q, Q.clone()
+    for _ in range(2):
+        K.sdpa_cached(q, o=o, scale=0.1, stream=_Stream(), **_long_call(200))
+    assert streams == [5]
+    assert asked == ([77, 77] if captured == 77 else [77])
+    if captured == 77:
+        assert not K._WORKSPACES
+        capturing.clear()
+        K.sdpa_cached(q, o=o, scale=0.1, stream=_Stream(), **_long_call(200))
+        assert asked == [77, 77, 77]
+    else:
+        assert used[0] == used[1]
     K.release_workspaces()

@@ -1025,3 +1025,59 @@ def test_two_threads_on_one_stream():
     assert not errors
     for w, g in zip(want, got):
         assert len(g) == 60 and all(torch.equal(a, b) for x in g for a, b in zip(w, x))
+
+
+def test_workspace_of_another_stream():
+    """A call on a stream that is not the current one, while the current one has still to
+    fill memory that it has given back: the call's workspace is not that memory."""
+    q, cache, t, n, _ = _attention_call([4000, 1333, 90], [1, 1, 1], 2, 4, 128, 32, INT8, 92, True)
+    dev = [q.cuda(), *[c.cuda() for c in cache], t.cuda(), n.cuda()]
+    want = torch.empty_like(dev[0])
+    K.sdpa_cached(*dev, want, 0.09)
+    side = torch.cuda.Stream()
+    out = [torch.empty_like(want) for _ in range(4)]
+    torch.cuda.synchronize()
+    for o in out:
+        K.release_workspaces()
+        blocks = [torch.empty(k << 20, dtype=torch.uint8, device="cuda") for k in (1, 2, 4, 8, 16, 32)]
+        torch.cuda._sleep(2_000_000)  # (about a millisecond)
+        for b in blocks:
+            b.fill_(255)
+        del b, blocks
+        K.sdpa_cached(*dev, o, 0.09, stream=side)
+        side.synchronize()
+    torch.cuda.synchronize()
+    assert all(torch.equal(want, o) for o in out)
+
+
+def test_captured_reductions_have_memory_of_their_own():
+    """Column sums in two graphs, replayed while eager ones, some larger, run between."""
+    prog = X.compile_expr(X.Leaf(0, F32))
+    g = _gen(93)
+    small, large = torch.randn(4096, 512, generator=g).cuda(), torch.randn(8192, 2048, generator=g).cuda()
+
+    def sums(x, o):
+        K.reduce(prog, [K.OperandMap(x)], "sum", [0], o, (0, 0) + tuple(x.shape))
+        return o
+
+    want, want_large = (sums(x, torch.empty(1, x.shape[1], device="cuda")) for x in (small, large))
+    K.release_workspaces()
+    xs = [torch.zeros_like(small) for _ in range(2)]
+    outs = [torch.empty(1, 512, device="cuda") for _ in range(2)]
+    graphs = []
+    for x, o in zip(xs, outs):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            sums(x, o)
+        graphs.append(graph)
+    for j in range(6):
+        for x, o, graph in zip(xs, outs, graphs):
+            x.copy_(small if j % 2 else -small)
+            graph.replay()
+        assert torch.equal(sums(large, torch.empty_like(want_large)), want_large)
+        junk = torch.full((8 << 20,), float("nan"), device="cuda")
+        for o in outs:
+            assert torch.equal(o, want if j % 2 else -want), j
+        del junk
+        torch.cuda.synchronize()
+    K.release_workspaces()

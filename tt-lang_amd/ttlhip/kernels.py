@@ -53,9 +53,7 @@ def _check_device(t: torch.Tensor, what: str) -> None:
 # kernels run in stream order, and a call's launches follow each other without
 # another's between them, because the buffer's lock is held from the lookup to
 # the last launch (ctypes lets other threads run meanwhile).  Calls on different
-# streams get different buffers.  A HIP graph captured over such a call
-# keeps the buffer's address: replaying it while eager calls run on the
-# same buffer from another stream races, as with any shared buffer.
+# streams get different buffers.
 class _Workspace:
     __slots__ = ("lock", "memory")
 
@@ -68,7 +66,20 @@ _WORKSPACES: dict = {}
 
 
 def _with_workspace(device: torch.device, stream, nbytes: int, sp: int, launch) -> None:
-    """launch(address) with `nbytes` of the workspace of the stream (pointer `sp`)."""
+    """launch(address) with `nbytes` of the workspace of the stream (pointer `sp`);
+    under capture with memory of the graph's own, which no eager call, no other
+    graph and no later, larger workspace has to do with."""
+    if stream is not None and (sp != L.stream_ptr() or
+                               device.index != torch._C._cuda_getDevice()):
+        # The allocator hands out memory that the current stream may still work on, in
+        # that stream's order: so it is asked on the stream that the launch goes to.
+        with torch.cuda.stream(stream):
+            _with_workspace(device, None, nbytes, sp, launch)
+        return
+    if torch.cuda.is_current_stream_capturing():
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        launch(ws.data_ptr())
+        return
     key = (device.index, sp)
     slot = _WORKSPACES.get(key)
     if slot is None:
@@ -76,26 +87,8 @@ def _with_workspace(device: torch.device, stream, nbytes: int, sp: int, launch) 
     with slot.lock:
         ws = slot.memory
         if ws is None or ws.numel() < nbytes:
-            ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
-            if stream is not None:
-                # allocated on the current stream, used on `stream`: keep the
-                # block from being handed out again before that stream's work
-                # on it has finished once this buffer is replaced
-                ws.record_stream(stream)
-            slot.memory = ws
+            slot.memory = ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
         launch(ws.data_ptr())
-
-
-def _with_workspace_or_graphs(device: torch.device, stream, nbytes: int, sp: int, launch) -> None:
-    """The same; under capture with memory of the graph's own, which no eager
-    call, no other graph and no later, larger workspace has to do with."""
-    if not torch.cuda.is_current_stream_capturing():
-        _with_workspace(device, stream, nbytes, sp, launch)
-        return
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
-    if stream is not None:
-        ws.record_stream(stream)
-    launch(ws.data_ptr())
 
 
 # The matmul's scratch (partial sums of products that divide K among several
@@ -992,6 +985,6 @@ def sdpa_cached(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
                ws, nbytes, sp)
 
     if nbytes:
-        _with_workspace_or_graphs(q.device, stream, nbytes, sp, launch)
+        _with_workspace(q.device, stream, nbytes, sp, launch)
     else:
         launch(0)
