@@ -527,7 +527,8 @@ typedef struct ttlh_kv_cache {
  * 127, 448) over the new tokens of the page and head, or the page's scale where it
  * holds earlier tokens under a larger one; where it holds them under a smaller
  * one their codes are scaled down and rounded again.  A value that is not finite
- * makes the scale NaN (and new codes 0): what reads that page and head is NaN.
+ * makes the scale NaN (and new codes 0): what reads that page and head is NaN, and stays so
+ * while tokens are appended; so does a scale found negative or not finite.
  * A page belongs to one sequence in a call.                                      */
 int ttlh_kv_cache_write(const ttlh_kv_cache* cache, const void* k, const void* v, int dtype,
                         int64_t k_token, int64_t k_head, int64_t v_token, int64_t v_head,

@@ -84,7 +84,7 @@ def write(k, v, k_cache, v_cache, k_scale, v_scale, table, lengths, starts=None)
                                   codes.dtype)
                     if run[0][0] > 0 and begin > 0:  # the page holds earlier tokens
                         old = float(scales[p, h])
-                        s = max(old, s) if math.isfinite(old) and math.isfinite(s) else math.nan
+                        s = max(old, s) if 0 <= old < math.inf and math.isfinite(s) else math.nan
                         if s > old:
                             slot = run[0][0]
                             codes[p, h, :slot] = to_code(

@@ -252,6 +252,7 @@ SOURCE = r"""
 #include "ttlh_kvcache.h"
 extern "C" float scale_for(float a, int f) { return ttlh::scale_for(a, f); }
 extern "C" float joined(float a, float b) { return ttlh::joined_scale(a, b); }
+extern "C" float sound(float a) { return ttlh::sound_scale(a); }
 static ttlh::CacheArgs args(const int32_t* t, int ld, int width, int pages, int shift, const int32_t* starts,
                             int tokens) {
   ttlh::CacheArgs c = {};
@@ -288,6 +289,7 @@ def rules(tmp_path_factory):
     lib.scale_for.restype = lib.joined.restype = ctypes.c_float
     lib.scale_for.argtypes = [ctypes.c_float, ctypes.c_int]
     lib.joined.argtypes = [ctypes.c_float, ctypes.c_float]
+    lib.sound.restype, lib.sound.argtypes = ctypes.c_float, [ctypes.c_float]
     lib.offset.restype = ctypes.c_int64
     return lib
 
@@ -490,3 +492,11 @@ def test_workspaces_come_from_the_launch_stream(monkeypatch, captured):
     else:
         assert used[0] == used[1]
     K.release_workspaces()
+
+
+def test_scales_that_readers_take_as_nan(rules):
+    for s in (-1.0, -1e-45, -math.inf, math.inf, math.nan):
+        assert math.isnan(rules.sound(s)) and math.isnan(rules.joined(rules.sound(s), 1.0))
+    for s in (0.0, -0.0, 1e-45, 2.0 ** -126, 3.0, 3.4028234e38):
+        s = ctypes.c_float(s).value
+        assert rules.sound(s) == s

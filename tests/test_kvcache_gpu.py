@@ -1081,3 +1081,22 @@ def test_captured_reductions_have_memory_of_their_own():
         del junk
         torch.cuda.synchronize()
     K.release_workspaces()
+
+
+@pytest.mark.parametrize("cdtype", [INT8, E4M3])
+@pytest.mark.parametrize("old", [-1.0, -1000.0, -math.inf, math.inf, -0.0])
+def test_write_behind_tokens_of_a_bad_scale(cdtype, old):
+    """A page that is NaN for its readers stays so while tokens are appended to it."""
+    for one in (True, False):
+        cache = _cache(2, 2, 16, 64, cdtype, 85)
+        _valid_codes(cache, None, None, None, 16)
+        cache[2][1, 0], cache[3][1, 1] = old, old
+        k = torch.randn(1, 2, 64, generator=_gen(86))
+        table = torch.tensor([[1]], dtype=torch.int32)
+        n = torch.tensor([5], dtype=torch.int32)
+        starts = None if one else torch.tensor([0, 1], dtype=torch.int32)
+        got = _run_write(k, k, cache, table, n, starts)
+        assert math.isnan(got[2][1, 0]) == (old != 0.0) and not math.isnan(got[2][1, 1])
+        q = torch.randn(1, 4, 64, generator=_gen(87)).to(BF16)
+        _check_attention(q, got, table, n, None, 0.125)
+        _run_write(k, k, got, table, torch.tensor([1], dtype=torch.int32), starts)

@@ -336,7 +336,7 @@ __global__ __launch_bounds__(256) void kv_write_kernel(const WriteArgs p) {
     const uint32_t m = max(max(part[z][0], part[z][1]), max(part[z][2], part[z][3]));
     float s = scale_for(__uint_as_float(m), FMT);
     if (lo > 0) {  // earlier tokens
-      const float old = *scale;
+      const float old = sound_scale(*scale);
       s = joined_scale(old, s);
       if (s > old)
         for (int t = t0; t < lo; t += kTokens) {
@@ -370,7 +370,7 @@ __global__ __launch_bounds__(256) void kv_write_one_kernel(const WriteArgs p) {
   Eight<T> x;
   x.load(static_cast<const T*>(z ? p.x[1] : p.x[0]) + b * (z ? p.token[1] : p.token[0]) +
              h * (z ? p.head[1] : p.head[0]) + e, p.vec);
-  const float old = *scale;
+  const float old = sound_scale(*scale);
   uint32_t m = x.largest();
 #pragma unroll
   for (int i = kPer / 2; i; i >>= 1)

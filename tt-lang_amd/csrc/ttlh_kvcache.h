@@ -102,8 +102,15 @@ TTLH_HD float scale_for(float a, int format) {
   return bits_float(static_cast<uint32_t>(s < 1 ? 1 : s) << 23);
 }
 
-// the scale of a page that holds earlier tokens under `old` and gets new ones that
-// need `need`: the larger; NaN stays
+// A page's scale as its readers take it: one that is negative or not finite is NaN,
+// and stays so while tokens are appended.  (Codes of a negative scale, scaled down, would
+// be codes of a finite one, or leave their range.)
+TTLH_HD float sound_scale(float s) {
+  return s >= 0.0f && s < bits_float(0x7f800000u) ? s : bits_float(0x7fc00000u);
+}
+
+// the scale of a page that holds earlier tokens under `old`, a sound_scale(), and gets
+// new ones that need `need`: the larger; NaN stays
 TTLH_HD float joined_scale(float old, float need) {
   if (!(old < bits_float(0x7f800000u)) || need != need) return bits_float(0x7fc00000u);
   return old > need ? old : need;
