@@ -537,7 +537,8 @@ int ttlh_kv_cache_write(const ttlh_kv_cache* cache, const void* k, const void* v
 /* O[t, h] = softmax over the positions j that token t (at position p) sees of
  * cap(scale Q[t, h] . K[j, h / (q_heads / heads)]) V[j, ..], with j <= p, and
  * j > p - window where window > 0; cap(x) = softcap tanh(x / softcap) (softcap from
- * 2^-16 to 2^16), or x where softcap = 0.  A token that sees nothing gets zeros, one
+ * 2^-16 to 2^16; right to 2^-22 softcap up to 128, above to 2^-21 of itself, beside the
+ * roundings of x), or x where softcap = 0.  A token that sees nothing gets zeros, one
  * that sees a page whose K or V scale is negative or not finite NaN.  Q, O: bf16 [tokens, q_heads,
  * dim], 16-byte aligned, strides multiples of 8.  fp32 scores and statistics.
  * `workspace`: ttlh_sdpa_cached_workspace_bytes of device memory, 16-byte aligned. */

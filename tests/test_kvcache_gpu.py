@@ -1100,3 +1100,65 @@ def test_write_behind_tokens_of_a_bad_scale(cdtype, old):
         q = torch.randn(1, 4, 64, generator=_gen(87)).to(BF16)
         _check_attention(q, got, table, n, None, 0.125)
         _run_write(k, k, got, table, torch.tensor([1], dtype=torch.int32), starts)
+
+
+@pytest.mark.parametrize("dim,group,tokens", [(64, 4, 1), (128, 4, 1), (128, 20, 1), (64, 30, 1), (64, 4, 40),
+                                              (128, 4, 40), (128, 8, 300)])
+@pytest.mark.parametrize("softcap", [100.0, 129.0, 1000.0, 1e4, 65536.0])
+def test_attention_of_close_scores_under_a_large_cap(softcap, dim, group, tokens):
+    """Two positions whose scores, up to 192, differ by so little that o is the difference of
+    two probabilities: p = 1 and p = 1 - i / 256, V = 1 and -1.  Both are numbers of bf16, and
+    scores that are right to 2^-10 leave them so (a step of bf16 below 1 is 2^-8): o = (1 - p)
+    / (1 + p) up to its rounding, 2^-8 of it, p's own error in the sum 1 + p, less than 2^-10
+    of it, and fp32's (64 + n) 2^-24.
+
+    The scores: sums of dim products that fp32 holds exactly, a few factors and the cap: 16
+    roundings of numbers up to 192 log2 e < 512, 2^-12.  softcap tanh(s / softcap) is flatter
+    than s, so i is whole only for large caps; where p is not near a number of bf16, its
+    rounding may go either way."""
+    heads, length = 8, 310
+    page = 32
+    pages = -(-length // page)
+    k = torch.full((pages, heads, page, dim), -127, dtype=torch.int8)
+    v = torch.zeros(pages, heads, page, dim, dtype=torch.int8)
+    k[0, :, :2] = 127
+    v[0, :, 0], v[0, :, 1] = 1, -1
+    ks, vs = torch.empty(pages, heads), torch.ones(pages, heads)
+    for h in range(heads):
+        k[0, h, 1, 3 * h] = 126  # one less in the sum
+        i = 1 + h % 3
+        ks[:, h] = -math.log(1 - i / 256) * 128 / dim
+    cache = [k, v, ks, vs]
+    q = torch.full((tokens, heads * group, dim), 1.0).to(BF16)
+    table = torch.arange(pages, dtype=torch.int32)[None]
+    n, starts = torch.tensor([length], dtype=torch.int32), torch.tensor([0, tokens], dtype=torch.int32)
+    scale = dim / 128
+    out = torch.full_like(q, 7.0).cuda()
+    K.sdpa_cached(q.cuda(), *[c.cuda() for c in cache], table.cuda(), n.cuda(), out, scale,
+                  starts=starts.cuda(), softcap=softcap)
+    got = out.cpu().double()
+    for h in range(heads):
+        s = torch.tensor([127.0 * dim, 127.0 * dim - 1], dtype=torch.float64) * float(ks[0, h]) * scale
+        assert float(s[0]) < 192
+        s = softcap * torch.tanh(s / softcap)
+        p = float(torch.exp(s[1] - s[0]))
+        near = round(p * 256) / 256
+        ref = (1 - near) / (1 + p)
+        off = 2.0 ** -10
+        tol = 2.0 ** -8 * ref + 2 * off * ref + 400 * 2.0 ** -24
+        if abs(near - p) > 2.0 ** -9 - off:  # (either neighbour)
+            tol += 2.0 ** -8
+        err = (got[:, h * group:(h + 1) * group] - ref).abs().max()
+        assert float(err) <= tol, (h, p, ref, float(err), tol)
+
+
+@pytest.mark.parametrize("news", [[1, 1], [130, 40]])
+@pytest.mark.parametrize("softcap,loud", [(129.0, 100.0), (1000.0, 300.0), (1000.0, 3000.0), (65536.0, 4.0)])
+def test_attention_large_caps(softcap, loud, news):
+    """Scores far below, about and far above the cap."""
+    q, cache, table, n, starts = _attention_call([300, 55], news, 2, 4, 128, 32, INT8, 88, loud=loud)
+    _check_attention(q, cache, table, n, starts, 0.09, softcap=softcap)
+    _check_attention(q, cache, table, n, starts, -0.09, window=50, softcap=softcap)
+    table[0, 2] = -1
+    cache[2][table[0, 7], 1] = math.nan
+    _check_attention(q, cache, table, n, starts, 0.09, softcap=softcap)

@@ -372,9 +372,22 @@ struct Subtiles {
   }
 };
 
-// C tanh(t) = C - 2 C / (1 + e^2t), from x = 2 t log2 e
+// C tanh(t) = C - 2 C / (1 + e^2t), from x = 2 t log2 e: off by 2^-22 C, whatever t is.
+// Up to C = 128 that is 2^-15 of a score, 1/64 of what the rounding of p to bf16 is.
+constexpr float kNearCap = 128.0f;
 __device__ __forceinline__ float capped(float x, float cap) {
   return __builtin_fmaf(-2.0f * cap, __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x)), cap);
+}
+// The same for larger C, off by 2^-21 of itself: up to |t| = 1/2 as t times a polynomial
+// in t^2 (tanh(t) / t at Chebyshev's nodes, right to 2^-26), above as above.
+__device__ __forceinline__ float capped_far(float x, float cap) {
+  const float w = x * x;  // 4 log2(e)^2 t^2
+  float q = __builtin_fmaf(w, 3.564945473e-6f, -9.181317000e-5f);
+  q = __builtin_fmaf(w, q, 1.922384137e-3f);
+  q = __builtin_fmaf(w, q, -4.003743082e-2f);
+  q = __builtin_fmaf(w, q, 1.0f);
+  const float y = x * (cap * 0.34657359028f) * q;  // (ln 2 / 2)
+  return w < 2.0813689810f ? y : capped(x, cap);
 }
 
 __device__ __forceinline__ float xor32_max(float x) {
@@ -533,7 +546,10 @@ struct Rows {
       for (int t = 0; t < 2; ++t)
 #pragma unroll
         for (int i = 0; i < 4; ++i) e[4 * t + i] = sc[r][t][i] * ks[t];
-      if (p.cap_log2 != 0.0f) {
+      if (p.cap_log2 > kNearCap * kLog2e) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) e[i] = capped_far(e[i], p.cap_log2);
+      } else if (p.cap_log2 != 0.0f) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) e[i] = capped(e[i], p.cap_log2);
       }
@@ -757,8 +773,10 @@ __global__ __launch_bounds__(kRowWaves * 64, rows_per_cu(D, MT)) void cached_row
 // NW waves: four, two workgroups on a CU, or (dim 128) eight, which share the decoding,
 // and one (see choose()).
 constexpr int kBlock = 64;
+// How scores are capped: not, as capped() does, as capped_far() does.
+constexpr int kUncapped = 0, kCapped = 1, kCappedFar = 2;
 
-template <int D, int FMT, bool CAP, int NW>
+template <int D, int FMT, int CAP, int NW>
 struct Tiles {
   static constexpr int ND = D / 32, NDC = D / 16;
   static constexpr int kChunks = D / 8;                           // of eight codes in a row
@@ -955,16 +973,20 @@ struct Tiles {
   };
   static __device__ __forceinline__ float nan_value() { return __int_as_float(0x7fc00000); }
   // Half T of an edge block: scores that are not seen, and those of bad pages.
-  // (Where scores are capped, C tanh t = C - 2 C u with u = 1 / (1 + e^2t), it takes
-  // the u that pair() left: u = inf is not seen.)
+  // (Where scores are capped it takes what pair() left: capped scores, or, with C tanh t =
+  // C - 2 C u, the u = 1 / (1 + e^2t), of which u = inf is not seen.)
   template <int T>
   __device__ __forceinline__ void hide(const Factors& k) {
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
       const int c = 2 * T + (r >> 3), j = k.pos + 32 * T + 8 * (r >> 2) + 4 * h + (r & 3);
       if ((k.bad >> c) & 1) cur[T][r] = nan_value();
-      if (!((k.there >> c) & 1) || j < from || j >= end) cur[T][r] = CAP ? INFINITY : -INFINITY;
+      if (!((k.there >> c) & 1) || j < from || j >= end) cur[T][r] = CAP == kCapped ? INFINITY : -INFINITY;
     }
+  }
+  // the factor of what settle() and again() find in cur, subtile c
+  __device__ __forceinline__ float factor(const Factors& k, int c) const {
+    return CAP == kCapped ? -2.0f * p.cap_log2 : CAP == kCappedFar ? 1.0f : k.ks[c];
   }
   // p times V's scale = 2^(x f + b) of scores 2 Q, 2 Q + 1 of half T: the K scale in f
   // (or, capped, in x) and V's in b.  (Accumulator r: position 32 T + 8 (r / 4) + 4 h +
@@ -972,13 +994,16 @@ struct Tiles {
   template <int T, int Q>
   __device__ __forceinline__ void pair(const Factors& k, float base) {
     constexpr int c = 2 * T + Q / 4;
-    const float f = CAP ? -2.0f * p.cap_log2 : k.ks[c], b = base + k.lv[c];
+    const float f = factor(k, c), b = base + k.lv[c];
     float e[2];
 #pragma unroll
     for (int z = 0; z < 2; ++z) {
       float x = cur[T][2 * Q + z];
-      if constexpr (CAP) {
+      if constexpr (CAP == kCapped) {
         x = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x * k.ks[c]));
+        cur[T][2 * Q + z] = x;
+      } else if constexpr (CAP == kCappedFar) {
+        x = capped_far(x * k.ks[c], p.cap_log2);
         cur[T][2 * Q + z] = x;
       }
       e[z] = __builtin_amdgcn_exp2f(__builtin_fmaf(x, f, b));
@@ -994,14 +1019,14 @@ struct Tiles {
     if constexpr (Q % 4 == 3) rs = Q == 3 ? part * k.iv[c] : __builtin_fmaf(part, k.iv[c], rs);
   }
   __device__ __forceinline__ float base() const {
-    return (CAP ? p.cap_log2 : 0.0f) - (m == -INFINITY ? 0.0f : m);
+    return (CAP == kCapped ? p.cap_log2 : 0.0f) - (m == -INFINITY ? 0.0f : m);
   }
   // The same for the whole of half T from what pair() left in cur.  (As asm, like the
   // products' rescaling below: in C++ a second set of P lives across the branch.)
   template <int T, int Q = 0>
   __device__ __forceinline__ void again(const Factors& k, float base) {
     constexpr int c = 2 * T + Q / 4;
-    const float f = CAP ? -2.0f * p.cap_log2 : k.ks[c], b = base + k.lv[c];
+    const float f = factor(k, c), b = base + k.lv[c];
     float e0, e1;
     asm volatile(
         "v_fma_f32 %1, %3, %5, %6\n\t"
@@ -1025,9 +1050,8 @@ struct Tiles {
         float x = cur[T][8 * c];
 #pragma unroll
         for (int r = 1; r < 8; ++r)
-          x = CAP ? fminf(x, cur[T][8 * c + r]) : fmaxf(x, cur[T][8 * c + r]);
-        const float f = CAP ? -2.0f * p.cap_log2 : k.ks[2 * T + c];
-        mx = fmaxf(mx, __builtin_fmaf(x, f, CAP ? p.cap_log2 : 0.0f));
+          x = CAP == kCapped ? fminf(x, cur[T][8 * c + r]) : fmaxf(x, cur[T][8 * c + r]);
+        mx = fmaxf(mx, __builtin_fmaf(x, factor(k, 2 * T + c), CAP == kCapped ? p.cap_log2 : 0.0f));
       }
       const float to = fmaxf(m, xor32_max(mx));
       const float alpha = to == m ? 1.0f : __builtin_amdgcn_exp2f(m - to);
@@ -1124,7 +1148,7 @@ struct Tiles {
   }
 };
 
-template <int D, int FMT, bool CAP, int NW>
+template <int D, int FMT, int CAP, int NW>
 __global__ __launch_bounds__(NW * 64, D == 64 && !CAP ? 3 : 2) void cached_tiles_kernel(
     const CachedArgs p) {
   constexpr int kRows = 32 * NW;
@@ -1446,14 +1470,21 @@ extern "C" int ttlh_sdpa_cached(const ttlh_kv_cache* cache, const void* Q, void*
       run(cached_rows_kernel<D, F, 2>, 64 * kRowWaves, cached_join_kernel<D, 32>);
     else if (x.bm == 48)
       run(cached_rows_kernel<D, F, 3>, 64 * kRowWaves, cached_join_kernel<D, 48>);
-    else if constexpr (D == 128) {
-      if (x.bm == 256)
-        softcap > 0.0f ? run(cached_tiles_kernel<D, F, true, 8>, 512, cached_join_kernel<D, 256>)
-                       : run(cached_tiles_kernel<D, F, false, 8>, 512, cached_join_kernel<D, 256>);
+    else {
+      const auto tiles = [&](auto cap) {
+        constexpr int C = decltype(cap)::value;
+        if constexpr (D == 128) {
+          if (x.bm == 256) run(cached_tiles_kernel<D, F, C, 8>, 512, cached_join_kernel<D, 256>);
+        }
+        if (x.bm == 128) run(cached_tiles_kernel<D, F, C, 4>, 256, cached_join_kernel<D, 128>);
+      };
+      if (softcap == 0.0f)
+        tiles(std::integral_constant<int, kUncapped>());
+      else if (softcap <= kNearCap)
+        tiles(std::integral_constant<int, kCapped>());
+      else
+        tiles(std::integral_constant<int, kCappedFar>());
     }
-    if (x.bm == 128)
-      softcap > 0.0f ? run(cached_tiles_kernel<D, F, true, 4>, 256, cached_join_kernel<D, 128>)
-                     : run(cached_tiles_kernel<D, F, false, 4>, 256, cached_join_kernel<D, 128>);
   };
   const std::integral_constant<int, 64> d64;
   const std::integral_constant<int, 128> d128;
