@@ -500,3 +500,19 @@ def test_scales_that_readers_take_as_nan(rules):
     for s in (0.0, -0.0, 1e-45, 2.0 ** -126, 3.0, 3.4028234e38):
         s = ctypes.c_float(s).value
         assert rules.sound(s) == s
+
+
+def test_caches_and_scales_that_overlap_are_refused():
+    """K's and V's codes or scales in one memory, whole or in part, would be written by both."""
+    both = torch.zeros(7, 2, 16, 64, dtype=INT8)
+    scales = torch.ones(7, 2)
+    for change in (dict(k_cache=both[:6], v_cache=both[1:]), dict(k_cache=both[1:], v_cache=both[:6]),
+                   dict(k_scale=scales[:6], v_scale=scales[:6]), dict(k_scale=scales[:6], v_scale=scales[1:])):
+        with pytest.raises(ValueError, match="one memory"):
+            K.kv_cache_write(X, X, **_call(**change))
+    two, sc = torch.zeros(12, 2, 16, 64, dtype=INT8), torch.ones(12, 2)
+    with pytest.raises(RuntimeError, match="no CPU path"):  # halves of one buffer are two
+        K.kv_cache_write(X, X, **_call(k_cache=two[:6], v_cache=two[6:], k_scale=sc[:6], v_scale=sc[6:]))
+    none, ns = torch.zeros(0, 2, 16, 64, dtype=INT8), torch.ones(0, 2)
+    with pytest.raises(RuntimeError, match="no CPU path"):  # and nothing has no memory
+        K.kv_cache_write(X, X, **_call(k_cache=none, v_cache=none.clone(), k_scale=ns, v_scale=ns.clone()))

@@ -935,8 +935,9 @@ def kv_cache_write(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_ca
                               lengths, starts)
     if heads != ch or dim != cd:
         raise ValueError(f"kv_cache_write: tokens of {(heads, dim)}, a cache of {(ch, cd)} (heads, dim)")
-    if k_cache.data_ptr() == v_cache.data_ptr() and tokens:
-        raise ValueError("kv_cache_write: k_cache and v_cache are one memory")
+    if tokens and (abs(k_cache.data_ptr() - v_cache.data_ptr()) < k_cache.numel()
+                   or abs(k_scale.data_ptr() - v_scale.data_ptr()) < 4 * k_scale.numel()):
+        raise ValueError("kv_cache_write: k_cache and v_cache, or their scales, are one memory")
     code = L.dtype_code(k.dtype)
     tensors = (k, v, k_cache, v_cache, k_scale, v_scale, table, lengths)
     _check_on_one_device("kv_cache_write", tensors if starts is None else tensors + (starts,), stream)
