@@ -516,3 +516,13 @@ def test_caches_and_scales_that_overlap_are_refused():
     none, ns = torch.zeros(0, 2, 16, 64, dtype=INT8), torch.ones(0, 2)
     with pytest.raises(RuntimeError, match="no CPU path"):  # and nothing has no memory
         K.kv_cache_write(X, X, **_call(k_cache=none, v_cache=none.clone(), k_scale=ns, v_scale=ns.clone()))
+
+
+def test_results_over_other_views_of_the_queries_are_refused():
+    """o may be q itself: with other strides, rows that others still read would be written."""
+    square = torch.zeros(6, 6, 64, dtype=torch.bfloat16)
+    a = _call(starts=torch.tensor([0, 2, 3, 6], dtype=torch.int32))
+    with pytest.raises(ValueError, match="another view"):
+        K.sdpa_cached(square, o=square.transpose(0, 1), scale=0.1, **a)
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        K.sdpa_cached(square, o=square, scale=0.1, **a)

@@ -973,6 +973,8 @@ def sdpa_cached(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
                          f"{(heads, cd)}")
     _check_distinct("sdpa_cached", "o", shape, ot, oh)
     qp, op = q.data_ptr(), o.data_ptr()
+    if op == qp and (ot != qt or oh != qh):
+        raise ValueError("sdpa_cached: o may be q itself, not another view of its memory")
     if (qp | op) & 15 or (qt | qh | ot | oh) & 7:
         raise ValueError("sdpa_cached: q and o must be 16-byte aligned with strides that are "
                          "multiples of 8")
