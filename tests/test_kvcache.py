@@ -526,3 +526,13 @@ def test_results_over_other_views_of_the_queries_are_refused():
         K.sdpa_cached(square, o=square.transpose(0, 1), scale=0.1, **a)
     with pytest.raises(RuntimeError, match="no CPU path"):
         K.sdpa_cached(square, o=square, scale=0.1, **a)
+
+
+def test_library_refuses_rows_past_31_bits():
+    """The rows of a sequence, new tokens x q heads of a cache head, are rounded up to a tile
+    in 32 bits."""
+    lib = L.load()
+    cache = _c_cache(heads=1, tokens=2 ** 28 - 1)
+    for q_heads in (8, 9):  # (2 ** 31 - 8 rows; more)
+        assert lib.ttlh_sdpa_cached(cache, 16, 16, q_heads, 512, 64, 512, 64, 0.1, 0, 0.0, None, 0,
+                                    None) == L.TTLH_EUNSUPPORTED

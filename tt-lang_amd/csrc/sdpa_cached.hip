@@ -1413,7 +1413,8 @@ extern "C" int ttlh_sdpa_cached(const ttlh_kv_cache* cache, const void* Q, void*
   if (st != TTLH_OK) return st;
   TTLH_REQUIRE(q_heads > 0 && q_heads % cache->heads == 0, TTLH_EINVAL,
                "ttlh_sdpa_cached: q heads must be a multiple of the cache's");
-  TTLH_REQUIRE(q_heads < 65536 && cache->tokens * q_heads < (int64_t(1) << 31), TTLH_EUNSUPPORTED,
+  // (rows, rounded up to a tile, fit an int)
+  TTLH_REQUIRE(q_heads < 65536 && cache->tokens * q_heads <= (int64_t(1) << 31) - 512, TTLH_EUNSUPPORTED,
                "ttlh_sdpa_cached: too many q heads or tokens");
   TTLH_REQUIRE(std::isfinite(scale), TTLH_EINVAL, "ttlh_sdpa_cached: scale must be finite");
   TTLH_REQUIRE(softcap == 0.0f || (softcap >= 0x1p-16f && softcap <= 0x1p16f), TTLH_EINVAL,
