@@ -536,3 +536,11 @@ def test_library_refuses_rows_past_31_bits():
     for q_heads in (8, 9):  # (2 ** 31 - 8 rows; more)
         assert lib.ttlh_sdpa_cached(cache, 16, 16, q_heads, 512, 64, 512, 64, 0.1, 0, 0.0, None, 0,
                                     None) == L.TTLH_EUNSUPPORTED
+
+
+def test_library_refuses_grids_past_32_bits_of_threads():
+    lib = L.load()
+    cache = _c_cache(heads=4, seqs=2 ** 22, tokens=2 ** 22, starts=None, width=200, table_ld=200)
+    need = lib.ttlh_sdpa_cached_workspace_bytes(cache, 4)
+    assert lib.ttlh_sdpa_cached(cache, 16, 16, 4, 256, 64, 256, 64, 0.1, 0, 0.0, 4096, need,
+                                None) == L.TTLH_EUNSUPPORTED

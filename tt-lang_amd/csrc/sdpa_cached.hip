@@ -1450,7 +1450,10 @@ extern "C" int ttlh_sdpa_cached(const ttlh_kv_cache* cache, const void* Q, void*
   a.part_ml = a.part_o + 2 * int64_t(x.target) * cache->heads * x.bm * cache->dim;
   a.chunk = reinterpret_cast<int32_t*>(a.part_ml + 2 * int64_t(x.target) * cache->heads * x.bm * 2);
   const int64_t items = (x.tiles + x.target) * cache->heads;
-  TTLH_REQUIRE(items < (int64_t(1) << 31), TTLH_EUNSUPPORTED, "ttlh_sdpa_cached: too many tiles");
+  static_assert(kRowWaves == 4, "256 threads, but for tiles of 256 rows");
+  const int threads = x.bm == 256 ? 512 : 256;  // (all workgroups' together fit 32 bits)
+  TTLH_REQUIRE(items * threads < (int64_t(1) << 32), TTLH_EUNSUPPORTED,
+               "ttlh_sdpa_cached: too many tiles");
   const dim3 grid(static_cast<uint32_t>(items));
   // (at most target tiles have several parts; rows of a tile: without starts no more
   // than the group.  Most workgroups of the join find nothing to do: few of them.)
@@ -1459,25 +1462,25 @@ extern "C" int ttlh_sdpa_cached(const ttlh_kv_cache* cache, const void* Q, void*
   const dim3 joins(static_cast<uint32_t>((x.tiles < x.target ? x.tiles : x.target) * cache->heads),
                    static_cast<uint32_t>(rounds < 8 ? rounds : 8));
   hipStream_t s = static_cast<hipStream_t>(stream);
-  const auto run = [&](auto kernel, int threads, auto join) {
+  const auto run = [&](auto kernel, auto join) {
     hipLaunchKernelGGL(kernel, grid, dim3(threads), 0, s, a);
     if (x.target) hipLaunchKernelGGL(join, joins, dim3(256), 0, s, a);
   };
   const auto pick = [&](auto dim, auto fmt) {
     constexpr int D = decltype(dim)::value, F = decltype(fmt)::value;
     if (x.bm == 16)
-      run(cached_rows_kernel<D, F, 1>, 64 * kRowWaves, cached_join_kernel<D, 16>);
+      run(cached_rows_kernel<D, F, 1>, cached_join_kernel<D, 16>);
     else if (x.bm == 32)
-      run(cached_rows_kernel<D, F, 2>, 64 * kRowWaves, cached_join_kernel<D, 32>);
+      run(cached_rows_kernel<D, F, 2>, cached_join_kernel<D, 32>);
     else if (x.bm == 48)
-      run(cached_rows_kernel<D, F, 3>, 64 * kRowWaves, cached_join_kernel<D, 48>);
+      run(cached_rows_kernel<D, F, 3>, cached_join_kernel<D, 48>);
     else {
       const auto tiles = [&](auto cap) {
         constexpr int C = decltype(cap)::value;
         if constexpr (D == 128) {
-          if (x.bm == 256) run(cached_tiles_kernel<D, F, C, 8>, 512, cached_join_kernel<D, 256>);
+          if (x.bm == 256) run(cached_tiles_kernel<D, F, C, 8>, cached_join_kernel<D, 256>);
         }
-        if (x.bm == 128) run(cached_tiles_kernel<D, F, C, 4>, 256, cached_join_kernel<D, 128>);
+        if (x.bm == 128) run(cached_tiles_kernel<D, F, C, 4>, cached_join_kernel<D, 128>);
       };
       if (softcap == 0.0f)
         tiles(std::integral_constant<int, kUncapped>());
