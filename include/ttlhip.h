@@ -539,8 +539,11 @@ int ttlh_kv_cache_write(const ttlh_kv_cache* cache, const void* k, const void* v
  * j > p - window where window > 0; cap(x) = softcap tanh(x / softcap) (softcap from
  * 2^-16 to 2^16; right to 2^-22 softcap up to 128, above to 2^-21 of itself, beside the
  * roundings of x), or x where softcap = 0.  A token that sees nothing gets zeros, one
- * that sees a page whose K or V scale is negative or not finite NaN.  Q, O: bf16 [tokens, q_heads,
- * dim], 16-byte aligned, strides multiples of 8.  fp32 scores and statistics.
+ * that sees a page whose K or V scale is negative or not finite NaN.  Codes of positions that
+ * no token of a sequence sees may be anything; among the others V's must be numbers
+ * (ttlh_kv_cache_write leaves no e4m3 NaN): a NaN there may reach tokens before it as well.
+ * Q, O: bf16 [tokens, q_heads, dim], 16-byte aligned, strides multiples of 8.  fp32 scores and
+ * statistics.
  * `workspace`: ttlh_sdpa_cached_workspace_bytes of device memory, 16-byte aligned. */
 int64_t ttlh_sdpa_cached_workspace_bytes(const ttlh_kv_cache* cache, int64_t q_heads);
 int ttlh_sdpa_cached(const ttlh_kv_cache* cache, const void* Q, void* O, int64_t q_heads,

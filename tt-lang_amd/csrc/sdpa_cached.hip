@@ -1082,7 +1082,7 @@ struct Tiles {
     }
   }
   template <int buf, int I = 0>
-  __device__ __forceinline__ void chain(const Factors& k, float b, int kb, int nb) {
+  __device__ __forceinline__ void chain(const Factors& k, float b, int kb) {
     product<I>(Ks[buf], Vs[buf]);
     __builtin_amdgcn_sched_barrier(0);
     constexpr int g = I / NDC, i = I % NDC;
@@ -1110,13 +1110,13 @@ struct Tiles {
       settle<1>(k);
       if (may_be_special(kb + 1)) clear_unseen(kb + 1);
     }
-    if constexpr (I + 1 < kProducts) chain<buf, I + 1>(k, b, kb, nb);
+    if constexpr (I + 1 < kProducts) chain<buf, I + 1>(k, b, kb);
   }
 
   // Block kb; the next one's codes (in registers) go to the other LDS buffers, and
   // those of the one after it follow into the registers.
   template <int buf>
-  __device__ __forceinline__ void block(int kb, int nb) {
+  __device__ __forceinline__ void block(int kb) {
     const uint16_t *Kc = Ks[buf], *Vc = Vs[buf];
     read<0>(Kc, Vc);
     read<1>(Kc, Vc);
@@ -1135,12 +1135,12 @@ struct Tiles {
       k.iv[t] = uniform(iv, at + t);
     }
     k.edge = is_special(kb);
-    chain<buf>(k, base(), kb, nb);
+    chain<buf>(k, base(), kb);
     load<kUnits - 1>(p.c.v, vraw, kb + 2);
     if (may_be_special(kb + 1)) restage_v(kb + 1);
   }
   // the same without the block itself
-  __device__ __forceinline__ void skip(int kb, int nb) {
+  __device__ __forceinline__ void skip(int kb) {
     clear_unseen(kb + 1);
     stage_all((kb & 1) ^ 1);
     restage_v(kb + 1);
@@ -1203,9 +1203,9 @@ __global__ __launch_bounds__(NW * 64, D == 64 && !CAP ? 3 : 2) void cached_tiles
   const auto step = [&](int kb, auto buf) {
     const int pos = s.begin + kb * kBlock;
     if (pos < wave_hi && pos + kBlock > wave_lo)
-      x.template block<decltype(buf)::value>(kb, nb);
+      x.template block<decltype(buf)::value>(kb);
     else
-      x.skip(kb, nb);
+      x.skip(kb);
     __syncthreads();
   };
   for (int kb = 0; kb < nb; kb += 2) {

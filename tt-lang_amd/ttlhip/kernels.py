@@ -959,8 +959,10 @@ def sdpa_cached(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
     multiples of 8; o may be q.  q heads share the cache's heads in equal groups; the
     other arguments are those of kv_cache_write().  Positions that the table does not
     name are not seen.  A token that sees nothing gets zeros, one that sees a page
-    with a negative or non-finite scale NaN.  Rows of o behind the last sequence's
-    tokens stay as they are."""
+    with a negative or non-finite scale NaN.  (Codes that are NaN, which a torch cast
+    to e4m3 makes of values past 448 and kv_cache_write() never does, may reach tokens
+    that do not see them.)  Rows of o behind the last sequence's tokens stay as they
+    are."""
     shape, qt, qh = _heads("sdpa_cached", "q", q)
     _, ot, oh = _heads("sdpa_cached", "o", o, shape)
     if q.dtype != torch.bfloat16 or o.dtype != torch.bfloat16:
