@@ -21,7 +21,7 @@ LIB = OUT_DIR / "libttlhip.so"
 OBJ_DIR = CSRC / "_build"
 
 SOURCES = ["runtime.hip", "eltwise.hip", "matmul.hip", "matmul_direct.hip", "bfp8.hip", "sdpa.hip", "layout.hip",
-           "kvcache.hip", "sdpa_cached.hip"]
+           "kvcache.hip", "sdpa_cached.hip", "fp8_rows.hip", "fp8_matmul.hip"]
 
 ARCH = "gfx950"
 

@@ -100,6 +100,9 @@ class KVCache(C.Structure):
 # ttlh_kv_cache formats of codes
 CACHE_INT8, CACHE_E4M3 = 0, 1
 
+# ttlh_fp8_glu activations
+GLU_SILU, GLU_GELU = 0, 1
+
 # The structs' layouts for struct.pack, which builds a launch's argument arrays
 # in a microsecond where one ctypes object per step takes about one each.
 INSTR_FMT, OPERAND_FMT, ROW_REDUCE_FMT = "3Bxff", "Qii6q", "QQiiQifQiiq"
@@ -165,6 +168,12 @@ SIGNATURES = {
                                 C.c_float, _vp, _i64, _vp]),
     "ttlh_rope": (_int, [_vp, _vp, _int, _vp, _int, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i64,
                          _i64, _int, C.c_float, _int, _vp]),
+    "ttlh_fp8_quant": (_int, [_vp, _i64, _int, _vp, _i64, _vp, _i64, _i64, _i64, _vp]),
+    "ttlh_fp8_rms_norm": (_int, [_vp, _i64, _vp, _i64, _vp, _i64, _int, _vp, _int, C.c_float, _vp,
+                                 _i64, _vp, _i64, _i64, _i64, _vp]),
+    "ttlh_fp8_glu": (_int, [_vp, _i64, _vp, _i64, _int, _int, _vp, _i64, _vp, _i64, _i64, _i64, _vp]),
+    "ttlh_matmul_fp8": (_int, [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _int, _i64, _i64,
+                               _i64, _i64, _vp]),
     "ttlh_last_error": (C.c_char_p, []),
     "ttlh_version": (_int, []),
 }

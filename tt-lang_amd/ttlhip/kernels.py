@@ -993,3 +993,221 @@ def sdpa_cached(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
         _with_workspace(q.device, stream, nbytes, sp, launch)
     else:
         launch(0)
+
+
+# --- linear layers in 8-bit floating point --------------------------------------
+
+FP8_GROUP = 128  # values of a row that share a scale (weights: of 128 rows)
+_E4M3, _E8M0 = torch.float8_e4m3fn, torch.float8_e8m0fnu
+GLU_ACTS = {"silu": L.GLU_SILU, "gelu": L.GLU_GELU}
+
+
+def fp8_scales(rows: int, dim: int, device=None) -> torch.Tensor:
+    """Memory for the scales of [rows, dim] values (of weights: a row for each 128 of
+    theirs): e8m0 [ceil(dim / 512), rows, 4], the scale of row r's values 128 g ..
+    128 g + 127 at [g // 4, r, g % 4]; all 2^-126, the scale of zeros."""
+    if rows < 0 or dim <= 0:
+        raise ValueError(f"fp8_scales: bad sizes {rows} x {dim}")
+    if device is None:
+        device = "cuda" if torch.cuda.is_available() else "cpu"
+    return torch.ones(-(-dim // (4 * FP8_GROUP)), rows, 4, dtype=torch.uint8, device=device).view(_E8M0)
+
+
+def fp8_weights(w: torch.Tensor):
+    """(codes, scales) of weights w [outputs, inputs] for matmul_fp8(): e4m3 codes with
+    the smallest power of two for each 128 x 128 block whose 448 fold holds it; made once,
+    with torch, where w is.  Weights that are not finite are refused."""
+    if w.dim() != 2 or w.shape[1] == 0 or not w.is_floating_point():
+        raise ValueError(f"fp8_weights: w must be a matrix of numbers, got {w.dtype} {tuple(w.shape)}")
+    w = w.detach().float()
+    if not bool(torch.isfinite(w).all()):
+        raise ValueError("fp8_weights: w must be finite")
+    n, k = w.shape
+    blocks, groups = -(-n // FP8_GROUP), -(-k // FP8_GROUP)
+    full = w.new_zeros(blocks * FP8_GROUP, groups * FP8_GROUP)
+    full[:n, :k] = w
+    full = full.view(blocks, FP8_GROUP, groups, FP8_GROUP)
+    m, e = torch.frexp(full.abs().amax((1, 3)))  # 448 = 0.875 x 2^9
+    e = torch.where(m > 0, e - 9 + (m > 0.875).int(), torch.full_like(e, -126)).clamp(min=-126)
+    codes = torch.ldexp(full, -e[:, None, :, None]).to(_E4M3).view(blocks * FP8_GROUP, -1)
+    scales = fp8_scales(blocks, k, w.device)
+    bits = torch.ones(blocks, 4 * scales.shape[0], dtype=torch.uint8, device=w.device)
+    bits[:, :groups] = (e + 127).to(torch.uint8)
+    scales.view(torch.uint8).copy_(bits.view(blocks, -1, 4).transpose(0, 1))
+    return codes[:n, :k].contiguous(), scales
+
+
+def _fp8_rows(what: str, name: str, t: torch.Tensor, shape=None):
+    """(shape, row stride) of t, [rows, dim] with unit stride along dim."""
+    s = t.shape
+    if len(s) != 2 or (shape is not None and s != shape):
+        raise ValueError(f"{what}: {name} must be [rows, dim]"
+                         f"{'' if shape is None else f' = {tuple(shape)}'}, got {tuple(s)}")
+    a, b = t.stride()
+    if b != 1 and s[1] > 1:
+        raise ValueError(f"{what}: {name} must have unit column stride")
+    return s, a if s[0] > 1 else s[1]
+
+
+def _fp8_scales(what: str, name: str, t: torch.Tensor, rows: int, dim: int) -> int:
+    """The stride of words, in dwords, of scales for [rows, dim] values."""
+    words = -(-dim // (4 * FP8_GROUP))
+    if t.dtype != _E8M0 or t.shape != (words, rows, 4):
+        raise ValueError(f"{what}: {name} must be float8_e8m0fnu [{words}, {rows}, 4] (fp8_scales()), got "
+                         f"{t.dtype} {tuple(t.shape)}")
+    a, b, c = t.stride()
+    if c != 1 or (b != 4 and rows > 1) or (a % 4 and words > 1) or t.data_ptr() % 4:
+        raise ValueError(f"{what}: {name} must have each row's four scales in one aligned dword, rows "
+                         f"beside each other")
+    return a // 4 if words > 1 else rows
+
+
+def _span(t: torch.Tensor):
+    """(first byte, past the last byte) that t can reach."""
+    size, last = t.element_size(), 0
+    for n, s in zip(t.shape, t.stride()):
+        last += (n - 1) * s
+    return t.data_ptr(), t.data_ptr() + (last + 1) * size
+
+
+def _apart(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two tensors have no memory in common; for matrices of one row pitch also
+    where the rows of one lie between those of the other."""
+    if a.numel() == 0 or b.numel() == 0:
+        return True
+    (a0, a1), (b0, b1) = _span(a), _span(b)
+    if a1 <= b0 or b1 <= a0:
+        return True
+    if a.dim() != 2 or b.dim() != 2 or a.shape[0] < 2 or b.shape[0] < 2:
+        return False
+    pitch = a.stride(0) * a.element_size()
+    if pitch <= 0 or pitch != b.stride(0) * b.element_size():
+        return False
+    wide_a, wide_b = a.shape[1] * a.element_size(), b.shape[1] * b.element_size()
+    d = (b0 - a0) % pitch
+    return wide_a <= d and d + wide_b <= pitch
+
+
+def _fp8_out(what: str, codes: torch.Tensor, scales: torch.Tensor, shape, others):
+    """(row stride of codes, stride of the scales' words) of an operator's outputs."""
+    rows, dim = shape
+    _, ld = _fp8_rows(what, "codes", codes, shape)
+    if codes.dtype != _E4M3:
+        raise ValueError(f"{what}: codes must be float8_e4m3fn, got {codes.dtype}")
+    if dim == 0:
+        raise ValueError(f"{what}: rows must have values")
+    sld = _fp8_scales(what, "scales", scales, rows, dim)
+    if (rows > 1 and ld < dim) or (scales.shape[0] > 1 and sld < rows):
+        raise ValueError(f"{what}: codes and scales must not repeat their elements")
+    for t in others + (scales,):
+        if not _apart(codes, t) or (t is not scales and not _apart(scales, t)):
+            raise ValueError(f"{what}: codes and scales must have memory of their own")
+    return ld, sld
+
+
+def quant_fp8(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, stream=None) -> None:
+    """x [rows, dim] (bf16 or f32, any row pitch) into e4m3 codes [rows, dim] with a scale
+    for each 128 values of a row (fp8_scales()): a value is code * scale.
+
+    A scale is the smallest power of two, from 2^-126 on, whose 448 fold holds its group;
+    a code is the quotient rounded to nearest, ties to even.  Groups past a row's last one
+    get the scale of zeros, 2^-126.  A value that is not finite makes its group's scale NaN
+    and its codes zeros."""
+    shape, ld = _fp8_rows("quant_fp8", "x", x)
+    cl, sl = _fp8_out("quant_fp8", codes, scales, shape, (x,))
+    code = L.dtype_code(x.dtype)
+    _check_on_one_device("quant_fp8", (x, codes, scales), stream)
+    L.call("ttlh_fp8_quant", x.data_ptr(), ld, code, codes.data_ptr(), cl, scales.data_ptr(), sl,
+           shape[0], shape[1], L.stream_ptr(stream))
+
+
+def rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor,
+                 eps: float = 1e-6, residual: Optional[torch.Tensor] = None,
+                 total: Optional[torch.Tensor] = None, stream=None) -> None:
+    """The root-mean-square norm t / sqrt(mean(t^2) + eps) * weight of t = x + residual
+    (or of x) into codes and scales as quant_fp8() makes them.
+
+    x, residual: bf16 or f32 [rows, dim], any row pitch; weight: bf16 or f32 [dim].
+    total: gets t, rounded to x's dtype; it may be residual or x itself.  The norm is that
+    of t before this rounding."""
+    shape, ld = _fp8_rows("rms_norm_fp8", "x", x)
+    if weight.shape != (shape[1],) or not weight.is_contiguous():
+        raise ValueError(f"rms_norm_fp8: weight must be contiguous [{shape[1]}], got {tuple(weight.shape)}")
+    tensors, rl, tl = (x, weight), 0, 0
+    for name, t in (("residual", residual), ("total", total)):
+        if t is None:
+            continue
+        _, s = _fp8_rows("rms_norm_fp8", name, t, shape)
+        if t.dtype != x.dtype:
+            raise ValueError(f"rms_norm_fp8: {name} must be {x.dtype} as x is, got {t.dtype}")
+        if name == "total":
+            tl = s
+            if shape[0] > 1 and s < shape[1]:
+                raise ValueError("rms_norm_fp8: total must not repeat its elements")
+            for other in tensors:
+                same = (other is not weight and t.data_ptr() == other.data_ptr()
+                        and t.stride() == other.stride())
+                if not same and not _apart(t, other):
+                    raise ValueError("rms_norm_fp8: total may be x or residual itself, not another view "
+                                     "of an operand's memory")
+        else:
+            rl = s
+        tensors += (t,)
+    cl, sl = _fp8_out("rms_norm_fp8", codes, scales, shape, tensors)
+    code, wcode = L.dtype_code(x.dtype), L.dtype_code(weight.dtype)
+    _check_on_one_device("rms_norm_fp8", tensors + (codes, scales), stream)
+    L.call("ttlh_fp8_rms_norm", x.data_ptr(), ld, 0 if residual is None else residual.data_ptr(), rl,
+           0 if total is None else total.data_ptr(), tl, code, weight.data_ptr(), wcode, eps,
+           codes.data_ptr(), cl, scales.data_ptr(), sl, shape[0], shape[1], L.stream_ptr(stream))
+
+
+def glu_fp8(gate: torch.Tensor, up: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor,
+            act: str = "silu", stream=None) -> None:
+    """The gated activation act(gate) * up into codes and scales as quant_fp8() makes
+    them.  gate, up: bf16 or f32 [rows, dim], any row pitch (the halves of one product's
+    result).  act: "silu", g / (1 + e^-g), or "gelu", g (1 + erf(g / sqrt 2)) / 2."""
+    shape, gl = _fp8_rows("glu_fp8", "gate", gate)
+    _, ul = _fp8_rows("glu_fp8", "up", up, shape)
+    if up.dtype != gate.dtype:
+        raise ValueError(f"glu_fp8: up must be {gate.dtype} as gate is, got {up.dtype}")
+    if act not in GLU_ACTS:
+        raise ValueError(f"glu_fp8: act must be one of {sorted(GLU_ACTS)}, got {act!r}")
+    cl, sl = _fp8_out("glu_fp8", codes, scales, shape, (gate, up))
+    code = L.dtype_code(gate.dtype)
+    _check_on_one_device("glu_fp8", (gate, up, codes, scales), stream)
+    L.call("ttlh_fp8_glu", gate.data_ptr(), gl, up.data_ptr(), ul, code, GLU_ACTS[act],
+           codes.data_ptr(), cl, scales.data_ptr(), sl, shape[0], shape[1], L.stream_ptr(stream))
+
+
+def matmul_fp8(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor,
+               c: torch.Tensor, stream=None) -> None:
+    """c [M, N] (bf16 or f32, any row pitch) = x [M, K] @ w [N, K]^T of e4m3 codes with
+    their scales: x's and x_scale from quant_fp8(), rms_norm_fp8() or glu_fp8(), w's, with a
+    scale for each 128 x 128 block, from fp8_weights().
+
+    K is a multiple of 16; rows of codes start on 16 bytes.  fp32 accumulation; for a bf16
+    result each eight neighbouring products are aligned to 2^-13 of the largest of them (the
+    fp8 matrix instruction), for an f32 result they are added as fp32 (bf16 instructions, at
+    half the rate).  A NaN scale makes its row (of w: the block's outputs) NaN."""
+    (M, K), xl = _fp8_rows("matmul_fp8", "x", x)
+    (N, kw), wl = _fp8_rows("matmul_fp8", "w", w)
+    shape, cl = _fp8_rows("matmul_fp8", "c", c)
+    if kw != K or shape != (M, N):
+        raise ValueError(f"matmul_fp8: shapes {(M, K)} @ {(N, kw)}^T -> {tuple(shape)}")
+    if x.dtype != _E4M3 or w.dtype != _E4M3:
+        raise ValueError(f"matmul_fp8: x and w must be float8_e4m3fn, got {x.dtype} and {w.dtype}")
+    if K == 0 or K % 16:
+        raise ValueError(f"matmul_fp8: K must be a positive multiple of 16, got {K}")
+    if (x.data_ptr() | w.data_ptr() | (xl if M > 1 else 0) | (wl if N > 1 else 0)) & 15:
+        raise ValueError("matmul_fp8: rows of x and w must start on 16 bytes")
+    xsl = _fp8_scales("matmul_fp8", "x_scale", x_scale, M, K)
+    wsl = _fp8_scales("matmul_fp8", "w_scale", w_scale, -(-N // FP8_GROUP), K)
+    if M > 1 and cl < N:
+        raise ValueError("matmul_fp8: c must not repeat its elements")
+    for t in (x, x_scale, w, w_scale):
+        if not _apart(c, t):
+            raise ValueError("matmul_fp8: c must have memory of its own")
+    code = L.dtype_code(c.dtype)
+    _check_on_one_device("matmul_fp8", (x, x_scale, w, w_scale, c), stream)
+    L.call("ttlh_matmul_fp8", x.data_ptr(), xl, x_scale.data_ptr(), xsl, w.data_ptr(), wl,
+           w_scale.data_ptr(), wsl, c.data_ptr(), code, cl, M, N, K, L.stream_ptr(stream))
