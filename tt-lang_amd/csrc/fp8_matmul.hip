@@ -6,22 +6,31 @@
 // instruction of its own, and one accumulator runs through all of K.
 //
 // The fp8 MFMA aligns the products of eight neighbouring k to 2^-13 of the largest of them
-// before it adds them (measured; sums of such eights are right to fp32): 2^-17 of a product's
-// size on average, far below the rounding of a bf16 result.  Results in fp32 (WIDE) keep fp32's
-// accuracy: codes times scale become bf16, which holds them exactly, and go through bf16 MFMAs,
-// at half the rate.
+// before it adds them (measured; sums of such eights are right to fp32), which leaves an error of
+// 2^-19 of the products' sizes on average, far below the rounding of a bf16 result.  Results in
+// fp32 (WIDE) keep fp32's accuracy: codes times scale become bf16, which holds them exactly, and go
+// through bf16 MFMAs, at half the rate.
 //
-// fp8_direct_kernel: few rows of x, HBM bound by w.  Operands go from memory straight into the
-// MFMA registers; a workgroup has a block of outputs and its waves divide K in words of 512,
-// each with all loads of a word in flight; their sums meet in LDS and are added in wave order.
-//
-// fp8_block_kernel: many rows, MFMA bound.  Stages of 64 codes of K reach LDS by direct-to-LDS
-// loads, two to three stages ahead in a ring of four buffers, one barrier a stage; a wave has
-// 128 x 128 (T = 4) or 64 x 64 results, and its fragments of a stage are read while the stage
-// before it is multiplied.  8192 x 22016 x 4096: 703 us, 2.1 PFLOP/s (64 x 64: 950 us).
+// Three kernels (choose_form, at the end, has the rule).  All of them bring whole lines of 128
+// codes, a group, to LDS by direct-to-LDS loads of eight lanes a row: lanes of one load that lie in
+// different rows, or halves of lines at different times, cost up to four times the rate at which a CU
+// takes them (64 bytes a clock), and that rate, not memory, bounds the middle sizes.  A chunk of 16
+// codes lies at its place XOR row / 2, so that an MFMA operand's reads meet no bank twice.  Codes past
+// K are loaded as zeros, from kZeros: no kernel has a case for the last group.
+//  * fp8_direct_kernel: few results.  The waves of a workgroup divide K, each with LDS of its own and
+//    no barrier, and their sums are added in wave order.  1 x 22016 x 4096 19.0 us (4.7 TB/s of
+//    weights; one quarter of the lanes' rate, straight to registers: 19.2, but 32 x 4096 x 11008 26.0 ->
+//    16.2), 64 x 4096 x 4096 6.9 us.
+//  * fp8_block_kernel: a ring of three buffers and one barrier a group, 64 x 64 to 128 x 256 results.
+//    512 x 4096 x 4096 15.0 us (halves of lines: 21), 2048 x 4096 x 4096 36.4 us.
+//  * fp8_large_kernel: 256 x 256, bf16 results.  8192 x 22016 x 4096 584 us (2.5 PFLOP/s; in stages of
+//    half lines and a ring of four 703), 8192^3 397 us (2.8 PFLOP/s): the MFMAs are busy 78% of the
+//    cycles, at the clock that the power cap leaves (1.5 GHz).
 
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
+#include <utility>
 
 #include "ttlh_common.h"
 #include "ttlh_fp8.h"
@@ -33,6 +42,30 @@ typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef __attribute__((address_space(3))) void lds_void;
+
+// s_waitcnt: at most n vector loads outstanding; all LDS reads done
+constexpr int vmcnt_imm(int n) { return 0x0F70 | (n & 0xF) | ((n >> 4) << 14); }
+constexpr int kLdsDone = 0xC07F;
+
+// until at most n rounds of LOADS loads are outstanding
+template <int LOADS>
+__device__ __forceinline__ void wait_behind(int n) {
+  static_assert(2 * LOADS < 64, "what the counter holds");
+  if (n >= 3) __builtin_amdgcn_s_waitcnt(vmcnt_imm(3 * LOADS < 63 ? 3 * LOADS : 63));
+  else if (n == 2) __builtin_amdgcn_s_waitcnt(vmcnt_imm(2 * LOADS));
+  else if (n == 1) __builtin_amdgcn_s_waitcnt(vmcnt_imm(LOADS));
+  else __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
+}
+
+// What is read in the place of codes past K.
+__device__ __attribute__((aligned(16))) const uint32_t kZeros[4] = {0u, 0u, 0u, 0u};
+
+// 16 bytes at src + k a lane, or zeros, to LDS: lane l's land at to + 16 l.
+__device__ __forceinline__ void load_lds(const uint8_t* src, int k, bool there, uint8_t* to) {
+  const uint8_t* from = there ? src + k : reinterpret_cast<const uint8_t*>(kZeros);
+  __builtin_amdgcn_global_load_lds(from, (lds_void*)to, 16, 0, 0);
+}
 
 struct Fp8Args {
   const uint8_t* x;
@@ -59,16 +92,14 @@ __device__ __forceinline__ i32x8 all8(const Frag& f) {
                static_cast<int>(f.hi[2]), static_cast<int>(f.hi[3])};
 }
 
-// eight codes (dwords a, b) times 2^(s - 127) as bf16; NaN where s is
+// eight codes (dwords a, b) times 2^(s - 127) as bf16; NaN where s is 255, whatever the codes are
 __device__ __forceinline__ bf16x8 widened(uint32_t a, uint32_t b, uint32_t s) {
   const float scale = __uint_as_float(s << 23);
   const bf16x2 p = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, scale, false);
   const bf16x2 q = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, scale, true);
   const bf16x2 r = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, scale, false);
   const bf16x2 t = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, scale, true);
-  bf16x8 v = {p[0], p[1], q[0], q[1], r[0], r[1], t[0], t[1]};
-  if (s == kScaleNan) v = __builtin_bit_cast(bf16x8, u32x4{0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u});
-  return v;
+  return bf16x8{p[0], p[1], q[0], q[1], r[0], r[1], t[0], t[1]};
 }
 
 // acc += A . B over one group; sa, sb: dwords of scales, the group's in byte J
@@ -128,109 +159,126 @@ __device__ __forceinline__ void store4(const Fp8Args& p, int row, int col, f32x4
   }
 }
 
-// eight neighbouring results of a row in bf16 (p.c_vec; c_vec8: as one store)
-__device__ __forceinline__ void store8(const Fp8Args& p, int row, int col, u32x4 v) {
-  if (row >= p.M || col >= p.N) return;
-  uint16_t* c = static_cast<uint16_t*>(p.c) + row * p.c_ld + col;
-  const int n = p.N - col;
-  if (p.c_vec8 && n >= 8) {
-    *reinterpret_cast<u32x4*>(c) = v;
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (i < n) c[i] = static_cast<uint16_t>(v[i >> 1] >> (16 * (i & 1)));
-  }
-}
-
-// MT x 16 rows of x, NT x 16 of w a workgroup.
-template <int MT, int NT, int WAVES, bool WIDE>
-__global__ __launch_bounds__(WAVES * 64) void fp8_direct_kernel(const Fp8Args p) {
+// MT x 16 rows of x, NT x 16 of w a workgroup; wave v of WAVES takes the groups v, v + WAVES ..
+// of K, AHEAD (2 to 4) of them in flight.
+template <int MT, int NT, int WAVES, int AHEAD, bool WIDE>
+__device__ __forceinline__ void fp8_direct(const Fp8Args& p) {
+  static_assert(WAVES % 4 == 0 && 128 % (NT * 16) == 0, "one byte of the scales a wave, one block of w's");
+  constexpr int kRows = (MT + NT) * 16;  // of a wave's group: those of w, then those of x
+  constexpr int kSlot = kRows * kFp8Group;
+  __shared__ __attribute__((aligned(16))) uint8_t b0[WAVES * kSlot], b1[WAVES * kSlot],
+      b2[AHEAD > 2 ? WAVES * kSlot : 16], b3[AHEAD > 3 ? WAVES * kSlot : 16];
   int bm, bn;
   block_of(p, bm, bn);
   // (uniform, and known to be: an MFMA behind a branch that the compiler takes for divergent
   // runs whether or not its lanes are masked)
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int r = lane & 15, q = lane >> 4;
+  const auto slot = [&](int a) -> uint8_t* {
+    return (a == 0 ? b0 : a == 1 ? b1 : a == 2 ? b2 : b3) + wave * kSlot;
+  };
   const int m0 = bm * MT * 16, n0 = bn * NT * 16;
-  const uint8_t *xp[MT], *wp[NT];
-  const uint32_t *xs[MT], *ws[NT];
-  // rows past the last one are read as the last one: they reach results that are not stored
+  const int groups = (p.K + kFp8Group - 1) / kFp8Group;
+  const int n = groups > wave ? (groups - wave + WAVES - 1) / WAVES : 0;  // of this wave
+
+  // Loads: eight rows of 128 codes an instruction, eight lanes a row (a row's 16 bytes by lanes 16
+  // apart, as the MFMA has them, are a quarter of the rate: 16 bytes a clock and CU).  Chunk c of
+  // row r of a tile lies at c ^ (r / 2 & 7).  Rows past the last one are read as the last one:
+  // they reach results that are not stored.
+  const int chunk = 16 * ((lane & 7) ^ (lane >> 4));  // of a tile's rows 0 to 7; of 8 to 15: ^ 64
+  const uint8_t* src[kRows / 8];
 #pragma unroll
-  for (int i = 0; i < MT; ++i) {
-    const int row = min(m0 + 16 * i + r, p.M - 1);
-    xp[i] = p.x + row * p.x_ld + 16 * q;
-    xs[i] = p.xs + row;
+  for (int i = 0; i < kRows / 8; ++i) {
+    const int row = 8 * i + (lane >> 3);
+    src[i] = (i < 2 * NT ? p.w + min(n0 + row, p.N - 1) * p.w_ld
+                         : p.x + min(m0 + row - 16 * NT, p.M - 1) * p.x_ld) + (i & 1 ? chunk ^ 64 : chunk);
   }
+  const int r = lane & 15, q = lane >> 4;
+  const uint8_t* ws = reinterpret_cast<const uint8_t*>(p.ws + n0 / kFp8Group) + (wave & 3);
+  const uint8_t* xs[MT];
 #pragma unroll
-  for (int j = 0; j < NT; ++j) {
-    const int row = min(n0 + 16 * j + r, p.N - 1);
-    wp[j] = p.w + row * p.w_ld + 16 * q;
-    ws[j] = p.ws + row / kFp8Group;
-  }
+  for (int i = 0; i < MT; ++i)
+    xs[i] = reinterpret_cast<const uint8_t*>(p.xs + min(m0 + 16 * i + r, p.M - 1)) + (wave & 3);
+  uint32_t sw[AHEAD], sx[AHEAD][MT];
+  const auto load = [&](int a, int i) {  // (past the wave's last group: zeros)
+    const int g = wave + WAVES * i, k = g * kFp8Group, word = min(g, groups - 1) >> 2;
+    const bool even = k + chunk < p.K, odd = k + (chunk ^ 64) < p.K;
+#pragma unroll
+    for (int j = 0; j < kRows / 8; ++j) load_lds(src[j], k, j & 1 ? odd : even, slot(a) + j * 1024);
+    sw[a] = ws[4 * word * p.ws_ld];
+#pragma unroll
+    for (int j = 0; j < MT; ++j) sx[a][j] = xs[j][4 * word * p.xs_ld];
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  constexpr int kLoads = kRows / 8 + 1 + MT;  // of a group
+
   f32x4 acc[MT][NT];
 #pragma unroll
   for (int i = 0; i < MT; ++i)
 #pragma unroll
     for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-  // chunk (of 16 codes) k .. of a lane, zeros past K
-  const auto chunk = [&](const uint8_t* base, int k) {
-    return k + 16 * q < p.K ? *reinterpret_cast<const u32x4*>(base + k) : u32x4{0u, 0u, 0u, 0u};
-  };
-  const int words = (p.K + kFp8Word - 1) / kFp8Word;
-  for (int word = wave; word < words; word += WAVES) {
-    const int k0 = word * kFp8Word;
-    uint32_t sx[MT], sw[NT];
-    Frag a[NT][4], b[MT][4];
-#pragma unroll
-    for (int j = 0; j < NT; ++j) sw[j] = ws[j][word * p.ws_ld];
-#pragma unroll
-    for (int i = 0; i < MT; ++i) sx[i] = xs[i][word * p.xs_ld];
-#pragma unroll
-    for (int g = 0; g < 4; ++g) {
-#pragma unroll
-      for (int j = 0; j < NT; ++j)
-        a[j][g] = Frag{chunk(wp[j], k0 + 128 * g), chunk(wp[j], k0 + 128 * g + 64)};
-#pragma unroll
-      for (int i = 0; i < MT; ++i)
-        b[i][g] = Frag{chunk(xp[i], k0 + 128 * g), chunk(xp[i], k0 + 128 * g + 64)};
-    }
+  // A lane has row r of a tile, chunks q and q + 4.
+  const int at_lo = r * kFp8Group + 16 * (q ^ (r >> 1)), at_hi = at_lo ^ 64;
+  const auto multiply = [&](int a) {
+    Frag w[NT], x[MT];
 #pragma unroll
     for (int j = 0; j < NT; ++j)
+      w[j] = Frag{*reinterpret_cast<const u32x4*>(slot(a) + j * 2048 + at_lo),
+                  *reinterpret_cast<const u32x4*>(slot(a) + j * 2048 + at_hi)};
 #pragma unroll
-      for (int i = 0; i < MT; ++i) {
-        acc[i][j] = mma16<WIDE, 0>(a[j][0], b[i][0], acc[i][j], sw[j], sx[i]);
-        // (a group past K has codes of zero, but its scale need not be a number)
-        if (k0 + 128 < p.K) acc[i][j] = mma16<WIDE, 1>(a[j][1], b[i][1], acc[i][j], sw[j], sx[i]);
-        if (k0 + 256 < p.K) acc[i][j] = mma16<WIDE, 2>(a[j][2], b[i][2], acc[i][j], sw[j], sx[i]);
-        if (k0 + 384 < p.K) acc[i][j] = mma16<WIDE, 3>(a[j][3], b[i][3], acc[i][j], sw[j], sx[i]);
-      }
+    for (int i = 0; i < MT; ++i)
+      x[i] = Frag{*reinterpret_cast<const u32x4*>(slot(a) + (NT + i) * 2048 + at_lo),
+                  *reinterpret_cast<const u32x4*>(slot(a) + (NT + i) * 2048 + at_hi)};
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int j = 0; j < NT; ++j) acc[i][j] = mma16<WIDE, 0>(w[j], x[i], acc[i][j], sw[a], sx[a][i]);
+    __builtin_amdgcn_sched_barrier(0);  // (the slot is read before it is loaded anew)
+  };
+#pragma unroll
+  for (int a = 0; a < AHEAD; ++a) load(a, a);
+  int i = 0;
+  for (; i + AHEAD < n; i += AHEAD) {
+#pragma unroll
+    for (int a = 0; a < AHEAD; ++a) {
+      wait_behind<kLoads>(AHEAD - 1);
+      multiply(a);
+      load(a, i + a + AHEAD);
+    }
   }
-  // a lane has four neighbouring results of row r: columns 16 j + 4 q ..
-  __shared__ f32x4 part[WAVES][MT * NT][64];
+#pragma unroll
+  for (int a = 0; a < AHEAD; ++a)
+    if (i + a < n) {
+      wait_behind<kLoads>(AHEAD - 1 - a);
+      multiply(a);
+    }
+  __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));  // (no load of a wave without groups is left to land)
+  __syncthreads();
+  // The waves' sums, where the codes were: a lane has four neighbouring results of row r, columns
+  // 16 j + 4 q ..
+  static_assert(MT * NT * 1024 <= kSlot, "a wave's sums fit its slot");
+  f32x4* part = reinterpret_cast<f32x4*>(b0);
 #pragma unroll
   for (int i = 0; i < MT; ++i)
 #pragma unroll
-    for (int j = 0; j < NT; ++j) part[wave][i * NT + j][lane] = acc[i][j];
+    for (int j = 0; j < NT; ++j) part[(wave * MT * NT + i * NT + j) * 64 + lane] = acc[i][j];
   __syncthreads();
   for (int t = wave; t < MT * NT; t += WAVES) {
-    f32x4 s = part[0][t][lane];
+    f32x4 s = part[t * 64 + lane];
 #pragma unroll
-    for (int v = 1; v < WAVES; ++v) s += part[v][t][lane];
+    for (int v = 1; v < WAVES; ++v) s += part[(v * MT * NT + t) * 64 + lane];
     store4(p, m0 + 16 * (t / NT) + r, n0 + 16 * (t % NT) + 4 * q, s);
   }
 }
 
-// --- many rows: through LDS ---------------------------------------------------------
+template <int MT, int NT, int WAVES, int AHEAD, bool WIDE>
+__global__ __launch_bounds__(WAVES * 64) void fp8_direct_kernel(const Fp8Args p) {
+  fp8_direct<MT, NT, WAVES, AHEAD, WIDE>(p);
+}
+
+// --- more results ---------------------------------------------------------------
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
-typedef __attribute__((address_space(3))) void lds_void;
 
-constexpr int kBlockThreads = 256;
-constexpr int kStage = 64;  // codes of K a stage
-
-// s_waitcnt: at most n vector loads outstanding; all LDS reads done
-constexpr int vmcnt_imm(int n) { return 0x0F70 | (n & 0xF) | ((n >> 4) << 14); }
-constexpr int kLdsDone = 0xC07F;
 
 // One k = 64 step of a 32 x 32 tile; e: the scales' byte
 template <bool WIDE, int E>
@@ -263,225 +311,423 @@ __device__ __forceinline__ void banded_block(const Fp8Args& p, int band, int& bm
   bm = b * band + in - bn * rows;
 }
 
-// A wave has T x T tiles of 32 x 32, four waves a block of 64 T x 64 T.
-template <int T, bool WIDE>
-__device__ __forceinline__ void fp8_block(const Fp8Args& p) {
-  constexpr int kRows = 64 * T;           // of x, and of w, a block
-  constexpr int kLoads = kRows / 64;      // of 16 bytes a thread for one operand's stage
-  __shared__ __attribute__((aligned(16))) uint8_t x0[kRows * kStage], x1[kRows * kStage],
-      x2[kRows * kStage], x3[kRows * kStage], w0[kRows * kStage], w1[kRows * kStage],
-      w2[kRows * kStage], w3[kRows * kStage];
-  const auto xbuf = [&](auto q) -> uint8_t* {
-    constexpr int Q = decltype(q)::value & 3;
-    return Q == 0 ? x0 : Q == 1 ? x1 : Q == 2 ? x2 : x3;
-  };
-  const auto wbuf = [&](auto q) -> uint8_t* {
-    constexpr int Q = decltype(q)::value & 3;
-    return Q == 0 ? w0 : Q == 1 ? w1 : Q == 2 ? w2 : w3;
-  };
-  int bm, bn;
-  banded_block(p, 4, bm, bn);
-  const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
-  const int wm = (wave & 1) * 32 * T, wn = (wave >> 1) * 32 * T;
-  const int m0 = bm * kRows, n0 = bn * kRows;
-
-  // a thread's loads of a stage: rows i 64 + t / 4; chunk c of row r lies at c ^ (r / 4 & 3)
-  const int chunk = 16 * ((t & 3) ^ (t >> 4 & 3));
-  const uint8_t *xsrc[kLoads], *wsrc[kLoads];
+// A tile of 32 x 32 results from row, col: a lane has row lane % 32 and the columns 8 r + 4 h ..
+// + 3 (r < 4, h = lane / 32).  WHOLE: bf16, all columns exist and eight are one aligned store; the
+// halves of two r change places, so that a lane has eight neighbours.
+template <bool WHOLE>
+__device__ __forceinline__ void store_tile(const Fp8Args& p, int row, int col, const f32x16& v) {
+  const int lane = threadIdx.x & 63, h = lane >> 5;
+  row += lane & 31;
+  if constexpr (!WHOLE) {
 #pragma unroll
-  for (int i = 0; i < kLoads; ++i) {
-    // (rows past the last one are read as the last one: they reach results that are not stored)
-    xsrc[i] = p.x + static_cast<int64_t>(min(m0 + 64 * i + (t >> 2), p.M - 1)) * p.x_ld + chunk;
-    wsrc[i] = p.w + static_cast<int64_t>(min(n0 + 64 * i + (t >> 2), p.N - 1)) * p.w_ld + chunk;
-  }
-  const int base = wave * 1024;  // where a wave's lanes land, 16 bytes each
-  const auto load_piece = [&](auto q, int k0, int i) {
-    if (i < kLoads)
-      __builtin_amdgcn_global_load_lds(xsrc[i] + k0, (lds_void*)(xbuf(q) + i * 4096 + base), 16, 0, 0);
-    else
-      __builtin_amdgcn_global_load_lds(wsrc[i - kLoads] + k0,
-                                       (lds_void*)(wbuf(q) + (i - kLoads) * 4096 + base), 16, 0, 0);
-  };
-  const int nk = (p.K + kStage - 1) / kStage, full = p.K / kStage;
-  // any stage; chunks past K are read as the last one, and not used
-  const auto load_stage = [&](auto q, int s) {
-    const int k0 = min(s * kStage, p.K - 16 - chunk);
+    for (int r = 0; r < 4; ++r)
+      store4(p, row, col + 8 * r + 4 * h, f32x4{v[4 * r], v[4 * r + 1], v[4 * r + 2], v[4 * r + 3]});
+  } else {
+    u32x4* c = reinterpret_cast<u32x4*>(static_cast<uint16_t*>(p.c) + row * p.c_ld + col + 8 * h);
 #pragma unroll
-    for (int i = 0; i < 2 * kLoads; ++i) load_piece(q, k0, i);
-  };
-
-  // fragments: row lane % 32 of a tile, chunks 2 h and 2 h + 1 with h = lane / 32
-  const int l32 = lane & 31, h = lane >> 5, xr = l32 >> 2 & 3;
-  const int at_lo = l32 * kStage + ((2 * h) ^ xr) * 16, at_hi = l32 * kStage + ((2 * h + 1) ^ xr) * 16;
-  struct Frags {
-    Frag w[T], x[T];
-  };
-  Frags f0, f1;
-  // piece y of the 4 T that read a stage's fragments
-  const auto read_piece = [&](auto q, Frags& f, int y) {
-    const uint8_t* b = y < 2 * T ? wbuf(q) + wn * kStage : xbuf(q) + wm * kStage;
-    const int i = (y < 2 * T ? y : y - 2 * T) >> 1;
-    const u32x4 v = *reinterpret_cast<const u32x4*>(b + i * 32 * kStage + (y & 1 ? at_hi : at_lo));
-    Frag& g = y < 2 * T ? f.w[i] : f.x[i];
-    if (y & 1) g.hi = v;
-    else g.lo = v;
-  };
-  const auto read_stage = [&](auto q, Frags& f, int s) {
-#pragma unroll
-    for (int y = 0; y < 4 * T; ++y) read_piece(q, f, y);
-    const int left = p.K - s * kStage;
-    if (left < kStage) {  // zeros past K
-      const u32x4 zero = {0u, 0u, 0u, 0u};
-#pragma unroll
-      for (int i = 0; i < T; ++i) {
-        if (32 * h >= left) f.w[i].lo = f.x[i].lo = zero;
-        if (32 * h + 16 >= left) f.w[i].hi = f.x[i].hi = zero;
-      }
-    }
-  };
-
-  f32x16 acc[T][T];  // [w tile][x tile]
-#pragma unroll
-  for (int i = 0; i < T; ++i)
-#pragma unroll
-    for (int j = 0; j < T; ++j)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
-
-  // scales of four stages (two groups: half a word of four)
-  const int words = (p.K + kFp8Word - 1) / kFp8Word;
-  const uint32_t* ws = p.ws + min(n0 + wn, p.N - 1) / kFp8Group;  // (a wave's rows of w are in one block)
-  const uint32_t* xs[T];
-#pragma unroll
-  for (int j = 0; j < T; ++j) xs[j] = p.xs + min(m0 + wm + 32 * j + l32, p.M - 1);
-  uint32_t sw, sx[T], next_w, next_x[T];
-  const auto load_scales = [&](int four) {  // stages 4 four ..
-    const int word = min(four >> 1, words - 1);
-    next_w = ws[word * p.ws_ld];
-#pragma unroll
-    for (int j = 0; j < T; ++j) next_x[j] = xs[j][word * p.xs_ld];
-  };
-  const auto take_scales = [&](int four) {
-    const int by = 16 * (four & 1);
-    sw = next_w >> by;
-#pragma unroll
-    for (int j = 0; j < T; ++j) sx[j] = next_x[j] >> by;
-  };
-
-  using I0 = std::integral_constant<int, 0>;
-  using I1 = std::integral_constant<int, 1>;
-  using I2 = std::integral_constant<int, 2>;
-  using I3 = std::integral_constant<int, 3>;
-  load_scales(0);
-  load_stage(I0(), 0);
-  if (1 < nk) load_stage(I1(), 1);
-  if (2 < nk) load_stage(I2(), 2);
-  if (3 < nk) load_stage(I3(), 3);
-  constexpr int kStageLoads = 2 * kLoads;
-  const auto wait_behind = [&](int stages) {  // at most so many stages' loads are outstanding
-    if (stages >= 3) __builtin_amdgcn_s_waitcnt(vmcnt_imm(3 * kStageLoads));
-    else if (stages == 2) __builtin_amdgcn_s_waitcnt(vmcnt_imm(2 * kStageLoads));
-    else if (stages == 1) __builtin_amdgcn_s_waitcnt(vmcnt_imm(kStageLoads));
-    else __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
-  };
-  wait_behind(min(nk - 1, 3));
-  __builtin_amdgcn_s_barrier();
-  read_stage(I0(), f0, 0);
-
-  // Stage s, in buffers Q = s % 4, whose fragments are in cur.  Behind the barrier every wave has
-  // read its fragments of stage s, so the buffers take stage s + 4, and stage s + 1 has landed.
-  // STEADY: stages up to s + 4 exist and are whole.
-  const auto stage = [&](auto qq, auto steady, Frags& cur, Frags& nxt, int s) {
-    constexpr int Q = decltype(qq)::value, E = Q >> 1;
-    constexpr bool STEADY = decltype(steady)::value;
-    using Next = std::integral_constant<int, (Q + 1) & 3>;
-    __builtin_amdgcn_s_waitcnt(kLdsDone);
-    if constexpr (STEADY) {
-      // (the scales' loads lie behind those of stage s + 1 in the second and third of four)
-      __builtin_amdgcn_s_waitcnt(vmcnt_imm(2 * kStageLoads + (Q == 1 || Q == 2 ? T + 1 : 0)));
-      __builtin_amdgcn_s_barrier();
-      constexpr int kMma = T * T, kReads = 4 * T;
-      int y = 0;
-#pragma unroll
-      for (int v = 0; v < kMma; ++v) {
-        const int i = v / T, j = v % T;
-        acc[i][j] = mma32<WIDE, E>(cur.w[i], cur.x[j], acc[i][j], sw, sx[j]);
-        // the reads in the first three quarters, so that they are done at the barrier
-        const int upto = min(kReads, (v + 1) * kReads * 4 / (3 * kMma));
-#pragma unroll
-        for (int z = 0; z < kReads; ++z)
-          if (z >= y && z < upto) read_piece(Next(), nxt, z);
-        y = upto;
-        // 2 T loads over T T steps
-        const int l0 = v * kStageLoads / kMma, l1 = (v + 1) * kStageLoads / kMma;
-#pragma unroll
-        for (int z = 0; z < kStageLoads; ++z)
-          if (z >= l0 && z < l1) load_piece(qq, (s + 4) * kStage, z);
-        __builtin_amdgcn_sched_barrier(0);
-      }
-    } else {
-      if (s + 1 < nk) wait_behind(min(nk - 2 - s, 2));
-      __builtin_amdgcn_s_barrier();
-      if (s + 1 < nk) read_stage(Next(), nxt, s + 1);
-      if (s + 4 < nk) load_stage(qq, s + 4);
-#pragma unroll
-      for (int i = 0; i < T; ++i)
-#pragma unroll
-        for (int j = 0; j < T; ++j) acc[i][j] = mma32<WIDE, E>(cur.w[i], cur.x[j], acc[i][j], sw, sx[j]);
-      __builtin_amdgcn_sched_barrier(0);
-    }
-  };
-  int s = 0;
-  for (; s + 8 <= full; s += 4) {
-    take_scales(s >> 2);
-    load_scales((s >> 2) + 1);
-    __builtin_amdgcn_sched_barrier(0);
-    stage(I0(), std::true_type(), f0, f1, s);
-    stage(I1(), std::true_type(), f1, f0, s + 1);
-    stage(I2(), std::true_type(), f0, f1, s + 2);
-    stage(I3(), std::true_type(), f1, f0, s + 3);
-  }
-  for (; s < nk; s += 4) {
-    take_scales(s >> 2);
-    load_scales((s >> 2) + 1);
-    stage(I0(), std::false_type(), f0, f1, s);
-    if (s + 1 < nk) stage(I1(), std::false_type(), f1, f0, s + 1);
-    if (s + 2 < nk) stage(I2(), std::false_type(), f0, f1, s + 2);
-    if (s + 3 < nk) stage(I3(), std::false_type(), f1, f0, s + 3);
-  }
-
-  // A lane has row lane % 32 of x's tiles and, of w's, columns 8 r + 4 h .. + 3 (r < 4).  bf16:
-  // the halves of two r change places, so that a lane has eight neighbours.
-#pragma unroll
-  for (int j = 0; j < T; ++j) {
-    const int row = m0 + wm + 32 * j + l32;
-#pragma unroll
-    for (int i = 0; i < T; ++i) {
-      const int col = n0 + wn + 32 * i;
-      if (p.c_f32 || !p.c_vec) {
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-          store4(p, row, col + 8 * r + 4 * h,
-                 f32x4{acc[i][j][4 * r], acc[i][j][4 * r + 1], acc[i][j][4 * r + 2], acc[i][j][4 * r + 3]});
-      } else {
-#pragma unroll
-        for (int r = 0; r < 4; r += 2) {
-          uint32_t a0 = cvt_pk_bf16x2(acc[i][j][4 * r], acc[i][j][4 * r + 1]);
-          uint32_t a1 = cvt_pk_bf16x2(acc[i][j][4 * r + 2], acc[i][j][4 * r + 3]);
-          uint32_t b0 = cvt_pk_bf16x2(acc[i][j][4 * r + 4], acc[i][j][4 * r + 5]);
-          uint32_t b1 = cvt_pk_bf16x2(acc[i][j][4 * r + 6], acc[i][j][4 * r + 7]);
-          const auto e = __builtin_amdgcn_permlane32_swap(a0, b0, false, false);
-          const auto o = __builtin_amdgcn_permlane32_swap(a1, b1, false, false);
-          store8(p, row, col + 8 * (r + h), u32x4{e[0], o[0], e[1], o[1]});
-        }
-      }
+    for (int r = 0; r < 4; r += 2) {
+      const auto e = __builtin_amdgcn_permlane32_swap(cvt_pk_bf16x2(v[4 * r], v[4 * r + 1]),
+                                                      cvt_pk_bf16x2(v[4 * r + 4], v[4 * r + 5]), false, false);
+      const auto o = __builtin_amdgcn_permlane32_swap(cvt_pk_bf16x2(v[4 * r + 2], v[4 * r + 3]),
+                                                      cvt_pk_bf16x2(v[4 * r + 6], v[4 * r + 7]), false, false);
+      if (row < p.M) c[r] = u32x4{e[0], o[0], e[1], o[1]};
     }
   }
 }
 
-template <int T, bool WIDE>
-__global__ __launch_bounds__(kBlockThreads, T == 4 ? 1 : 2) void fp8_block_kernel(const Fp8Args p) {
-  fp8_block<T, WIDE>(p);
+// Results of TX x TW tiles, acc[i][j] tile i of x's rows and j of w's.
+template <int TX, int TW>
+__device__ __forceinline__ void store_tiles(const Fp8Args& p, int m0, int n0, const f32x16 (&acc)[TX][TW]) {
+  const bool whole = !p.c_f32 && p.c_vec8 && n0 + 32 * TW <= p.N;
+  if (whole) {
+#pragma unroll
+    for (int i = 0; i < TX; ++i)
+#pragma unroll
+      for (int j = 0; j < TW; ++j) store_tile<true>(p, m0 + 32 * i, n0 + 32 * j, acc[i][j]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < TX; ++i)
+#pragma unroll
+      for (int j = 0; j < TW; ++j) store_tile<false>(p, m0 + 32 * i, n0 + 32 * j, acc[i][j]);
+  }
+}
+
+// The scales of a wave's TX x 32 rows of x (a lane's in each tile) and of its rows of w, which are
+// in one block: a word, four groups, at a time, one ahead.
+template <int TX>
+struct Scales {
+  const uint32_t* ws;
+  const uint32_t* xs[TX];
+  uint32_t w, x[TX], next_w, next_x[TX];
+  int words;
+  uint32_t past;  // bytes of the last word that are of no group: those scales may be anything
+  static constexpr int kLoads = TX + 1;
+
+  __device__ __forceinline__ Scales(const Fp8Args& p, int m, int n) {
+    words = (p.K + kFp8Word - 1) / kFp8Word;
+    const int last = (p.K - 1) / kFp8Group & 3;
+    past = last == 3 ? 0u : ~0u << (8 * last + 8);
+    ws = p.ws + min(n, p.N - 1) / kFp8Group;
+#pragma unroll
+    for (int i = 0; i < TX; ++i) xs[i] = p.xs + min(m + 32 * i + static_cast<int>(threadIdx.x & 31), p.M - 1);
+    load(p, 0);
+  }
+  __device__ __forceinline__ void load(const Fp8Args& p, int word) {
+    word = min(word, words - 1);
+    next_w = ws[word * p.ws_ld];
+#pragma unroll
+    for (int i = 0; i < TX; ++i) next_x[i] = xs[i][word * p.xs_ld];
+  }
+  __device__ __forceinline__ void take(const Fp8Args& p, int word) {
+    const uint32_t none = word == words - 1 ? past : 0u;  // (their codes are zeros, their scale 1 / 2^127)
+    w = next_w & ~none;
+#pragma unroll
+    for (int i = 0; i < TX; ++i) x[i] = next_x[i] & ~none;
+    load(p, word + 1);
+    __builtin_amdgcn_sched_barrier(0);  // (the waits below count these loads)
+  }
+};
+
+template <typename F, int... I>
+__device__ __forceinline__ void each_until(F f, std::integer_sequence<int, I...>) {
+  (void)(f(std::integral_constant<int, I>()) && ...);
+}
+
+// A wave has TX x TW tiles of 32 x 32 (of x's rows, of w's), four waves a block of 64 TX x 64 TW; a
+// ring of RING (3 or 4) buffers.  A group's fragments are read while the one before it is multiplied.
+template <int TX, int TW, int RING, bool WIDE>
+__device__ __forceinline__ void fp8_block(const Fp8Args& p) {
+  constexpr int kXBytes = 64 * TX * kFp8Group, kWBytes = 64 * TW * kFp8Group;
+  __shared__ __attribute__((aligned(16))) uint8_t x0[kXBytes], x1[kXBytes], x2[kXBytes],
+      x3[RING > 3 ? kXBytes : 16], w0[kWBytes], w1[kWBytes], w2[kWBytes], w3[RING > 3 ? kWBytes : 16];
+  const auto xbuf = [&](auto q) -> uint8_t* {
+    constexpr int Q = decltype(q)::value % RING;
+    return Q == 0 ? x0 : Q == 1 ? x1 : Q == 2 ? x2 : x3;
+  };
+  const auto wbuf = [&](auto q) -> uint8_t* {
+    constexpr int Q = decltype(q)::value % RING;
+    return Q == 0 ? w0 : Q == 1 ? w1 : Q == 2 ? w2 : w3;
+  };
+  const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
+  int bm, bn;
+  banded_block(p, 4, bm, bn);
+  const int wm = (wave & 1) * 32 * TX, wn = (wave >> 1) * 32 * TW;
+  const int m0 = bm * 64 * TX, n0 = bn * 64 * TW;
+  const int groups = (p.K + kFp8Group - 1) / kFp8Group;
+
+  // a thread's loads of a group: rows 32 i + t / 8; chunk c of row r lies at c ^ (r / 2 & 7)
+  const int chunk = 16 * ((t & 7) ^ (t >> 4 & 7));
+  const uint8_t *xsrc[2 * TX], *wsrc[2 * TW];
+  // (rows past the last one are read as the last one: they reach results that are not stored)
+#pragma unroll
+  for (int i = 0; i < 2 * TX; ++i)
+    xsrc[i] = p.x + static_cast<int64_t>(min(m0 + 32 * i + (t >> 3), p.M - 1)) * p.x_ld + chunk;
+#pragma unroll
+  for (int i = 0; i < 2 * TW; ++i)
+    wsrc[i] = p.w + static_cast<int64_t>(min(n0 + 32 * i + (t >> 3), p.N - 1)) * p.w_ld + chunk;
+  const int base = wave * 1024;  // where a wave's lanes land
+  constexpr int kLoads = 2 * (TX + TW);
+  const auto load_piece = [&](auto q, int k, bool there, int i) {
+    if (i < 2 * TX)
+      load_lds(xsrc[i], k, there, xbuf(q) + i * 4096 + base);
+    else
+      load_lds(wsrc[i - 2 * TX], k, there, wbuf(q) + (i - 2 * TX) * 4096 + base);
+  };
+
+  // fragments: row lane % 32 of a tile, chunks 4 k + 2 h and 4 k + 2 h + 1 of 64 codes k, h = lane / 32
+  const int l32 = lane & 31, h = lane >> 5;
+  int at[4];
+#pragma unroll
+  for (int c = 0; c < 4; ++c) at[c] = l32 * kFp8Group + ((4 * (c >> 1) + 2 * h + (c & 1)) ^ (l32 >> 1 & 7)) * 16;
+  struct Frags {
+    Frag w[TW][2], x[TX][2];
+  };
+  Frags f0, f1;
+  constexpr int kReads = 4 * (TX + TW);
+  const auto read_piece = [&](auto q, Frags& f, int y) {  // all of the first 64 codes, then the others
+    const int k = y / (kReads / 2), z = y % (kReads / 2);
+    const uint8_t* b = z < 2 * TW ? wbuf(q) + wn * kFp8Group : xbuf(q) + wm * kFp8Group;
+    const int i = (z < 2 * TW ? z : z - 2 * TW) >> 1;
+    const u32x4 v = *reinterpret_cast<const u32x4*>(b + i * 32 * kFp8Group + at[2 * k + (z & 1)]);
+    Frag& g = z < 2 * TW ? f.w[i][k] : f.x[i][k];
+    if (z & 1) g.hi = v;
+    else g.lo = v;
+  };
+
+  f32x16 acc[TX][TW];
+#pragma unroll
+  for (int i = 0; i < TX; ++i)
+#pragma unroll
+    for (int j = 0; j < TW; ++j)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
+
+  Scales<TX> scale(p, m0 + wm, n0 + wn);
+  each_until([&](auto q) {
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i)
+      load_piece(q, decltype(q)::value * kFp8Group, decltype(q)::value * kFp8Group + chunk < p.K, i);
+    return true;
+  }, std::make_integer_sequence<int, RING>());
+  wait_behind<kLoads>(RING - 1);
+  __builtin_amdgcn_s_barrier();
+#pragma unroll
+  for (int y = 0; y < kReads; ++y) read_piece(std::integral_constant<int, 0>(), f0, y);
+
+  // Group s = U of a turn of the loop, whose fragments are in cur.  Behind the barrier every wave
+  // has read its fragments of group s, so its buffers take group s + RING (past the last one:
+  // zeros), and group s + 1 has landed.
+  const auto group = [&](auto uu, Frags& cur, Frags& nxt, int s) {
+    constexpr int U = decltype(uu)::value, E = U % 4;
+    using Next = std::integral_constant<int, U + 1>;
+    if constexpr (E == 0) scale.take(p, s >> 2);
+    const int k2 = (s + RING) * kFp8Group;
+    const bool there = k2 + chunk < p.K;
+    __builtin_amdgcn_s_waitcnt(kLdsDone);
+    // (are the scales' loads, at a word's first group, among those behind group s + 1's?)
+    __builtin_amdgcn_s_waitcnt(vmcnt_imm((RING - 2) * kLoads + (E <= RING - 2 ? Scales<TX>::kLoads : 0)));
+    __builtin_amdgcn_s_barrier();
+    constexpr int kMma = 2 * TX * TW;
+#pragma unroll
+    for (int v = 0; v < kMma; ++v) {
+      const int k = v / (TX * TW), i = v / TW % TX, j = v % TW;
+      acc[i][j] = mma32<WIDE, E>(cur.w[j][k], cur.x[i][k], acc[i][j], scale.w, scale.x[i]);
+      // the reads in the first three quarters, so that they are done at the barrier
+      const int r0 = min(kReads, v * kReads * 4 / (3 * kMma)), r1 = min(kReads, (v + 1) * kReads * 4 / (3 * kMma));
+#pragma unroll
+      for (int z = 0; z < kReads; ++z)
+        if (z >= r0 && z < r1) read_piece(Next(), nxt, z);
+      const int l0 = v * kLoads / kMma, l1 = (v + 1) * kLoads / kMma;
+#pragma unroll
+      for (int z = 0; z < kLoads; ++z)
+        if (z >= l0 && z < l1) load_piece(uu, k2, there, z);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    return s + 1 < groups;
+  };
+  constexpr int kTurn = RING == 3 ? 12 : 4;
+  for (int s = 0; s < groups; s += kTurn)
+    each_until([&](auto uu) {
+      constexpr int U = decltype(uu)::value;
+      return U % 2 ? group(uu, f1, f0, s + U) : group(uu, f0, f1, s + U);
+    }, std::make_integer_sequence<int, kTurn>());
+  __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));  // (no load is left to land in LDS that another has by then)
+  store_tiles(p, m0 + wm, n0 + wn, acc);
+}
+
+template <int TX, int TW, int RING, bool WIDE>
+__global__ __launch_bounds__(256, TX * TW * RING < 8 ? 2 : 1) void fp8_block_kernel(const Fp8Args p) {
+  fp8_block<TX, TW, RING, WIDE>(p);
+}
+
+// 256 x 256 results a workgroup, 128 x 128 a wave.  Two buffers of a group are all that LDS holds, so
+// a buffer is given back in parts.  A wave keeps all fragments of w of a group, and goes through
+// x's four tiles in turn, one read ahead; while the last one is multiplied it reads the next
+// group's of w and its first of x.  Two barriers a group s:
+//  * behind tile 0: everyone has read w and x's tiles 0 and 1 of s, whose memory takes those of s + 2;
+//    tiles 2 and 3 of s have landed;
+//  * behind tile 2: everyone has read x's tiles 2 and 3; w and tiles 0 and 1 of s + 1 have landed.
+// Loads are 32 to 48 MFMAs ahead of their use.
+__device__ __forceinline__ void fp8_large(const Fp8Args& p) {
+  constexpr int kBytes = 256 * kFp8Group;
+  __shared__ __attribute__((aligned(16))) uint8_t xa0[kBytes / 2], xb0[kBytes / 2], xa1[kBytes / 2],
+      xb1[kBytes / 2], w0[kBytes], w1[kBytes];  // xa: tiles 0 and 1 of both halves of the rows
+  const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
+  int bm, bn;
+  banded_block(p, 4, bm, bn);
+  const int wm = wave & 1, wn = wave >> 1;
+  const int m0 = bm * 256, n0 = bn * 256;
+  const int groups = (p.K + kFp8Group - 1) / kFp8Group;
+
+  // a thread's loads: rows 32 i + t / 8; chunk c of row r lies at c ^ (r / 2 & 7).  Row 32 (4 m + i)
+  // of x is tile i of half m: piece 2 m + (i & 1) of xa or xb.
+  const int chunk = 16 * ((t & 7) ^ (t >> 4 & 7));
+  const uint8_t *xsrc[8], *wsrc[8];
+  // (rows past the last one are read as the last one: they reach results that are not stored)
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    xsrc[i] = p.x + static_cast<int64_t>(min(m0 + 32 * i + (t >> 3), p.M - 1)) * p.x_ld + chunk;
+    wsrc[i] = p.w + static_cast<int64_t>(min(n0 + 32 * i + (t >> 3), p.N - 1)) * p.w_ld + chunk;
+  }
+  const int base = wave * 1024;
+  const auto load_xa = [&](auto q, int k, bool there, int z) {
+    load_lds(xsrc[4 * (z >> 1) + (z & 1)], k, there, (decltype(q)::value & 1 ? xa1 : xa0) + z * 4096 + base);
+  };
+  const auto load_xb = [&](auto q, int k, bool there, int z) {
+    load_lds(xsrc[4 * (z >> 1) + 2 + (z & 1)], k, there, (decltype(q)::value & 1 ? xb1 : xb0) + z * 4096 + base);
+  };
+  const auto load_w = [&](auto q, int k, bool there, int z) {
+    load_lds(wsrc[z], k, there, (decltype(q)::value & 1 ? w1 : w0) + z * 4096 + base);
+  };
+
+  const int l32 = lane & 31, h = lane >> 5;
+  int at[4];
+#pragma unroll
+  for (int c = 0; c < 4; ++c) at[c] = l32 * kFp8Group + ((4 * (c >> 1) + 2 * h + (c & 1)) ^ (l32 >> 1 & 7)) * 16;
+  Frag fw[4][2], fx[2][2];
+  // chunk y of four of x's tile i, of w's tile j
+  const auto read_x = [&](auto q, int i, int y) {
+    constexpr bool Q = decltype(q)::value & 1;
+    const uint8_t* from = (i < 2 ? (Q ? xa1 : xa0) : (Q ? xb1 : xb0)) + (2 * wm + (i & 1)) * 4096;
+    const u32x4 v = *reinterpret_cast<const u32x4*>(from + at[y]);
+    Frag& g = fx[i & 1][y >> 1];
+    if (y & 1) g.hi = v;
+    else g.lo = v;
+  };
+  const auto read_w = [&](auto q, int j, int y) {
+    constexpr bool Q = decltype(q)::value & 1;
+    const u32x4 v = *reinterpret_cast<const u32x4*>((Q ? w1 : w0) + (4 * wn + j) * 4096 + at[y]);
+    Frag& g = fw[j][y >> 1];
+    if (y & 1) g.hi = v;
+    else g.lo = v;
+  };
+
+  f32x16 acc[4][4];  // [x tile][w tile]
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
+
+  using I0 = std::integral_constant<int, 0>;
+  using I1 = std::integral_constant<int, 1>;
+  Scales<4> scale(p, m0 + 128 * wm, n0 + 128 * wn);
+  // the first group, and of the second what the first one's turn does not load
+  {
+    const bool first = chunk < p.K, second = kFp8Group + chunk < p.K;
+#pragma unroll
+    for (int z = 0; z < 4; ++z) load_xa(I0(), 0, first, z);
+#pragma unroll
+    for (int z = 0; z < 8; ++z) load_w(I0(), 0, first, z);
+#pragma unroll
+    for (int z = 0; z < 4; ++z) load_xb(I0(), 0, first, z);
+#pragma unroll
+    for (int z = 0; z < 4; ++z) load_xa(I1(), kFp8Group, second, z);
+#pragma unroll
+    for (int z = 0; z < 8; ++z) load_w(I1(), kFp8Group, second, z);
+#pragma unroll
+    for (int z = 0; z < 2; ++z) load_xb(I1(), kFp8Group, second, z);
+  }
+  __builtin_amdgcn_s_waitcnt(vmcnt_imm(14));
+  __builtin_amdgcn_s_barrier();
+#pragma unroll
+  for (int y = 0; y < 4; ++y) read_x(I0(), 0, y);
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+#pragma unroll
+    for (int y = 0; y < 4; ++y) read_w(I0(), j, y);
+
+  const auto group = [&](auto uu, int s) {  // group s = U of a word
+    constexpr int U = decltype(uu)::value;
+    using Next = std::integral_constant<int, U + 1>;
+    if constexpr (U == 0) scale.take(p, s >> 2);
+    // (past the last group: zeros)
+    const int k1 = (s + 1) * kFp8Group, k2 = (s + 2) * kFp8Group;
+    const bool there1 = k1 + chunk < p.K, there2 = k2 + chunk < p.K;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+#pragma unroll
+      for (int v = 0; v < 8; ++v) {
+        const int j = v >> 1, k = v & 1;
+        acc[i][j] = mma32<false, U>(fw[j][k], fx[i & 1][k], acc[i][j], scale.w, scale.x[i]);
+        if (v < 4) {  // the next tile of x
+          if (i < 3) read_x(uu, i + 1, v);
+          else read_x(Next(), 0, v);
+        }
+        if (i == 3 && k == 1)  // w's tile j of this group has been multiplied
+#pragma unroll
+          for (int y = 0; y < 4; ++y) read_w(Next(), j, y);
+        // behind the first barrier 12 loads in 16 MFMAs, behind the second 4 in 16
+        if (i == 0 && (v & 3) == 3) load_xb(Next(), k1, there1, 2 + (v >> 2));
+        if (i == 1 || i == 2) {
+          const int u = 8 * (i - 1) + v, z = u * 3 / 4;
+          if ((u + 1) * 3 / 4 > z) {
+            if (z < 4) load_xa(uu, k2, there2, z);
+            else load_w(uu, k2, there2, z - 4);
+          }
+        }
+        if (i == 3 && (v & 3) == 3) load_xb(uu, k2, there2, v >> 2);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      if (i == 0 || i == 2) {
+        __builtin_amdgcn_s_waitcnt(kLdsDone);
+        // Behind the loads that have to have landed there are 16 (12 of the group after the next,
+        // four of the next one's tiles 2 and 3), and in a word's first group the scales' five.
+        __builtin_amdgcn_s_waitcnt(vmcnt_imm(16 + (U == 0 ? Scales<4>::kLoads : 0)));
+        __builtin_amdgcn_s_barrier();
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+  };
+  // (whole words: groups past the last one are zeros, and an exit in the middle of the turn would cost
+  // the registers that hold the sums)
+  for (int s = 0; s < groups; s += 4) {
+    group(I0(), s);
+    group(I1(), s + 1);
+    group(std::integral_constant<int, 2>(), s + 2);
+    group(std::integral_constant<int, 3>(), s + 3);
+  }
+  __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));  // (no load is left to land in LDS that another has by then)
+  store_tiles(p, m0 + 128 * wm, n0 + 128 * wn, acc);
+}
+
+__global__ __launch_bounds__(256, 1) void fp8_large_kernel(const Fp8Args p) { fp8_large(p); }
+
+// --- which of them ------------------------------------------------------------------
+
+// A kernel's block of results, and how long a group of K takes it, in us, measured with cold
+// weights: with a few workgroups on the chip, with one on each of its CUs, and for each of several
+// that share a CU (0: a CU has one at a time); for results in bf16 and in f32.
+struct Form {
+  int bm, bn, waves;
+  struct {
+    float few, full, each;
+  } t[2];
+};
+constexpr Form kForms[] = {
+    {16, 16, 8, {{0.08f, 0.085f, 0.07f}, {0.08f, 0.085f, 0.08f}}},
+    {32, 16, 8, {{0.08f, 0.097f, 0.13f}, {0.08f, 0.097f, 0.13f}}},
+    {32, 32, 4, {{0.14f, 0.156f, 0.11f}, {0.15f, 0.16f, 0.13f}}},
+    {32, 32, 8, {{0.11f, 0.135f, 0.0f}, {0.12f, 0.138f, 0.0f}}},
+    {32, 64, 4, {{0.178f, 0.206f, 0.0f}, {0.235f, 0.25f, 0.0f}}},
+    {64, 64, 4, {{0.25f, 0.28f, 0.0f}, {0.345f, 0.385f, 0.0f}}},
+    {64, 64, 4, {{0.25f, 0.275f, 0.23f}, {0.41f, 0.456f, 0.35f}}},
+    {64, 128, 4, {{0.306f, 0.39f, 0.37f}, {0.565f, 0.675f, 0.59f}}},
+    {128, 128, 4, {{0.4f, 0.61f, 0.0f}, {0.8f, 1.1f, 0.0f}}},
+    {128, 256, 4, {{0.65f, 1.06f, 0.0f}, {1.37f, 1.97f, 0.0f}}},
+    {256, 256, 4, {{1.0f, 1.65f, 0.0f}, {1e9f, 1e9f, 0.0f}}},
+};
+constexpr float kBytesPerUs = 5.15e6f;  // of a large copy
+
+// The one that takes the least time a group of K: rounds of workgroups where a CU has one, their
+// number and that of the fullest CU on average where it has several, and never less than the codes
+// take from memory; the smaller blocks where that decides.  64 x 22016 x 4096: 25.6 us with 64 x 128
+// (29 x 128 and 26.5 x 128 x 128, 31.5 of 32 x 32); 512 x 4096 x 4096: 15.0 (16.9 with 64 x 64, 21.7
+// with 128 x 128); 2048 x 4096 x 4096: 36.4 with 128 x 256 (45 with 256 x 256, 47 with 128 x 128).
+int choose_form(const Fp8Args& a) {
+  const float memory = 128.0f * (static_cast<float>(a.M) + static_cast<float>(a.N)) / kBytesPerUs;
+  int best = 0;
+  float least = 0.0f;
+  for (int i = 0; i < static_cast<int>(sizeof(kForms) / sizeof(kForms[0])); ++i) {
+    const Form& f = kForms[i];
+    const auto& t = f.t[a.c_f32];
+    const int64_t blocks = static_cast<int64_t>((a.M + f.bm - 1) / f.bm) * ((a.N + f.bn - 1) / f.bn);
+    const float n = static_cast<float>(blocks) / num_cus();
+    float time;
+    if (n <= 1.0f)
+      time = t.few + (t.full - t.few) * n;
+    else if (t.each == 0.0f)
+      time = t.full * std::ceil(n);
+    else
+      time = std::max(t.full, t.each * 0.5f * (n + std::ceil(n)));
+    time = std::max(time, memory);
+    if (i == 0 || time < least) {
+      best = i;
+      least = time;
+    }
+  }
+  return best;
 }
 
 }  // namespace
@@ -526,22 +772,28 @@ extern "C" int ttlh_matmul_fp8(const void* x, int64_t x_ld, const void* x_scale,
   a.c_f32 = c_dtype == TTLH_F32;
   a.c_vec = reinterpret_cast<uintptr_t>(c) % (4 * size) == 0 && c_ld % 4 == 0;
   a.c_vec8 = reinterpret_cast<uintptr_t>(c) % 16 == 0 && c_ld % 8 == 0;
+  const int i = choose_form(a);
+  a.grid_m = static_cast<int32_t>((M + kForms[i].bm - 1) / kForms[i].bm);
+  a.grid_n = static_cast<int32_t>((N + kForms[i].bn - 1) / kForms[i].bn);
+  TTLH_REQUIRE(static_cast<int64_t>(a.grid_m) * a.grid_n < (int64_t(1) << 31), TTLH_EUNSUPPORTED,
+               "%s: too many blocks of results", fn);
+  const dim3 grid(static_cast<uint32_t>(a.grid_m) * a.grid_n);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  const auto run = [&](auto kernel, int bm, int bn, int waves) {
-    a.grid_m = static_cast<int32_t>((M + bm - 1) / bm);
-    a.grid_n = static_cast<int32_t>((N + bn - 1) / bn);
-    if (static_cast<int64_t>(a.grid_m) * a.grid_n >= (int64_t(1) << 31)) {
-      set_error("%s: too many blocks of results", fn);
-      return static_cast<int>(TTLH_EUNSUPPORTED);
-    }
-    hipLaunchKernelGGL(kernel, dim3(static_cast<uint32_t>(a.grid_m) * a.grid_n), dim3(waves * 64), 0, s, a);
-    return check_launch("fp8_direct_kernel");
+  const auto run = [&](auto narrow, auto wide) {
+    hipLaunchKernelGGL(a.c_f32 ? wide : narrow, grid, dim3(64 * kForms[i].waves), 0, s, a);
+    return check_launch("a kernel of ttlh_matmul_fp8");
   };
-  if (M > 64) {
-    if (a.c_f32) return run(fp8_block_kernel<2, true>, 128, 128, 4);
-    if (M * N >= 192 * 65536) return run(fp8_block_kernel<4, false>, 256, 256, 4);
-    return run(fp8_block_kernel<2, false>, 128, 128, 4);
+  switch (i) {
+    case 0: return run(fp8_direct_kernel<1, 1, 8, 2, false>, fp8_direct_kernel<1, 1, 8, 2, true>);
+    case 1: return run(fp8_direct_kernel<2, 1, 8, 2, false>, fp8_direct_kernel<2, 1, 8, 2, true>);
+    case 2: return run(fp8_direct_kernel<2, 2, 4, 2, false>, fp8_direct_kernel<2, 2, 4, 2, true>);
+    case 3: return run(fp8_direct_kernel<2, 2, 8, 2, false>, fp8_direct_kernel<2, 2, 8, 2, true>);
+    case 4: return run(fp8_direct_kernel<2, 4, 4, 2, false>, fp8_direct_kernel<2, 4, 4, 2, true>);
+    case 5: return run(fp8_direct_kernel<4, 4, 4, 2, false>, fp8_direct_kernel<4, 4, 4, 2, true>);
+    case 6: return run(fp8_block_kernel<1, 1, 3, false>, fp8_block_kernel<1, 1, 3, true>);
+    case 7: return run(fp8_block_kernel<1, 2, 3, false>, fp8_block_kernel<1, 2, 3, true>);
+    case 8: return run(fp8_block_kernel<2, 2, 3, false>, fp8_block_kernel<2, 2, 3, true>);
+    case 9: return run(fp8_block_kernel<2, 4, 3, false>, fp8_block_kernel<2, 4, 3, true>);
+    default: return run(fp8_large_kernel, fp8_large_kernel);  // (bf16 results alone)
   }
-  if (a.c_f32) return M <= 16 ? run(fp8_direct_kernel<1, 1, 8, true>, 16, 16, 8) : run(fp8_direct_kernel<2, 2, 8, true>, 32, 32, 8);
-  return M <= 16 ? run(fp8_direct_kernel<1, 1, 8, false>, 16, 16, 8) : run(fp8_direct_kernel<2, 2, 8, false>, 32, 32, 8);
 }
