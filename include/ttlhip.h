@@ -599,6 +599,11 @@ int ttlh_fp8_glu(const void* gate, int64_t gate_ld, const void* up, int64_t up_l
 int ttlh_matmul_fp8(const void* x, int64_t x_ld, const void* x_scale, int64_t xs_ld, const void* w,
                     int64_t w_ld, const void* w_scale, int64_t ws_ld, void* c, int c_dtype,
                     int64_t c_ld, int64_t M, int64_t N, int64_t K, void* stream);
+/* Which of its kernels a product runs on (for tests and profiles; by its sizes and C's dtype
+ * alone): 0 to 5 divide K among waves, blocks of 16 x 16, 32 x 16, 32 x 32 with four and with
+ * eight waves, 32 x 64, 64 x 64 results (rows x columns of C); 6 to 9 share their loads, 64 x 64,
+ * 64 x 128, 128 x 128, 128 x 256; 10 is that of 256 x 256.                             */
+int ttlh_matmul_fp8_form(int64_t M, int64_t N, int c_dtype);
 
 /* ------------------------------------------------------------------------ */
 const char* ttlh_last_error(void);

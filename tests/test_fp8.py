@@ -63,7 +63,7 @@ def test_bad_outputs_are_refused(change):
 
 def test_codes_and_scales_of_one_memory_are_refused():
     m = torch.zeros(2, 6, 1280, dtype=torch.uint8)
-    with pytest.raises(ValueError, match="memory of their own"):
+    with pytest.raises(ValueError, match="memory in common"):
         K.quant_fp8(X, m.view(E4M3)[0, :, :640], m.view(-1)[:48].view(2, 6, 4).view(E8M0))
 
 
@@ -145,7 +145,7 @@ def test_products_into_half_precision_or_their_operands_are_refused():
     with pytest.raises(TypeError):
         K.matmul_fp8(**_product(c=torch.zeros(6, 300, dtype=torch.half)))
     m = torch.zeros(6, 640, dtype=torch.uint8)
-    with pytest.raises(ValueError, match="memory of its own"):
+    with pytest.raises(ValueError, match="memory in common"):
         K.matmul_fp8(**_product(x=m.view(E4M3), c=m.view(BF16)[:, 10:310]))
 
 

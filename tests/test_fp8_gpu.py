@@ -20,6 +20,7 @@ import pytest
 import torch
 
 from oracle import fp8 as R
+from ttlhip import _lib as L
 from ttlhip import kernels as K
 
 pytestmark = pytest.mark.gpu
@@ -337,6 +338,89 @@ def _multiply(x, xs, w, ws, dtype, ld=None):
 def test_matmul(M, N, k, dtype):
     ops = _operands(M, N, k, _gen(M + N + k))
     _check_product(_multiply(*ops, dtype), *ops)
+
+
+def _form(M, N, dtype):
+    return L.load().ttlh_matmul_fp8_form(M, N, L.dtype_code(dtype))
+
+
+# sizes off every block, for each of the kernels; K of one group, of a turn of a ring and a part,
+# of many
+FORMS = [(5, 1000), (20, 4090), (40, 6100), (40, 4090), (100, 4000), (40, 12000), (200, 4100), (300, 6100),
+         (1000, 4000), (2000, 3990), (3990, 4000)]
+FORMS_F32 = [(5, 1000), (20, 4090), (40, 6100), (40, 4090), (100, 4000), (250, 4000), (1000, 1507), (500, 4090),
+             (1000, 4090), (2000, 4090)]
+
+
+def test_the_products_below_reach_every_kernel():
+    assert {_form(M, N, BF16) for M, N in FORMS} == set(range(11)), [_form(M, N, BF16) for M, N in FORMS]
+    assert {_form(M, N, F32) for M, N in FORMS_F32} == set(range(10)), [_form(M, N, F32) for M, N in FORMS_F32]
+
+
+@pytest.mark.parametrize("M,N,dtype", [(*s, BF16) for s in FORMS] + [(*s, F32) for s in FORMS_F32])
+@pytest.mark.parametrize("k", [16, 400, 528, 1680])
+def test_each_kernel(M, N, dtype, k):
+    ops = _operands(M, N, k, _gen(M + k))
+    _check_product(_multiply(*ops, dtype, ld=N + (k % 3)), *ops)
+
+
+@pytest.mark.parametrize("M,N,dtype", [(*s, BF16) for s in FORMS] + [(*s, F32) for s in FORMS_F32])
+def test_each_kernel_marks_rows_and_blocks_of_nan_scales(M, N, dtype):
+    """NaN scales, and anything at all in the bytes of groups that do not exist."""
+    x, xs, w, ws = _operands(M, N, 640, _gen(M))
+    xs.view(torch.uint8)[0, 2, 3], ws.view(torch.uint8)[1, 1, 0] = 255, 255
+    x[2, 384:512] = 0  # as the operators leave it
+    c = _multiply(x, xs, w, ws, dtype)
+    nan = torch.zeros(M, N, dtype=torch.bool)
+    nan[2], nan[:, 128:256] = True, True
+    assert torch.equal(torch.isnan(c), nan)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_long_rows(dtype):
+    ops = _operands(3, 40, 70000, _gen(1))
+    _check_product(_multiply(*ops, dtype), *ops)
+
+
+def test_weights_past_32_bits():
+    """Codes of w and results further than 2^32 bytes from their first one."""
+    k, n, rows = 4096, (1 << 20) + 300, 3
+    g = torch.Generator(device="cuda").manual_seed(3)
+    w = torch.randint(0, 0x7F, (n, k), generator=g, device="cuda", dtype=torch.uint8).view(E4M3)
+    ws = torch.randint(110, 120, (8, -(-n // 128), 4), generator=g, device="cuda", dtype=torch.uint8).view(E8M0)
+    x, xs, _, _ = _operands(rows, 16, k, _gen(2))
+    c = torch.empty(rows, n, dtype=BF16, device="cuda")
+    K.matmul_fp8(x.cuda(), xs.cuda(), w, ws, c)
+    tail = (n - 300) // 128 * 128
+    _check_product(c[:, tail:].cpu(), x, xs, w[tail:].cpu(), ws[:, tail // 128:].cpu())
+    _check_product(c[:, :256].cpu(), x, xs, w[:256].cpu(), ws[:, :2].cpu())
+    # the same codes as x: rows of x past 2^32
+    m = n
+    xs2 = torch.randint(110, 120, (8, m, 4), generator=g, device="cuda", dtype=torch.uint8).view(E8M0)
+    _, _, w2, ws2 = _operands(1, 24, k, _gen(4))
+    c = torch.empty(m, 2100, dtype=BF16, device="cuda")[:, :24]  # (and results past 2^32)
+    K.matmul_fp8(w, xs2, w2.cuda(), ws2.cuda(), c)
+    _check_product(c[-300:].cpu(), w[-300:].cpu(), xs2[:, -300:].cpu(), w2, ws2)
+    _check_product(c[:100].cpu(), w[:100].cpu(), xs2[:, :100].cpu(), w2, ws2)
+
+
+def test_rows_past_32_bits():
+    """Values, codes and sums further than 2^32 bytes from the first."""
+    rows, dim = 700_000, 4096
+    x = torch.zeros(rows, dim, dtype=BF16, device="cuda")
+    ends = torch.tensor([0, 1, rows // 2, rows - 2, rows - 1])
+    part = _values(5, dim, _gen(3), BF16, 0.5)
+    x[ends.cuda()] = part.cuda()
+    codes = torch.empty(rows, dim, dtype=E4M3, device="cuda")
+    scales = K.fp8_scales(rows, dim)
+    K.quant_fp8(x, codes, scales)
+    pick = lambda: (codes.view(torch.uint8)[ends.cuda()].cpu().view(E4M3),  # noqa: E731
+                    scales.view(torch.uint8)[:, ends.cuda()].cpu().view(E8M0))
+    _check(part.double(), *pick(), 0.0)
+    codes.view(torch.uint8).zero_()
+    K.rms_norm_fp8(x, torch.ones(dim, device="cuda"), codes, scales, residual=x, total=x)
+    _check(R.rms_norm(part, torch.ones(dim), 1e-6, part)[1], *pick(), D_NORM)
+    assert torch.equal(x[ends.cuda()].cpu(), part + part)
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32])

@@ -705,14 +705,14 @@ constexpr float kBytesPerUs = 5.15e6f;  // of a large copy
 // take from memory; the smaller blocks where that decides.  64 x 22016 x 4096: 25.6 us with 64 x 128
 // (29 x 128 and 26.5 x 128 x 128, 31.5 of 32 x 32); 512 x 4096 x 4096: 15.0 (16.9 with 64 x 64, 21.7
 // with 128 x 128); 2048 x 4096 x 4096: 36.4 with 128 x 256 (45 with 256 x 256, 47 with 128 x 128).
-int choose_form(const Fp8Args& a) {
-  const float memory = 128.0f * (static_cast<float>(a.M) + static_cast<float>(a.N)) / kBytesPerUs;
+int choose_form(int64_t M, int64_t N, bool f32) {
+  const float memory = 128.0f * (static_cast<float>(M) + static_cast<float>(N)) / kBytesPerUs;
   int best = 0;
   float least = 0.0f;
   for (int i = 0; i < static_cast<int>(sizeof(kForms) / sizeof(kForms[0])); ++i) {
     const Form& f = kForms[i];
-    const auto& t = f.t[a.c_f32];
-    const int64_t blocks = static_cast<int64_t>((a.M + f.bm - 1) / f.bm) * ((a.N + f.bn - 1) / f.bn);
+    const auto& t = f.t[f32];
+    const int64_t blocks = ((M + f.bm - 1) / f.bm) * ((N + f.bn - 1) / f.bn);
     const float n = static_cast<float>(blocks) / num_cus();
     float time;
     if (n <= 1.0f)
@@ -772,7 +772,7 @@ extern "C" int ttlh_matmul_fp8(const void* x, int64_t x_ld, const void* x_scale,
   a.c_f32 = c_dtype == TTLH_F32;
   a.c_vec = reinterpret_cast<uintptr_t>(c) % (4 * size) == 0 && c_ld % 4 == 0;
   a.c_vec8 = reinterpret_cast<uintptr_t>(c) % 16 == 0 && c_ld % 8 == 0;
-  const int i = choose_form(a);
+  const int i = choose_form(M, N, a.c_f32);
   a.grid_m = static_cast<int32_t>((M + kForms[i].bm - 1) / kForms[i].bm);
   a.grid_n = static_cast<int32_t>((N + kForms[i].bn - 1) / kForms[i].bn);
   TTLH_REQUIRE(static_cast<int64_t>(a.grid_m) * a.grid_n < (int64_t(1) << 31), TTLH_EUNSUPPORTED,
@@ -796,4 +796,8 @@ extern "C" int ttlh_matmul_fp8(const void* x, int64_t x_ld, const void* x_scale,
     case 9: return run(fp8_block_kernel<2, 4, 3, false>, fp8_block_kernel<2, 4, 3, true>);
     default: return run(fp8_large_kernel, fp8_large_kernel);  // (bf16 results alone)
   }
+}
+
+extern "C" int ttlh_matmul_fp8_form(int64_t M, int64_t N, int c_dtype) {
+  return M > 0 && N > 0 ? choose_form(M, N, c_dtype == TTLH_F32) : 0;
 }

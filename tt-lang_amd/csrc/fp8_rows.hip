@@ -30,53 +30,57 @@ typedef uint2 uint2u __attribute__((aligned(1)));
 
 template <typename T>
 struct Eight {
-  float v[8];
-  // n: how many of them there are; zeros in the place of the others
+  u32x4 w[sizeof(T) / 2];
+  // n: how many of them there are.  All eight, or zeros; nothing waits for the values here, so that
+  // loads of several operands are under way at once.
   __device__ __forceinline__ void load(const T* p, int n) {
+#pragma unroll
+    for (int h = 0; h < static_cast<int>(sizeof(T) / 2); ++h) w[h] = u32x4{0u, 0u, 0u, 0u};
     if (n >= 8) {
-      if constexpr (sizeof(T) == 2) {
-        const u32x4 w = *reinterpret_cast<const u32x4u*>(p);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          v[2 * i] = __uint_as_float(w[i] << 16);
-          v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-        }
-      } else {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const u32x4 w = *reinterpret_cast<const u32x4u*>(p + 4 * h);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) v[4 * h + i] = __uint_as_float(w[i]);
-        }
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = i < n ? to_f32(p[i]) : 0.0f;
+      for (int h = 0; h < static_cast<int>(sizeof(T) / 2); ++h)
+        w[h] = *reinterpret_cast<const u32x4u*>(p + h * (16 / sizeof(T)));
     }
   }
-  __device__ __forceinline__ void store(T* p, int n) const {
-    if (n >= 8) {
-      if constexpr (sizeof(T) == 2) {
-        u32x4 w;
+  // the first n of fewer than eight: a row's end
+  __device__ __forceinline__ void load_end(const T* p, int n) {
+    if (n <= 0 || n >= 8) return;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] = cvt_pk_bf16x2(v[2 * i], v[2 * i + 1]);
-        *reinterpret_cast<u32x4u*>(p) = w;
-      } else {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          u32x4 w;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) w[i] = __float_as_uint(v[4 * h + i]);
-          *reinterpret_cast<u32x4u*>(p + 4 * h) = w;
-        }
+    for (int i = 0; i < 7; ++i)
+      if (i < n) {
+        if constexpr (sizeof(T) == 2)
+          w[0][i / 2] |= static_cast<uint32_t>(p[i]) << (16 * (i & 1));
+        else
+          w[i / 4][i % 4] = __float_as_uint(p[i]);
       }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (i < n) p[i] = from_f32<T>(v[i]);
-    }
+  }
+  __device__ __forceinline__ float operator[](int i) const {
+    if constexpr (sizeof(T) == 2)
+      return __uint_as_float(i & 1 ? w[0][i / 2] & 0xffff0000u : w[0][i / 2] << 16);
+    else
+      return __uint_as_float(w[i / 4][i % 4]);
   }
 };
+
+template <typename T>
+__device__ __forceinline__ void store_eight(T* p, int n, const float (&v)[8]) {
+  if (n >= 8) {
+    if constexpr (sizeof(T) == 2) {
+      *reinterpret_cast<u32x4u*>(p) = u32x4{cvt_pk_bf16x2(v[0], v[1]), cvt_pk_bf16x2(v[2], v[3]),
+                                            cvt_pk_bf16x2(v[4], v[5]), cvt_pk_bf16x2(v[6], v[7])};
+    } else {
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        *reinterpret_cast<u32x4u*>(p + 4 * h) =
+            u32x4{__float_as_uint(v[4 * h]), __float_as_uint(v[4 * h + 1]), __float_as_uint(v[4 * h + 2]),
+                  __float_as_uint(v[4 * h + 3])};
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 7; ++i)
+      if (i < n) p[i] = from_f32<T>(v[i]);
+  }
+}
 
 // the largest x of a row of 16 lanes, in each of them
 __device__ __forceinline__ uint32_t row_max(uint32_t x) {
@@ -109,9 +113,12 @@ __device__ __forceinline__ void emit(const float (&y)[8], F exact, int n, uint8_
   int s = scale_code(m);
   if constexpr (!EXACT) {
     if (__any(scale_open(m) && s != kScaleNan)) {
+      // (the largest is among the values within the errors of two)
+      uint32_t near = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) near |= (__float_as_uint(y[i]) & 0x7fffffffu) + 128u >= m ? 1u << i : 0u;
       double big = 0.0;
-#pragma unroll 1
-      for (int i = 0; i < n; ++i) big = fmax(big, fabs(exact(i)));
+      for (; near; near &= near - 1) big = fmax(big, fabs(exact(__ffs(near) - 1)));
 #pragma unroll
       for (int i = 8; i; i >>= 1) big = fmax(big, __shfl_xor(big, i));
       if (scale_open(m) && s != kScaleNan)
@@ -119,11 +126,9 @@ __device__ __forceinline__ void emit(const float (&y)[8], F exact, int n, uint8_
     }
   }
   const float inv = __uint_as_float(inverse_scale_bits(s));
-  float v[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = s == kScaleNan ? 0.0f : y[i] * inv;
-  const uint2 w = {four_codes<TTLH_CACHE_E4M3>(v[0], v[1], v[2], v[3]),
-                   four_codes<TTLH_CACHE_E4M3>(v[4], v[5], v[6], v[7])};
+  uint2 w = {four_codes<TTLH_CACHE_E4M3>(y[0] * inv, y[1] * inv, y[2] * inv, y[3] * inv),
+             four_codes<TTLH_CACHE_E4M3>(y[4] * inv, y[5] * inv, y[6] * inv, y[7] * inv)};
+  if (s == kScaleNan) w = uint2{0u, 0u};
   if (n >= 8) {
     *reinterpret_cast<uint2u*>(codes) = w;
   } else {
@@ -142,36 +147,90 @@ __device__ __forceinline__ void emit(const float (&y)[8], F exact, int n, uint8_
 
 constexpr int kActNone = -1;
 
-// exp(x): 2^(x log2 e) with the product's rounding error and the constant's tail put back
-// (one unit in the last place; x at most 88 in magnitude where that matters)
-__device__ __forceinline__ float exp_f32(float x) {
-  constexpr float kL2E = 1.44269502e+00f, kL2ELo = 1.92596299e-08f, kLn2 = 6.93147182e-01f;
-  const float t = x * kL2E;
-  const float lo = __builtin_fmaf(x, kL2ELo, __builtin_fmaf(x, kL2E, -t));
-  const float p = __builtin_amdgcn_exp2f(t);
-  return fabsf(t) < 128.0f ? __builtin_fmaf(p, lo * kLn2, p) : p;
+// exp(x) for x <= 0, to a unit in the last place: 2^n 2^f with n + f = x log2 e, f from -1/2 to 1/2;
+// results below 2^-126 keep their last place too.  (-150: zero, and NaN; a caller's product with x
+// is what says NaN)
+__device__ __forceinline__ float exp_down(float x) {
+  constexpr float kL2E = 1.44269502e+00f, kL2ELo = 1.92596299e-08f;
+  x = fmaxf(x, -150.0f);
+  const float n = rintf(x * kL2E);
+  const float f = __builtin_fmaf(x, kL2ELo, __builtin_fmaf(x, kL2E, -n));
+  return __builtin_amdgcn_ldexpf(__builtin_amdgcn_exp2f(f), static_cast<int>(n));
 }
 
+// 1 / d for d from 1 to 2, to one unit in the last place
+__device__ __forceinline__ float reciprocal(float d) {
+  const float r = __builtin_amdgcn_rcpf(d);
+  return __builtin_fmaf(__builtin_fmaf(-d, r, 1.0f), r, r);
+}
+
+// silu: with e = exp(-|g|), g / (1 + e) or g e / (1 + e), so that nothing overflows.
+// gelu: g times the normal distribution's integral up to g, which below 0 is exp(-g^2 / 2) times a
+// function that falls from 1/2 like 1 / |g|: a polynomial in s = (|g| - 4) / (|g| + 4), fitted
+// (least relative error, up to |g| = 14.5: 2^-25.9, evaluated in fp32 2^-21.5; beyond that the
+// exponential is zero).  The library's complementary error function took three times as long:
+// 4099 x 11008 bf16 89 us.
 template <int ACT>
 __device__ __forceinline__ float gated(float g, float u) {
-  if constexpr (ACT == TTLH_GLU_SILU)
-    return g / (1.0f + exp_f32(-g)) * u;
-  else {
-    // erfc(z + lo) = erfc(z) (1 - 2 z lo) to 2^-24 where z > 0, whose rounding error lo
-    // would count 2 z^2 times
-    constexpr float kC = -0.707106769f, kCLo = -1.21016175e-08f;  // -1 / sqrt 2
-    const float z = g * kC;
-    const float lo = __builtin_fmaf(g, kCLo, __builtin_fmaf(g, kC, -z));
-    const float e = erfcf(z);
-    return 0.5f * g * (z > 0.0f && z < 16.0f ? __builtin_fmaf(-2.0f * z * lo, e, e) : e) * u;
+  const float x = fabsf(g);
+  if constexpr (ACT == TTLH_GLU_SILU) {
+    const float e = exp_down(-x);
+    return (g < 0.0f ? g * e : g) * reciprocal(1.0f + e) * u;
+  } else {
+    const float z = fminf(x, 16.0f);  // (the exponential is zero there)
+    const float s = (z - 4.0f) * __builtin_amdgcn_rcpf(z + 4.0f);
+    float h = -6.528619269374758e-05f;
+    h = __builtin_fmaf(h, s, -0.00016782732564024627f);
+    h = __builtin_fmaf(h, s, 0.0006577639142051339f);
+    h = __builtin_fmaf(h, s, 0.0005025526625104249f);
+    h = __builtin_fmaf(h, s, -0.008497918024659157f);
+    h = __builtin_fmaf(h, s, 0.030865497887134552f);
+    h = __builtin_fmaf(h, s, -0.07170674204826355f);
+    h = __builtin_fmaf(h, s, 0.12437920272350311f);
+    h = __builtin_fmaf(h, s, -0.17039774358272552f);
+    h = __builtin_fmaf(h, s, 0.09441064298152924f);
+    // 2^(n + f) = exp(-z^2 / 2), with the square's rounding error and the constant's tail
+    constexpr float kC = -0.7213475108146667f, kCLo = -9.6298149e-09f;  // -log2 e / 2
+    const float q = z * z, n = rintf(q * kC);
+    float f = __builtin_fmaf(q, kCLo, __builtin_fmaf(q, kC, -n));
+    f = __builtin_fmaf(__builtin_fmaf(z, z, -q), kC, f);
+    h = __builtin_amdgcn_ldexpf(h * __builtin_amdgcn_exp2f(f), static_cast<int>(n));
+    return g * (g < 0.0f ? h : 1.0f - h) * u;
   }
 }
+// The same in fp64, to 2^-40, in few registers (the rare path decides the kernel's number of them,
+// and with it how many waves a SIMD has).  The integral of the normal distribution below -x: up to
+// x = 3 one half less the series phi(x) (x + x^3 / 3 + x^5 / 15 ..), from there on the continued
+// fraction phi(x) / (x + 1 / (x + 2 / (x + 3 / ..))).
 template <int ACT>
 __device__ __forceinline__ double gated64(double g, double u) {
-  if constexpr (ACT == TTLH_GLU_SILU)
-    return g / (1.0 + exp(-g)) * u;
-  else
-    return 0.5 * g * erfc(g * -0.70710678118654752440) * u;
+  const double x = fabs(g);
+  if constexpr (ACT == TTLH_GLU_SILU) {
+    const double e = exp(-x);
+    return (g < 0.0 ? g * e : g) / (1.0 + e) * u;
+  } else {
+    const double phi = 0.39894228040143267794 * exp(-0.5 * x * x);
+    const auto over = [](double d) {
+      const double r = __builtin_amdgcn_rcp(d);
+      return fma(fma(-d, r, 1.0), r, r);
+    };
+    double h;
+    if (x < 3.0) {
+      double term = x, sum = x;
+#pragma unroll 1
+      for (int i = 3; i < 100; i += 2) {
+        term *= x * x * over(i);
+        sum += term;
+      }
+      h = 0.5 - phi * sum;
+    } else {
+      double f = x;
+#pragma unroll 1
+      for (int i = 60; i > 0; --i) f = fma(static_cast<double>(i), over(f), x);
+      h = phi / f;
+    }
+    return g * (g < 0.0 ? h : 1.0 - h) * u;
+  }
 }
 
 struct UnitArgs {
@@ -179,35 +238,30 @@ struct UnitArgs {
   const void* b;
   int64_t a_ld, b_ld;
   Out o;
-  int32_t rows, dim, words;
-  int32_t blocks;  // workgroups of a row
+  int32_t units, dim, words;  // a unit: a word of a row
 };
 
 template <typename T, int ACT>
 __global__ __launch_bounds__(kThreads) void fp8_units_kernel(const UnitArgs p) {
-  const int row = blockIdx.x / p.blocks;
-  const int word = (blockIdx.x - row * p.blocks) * (kThreads / 64) +
-                   __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  if (word >= p.words) return;
+  const int unit = blockIdx.x * (kThreads / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (unit >= p.units) return;
+  const int row = unit / p.words, word = unit - row * p.words;
   const int at = word * kFp8Word + (threadIdx.x & 63) * 8, n = p.dim - at;
   const T* pa = static_cast<const T*>(p.a) + row * p.a_ld + at;
   const T* pb = static_cast<const T*>(p.b) + row * p.b_ld + at;
   uint8_t* codes = p.o.codes + row * p.o.codes_ld + at;
   uint32_t* to = p.o.scales + word * p.o.scales_ld + row;
-  Eight<T> a;
+  Eight<T> a, b;
   a.load(pa, n);
-  if constexpr (ACT == kActNone) {
-    emit<true>(a.v, 0, n, codes, to);
-  } else {
-    Eight<T> b;
-    b.load(pb, n);
-    float y[8];
+  if constexpr (ACT != kActNone) b.load(pb, n);
+  a.load_end(pa, n);
+  if constexpr (ACT != kActNone) b.load_end(pb, n);
+  float y[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] = gated<ACT>(a.v[i], b.v[i]);
-    emit<false>(y, [&](int i) {
-      return gated64<ACT>(static_cast<double>(to_f32(pa[i])), static_cast<double>(to_f32(pb[i])));
-    }, min(n, 8), codes, to);
-  }
+  for (int i = 0; i < 8; ++i) y[i] = ACT == kActNone ? a[i] : gated<ACT == kActNone ? 0 : ACT>(a[i], b[i]);
+  emit<ACT == kActNone>(y, [&](int i) {
+    return gated64<ACT == kActNone ? 0 : ACT>(static_cast<double>(to_f32(pa[i])), static_cast<double>(to_f32(pb[i])));
+  }, min(n, 8), codes, to);
 }
 
 // --- the norm --------------------------------------------------------------------
@@ -222,6 +276,7 @@ struct NormArgs {
   int32_t rows, dim;
   int32_t weight_f32;
   float eps;
+  double by_dim;  // 1 / dim
 };
 
 // the sum of x over the LANES (64, or all of a workgroup of 256) that have a row
@@ -241,82 +296,93 @@ __device__ __forceinline__ double row_sum(double x) {
 }
 
 // LANES lanes have a row, SWEEPS x 8 values each, which stay in registers between the sum
-// of squares (in fp64: a group near a scale's border needs the exact norm) and the codes.
-// SWEEPS 0: any length, read twice.
+// of squares (in fp64: a group near a scale's border needs the exact norm) and the codes.  SWEEPS 0:
+// any length, read twice.
 template <typename T, int LANES, int SWEEPS>
-__global__ __launch_bounds__(kThreads) void fp8_norm_kernel(const NormArgs p) {
-  constexpr int kStep = LANES * 8;
-  const int row = blockIdx.x * (kThreads / LANES) + (LANES == 64 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0);
+__global__ __launch_bounds__(LANES > kThreads ? LANES : kThreads) void fp8_norm_kernel(const NormArgs p) {
+  constexpr int kStep = LANES * 8, kKept = SWEEPS ? SWEEPS : 1;
+  const int row = LANES > 64 ? blockIdx.x
+                             : blockIdx.x * (kThreads / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lane = threadIdx.x & (LANES - 1);
   if (row >= p.rows) return;  // (a whole wave of its own where LANES is 64)
   const T* x = static_cast<const T*>(p.x) + row * p.x_ld;
   const T* r = p.residual ? static_cast<const T*>(p.residual) + row * p.residual_ld : nullptr;
   T* total = p.total ? static_cast<T*>(p.total) + row * p.total_ld : nullptr;
-  const auto read = [&](int at, Eight<T>& t) {
-    const int n = p.dim - at;
-    t.load(x + at, n);
-    if (r) {
-      Eight<T> more;
-      more.load(r + at, n);
+  // the values of SWEEPS places from lane * 8 + at on
+  Eight<T> v[kKept], more[kKept];
+  const auto read = [&](int at) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) t.v[i] += more.v[i];
+    for (int i = 0; i < kKept; ++i) {
+      const int k = at + lane * 8 + i * kStep;
+      v[i].load(x + k, p.dim - k);
+      if (r) more[i].load(r + k, p.dim - k);
+    }
+#pragma unroll
+    for (int i = 0; i < kKept; ++i) {
+      const int k = at + lane * 8 + i * kStep;
+      v[i].load_end(x + k, p.dim - k);
+      if (r) more[i].load_end(r + k, p.dim - k);
     }
   };
+  const auto value = [&](int i, int e) { return r ? v[i][e] + more[i][e] : v[i][e]; };
   double sum = 0.0;
-  const auto add = [&](const Eight<T>& t) {
+  const auto add = [&]() {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) sum = fma(static_cast<double>(t.v[i]), static_cast<double>(t.v[i]), sum);
+    for (int i = 0; i < kKept; ++i)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const double d = static_cast<double>(value(i, e));
+        sum = fma(d, d, sum);
+      }
   };
-  Eight<T> t[SWEEPS ? SWEEPS : 1];
   if constexpr (SWEEPS > 0) {
-#pragma unroll
-    for (int i = 0; i < SWEEPS; ++i) read(lane * 8 + i * kStep, t[i]);
-#pragma unroll
-    for (int i = 0; i < SWEEPS; ++i) add(t[i]);
+    read(0);
+    add();
   } else {
-    for (int at = lane * 8; at < p.dim; at += kStep) {
-      read(at, t[0]);
-      add(t[0]);
+    for (int at = 0; at < p.dim; at += kStep) {
+      read(at);
+      add();
     }
   }
-  sum = row_sum<LANES>(sum);
-  const double by = 1.0 / sqrt(sum / p.dim + static_cast<double>(p.eps));
+  // 1 / sqrt(mean + eps), the hardware's to 2^-14 and better, twice as many places a step
+  const double a = row_sum<LANES>(sum) * p.by_dim + static_cast<double>(p.eps);
+  double by = __builtin_amdgcn_rsq(a);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) by = fma(by * 0.5, fma(-a * by, by, 1.0), by);
+  if (a > 1.7e308) by = 0.0;  // (infinite: its values make their own groups NaN)
   const float by32 = static_cast<float>(by);
-  const auto write = [&](int at, const Eight<T>& t) {
-    const int n = p.dim - at;
-    float w[8], y[8];
-    if (p.weight_f32) {
-      Eight<float> e;
-      e.load(static_cast<const float*>(p.weight) + at, n);
+  const int from = __builtin_amdgcn_readfirstlane(lane >> 6) * kFp8Word;
+  const auto write = [&](int i, int word) {  // (whole waves: one has a word of the row or is past it)
+    const int at = word * kFp8Word + (lane & 63) * 8, n = p.dim - at;
+    float t[8], y[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) w[i] = e.v[i];
-    } else {
-      Eight<uint16_t> e;
-      e.load(static_cast<const uint16_t*>(p.weight) + at, n);
+    for (int e = 0; e < 8; ++e) t[e] = value(i, e);
+    const auto weigh = [&](auto type) {
+      typedef decltype(type) W;
+      Eight<W> w;
+      w.load(static_cast<const W*>(p.weight) + at, n);
+      w.load_end(static_cast<const W*>(p.weight) + at, n);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) w[i] = e.v[i];
-    }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] = t.v[i] * by32 * w[i];
-    emit<false>(y, [&](int i) {
-      double v = to_f32(x[at + i]);
-      if (r) v += static_cast<double>(to_f32(r[at + i]));
-      const double g = p.weight_f32 ? static_cast<const float*>(p.weight)[at + i]
-                                    : to_f32(static_cast<const uint16_t*>(p.weight)[at + i]);
-      return v * by * g;
-    }, min(n, 8), p.o.codes + row * p.o.codes_ld + at,
-                p.o.scales + (at / kFp8Word) * p.o.scales_ld + row);
-    if (total) t.store(total + at, n);  // (after the values are read: total may be x or residual)
+      for (int e = 0; e < 8; ++e) y[e] = t[e] * by32 * w[e];
+    };
+    p.weight_f32 ? weigh(float()) : weigh(uint16_t());
+    emit<false>(y, [&](int e) {
+      double d = to_f32(x[at + e]);
+      if (r) d += static_cast<double>(to_f32(r[at + e]));
+      const double g = p.weight_f32 ? static_cast<const float*>(p.weight)[at + e]
+                                    : to_f32(static_cast<const uint16_t*>(p.weight)[at + e]);
+      return d * by * g;
+    }, min(n, 8), p.o.codes + row * p.o.codes_ld + at, p.o.scales + word * p.o.scales_ld + row);
+    if (total) store_eight(total + at, n, t);  // (after the values are read: total may be x or residual)
   };
-  // (whole waves: one has a word of the row or is past it)
   if constexpr (SWEEPS > 0) {
 #pragma unroll
     for (int i = 0; i < SWEEPS; ++i)
-      if ((lane & ~63) * 8 + i * kStep < p.dim) write(lane * 8 + i * kStep, t[i]);
+      if (from + i * kStep < p.dim) write(i, (from + i * kStep) / kFp8Word);
   } else {
-    for (int at = lane * 8; at - (lane & 63) * 8 < p.dim; at += kStep) {
-      read(at, t[0]);
-      write(at, t[0]);
+    for (int at = 0; at + from < p.dim; at += kStep) {
+      read(at);
+      write(0, (at + from) / kFp8Word);
     }
   }
 }
@@ -354,12 +420,12 @@ int run_units(const char* fn, const void* a, int64_t a_ld, const void* b, int64_
   p.b = b;
   p.a_ld = a_ld;
   p.b_ld = b_ld;
-  p.rows = static_cast<int32_t>(rows);
+  const int64_t words = (dim + kFp8Word - 1) / kFp8Word, units = rows * words;
+  TTLH_REQUIRE(units < (int64_t(1) << 31) - kThreads / 64, TTLH_EUNSUPPORTED, "%s: too many rows or values", fn);
+  p.units = static_cast<int32_t>(units);
   p.dim = static_cast<int32_t>(dim);
-  p.words = static_cast<int32_t>((dim + kFp8Word - 1) / kFp8Word);
-  p.blocks = (p.words + kThreads / 64 - 1) / (kThreads / 64);
-  TTLH_REQUIRE(rows * p.blocks < (int64_t(1) << 31), TTLH_EUNSUPPORTED, "%s: too many rows or values", fn);
-  const dim3 grid(static_cast<uint32_t>(rows * p.blocks));
+  p.words = static_cast<int32_t>(words);
+  const dim3 grid(static_cast<uint32_t>((units + kThreads / 64 - 1) / (kThreads / 64)));
   hipStream_t s = static_cast<hipStream_t>(stream);
   const auto run = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(kThreads), 0, s, p); };
   const auto pick = [&](auto value) {
@@ -426,21 +492,30 @@ extern "C" int ttlh_fp8_rms_norm(const void* x, int64_t x_ld, const void* residu
   p.dim = static_cast<int32_t>(dim);
   p.weight_f32 = weight_dtype == TTLH_F32;
   p.eps = eps;
+  p.by_dim = 1.0 / static_cast<double>(dim);
   hipStream_t s = static_cast<hipStream_t>(stream);
+  // a wave a row up to 2048 values (8192 x 1024 bf16: 9.4 us, a workgroup a row 13.0), then a workgroup
   const auto run = [&](auto kernel, int lanes) {
-    const int per = kThreads / lanes;
-    hipLaunchKernelGGL(kernel, dim3(static_cast<uint32_t>((rows + per - 1) / per)), dim3(kThreads), 0, s, p);
+    const int per = lanes > 64 ? 1 : kThreads / 64;
+    hipLaunchKernelGGL(kernel, dim3(static_cast<uint32_t>((rows + per - 1) / per)),
+                       dim3(lanes > kThreads ? lanes : kThreads), 0, s, p);
   };
   const auto pick = [&](auto value) {
     typedef decltype(value) T;
     if (dim <= 512)
       run(fp8_norm_kernel<T, 64, 1>, 64);
+    else if (dim <= 1024)
+      run(fp8_norm_kernel<T, 64, 2>, 64);
     else if (dim <= 2048)
-      run(fp8_norm_kernel<T, 256, 1>, 256);
+      run(fp8_norm_kernel<T, 64, 4>, 64);
     else if (dim <= 4096)
       run(fp8_norm_kernel<T, 256, 2>, 256);
     else if (dim <= 8192)
       run(fp8_norm_kernel<T, 256, 4>, 256);
+    else if (dim <= 12288)
+      run(fp8_norm_kernel<T, 512, 3>, 512);
+    else if (dim <= 16384)
+      run(fp8_norm_kernel<T, 512, 4>, 512);
     else
       run(fp8_norm_kernel<T, 256, 0>, 256);
   };

@@ -174,6 +174,7 @@ SIGNATURES = {
     "ttlh_fp8_glu": (_int, [_vp, _i64, _vp, _i64, _int, _int, _vp, _i64, _vp, _i64, _i64, _i64, _vp]),
     "ttlh_matmul_fp8": (_int, [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _int, _i64, _i64,
                                _i64, _i64, _vp]),
+    "ttlh_matmul_fp8_form": (_int, [_i64, _i64, _int]),
     "ttlh_last_error": (C.c_char_p, []),
     "ttlh_version": (_int, []),
 }

@@ -1049,33 +1049,30 @@ def _fp8_rows(what: str, name: str, t: torch.Tensor, shape=None):
     return s, a if s[0] > 1 else s[1]
 
 
-def _fp8_scales(what: str, name: str, t: torch.Tensor, rows: int, dim: int) -> int:
-    """The stride of words, in dwords, of scales for [rows, dim] values."""
+def _fp8_scales(what: str, name: str, t: torch.Tensor, rows: int, dim: int):
+    """(address, stride of words in dwords) of scales for [rows, dim] values."""
     words = -(-dim // (4 * FP8_GROUP))
     if t.dtype != _E8M0 or t.shape != (words, rows, 4):
         raise ValueError(f"{what}: {name} must be float8_e8m0fnu [{words}, {rows}, 4] (fp8_scales()), got "
                          f"{t.dtype} {tuple(t.shape)}")
     a, b, c = t.stride()
-    if c != 1 or (b != 4 and rows > 1) or (a % 4 and words > 1) or t.data_ptr() % 4:
+    at = t.data_ptr()
+    if c != 1 or (b != 4 and rows > 1) or (a % 4 and words > 1) or at % 4:
         raise ValueError(f"{what}: {name} must have each row's four scales in one aligned dword, rows "
                          f"beside each other")
-    return a // 4 if words > 1 else rows
-
-
-def _span(t: torch.Tensor):
-    """(first byte, past the last byte) that t can reach."""
-    size, last = t.element_size(), 0
-    for n, s in zip(t.shape, t.stride()):
-        last += (n - 1) * s
-    return t.data_ptr(), t.data_ptr() + (last + 1) * size
+    return at, a // 4 if words > 1 else rows
 
 
 def _apart(a: torch.Tensor, b: torch.Tensor) -> bool:
-    """Whether two tensors have no memory in common; for matrices of one row pitch also
-    where the rows of one lie between those of the other."""
-    if a.numel() == 0 or b.numel() == 0:
-        return True
-    (a0, a1), (b0, b1) = _span(a), _span(b)
+    """Whether two matrices have no memory in common: one ends before the other begins, or
+    they have one row pitch, and the rows of one lie between those of the other."""
+    ends = []
+    for t in (a, b):
+        if t.numel() == 0:
+            return True
+        last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
+        ends.append((t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()))
+    (a0, a1), (b0, b1) = ends
     if a1 <= b0 or b1 <= a0:
         return True
     if a.dim() != 2 or b.dim() != 2 or a.shape[0] < 2 or b.shape[0] < 2:
@@ -1088,21 +1085,31 @@ def _apart(a: torch.Tensor, b: torch.Tensor) -> bool:
     return wide_a <= d and d + wide_b <= pitch
 
 
-def _fp8_out(what: str, codes: torch.Tensor, scales: torch.Tensor, shape, others):
-    """(row stride of codes, stride of the scales' words) of an operator's outputs."""
+def _check_apart(what: str, outs, ins) -> None:
+    """outs, ins: (first byte, past the last byte, name, tensor).  No output has memory in
+    common with an operand or another output."""
+    for i, (a, b, name, t) in enumerate(outs):
+        for c, d, other, u in ins + outs[i + 1:]:
+            if a < d and c < b and not _apart(t, u):
+                raise ValueError(f"{what}: {name} and {other} have memory in common")
+
+
+def _fp8_out(what: str, codes: torch.Tensor, scales: torch.Tensor, shape):
+    """(address, row stride of codes, address, stride of the scales' words, both for
+    _check_apart) of an operator's outputs."""
     rows, dim = shape
     _, ld = _fp8_rows(what, "codes", codes, shape)
     if codes.dtype != _E4M3:
         raise ValueError(f"{what}: codes must be float8_e4m3fn, got {codes.dtype}")
     if dim == 0:
         raise ValueError(f"{what}: rows must have values")
-    sld = _fp8_scales(what, "scales", scales, rows, dim)
-    if (rows > 1 and ld < dim) or (scales.shape[0] > 1 and sld < rows):
+    sp, sld = _fp8_scales(what, "scales", scales, rows, dim)
+    words = scales.shape[0]
+    if (rows > 1 and ld < dim) or (words > 1 and sld < rows):
         raise ValueError(f"{what}: codes and scales must not repeat their elements")
-    for t in others + (scales,):
-        if not _apart(codes, t) or (t is not scales and not _apart(scales, t)):
-            raise ValueError(f"{what}: codes and scales must have memory of their own")
-    return ld, sld
+    cp = codes.data_ptr()
+    return cp, ld, sp, sld, [(cp, cp + (rows - 1) * ld + dim, "codes", codes),
+                             (sp, sp + 4 * ((words - 1) * sld + rows), "scales", scales)]
 
 
 def quant_fp8(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, stream=None) -> None:
@@ -1114,11 +1121,16 @@ def quant_fp8(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, stream
     get the scale of zeros, 2^-126.  A value that is not finite makes its group's scale NaN
     and its codes zeros."""
     shape, ld = _fp8_rows("quant_fp8", "x", x)
-    cl, sl = _fp8_out("quant_fp8", codes, scales, shape, (x,))
+    cp, cl, sp, sl, outs = _fp8_out("quant_fp8", codes, scales, shape)
     code = L.dtype_code(x.dtype)
+    rows, dim = shape
+    if rows:
+        xp = x.data_ptr()
+        _check_apart("quant_fp8", outs, [(xp, xp + ((rows - 1) * ld + dim) * x.element_size(), "x", x)])
+    else:
+        xp = 0
     _check_on_one_device("quant_fp8", (x, codes, scales), stream)
-    L.call("ttlh_fp8_quant", x.data_ptr(), ld, code, codes.data_ptr(), cl, scales.data_ptr(), sl,
-           shape[0], shape[1], L.stream_ptr(stream))
+    L.call("ttlh_fp8_quant", xp, ld, code, cp, cl, sp, sl, rows, dim, L.stream_ptr(stream))
 
 
 def rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor,
@@ -1130,35 +1142,46 @@ def rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, codes: torch.Tensor, sca
     x, residual: bf16 or f32 [rows, dim], any row pitch; weight: bf16 or f32 [dim].
     total: gets t, rounded to x's dtype; it may be residual or x itself.  The norm is that
     of t before this rounding."""
-    shape, ld = _fp8_rows("rms_norm_fp8", "x", x)
-    if weight.shape != (shape[1],) or not weight.is_contiguous():
-        raise ValueError(f"rms_norm_fp8: weight must be contiguous [{shape[1]}], got {tuple(weight.shape)}")
-    tensors, rl, tl = (x, weight), 0, 0
-    for name, t in (("residual", residual), ("total", total)):
-        if t is None:
-            continue
-        _, s = _fp8_rows("rms_norm_fp8", name, t, shape)
-        if t.dtype != x.dtype:
-            raise ValueError(f"rms_norm_fp8: {name} must be {x.dtype} as x is, got {t.dtype}")
-        if name == "total":
-            tl = s
-            if shape[0] > 1 and s < shape[1]:
-                raise ValueError("rms_norm_fp8: total must not repeat its elements")
-            for other in tensors:
-                same = (other is not weight and t.data_ptr() == other.data_ptr()
-                        and t.stride() == other.stride())
-                if not same and not _apart(t, other):
-                    raise ValueError("rms_norm_fp8: total may be x or residual itself, not another view "
-                                     "of an operand's memory")
-        else:
-            rl = s
-        tensors += (t,)
-    cl, sl = _fp8_out("rms_norm_fp8", codes, scales, shape, tensors)
-    code, wcode = L.dtype_code(x.dtype), L.dtype_code(weight.dtype)
-    _check_on_one_device("rms_norm_fp8", tensors + (codes, scales), stream)
-    L.call("ttlh_fp8_rms_norm", x.data_ptr(), ld, 0 if residual is None else residual.data_ptr(), rl,
-           0 if total is None else total.data_ptr(), tl, code, weight.data_ptr(), wcode, eps,
-           codes.data_ptr(), cl, scales.data_ptr(), sl, shape[0], shape[1], L.stream_ptr(stream))
+    what = "rms_norm_fp8"
+    shape, ld = _fp8_rows(what, "x", x)
+    rows, dim = shape
+    if weight.shape != (dim,) or not weight.is_contiguous():
+        raise ValueError(f"{what}: weight must be contiguous [{dim}], got {tuple(weight.shape)}")
+    cp, cl, sp, sl, outs = _fp8_out(what, codes, scales, shape)
+    dtype = x.dtype
+    code, wcode = L.dtype_code(dtype), L.dtype_code(weight.dtype)
+    size = 4 if code == L.TTLH_F32 else 2
+    xp, wp = x.data_ptr(), weight.data_ptr()
+    ins = [(xp, xp + ((rows - 1) * ld + dim) * size, "x", x),
+           (wp, wp + dim * weight.element_size(), "weight", weight)]
+    tensors = [x, weight, codes, scales]
+    rp = rl = tp = tl = 0
+    if residual is not None:
+        _, rl = _fp8_rows(what, "residual", residual, shape)
+        if residual.dtype != dtype:
+            raise ValueError(f"{what}: residual must be {dtype} as x is, got {residual.dtype}")
+        rp = residual.data_ptr()
+        ins.append((rp, rp + ((rows - 1) * rl + dim) * size, "residual", residual))
+        tensors.append(residual)
+    if total is not None:
+        _, tl = _fp8_rows(what, "total", total, shape)
+        if total.dtype != dtype:
+            raise ValueError(f"{what}: total must be {dtype} as x is, got {total.dtype}")
+        if rows > 1 and tl < dim:
+            raise ValueError(f"{what}: total must not repeat its elements")
+        tp = total.data_ptr()
+        tensors.append(total)
+        span = (tp, tp + ((rows - 1) * tl + dim) * size, "total", total)
+        # (x or residual itself: each element is read before its sum is written)
+        itself = [i for i in ins if i[2] != "weight" and i[0] == tp and (rl if i[2] == "residual" else ld) == tl]
+        if rows:
+            _check_apart(what, [span], [i for i in ins if i not in itself])
+        ins.append(span)
+    if rows:
+        _check_apart(what, outs, ins)
+    _check_on_one_device(what, tensors, stream)
+    L.call("ttlh_fp8_rms_norm", xp, ld, rp, rl, tp, tl, code, wp, wcode, eps, cp, cl, sp, sl, rows, dim,
+           L.stream_ptr(stream))
 
 
 def glu_fp8(gate: torch.Tensor, up: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor,
@@ -1170,13 +1193,19 @@ def glu_fp8(gate: torch.Tensor, up: torch.Tensor, codes: torch.Tensor, scales: t
     _, ul = _fp8_rows("glu_fp8", "up", up, shape)
     if up.dtype != gate.dtype:
         raise ValueError(f"glu_fp8: up must be {gate.dtype} as gate is, got {up.dtype}")
-    if act not in GLU_ACTS:
+    kind = GLU_ACTS.get(act)
+    if kind is None:
         raise ValueError(f"glu_fp8: act must be one of {sorted(GLU_ACTS)}, got {act!r}")
-    cl, sl = _fp8_out("glu_fp8", codes, scales, shape, (gate, up))
+    cp, cl, sp, sl, outs = _fp8_out("glu_fp8", codes, scales, shape)
     code = L.dtype_code(gate.dtype)
+    rows, dim = shape
+    gp, up_ = gate.data_ptr(), up.data_ptr()
+    if rows:
+        size = gate.element_size()
+        _check_apart("glu_fp8", outs, [(gp, gp + ((rows - 1) * gl + dim) * size, "gate", gate),
+                                       (up_, up_ + ((rows - 1) * ul + dim) * size, "up", up)])
     _check_on_one_device("glu_fp8", (gate, up, codes, scales), stream)
-    L.call("ttlh_fp8_glu", gate.data_ptr(), gl, up.data_ptr(), ul, code, GLU_ACTS[act],
-           codes.data_ptr(), cl, scales.data_ptr(), sl, shape[0], shape[1], L.stream_ptr(stream))
+    L.call("ttlh_fp8_glu", gp, gl, up_, ul, code, kind, cp, cl, sp, sl, rows, dim, L.stream_ptr(stream))
 
 
 def matmul_fp8(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor,
@@ -1189,25 +1218,30 @@ def matmul_fp8(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale:
     result each eight neighbouring products are aligned to 2^-13 of the largest of them (the
     fp8 matrix instruction), for an f32 result they are added as fp32 (bf16 instructions, at
     half the rate).  A NaN scale makes its row (of w: the block's outputs) NaN."""
-    (M, K), xl = _fp8_rows("matmul_fp8", "x", x)
-    (N, kw), wl = _fp8_rows("matmul_fp8", "w", w)
-    shape, cl = _fp8_rows("matmul_fp8", "c", c)
+    what = "matmul_fp8"
+    (M, K), xl = _fp8_rows(what, "x", x)
+    (N, kw), wl = _fp8_rows(what, "w", w)
+    shape, cl = _fp8_rows(what, "c", c)
     if kw != K or shape != (M, N):
-        raise ValueError(f"matmul_fp8: shapes {(M, K)} @ {(N, kw)}^T -> {tuple(shape)}")
+        raise ValueError(f"{what}: shapes {(M, K)} @ {(N, kw)}^T -> {tuple(shape)}")
     if x.dtype != _E4M3 or w.dtype != _E4M3:
-        raise ValueError(f"matmul_fp8: x and w must be float8_e4m3fn, got {x.dtype} and {w.dtype}")
+        raise ValueError(f"{what}: x and w must be float8_e4m3fn, got {x.dtype} and {w.dtype}")
     if K == 0 or K % 16:
-        raise ValueError(f"matmul_fp8: K must be a positive multiple of 16, got {K}")
-    if (x.data_ptr() | w.data_ptr() | (xl if M > 1 else 0) | (wl if N > 1 else 0)) & 15:
-        raise ValueError("matmul_fp8: rows of x and w must start on 16 bytes")
-    xsl = _fp8_scales("matmul_fp8", "x_scale", x_scale, M, K)
-    wsl = _fp8_scales("matmul_fp8", "w_scale", w_scale, -(-N // FP8_GROUP), K)
+        raise ValueError(f"{what}: K must be a positive multiple of 16, got {K}")
+    xp, wp, cp = x.data_ptr(), w.data_ptr(), c.data_ptr()
+    if (xp | wp | (xl if M > 1 else 0) | (wl if N > 1 else 0)) & 15:
+        raise ValueError(f"{what}: rows of x and w must start on 16 bytes")
+    blocks, words = -(-N // FP8_GROUP), -(-K // (4 * FP8_GROUP))
+    xsp, xsl = _fp8_scales(what, "x_scale", x_scale, M, K)
+    wsp, wsl = _fp8_scales(what, "w_scale", w_scale, blocks, K)
     if M > 1 and cl < N:
-        raise ValueError("matmul_fp8: c must not repeat its elements")
-    for t in (x, x_scale, w, w_scale):
-        if not _apart(c, t):
-            raise ValueError("matmul_fp8: c must have memory of its own")
+        raise ValueError(f"{what}: c must not repeat its elements")
     code = L.dtype_code(c.dtype)
-    _check_on_one_device("matmul_fp8", (x, x_scale, w, w_scale, c), stream)
-    L.call("ttlh_matmul_fp8", x.data_ptr(), xl, x_scale.data_ptr(), xsl, w.data_ptr(), wl,
-           w_scale.data_ptr(), wsl, c.data_ptr(), code, cl, M, N, K, L.stream_ptr(stream))
+    if M and N:
+        _check_apart(what, [(cp, cp + ((M - 1) * cl + N) * (4 if code == L.TTLH_F32 else 2), "c", c)],
+                     [(xp, xp + (M - 1) * xl + K, "x", x), (wp, wp + (N - 1) * wl + K, "w", w),
+                      (xsp, xsp + 4 * ((words - 1) * xsl + M), "x_scale", x_scale),
+                      (wsp, wsp + 4 * ((words - 1) * wsl + blocks), "w_scale", w_scale)])
+    _check_on_one_device(what, (x, x_scale, w, w_scale, c), stream)
+    L.call("ttlh_matmul_fp8", xp, xl, xsp, xsl, wp, wl, wsp, wsl, cp, code, cl, M, N, K,
+           L.stream_ptr(stream))
