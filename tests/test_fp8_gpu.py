@@ -358,7 +358,7 @@ def test_the_products_below_reach_every_kernel():
 
 
 @pytest.mark.parametrize("M,N,dtype", [(*s, BF16) for s in FORMS] + [(*s, F32) for s in FORMS_F32])
-@pytest.mark.parametrize("k", [16, 400, 528, 1680])
+@pytest.mark.parametrize("k", [16, 400, 528, 1680, 128, 1408])
 def test_each_kernel(M, N, dtype, k):
     ops = _operands(M, N, k, _gen(M + k))
     _check_product(_multiply(*ops, dtype, ld=N + (k % 3)), *ops)

@@ -16,16 +16,19 @@
 // different rows, or halves of lines at different times, cost up to four times the rate at which a CU
 // takes them (64 bytes a clock), and that rate, not memory, bounds the middle sizes.  A chunk of 16
 // codes lies at its place XOR row / 2, so that an MFMA operand's reads meet no bank twice.  Codes past
-// K are loaded as zeros, from kZeros: no kernel has a case for the last group.
+// K are loaded as zeros, from kZeros: no kernel has a case for the last group.  With all CUs loading, each
+// gets about 65 KB a us from its XCD's L2 (32 bytes a clock), and middle sizes run at that: 512 x 4096 x
+// 4096 in blocks of 64 x 128 takes 201 MB so, 12 us of its 15.  (Dividing K among workgroups too, their
+// parts joined by the last to arrive, brought 32 x 4096 x 11008 from 16.7 to 16.3 us and nothing else.)
 //  * fp8_direct_kernel: few results.  The waves of a workgroup divide K, each with LDS of its own and
 //    no barrier, and their sums are added in wave order.  1 x 22016 x 4096 19.0 us (4.7 TB/s of
 //    weights; one quarter of the lanes' rate, straight to registers: 19.2, but 32 x 4096 x 11008 26.0 ->
 //    16.2), 64 x 4096 x 4096 6.9 us.
 //  * fp8_block_kernel: a ring of three buffers and one barrier a group, 64 x 64 to 128 x 256 results.
 //    512 x 4096 x 4096 15.0 us (halves of lines: 21), 2048 x 4096 x 4096 36.4 us.
-//  * fp8_large_kernel: 256 x 256, bf16 results.  8192 x 22016 x 4096 584 us (2.5 PFLOP/s; in stages of
-//    half lines and a ring of four 703), 8192^3 397 us (2.8 PFLOP/s): the MFMAs are busy 78% of the
-//    cycles, at the clock that the power cap leaves (1.5 GHz).
+//  * fp8_large_kernel: 256 x 256, bf16 results.  8192 x 22016 x 4096 555 to 595 us by the box (2.5 to
+//    2.7 PFLOP/s; in stages of half lines and a ring of four 703), 8192^3 380 to 400 us (2.8 PFLOP/s):
+//    the MFMAs are busy 78% of the cycles, at the clock that the power cap leaves (1.5 GHz).
 
 #include <algorithm>
 #include <cmath>
@@ -527,7 +530,11 @@ __global__ __launch_bounds__(256, TX * TW * RING < 8 ? 2 : 1) void fp8_block_ker
 //  * behind tile 0: everyone has read w and x's tiles 0 and 1 of s, whose memory takes those of s + 2;
 //    tiles 2 and 3 of s have landed;
 //  * behind tile 2: everyone has read x's tiles 2 and 3; w and tiles 0 and 1 of s + 1 have landed.
-// Loads are 32 to 48 MFMAs ahead of their use.
+// Loads are 32 to 48 MFMAs ahead of their use.  CUT: K ends inside a group.  Without that the loads need
+// no choice between codes and zeros: two vector instructions a load fewer, and 1.3% less time, since
+// what bounds this kernel is power (workgroups set apart in time by up to 6 us, so that their stores do
+// not meet: no change).
+template <bool CUT>
 __device__ __forceinline__ void fp8_large(const Fp8Args& p) {
   constexpr int kBytes = 256 * kFp8Group;
   __shared__ __attribute__((aligned(16))) uint8_t xa0[kBytes / 2], xb0[kBytes / 2], xa1[kBytes / 2],
@@ -550,15 +557,24 @@ __device__ __forceinline__ void fp8_large(const Fp8Args& p) {
     wsrc[i] = p.w + static_cast<int64_t>(min(n0 + 32 * i + (t >> 3), p.N - 1)) * p.w_ld + chunk;
   }
   const int base = wave * 1024;
+  const auto load = [&](const uint8_t* src, int k, bool there, uint8_t* to) {
+    if constexpr (CUT)
+      load_lds(src, k, there, to);
+    else
+      __builtin_amdgcn_global_load_lds(src + k, (lds_void*)to, 16, 0, 0);
+  };
   const auto load_xa = [&](auto q, int k, bool there, int z) {
-    load_lds(xsrc[4 * (z >> 1) + (z & 1)], k, there, (decltype(q)::value & 1 ? xa1 : xa0) + z * 4096 + base);
+    load(xsrc[4 * (z >> 1) + (z & 1)], k, there, (decltype(q)::value & 1 ? xa1 : xa0) + z * 4096 + base);
   };
   const auto load_xb = [&](auto q, int k, bool there, int z) {
-    load_lds(xsrc[4 * (z >> 1) + 2 + (z & 1)], k, there, (decltype(q)::value & 1 ? xb1 : xb0) + z * 4096 + base);
+    load(xsrc[4 * (z >> 1) + 2 + (z & 1)], k, there, (decltype(q)::value & 1 ? xb1 : xb0) + z * 4096 + base);
   };
   const auto load_w = [&](auto q, int k, bool there, int z) {
-    load_lds(wsrc[z], k, there, (decltype(q)::value & 1 ? w1 : w0) + z * 4096 + base);
+    load(wsrc[z], k, there, (decltype(q)::value & 1 ? w1 : w0) + z * 4096 + base);
   };
+  // where group s begins; past the last one CUT: zeros, else the last one's codes again (their scales
+  // are then 2^-127, and products of 2^-254 add nothing)
+  const auto begin = [&](int s) { return (CUT ? s : min(s, groups - 1)) * kFp8Group; };
 
   const int l32 = lane & 31, h = lane >> 5;
   int at[4];
@@ -595,7 +611,8 @@ __device__ __forceinline__ void fp8_large(const Fp8Args& p) {
   Scales<4> scale(p, m0 + 128 * wm, n0 + 128 * wn);
   // the first group, and of the second what the first one's turn does not load
   {
-    const bool first = chunk < p.K, second = kFp8Group + chunk < p.K;
+    const int second_k = begin(1);
+    const bool first = chunk < p.K, second = second_k + chunk < p.K;
 #pragma unroll
     for (int z = 0; z < 4; ++z) load_xa(I0(), 0, first, z);
 #pragma unroll
@@ -603,11 +620,11 @@ __device__ __forceinline__ void fp8_large(const Fp8Args& p) {
 #pragma unroll
     for (int z = 0; z < 4; ++z) load_xb(I0(), 0, first, z);
 #pragma unroll
-    for (int z = 0; z < 4; ++z) load_xa(I1(), kFp8Group, second, z);
+    for (int z = 0; z < 4; ++z) load_xa(I1(), second_k, second, z);
 #pragma unroll
-    for (int z = 0; z < 8; ++z) load_w(I1(), kFp8Group, second, z);
+    for (int z = 0; z < 8; ++z) load_w(I1(), second_k, second, z);
 #pragma unroll
-    for (int z = 0; z < 2; ++z) load_xb(I1(), kFp8Group, second, z);
+    for (int z = 0; z < 2; ++z) load_xb(I1(), second_k, second, z);
   }
   __builtin_amdgcn_s_waitcnt(vmcnt_imm(14));
   __builtin_amdgcn_s_barrier();
@@ -622,8 +639,7 @@ __device__ __forceinline__ void fp8_large(const Fp8Args& p) {
     constexpr int U = decltype(uu)::value;
     using Next = std::integral_constant<int, U + 1>;
     if constexpr (U == 0) scale.take(p, s >> 2);
-    // (past the last group: zeros)
-    const int k1 = (s + 1) * kFp8Group, k2 = (s + 2) * kFp8Group;
+    const int k1 = begin(s + 1), k2 = begin(s + 2);
     const bool there1 = k1 + chunk < p.K, there2 = k2 + chunk < p.K;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -672,7 +688,10 @@ __device__ __forceinline__ void fp8_large(const Fp8Args& p) {
   store_tiles(p, m0 + 128 * wm, n0 + 128 * wn, acc);
 }
 
-__global__ __launch_bounds__(256, 1) void fp8_large_kernel(const Fp8Args p) { fp8_large(p); }
+template <bool CUT>
+__global__ __launch_bounds__(256, 1) void fp8_large_kernel(const Fp8Args p) {
+  fp8_large<CUT>(p);
+}
 
 // --- which of them ------------------------------------------------------------------
 
@@ -794,7 +813,9 @@ extern "C" int ttlh_matmul_fp8(const void* x, int64_t x_ld, const void* x_scale,
     case 7: return run(fp8_block_kernel<1, 2, 3, false>, fp8_block_kernel<1, 2, 3, true>);
     case 8: return run(fp8_block_kernel<2, 2, 3, false>, fp8_block_kernel<2, 2, 3, true>);
     case 9: return run(fp8_block_kernel<2, 4, 3, false>, fp8_block_kernel<2, 4, 3, true>);
-    default: return run(fp8_large_kernel, fp8_large_kernel);  // (bf16 results alone)
+    default:  // (bf16 results alone)
+      return K % kFp8Group ? run(fp8_large_kernel<true>, fp8_large_kernel<true>)
+                           : run(fp8_large_kernel<false>, fp8_large_kernel<false>);
   }
 }
 
