@@ -581,7 +581,8 @@ int ttlh_rope(const void* x, void* out, int dtype, const void* positions, int po
 int ttlh_fp8_quant(const void* x, int64_t x_ld, int dtype, void* codes, int64_t codes_ld,
                    void* scales, int64_t scales_ld, int64_t rows, int64_t dim, void* stream);
 /* t = x + residual (null: x); y = t / sqrt(mean(t^2) + eps) * weight [dim]; total (may be
- * null, or x or residual itself): t rounded to dtype.  y is of the sum before its rounding.  */
+ * null, or x or residual itself): t rounded to dtype.  y is of the sum before its rounding.
+ * eps is positive.  */
 int ttlh_fp8_rms_norm(const void* x, int64_t x_ld, const void* residual, int64_t residual_ld,
                       void* total, int64_t total_ld, int dtype, const void* weight,
                       int weight_dtype, float eps, void* codes, int64_t codes_ld, void* scales,

@@ -104,7 +104,7 @@ def test_bad_norms_are_refused(change):
         K.rms_norm_fp8(**a)
 
 
-@pytest.mark.parametrize("eps", [-1e-6, float("nan"), float("inf")])
+@pytest.mark.parametrize("eps", [-1e-6, 0.0, 1e-50, float("nan"), float("inf")])
 def test_the_library_refuses_a_bad_eps(eps):
     lib = L.load()
     st = lib.ttlh_fp8_rms_norm(16, 640, 0, 0, 0, 0, 0, 16, 0, eps, 16, 640, 16, 6, 6, 640, None)
@@ -171,23 +171,34 @@ def test_rows_of_one_buffer_may_lie_beside_each_other():
 def test_the_library_refuses_what_it_cannot_run():
     lib = L.load()
 
-    def quant(dtype=0, codes=16, scales=16, rows=6, dim=640, x=16):
-        return lib.ttlh_fp8_quant(x, 640, dtype, codes, 640, scales, 6, rows, dim, None)
+    def quant(dtype=0, codes=16, scales=16, rows=6, dim=640, x=16, ld=1 << 40, sl=1 << 40):
+        return lib.ttlh_fp8_quant(x, ld, dtype, codes, ld, scales, sl, rows, dim, None)
 
     assert quant(dim=0) == quant(rows=-1) == quant(dtype=2) == L.TTLH_EINVAL
     assert quant(x=None) == quant(codes=None) == quant(scales=None) == quant(scales=18) == L.TTLH_EINVAL
     assert quant(rows=1 << 31) == quant(dim=1 << 31) == L.TTLH_EUNSUPPORTED
     assert quant(rows=(1 << 31) - 1, dim=4096) == L.TTLH_EUNSUPPORTED
+    assert quant(sl=5) == quant(ld=639) == L.TTLH_EINVAL
+    # more threads than a launch has
+    assert quant(rows=1 << 26, dim=512, ld=512) == quant(rows=1 << 22, dim=8192, ld=8192, sl=1 << 22) == L.TTLH_EUNSUPPORTED
+
+    def norm(rows=6, dim=640, ld=640, tl=640, sl=6):
+        return lib.ttlh_fp8_rms_norm(16, ld, 0, 0, 16, tl, 0, 16, 0, 1e-6, 16, ld, 16, sl, rows, dim, None)
+
+    assert norm(tl=639) == norm(ld=639) == norm(sl=5) == L.TTLH_EINVAL
+    assert norm(rows=1 << 26, sl=1 << 26) == norm(rows=1 << 23, dim=4096, ld=4096, tl=4096, sl=1 << 23) == L.TTLH_EUNSUPPORTED
     assert quant(rows=0, x=None) == L.TTLH_OK
     assert lib.ttlh_fp8_glu(16, 640, 16, 640, 0, 2, 16, 640, 16, 6, 6, 640, None) == L.TTLH_EINVAL
 
-    def product(x=16, xl=640, w=16, wl=640, c=16, cd=0, M=6, N=300, K=640, xs=16):
-        return lib.ttlh_matmul_fp8(x, xl, xs, 6, w, wl, 16, 3, c, cd, 300, M, N, K, None)
+    def product(x=16, xl=640, w=16, wl=640, c=16, cd=0, M=6, N=300, K=640, xs=16, cl=1 << 30):
+        return lib.ttlh_matmul_fp8(x, xl, xs, 6, w, wl, 16, 3, c, cd, cl, M, N, K, None)
 
     assert product(K=632) == product(K=0) == product(x=24) == product(xl=648) == L.TTLH_EINVAL
     assert product(wl=632) == product(cd=5) == product(c=17) == product(xs=18) == L.TTLH_EINVAL
     assert product(x=None) == product(w=None) == product(c=None) == product(xs=None) == L.TTLH_EINVAL
     assert product(M=1 << 28) == product(K=1 << 29) == L.TTLH_EUNSUPPORTED
+    assert product(cl=299) == L.TTLH_EINVAL
+    assert product(M=1, N=1 << 27, K=16) == product(M=1 << 27, N=1 << 27) == L.TTLH_EUNSUPPORTED  # blocks
     assert product(M=0, x=None) == product(N=0, c=None) == L.TTLH_OK
 
 

@@ -224,6 +224,40 @@ def test_scales_at_their_borders_are_the_exact_ones(dim):
     _check(y, codes.cpu(), scales.cpu(), D_NORM)
 
 
+@pytest.mark.parametrize("dim", [128, 1, 9, 300, 5000])
+def test_scales_at_their_borders_with_a_sum(dim):
+    """The same of f32 sums that fp32 rounds, in rows that end inside a wave's words: the norm is that
+    of the exact sum, and lanes past the row's end have no part in the decision."""
+    g = _gen(dim + 5)
+    rows = 64
+    x = _values(1, dim, g, F32, 0.0)
+    x = (x.double() * (1 + torch.arange(rows)[:, None] * 2.0 ** -24)).float()
+    r = _values(rows, dim, g, F32, 0.0) * 2.0 ** -9
+    y0 = R.rms_norm(x, torch.ones(dim), 1e-6, r)[1]
+    w = torch.ones(dim)
+    for k in range(0, dim, 128):
+        at = k + int(y0[0, k:k + 128].abs().argmax())
+        w[at] = 1.75 * 2.0 ** 5 / abs(float(y0[0, at]))
+    y = R.rms_norm(x, w, 1e-6, r)[1]
+    _, codes, _, scales = _out(rows, dim)
+    K.rms_norm_fp8(x.cuda(), w.cuda(), codes, scales, residual=r.cuda())
+    _check(y, codes.cpu(), scales.cpu(), D_NORM)
+
+
+@pytest.mark.parametrize("act,d", [("silu", D_SILU), ("gelu", D_GELU)])
+def test_an_open_scale_beside_a_row_that_ends(act, d):
+    """One group at its border, the wave's others past the end of the tensor or all zeros."""
+    for dim in (5, 128, 130, 384):
+        gate = torch.full((2, dim), 0.5)
+        gate[:, 128:256] = 0
+        up = torch.full((2, dim), 0.25)
+        one = float(R.glu(torch.tensor([[2.0]]), torch.ones(1, 1), act))
+        gate[1, 3], up[1, 3] = 2.0, torch.tensor(448.0 / one).float()
+        _, codes, _, scales = _out(2, dim)
+        K.glu_fp8(gate.cuda(), up.cuda(), codes, scales, act=act)
+        _check(R.glu(gate, up, act), codes.cpu(), scales.cpu(), d)
+
+
 # --- the gate ---------------------------------------------------------------------
 
 

@@ -26,7 +26,7 @@
 //    16.2), 64 x 4096 x 4096 6.9 us.
 //  * fp8_block_kernel: a ring of three buffers and one barrier a group, 64 x 64 to 128 x 256 results.
 //    512 x 4096 x 4096 15.0 us (halves of lines: 21), 2048 x 4096 x 4096 36.4 us.
-//  * fp8_large_kernel: 256 x 256, bf16 results.  8192 x 22016 x 4096 555 to 595 us by the box (2.5 to
+//  * fp8_large_kernel: 256 x 256, bf16 results.  8192 x 22016 x 4096 555 to 595 us by the card (2.5 to
 //    2.7 PFLOP/s; in stages of half lines and a ring of four 703), 8192^3 380 to 400 us (2.8 PFLOP/s):
 //    the MFMAs are busy 78% of the cycles, at the clock that the power cap leaves (1.5 GHz).
 
@@ -774,6 +774,7 @@ extern "C" int ttlh_matmul_fp8(const void* x, int64_t x_ld, const void* x_scale,
                TTLH_EINVAL, "%s: the scales must be 4-byte aligned", fn);
   const int size = c_dtype == TTLH_BF16 ? 2 : 4;
   TTLH_REQUIRE(reinterpret_cast<uintptr_t>(c) % size == 0, TTLH_EINVAL, "%s: C is off its elements", fn);
+  TTLH_REQUIRE(M == 1 || c_ld >= N, TTLH_EINVAL, "%s: rows of C lie on one another", fn);
   Fp8Args a;
   a.x = static_cast<const uint8_t*>(x);
   a.w = static_cast<const uint8_t*>(w);
@@ -794,8 +795,9 @@ extern "C" int ttlh_matmul_fp8(const void* x, int64_t x_ld, const void* x_scale,
   const int i = choose_form(M, N, a.c_f32);
   a.grid_m = static_cast<int32_t>((M + kForms[i].bm - 1) / kForms[i].bm);
   a.grid_n = static_cast<int32_t>((N + kForms[i].bn - 1) / kForms[i].bn);
-  TTLH_REQUIRE(static_cast<int64_t>(a.grid_m) * a.grid_n < (int64_t(1) << 31), TTLH_EUNSUPPORTED,
-               "%s: too many blocks of results", fn);
+  // (a launch has less than 2^32 threads)
+  TTLH_REQUIRE(static_cast<int64_t>(a.grid_m) * a.grid_n < (int64_t(1) << 26) / kForms[i].waves,
+               TTLH_EUNSUPPORTED, "%s: too many blocks of results", fn);
   const dim3 grid(static_cast<uint32_t>(a.grid_m) * a.grid_n);
   hipStream_t s = static_cast<hipStream_t>(stream);
   const auto run = [&](auto narrow, auto wide) {

@@ -112,16 +112,19 @@ __device__ __forceinline__ void emit(const float (&y)[8], F exact, int n, uint8_
   m = row_max(m);
   int s = scale_code(m);
   if constexpr (!EXACT) {
-    if (__any(scale_open(m) && s != kScaleNan)) {
-      // (the largest is among the values within the errors of two)
+    const bool open = scale_open(m) && s != kScaleNan;
+    if (__any(open)) {
+      // The largest is among the values within the errors of two.  (Of an open group alone: in one of
+      // zeros, past the row's end too, every value is that near.)
       uint32_t near = 0;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) near |= (__float_as_uint(y[i]) & 0x7fffffffu) + 128u >= m ? 1u << i : 0u;
+      for (int i = 0; i < 8; ++i)
+        near |= open && (__float_as_uint(y[i]) & 0x7fffffffu) + 128u >= m ? 1u << i : 0u;
       double big = 0.0;
       for (; near; near &= near - 1) big = fmax(big, fabs(exact(__ffs(near) - 1)));
 #pragma unroll
       for (int i = 8; i; i >>= 1) big = fmax(big, __shfl_xor(big, i));
-      if (scale_open(m) && s != kScaleNan)
+      if (open)
         s = scale_code64(static_cast<uint64_t>(__double_as_longlong(big)));
     }
   }
@@ -279,7 +282,7 @@ struct NormArgs {
   double by_dim;  // 1 / dim
 };
 
-// the sum of x over the LANES (64, or all of a workgroup of 256) that have a row
+// the sum of x over the LANES (64, or a whole workgroup) that have a row
 template <int LANES>
 __device__ __forceinline__ double row_sum(double x) {
 #pragma unroll
@@ -297,8 +300,9 @@ __device__ __forceinline__ double row_sum(double x) {
 
 // LANES lanes have a row, SWEEPS x 8 values each, which stay in registers between the sum
 // of squares (in fp64: a group near a scale's border needs the exact norm) and the codes.  SWEEPS 0:
-// any length, read twice.
-template <typename T, int LANES, int SWEEPS>
+// any length, read twice.  SUM: there is a residual (asked in the kernel, 4099 x 11008 bf16 without one
+// took 48 us in place of 34).
+template <typename T, bool SUM, int LANES, int SWEEPS>
 __global__ __launch_bounds__(LANES > kThreads ? LANES : kThreads) void fp8_norm_kernel(const NormArgs p) {
   constexpr int kStep = LANES * 8, kKept = SWEEPS ? SWEEPS : 1;
   const int row = LANES > 64 ? blockIdx.x
@@ -306,32 +310,33 @@ __global__ __launch_bounds__(LANES > kThreads ? LANES : kThreads) void fp8_norm_
   const int lane = threadIdx.x & (LANES - 1);
   if (row >= p.rows) return;  // (a whole wave of its own where LANES is 64)
   const T* x = static_cast<const T*>(p.x) + row * p.x_ld;
-  const T* r = p.residual ? static_cast<const T*>(p.residual) + row * p.residual_ld : nullptr;
+  const T* r = SUM ? static_cast<const T*>(p.residual) + row * p.residual_ld : nullptr;
   T* total = p.total ? static_cast<T*>(p.total) + row * p.total_ld : nullptr;
   // the values of SWEEPS places from lane * 8 + at on
-  Eight<T> v[kKept], more[kKept];
+  Eight<T> v[kKept], more[SUM ? kKept : 1];
   const auto read = [&](int at) {
 #pragma unroll
     for (int i = 0; i < kKept; ++i) {
       const int k = at + lane * 8 + i * kStep;
       v[i].load(x + k, p.dim - k);
-      if (r) more[i].load(r + k, p.dim - k);
+      if constexpr (SUM) more[i].load(r + k, p.dim - k);
     }
 #pragma unroll
     for (int i = 0; i < kKept; ++i) {
       const int k = at + lane * 8 + i * kStep;
       v[i].load_end(x + k, p.dim - k);
-      if (r) more[i].load_end(r + k, p.dim - k);
+      if constexpr (SUM) more[i].load_end(r + k, p.dim - k);
     }
   };
-  const auto value = [&](int i, int e) { return r ? v[i][e] + more[i][e] : v[i][e]; };
+  const auto value = [&](int i, int e) { return SUM ? v[i][e] + more[SUM ? i : 0][e] : v[i][e]; };
   double sum = 0.0;
   const auto add = [&]() {
 #pragma unroll
     for (int i = 0; i < kKept; ++i)
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const double d = static_cast<double>(value(i, e));
+        double d = v[i][e];
+        if constexpr (SUM) d += static_cast<double>(more[i][e]);
         sum = fma(d, d, sum);
       }
   };
@@ -368,7 +373,7 @@ __global__ __launch_bounds__(LANES > kThreads ? LANES : kThreads) void fp8_norm_
     p.weight_f32 ? weigh(float()) : weigh(uint16_t());
     emit<false>(y, [&](int e) {
       double d = to_f32(x[at + e]);
-      if (r) d += static_cast<double>(to_f32(r[at + e]));
+      if constexpr (SUM) d += static_cast<double>(to_f32(r[at + e]));
       const double g = p.weight_f32 ? static_cast<const float*>(p.weight)[at + e]
                                     : to_f32(static_cast<const uint16_t*>(p.weight)[at + e]);
       return d * by * g;
@@ -395,9 +400,11 @@ int check_rows(const char* fn, int64_t rows, int64_t dim, int dtype) {
   return TTLH_OK;
 }
 
-int check_out(const char* fn, int64_t rows, void* codes, int64_t codes_ld, void* scales,
+int check_out(const char* fn, int64_t rows, int64_t dim, void* codes, int64_t codes_ld, void* scales,
               int64_t scales_ld, Out* o) {
   TTLH_REQUIRE(codes && scales, TTLH_EINVAL, "%s: null pointer", fn);
+  TTLH_REQUIRE((rows == 1 || codes_ld >= dim) && (dim <= kFp8Word || scales_ld >= rows), TTLH_EINVAL,
+               "%s: rows of codes or words of scales lie on one another", fn);
   TTLH_REQUIRE((reinterpret_cast<uintptr_t>(scales) & 3) == 0, TTLH_EINVAL,
                "%s: the scales must be 4-byte aligned", fn);
   o->codes = static_cast<uint8_t*>(codes);
@@ -413,7 +420,7 @@ int run_units(const char* fn, const void* a, int64_t a_ld, const void* b, int64_
   int st = check_rows(fn, rows, dim, dtype);
   if (st != TTLH_OK || rows == 0) return st;
   UnitArgs p;
-  st = check_out(fn, rows, codes, codes_ld, scales, scales_ld, &p.o);
+  st = check_out(fn, rows, dim, codes, codes_ld, scales, scales_ld, &p.o);
   if (st != TTLH_OK) return st;
   TTLH_REQUIRE(a && b, TTLH_EINVAL, "%s: null pointer", fn);
   p.a = a;
@@ -421,7 +428,8 @@ int run_units(const char* fn, const void* a, int64_t a_ld, const void* b, int64_
   p.a_ld = a_ld;
   p.b_ld = b_ld;
   const int64_t words = (dim + kFp8Word - 1) / kFp8Word, units = rows * words;
-  TTLH_REQUIRE(units < (int64_t(1) << 31) - kThreads / 64, TTLH_EUNSUPPORTED, "%s: too many rows or values", fn);
+  // (a launch has less than 2^32 threads)
+  TTLH_REQUIRE(units <= (int64_t(1) << 26) - kThreads / 64, TTLH_EUNSUPPORTED, "%s: too many rows or values", fn);
   p.units = static_cast<int32_t>(units);
   p.dim = static_cast<int32_t>(dim);
   p.words = static_cast<int32_t>(words);
@@ -475,12 +483,16 @@ extern "C" int ttlh_fp8_rms_norm(const void* x, int64_t x_ld, const void* residu
   if (st != TTLH_OK) return st;
   TTLH_REQUIRE(weight_dtype == TTLH_BF16 || weight_dtype == TTLH_F32, TTLH_EINVAL,
                "%s: bf16 or f32 weights", fn);
-  TTLH_REQUIRE(eps >= 0.0f && std::isfinite(eps), TTLH_EINVAL, "%s: eps must be finite and not negative", fn);
+  // (positive: 1 / sqrt of it is a number in fp32, whatever the row)
+  TTLH_REQUIRE(eps > 0.0f && std::isfinite(eps), TTLH_EINVAL, "%s: eps must be positive and finite", fn);
   if (rows == 0) return TTLH_OK;
   NormArgs p;
-  st = check_out(fn, rows, codes, codes_ld, scales, scales_ld, &p.o);
+  st = check_out(fn, rows, dim, codes, codes_ld, scales, scales_ld, &p.o);
   if (st != TTLH_OK) return st;
   TTLH_REQUIRE(x && weight, TTLH_EINVAL, "%s: null pointer", fn);
+  TTLH_REQUIRE(!total || rows == 1 || total_ld >= dim, TTLH_EINVAL, "%s: rows of the sum lie on one another", fn);
+  // (a launch has less than 2^32 threads: 64, 256 or 512 a row)
+  TTLH_REQUIRE(rows < (int64_t(1) << (dim <= 2048 ? 26 : 23)), TTLH_EUNSUPPORTED, "%s: too many rows", fn);
   p.x = x;
   p.residual = residual;
   p.total = total;
@@ -500,25 +512,29 @@ extern "C" int ttlh_fp8_rms_norm(const void* x, int64_t x_ld, const void* residu
     hipLaunchKernelGGL(kernel, dim3(static_cast<uint32_t>((rows + per - 1) / per)),
                        dim3(lanes > kThreads ? lanes : kThreads), 0, s, p);
   };
-  const auto pick = [&](auto value) {
+  const auto pick = [&](auto value, auto sum) {
     typedef decltype(value) T;
+    constexpr bool S = decltype(sum)::value;
     if (dim <= 512)
-      run(fp8_norm_kernel<T, 64, 1>, 64);
+      run(fp8_norm_kernel<T, S, 64, 1>, 64);
     else if (dim <= 1024)
-      run(fp8_norm_kernel<T, 64, 2>, 64);
+      run(fp8_norm_kernel<T, S, 64, 2>, 64);
     else if (dim <= 2048)
-      run(fp8_norm_kernel<T, 64, 4>, 64);
+      run(fp8_norm_kernel<T, S, 64, 4>, 64);
     else if (dim <= 4096)
-      run(fp8_norm_kernel<T, 256, 2>, 256);
+      run(fp8_norm_kernel<T, S, 256, 2>, 256);
     else if (dim <= 8192)
-      run(fp8_norm_kernel<T, 256, 4>, 256);
+      run(fp8_norm_kernel<T, S, 256, 4>, 256);
     else if (dim <= 12288)
-      run(fp8_norm_kernel<T, 512, 3>, 512);
+      run(fp8_norm_kernel<T, S, 512, 3>, 512);
     else if (dim <= 16384)
-      run(fp8_norm_kernel<T, 512, 4>, 512);
+      run(fp8_norm_kernel<T, S, 512, 4>, 512);
     else
-      run(fp8_norm_kernel<T, 256, 0>, 256);
+      run(fp8_norm_kernel<T, S, 256, 0>, 256);
   };
-  dtype == TTLH_BF16 ? pick(uint16_t()) : pick(float());
+  const auto sums = [&](auto value) {
+    residual ? pick(value, std::true_type()) : pick(value, std::false_type());
+  };
+  dtype == TTLH_BF16 ? sums(uint16_t()) : sums(float());
   return check_launch("fp8_norm_kernel");
 }

@@ -1139,8 +1139,8 @@ def rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, codes: torch.Tensor, sca
     """The root-mean-square norm t / sqrt(mean(t^2) + eps) * weight of t = x + residual
     (or of x) into codes and scales as quant_fp8() makes them.
 
-    x, residual: bf16 or f32 [rows, dim], any row pitch; weight: bf16 or f32 [dim].
-    total: gets t, rounded to x's dtype; it may be residual or x itself.  The norm is that
+    x, residual: bf16 or f32 [rows, dim], any row pitch; weight: bf16 or f32 [dim]; eps
+    positive.  total: gets t, rounded to x's dtype; it may be residual or x itself.  The norm is that
     of t before this rounding."""
     what = "rms_norm_fp8"
     shape, ld = _fp8_rows(what, "x", x)
