@@ -258,6 +258,58 @@ def test_an_open_scale_beside_a_row_that_ends(act, d):
         _check(R.glu(gate, up, act), codes.cpu(), scales.cpu(), d)
 
 
+def _check_exact(y, codes, scales):
+    """Every code is the one rounding of the exact value."""
+    s = R.scales(y)
+    assert torch.equal(R.by_row(scales, s.shape[1]), s)
+    e = R.e4m3(y / R.each(s, y.shape[1]))
+    bad = codes.double() != e
+    assert not bad.any(), (int(bad.sum()), bad.nonzero()[:4], codes.double()[bad][:4], e[bad][:4])
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("rows,dim", [(1000, 1000), (1000, 2890), (200, 9000), (60, 20000)])
+def test_codes_of_a_norm_are_the_exact_ones(rows, dim, dtype):
+    """Two in a million values lie so near the middle between two codes that fp32 takes the other."""
+    g = _gen(rows + dim)
+    x, r = _values(rows, dim, g, dtype), _values(rows, dim, g, dtype)
+    w = _values(1, dim, g, F32, 0.2)[0]
+    total, y = R.rms_norm(x, w, 1e-6, r)
+    _, codes, _, scales = _out(rows, dim)
+    K.rms_norm_fp8(x.cuda(), w.cuda(), codes, scales, residual=r.cuda())
+    _check_exact(y, codes.cpu(), scales.cpu())
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+def test_codes_of_a_gate_are_the_exact_ones(act, dtype):
+    """Of values as they come, and of gates that fp32 takes for open, whose products with bf16 values
+    are often in the middle between two codes."""
+    g = _gen(9)
+    gate, up = 2 * torch.randn(500, 2000, generator=g), _values(500, 2000, g, dtype)
+    at = torch.tensor([-7.0, 6.0, 7.0, 7.5, 8.0, 10.0, 14.0, 20.0, 28.0])
+    gate[250:] = at[torch.randint(len(at), (250, 2000), generator=g)]
+    up[250:] = up[250:].to(BF16).to(dtype)
+    gate = gate.to(dtype)
+    _, codes, _, scales = _out(500, 2000)
+    K.glu_fp8(gate.cuda(), up.cuda(), codes, scales, act=act)
+    _check_exact(R.glu(gate, up, act), codes.cpu(), scales.cpu())
+
+
+@pytest.mark.parametrize("dim", [1, 7, 129, 640])
+def test_values_between_two_codes_at_a_row_s_end(dim):
+    """All of a row's values but the largest are in the middle between two codes."""
+    up = torch.tensor([17.0, 19.0, 21.0, 23.0, 25.0])[torch.arange(dim) % 5].repeat(3, 1) / 16
+    up[:, ::128] = 28.0
+    gate = torch.full((3, dim), 64.0)
+    gate[1], up[2] = 8.0, -up[2]
+    for act in ("silu", "gelu"):
+        wide, codes, s, scales = _out(3, dim)
+        K.glu_fp8(gate.to(BF16).cuda(), up.to(BF16).cuda(), codes, scales, act=act)
+        _check_exact(R.glu(gate.to(BF16), up.to(BF16), act), codes.cpu(), scales.cpu())
+        _untouched(wide, s, dim)
+
+
 # --- the gate ---------------------------------------------------------------------
 
 

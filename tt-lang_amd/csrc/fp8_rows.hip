@@ -9,7 +9,10 @@
 // Values are computed in fp32.  A scale, though, steps by two where its group's largest
 // value crosses 448 x 2^n, so that an error of one unit in the last place there changes
 // 128 codes; a group whose largest value comes within 32 units of such a border (one in
-// 10^5) is therefore decided in fp64.  Scales are those of the exact values.
+// 10^5) is therefore decided in fp64.  So is a code whose value is within 2^-20 of the middle between
+// two (one in 10^5; found where the codes of the value a little up and a little down differ, two
+// instructions a value).  Scales and codes are those of the exact values, but for magnitudes below
+// 2^-126 (of a gate's exponential, too), of which fp32 has less than 24 bits.
 
 #include <cmath>
 #include <type_traits>
@@ -100,16 +103,40 @@ struct Out {
   int64_t codes_ld, scales_ld;  // bytes; dwords from a word of all rows to the next
 };
 
+__device__ __forceinline__ uint2 eight_codes(const float (&y)[8], float by) {
+  return uint2{four_codes<TTLH_CACHE_E4M3>(y[0] * by, y[1] * by, y[2] * by, y[3] * by),
+               four_codes<TTLH_CACHE_E4M3>(y[4] * by, y[5] * by, y[6] * by, y[7] * by)};
+}
+
+// The code of x, rounded once: to fp32 towards zero, with the last place odd where something was
+// lost, then to the nearest code.
+__device__ __forceinline__ uint32_t code_of(double x) {
+  const float f = static_cast<float>(x);
+  const double back = static_cast<double>(f);
+  uint32_t b = __float_as_uint(f);
+  if (back != x) b = (fabs(back) > fabs(x) ? b - 1u : b) | 1u;
+  return four_codes<TTLH_CACHE_E4M3>(__uint_as_float(b), 0.0f, 0.0f, 0.0f) & 255u;
+}
+
+// No value that decides a code or a scale is off by more, relative to its size (gelu: 9 x 2^-24).
+constexpr float kNear = 0x1p-20f;
+
 // The codes of a wave's 512 values (n of a lane's eight exist) and their scales, to
 // `codes` (the lane's) and `word`.  exact(i): value i in fp64, where fp32 does not decide
-// a scale.
+// a scale or a code.
 template <bool EXACT, typename F>
 __device__ __forceinline__ void emit(const float (&y)[8], F exact, int n, uint8_t* codes,
                                      uint32_t* word) {
-  uint32_t m = 0;
+  // the largest magnitude's bits (NaN: the largest): of the positive values as signed numbers, of the
+  // negative ones as unsigned, without clearing eight signs
+  int positive = 0;
+  uint32_t negative = 0;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(y[i]) & 0x7fffffffu);
-  m = row_max(m);
+  for (int i = 0; i < 8; ++i) {
+    positive = max(positive, static_cast<int>(__float_as_uint(y[i])));
+    negative = max(negative, __float_as_uint(y[i]));
+  }
+  const uint32_t m = row_max(max(static_cast<uint32_t>(positive), negative & 0x7fffffffu));
   int s = scale_code(m);
   if constexpr (!EXACT) {
     const bool open = scale_open(m) && s != kScaleNan;
@@ -129,8 +156,22 @@ __device__ __forceinline__ void emit(const float (&y)[8], F exact, int n, uint8_
     }
   }
   const float inv = __uint_as_float(inverse_scale_bits(s));
-  uint2 w = {four_codes<TTLH_CACHE_E4M3>(y[0] * inv, y[1] * inv, y[2] * inv, y[3] * inv),
-             four_codes<TTLH_CACHE_E4M3>(y[4] * inv, y[5] * inv, y[6] * inv, y[7] * inv)};
+  uint2 w = eight_codes(y, EXACT ? inv : inv * (1.0f + kNear));
+  if constexpr (!EXACT) {
+    const uint2 v = eight_codes(y, inv * (1.0f - kNear));
+    const uint2 differ = {w.x ^ v.x, w.y ^ v.y};
+    // (zeros, past the row's end too, do not)
+    if (__any((differ.x | differ.y) != 0)) {
+      uint64_t open = s == kScaleNan ? 0u : static_cast<uint64_t>(differ.y) << 32 | differ.x;
+      while (open) {
+        const int i = __builtin_ctzll(open) >> 3, at = 8 * (i & 3);
+        const uint32_t c = code_of(exact(i) * static_cast<double>(inv));
+        if (i < 4) w.x = (w.x & ~(255u << at)) | c << at;
+        else w.y = (w.y & ~(255u << at)) | c << at;
+        open &= ~(uint64_t(255) << (8 * i));
+      }
+    }
+  }
   if (s == kScaleNan) w = uint2{0u, 0u};
   if (n >= 8) {
     *reinterpret_cast<uint2u*>(codes) = w;
@@ -150,12 +191,18 @@ __device__ __forceinline__ void emit(const float (&y)[8], F exact, int n, uint8_
 
 constexpr int kActNone = -1;
 
+// x, or lo or hi where it is past them; a NaN: lo.  (fminf and fmaxf take two instructions each, the
+// first to make NaN quiet: 2 of gelu's 36 a value)
+__device__ __forceinline__ float within(float x, float lo, float hi) {
+  return __builtin_amdgcn_fmed3f(x, lo, hi);
+}
+
 // exp(x) for x <= 0, to a unit in the last place: 2^n 2^f with n + f = x log2 e, f from -1/2 to 1/2;
 // results below 2^-126 keep their last place too.  (-150: zero, and NaN; a caller's product with x
 // is what says NaN)
 __device__ __forceinline__ float exp_down(float x) {
   constexpr float kL2E = 1.44269502e+00f, kL2ELo = 1.92596299e-08f;
-  x = fmaxf(x, -150.0f);
+  x = within(x, -150.0f, 0.0f);
   const float n = rintf(x * kL2E);
   const float f = __builtin_fmaf(x, kL2ELo, __builtin_fmaf(x, kL2E, -n));
   return __builtin_amdgcn_ldexpf(__builtin_amdgcn_exp2f(f), static_cast<int>(n));
@@ -173,14 +220,14 @@ __device__ __forceinline__ float reciprocal(float d) {
 // (least relative error, up to |g| = 14.5: 2^-25.9, evaluated in fp32 2^-21.5; beyond that the
 // exponential is zero).  The library's complementary error function took three times as long:
 // 4099 x 11008 bf16 89 us.
-template <int ACT>
+template <int ACT, bool BF16>
 __device__ __forceinline__ float gated(float g, float u) {
   const float x = fabsf(g);
   if constexpr (ACT == TTLH_GLU_SILU) {
     const float e = exp_down(-x);
     return (g < 0.0f ? g * e : g) * reciprocal(1.0f + e) * u;
   } else {
-    const float z = fminf(x, 16.0f);  // (the exponential is zero there)
+    const float z = within(x, 0.0f, 16.0f);  // (the exponential is zero there)
     const float s = (z - 4.0f) * __builtin_amdgcn_rcpf(z + 4.0f);
     float h = -6.528619269374758e-05f;
     h = __builtin_fmaf(h, s, -0.00016782732564024627f);
@@ -192,13 +239,13 @@ __device__ __forceinline__ float gated(float g, float u) {
     h = __builtin_fmaf(h, s, 0.12437920272350311f);
     h = __builtin_fmaf(h, s, -0.17039774358272552f);
     h = __builtin_fmaf(h, s, 0.09441064298152924f);
-    // 2^(n + f) = exp(-z^2 / 2), with the square's rounding error and the constant's tail
+    // 2^(n + f) = exp(-z^2 / 2), with the square's rounding error (of bf16: none) and the constant's tail
     constexpr float kC = -0.7213475108146667f, kCLo = -9.6298149e-09f;  // -log2 e / 2
     const float q = z * z, n = rintf(q * kC);
     float f = __builtin_fmaf(q, kCLo, __builtin_fmaf(q, kC, -n));
-    f = __builtin_fmaf(__builtin_fmaf(z, z, -q), kC, f);
+    if constexpr (!BF16) f = __builtin_fmaf(__builtin_fmaf(z, z, -q), kC, f);
     h = __builtin_amdgcn_ldexpf(h * __builtin_amdgcn_exp2f(f), static_cast<int>(n));
-    return g * (g < 0.0f ? h : 1.0f - h) * u;
+    return __builtin_fmaf(-x, h, within(g, 0.0f, 3.4028235e38f)) * u;
   }
 }
 // The same in fp64, to 2^-40, in few registers (the rare path decides the kernel's number of them,
@@ -261,7 +308,8 @@ __global__ __launch_bounds__(kThreads) void fp8_units_kernel(const UnitArgs p) {
   if constexpr (ACT != kActNone) b.load_end(pb, n);
   float y[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) y[i] = ACT == kActNone ? a[i] : gated<ACT == kActNone ? 0 : ACT>(a[i], b[i]);
+  for (int i = 0; i < 8; ++i)
+    y[i] = ACT == kActNone ? a[i] : gated<ACT == kActNone ? 0 : ACT, sizeof(T) == 2>(a[i], b[i]);
   emit<ACT == kActNone>(y, [&](int i) {
     return gated64<ACT == kActNone ? 0 : ACT>(static_cast<double>(to_f32(pa[i])), static_cast<double>(to_f32(pb[i])));
   }, min(n, 8), codes, to);
