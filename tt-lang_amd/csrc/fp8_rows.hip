@@ -192,7 +192,7 @@ __device__ __forceinline__ void emit(const float (&y)[8], F exact, int n, uint8_
 constexpr int kActNone = -1;
 
 // x, or lo or hi where it is past them; a NaN: lo.  (fminf and fmaxf take two instructions each, the
-// first to make NaN quiet: 2 of gelu's 36 a value)
+// first to make NaN quiet: gelu 4099 x 11008 62 -> 58 us without them)
 __device__ __forceinline__ float within(float x, float lo, float hi) {
   return __builtin_amdgcn_fmed3f(x, lo, hi);
 }
@@ -349,7 +349,7 @@ __device__ __forceinline__ double row_sum(double x) {
 // LANES lanes have a row, SWEEPS x 8 values each, which stay in registers between the sum
 // of squares (in fp64: a group near a scale's border needs the exact norm) and the codes.  SWEEPS 0:
 // any length, read twice.  SUM: there is a residual (asked in the kernel, 4099 x 11008 bf16 without one
-// took 48 us in place of 34).
+// took 48 us in place of 35).
 template <typename T, bool SUM, int LANES, int SWEEPS>
 __global__ __launch_bounds__(LANES > kThreads ? LANES : kThreads) void fp8_norm_kernel(const NormArgs p) {
   constexpr int kStep = LANES * 8, kKept = SWEEPS ? SWEEPS : 1;
