@@ -251,7 +251,8 @@ __device__ __forceinline__ float gated(float g, float u) {
 // The same in fp64, to 2^-40, in few registers (the rare path decides the kernel's number of them,
 // and with it how many waves a SIMD has).  The integral of the normal distribution below -x: up to
 // x = 3 one half less the series phi(x) (x + x^3 / 3 + x^5 / 15 ..), from there on the continued
-// fraction phi(x) / (x + 1 / (x + 2 / (x + 3 / ..))).
+// fraction phi(x) / (x + 1 / (x + 2 / (x + 3 / ..))), both as far as x asks for.  (4099 x 11008 bf16, all
+// gates 8, so that one product in 16 lies between two codes: 147 us; with 49 and 60 steps always, 280)
 template <int ACT>
 __device__ __forceinline__ double gated64(double g, double u) {
   const double x = fabs(g);
@@ -268,7 +269,7 @@ __device__ __forceinline__ double gated64(double g, double u) {
     if (x < 3.0) {
       double term = x, sum = x;
 #pragma unroll 1
-      for (int i = 3; i < 100; i += 2) {
+      for (int i = 3, end = 30 + static_cast<int>(20.0 * x); i < end; i += 2) {
         term *= x * x * over(i);
         sum += term;
       }
@@ -276,7 +277,7 @@ __device__ __forceinline__ double gated64(double g, double u) {
     } else {
       double f = x;
 #pragma unroll 1
-      for (int i = 60; i > 0; --i) f = fma(static_cast<double>(i), over(f), x);
+      for (int i = 6 + static_cast<int>(560.0 * over(x * x)); i > 0; --i) f = fma(static_cast<double>(i), over(f), x);
       h = phi / f;
     }
     return g * (g < 0.0 ? h : 1.0 - h) * u;
