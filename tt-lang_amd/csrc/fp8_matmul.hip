@@ -212,7 +212,8 @@ __device__ __forceinline__ void fp8_direct(const Fp8Args& p) {
     for (int j = 0; j < MT; ++j) sx[a][j] = xs[j][4 * word * p.xs_ld];
     __builtin_amdgcn_sched_barrier(0);
   };
-  constexpr int kLoads = kRows / 8 + 1 + MT;  // of a group
+  // of a group (the scales are bytes at any address, which no scalar load reads: vmcnt sees them all)
+  constexpr int kLoads = kRows / 8 + 1 + MT;
 
   f32x4 acc[MT][NT];
 #pragma unroll
@@ -364,7 +365,10 @@ struct Scales {
   uint32_t w, x[TX], next_w, next_x[TX];
   int words;
   uint32_t past;  // bytes of the last word that are of no group: those scales may be anything
-  static constexpr int kLoads = TX + 1;
+  // What the waits below count: the vector loads that load() cannot do without, x's, whose addresses are a
+  // lane's own.  w's address is the same for a wave, so its load may be a scalar one, which vmcnt does not
+  // see; where it is a vector load, the waits are one load stricter than they have to be.
+  static constexpr int kLoads = TX;
 
   __device__ __forceinline__ Scales(const Fp8Args& p, int m, int n) {
     words = (p.K + kFp8Word - 1) / kFp8Word;
@@ -669,7 +673,7 @@ __device__ __forceinline__ void fp8_large(const Fp8Args& p) {
       if (i == 0 || i == 2) {
         __builtin_amdgcn_s_waitcnt(kLdsDone);
         // Behind the loads that have to have landed there are 16 (12 of the group after the next,
-        // four of the next one's tiles 2 and 3), and in a word's first group the scales' five.
+        // four of the next one's tiles 2 and 3), and in a word's first group the scales' four or five.
         __builtin_amdgcn_s_waitcnt(vmcnt_imm(16 + (U == 0 ? Scales<4>::kLoads : 0)));
         __builtin_amdgcn_s_barrier();
         __builtin_amdgcn_sched_barrier(0);
