@@ -180,6 +180,8 @@ __device__ __forceinline__ void emit(const float (&y)[8], F exact, int n, uint8_
     for (int i = 0; i < 8; ++i)
       if (i < n) codes[i] = static_cast<uint8_t>((i < 4 ? w.x : w.y) >> (8 * (i & 3)));
   }
+  // (a group past the row's end: what a norm makes of its zeros is NaN where the row holds one)
+  if (!EXACT && n <= 0) s = kScaleLeast;
   const uint32_t four = static_cast<uint32_t>(__builtin_amdgcn_readlane(s, 0)) |
                         static_cast<uint32_t>(__builtin_amdgcn_readlane(s, 16)) << 8 |
                         static_cast<uint32_t>(__builtin_amdgcn_readlane(s, 32)) << 16 |
