@@ -8,8 +8,12 @@
 // The fp8 MFMA aligns the products of eight neighbouring k to 2^-13 of the largest of them
 // before it adds them (measured; sums of such eights are right to fp32), which leaves an error of
 // 2^-19 of the products' sizes on average, far below the rounding of a bf16 result.  Results in
-// fp32 (WIDE) keep fp32's accuracy: codes times scale become bf16, which holds them exactly, and go
-// through bf16 MFMAs, at half the rate.
+// fp32 (WIDE) keep fp32's accuracy: codes become bf16, which holds them exactly times a power of two in
+// bf16's range, and go through bf16 MFMAs, at half the rate.  The exponents of a group's two scales are divided
+// between the operands so that both are in that range (wide_w, wide_x); where the sum of the two leaves no
+// such division (x's values from some 2^104 on, of weights of ordinary size), the rows of x concerned are
+// computed again at the end, group by group, with the scales applied to the sums (4096^3 with one such row
+// 475 us in place of 123; with one NaN row, whose results the same code writes, 131).
 //
 // Three kernels (choose_form, at the end, has the rule).  All of them bring whole lines of 128
 // codes, a group, to LDS by direct-to-LDS loads of eight lanes a row: lanes of one load that lie in
@@ -96,8 +100,8 @@ __device__ __forceinline__ i32x8 all8(const Frag& f) {
 }
 
 // eight codes (dwords a, b) times 2^(s - 127) as bf16; NaN where s is 255, whatever the codes are
-__device__ __forceinline__ bf16x8 widened(uint32_t a, uint32_t b, uint32_t s) {
-  const float scale = __uint_as_float(s << 23);
+__device__ __forceinline__ bf16x8 widened(uint32_t a, uint32_t b, int s) {
+  const float scale = __uint_as_float(static_cast<uint32_t>(s) << 23);
   const bf16x2 p = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, scale, false);
   const bf16x2 q = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, scale, true);
   const bf16x2 r = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, scale, false);
@@ -105,21 +109,27 @@ __device__ __forceinline__ bf16x8 widened(uint32_t a, uint32_t b, uint32_t s) {
   return bf16x8{p[0], p[1], q[0], q[1], r[0], r[1], t[0], t[1]};
 }
 
-// acc += A . B over one group; sa, sb: dwords of scales, the group's in byte J
+// byte J of a dword of scales
+template <int J>
+__device__ __forceinline__ int scale_byte(uint32_t s) {
+  return static_cast<int>(s >> (8 * J) & 255);
+}
+
+// acc += A . B over one group; sa, sb: dwords of scales, the group's in byte J (WIDE: the operands'
+// scales, of wide_w and wide_x)
 template <bool WIDE, int J>
 __device__ __forceinline__ f32x4 mma16(const Frag& a, const Frag& b, f32x4 acc, uint32_t sa, uint32_t sb) {
   if constexpr (!WIDE) {
     return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(all8(a), all8(b), acc, 0, 0, J, static_cast<int>(sa), J,
                                                             static_cast<int>(sb));
   } else {
-    const uint32_t ea = sa >> (8 * J) & 255, eb = sb >> (8 * J) & 255;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const u32x4 u = h ? a.hi : a.lo, v = h ? b.hi : b.lo;
 #pragma unroll
       for (int i = 0; i < 2; ++i)
-        acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widened(u[2 * i], u[2 * i + 1], ea),
-                                                      widened(v[2 * i], v[2 * i + 1], eb), acc, 0, 0, 0);
+        acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widened(u[2 * i], u[2 * i + 1], sa),
+                                                      widened(v[2 * i], v[2 * i + 1], sb), acc, 0, 0, 0);
     }
     return acc;
   }
@@ -161,6 +171,91 @@ __device__ __forceinline__ void store4(const Fp8Args& p, int row, int col, f32x4
     }
   }
 }
+
+// Rows of x whose scales leave bf16's range, into fp32: a lane's results of a tile of T x T (T 16: four,
+// 32: sixteen), of x's row `row` and w's from `col` on, over the groups from `first` on in steps of `step`.
+// The codes as they are, exact in bf16, make a group's sums, which the scales are then applied to.
+template <int T>
+struct FarTile {
+  typedef float Sums __attribute__((ext_vector_type(T == 16 ? 4 : 16)));
+  static constexpr int kK = T == 16 ? 32 : 16;  // of an MFMA: a lane has eight codes of it
+
+  static __device__ __forceinline__ Sums of(const Fp8Args& p, int row, int col, int first, int step) {
+    const int lane = threadIdx.x & 63, at = 8 * (lane / T);
+    row = min(row, p.M - 1);
+    const uint8_t* x = p.x + row * p.x_ld + at;
+    const uint8_t* w = p.w + min(col + lane % T, p.N - 1) * p.w_ld + at;
+    const uint32_t* xs = p.xs + row;
+    const uint32_t* ws = p.ws + min(col, p.N - 1) / kFp8Group;
+    Sums sum;
+#pragma unroll
+    for (int r = 0; r < T * T / 64; ++r) sum[r] = 0.0f;
+    const int groups = (p.K + kFp8Group - 1) / kFp8Group;
+#pragma unroll 1
+    for (int g = first; g < groups; g += step) {
+      Sums s;
+#pragma unroll
+      for (int r = 0; r < T * T / 64; ++r) s[r] = 0.0f;
+#pragma unroll
+      for (int k = g * kFp8Group, i = 0; i < kFp8Group / kK; ++i, k += kK) {
+        u32x2 a = {0u, 0u}, b = {0u, 0u};
+        if (k + at < p.K) {  // (K is a multiple of 16: all eight exist)
+          a = *reinterpret_cast<const u32x2*>(w + k);
+          b = *reinterpret_cast<const u32x2*>(x + k);
+        }
+        const bf16x8 u = widened(a[0], a[1], 127), v = widened(b[0], b[1], 127);
+        if constexpr (T == 16)
+          s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(u, v, s, 0, 0, 0);
+        else
+          s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(u, v, s, 0, 0, 0);
+      }
+      int ex, ew;
+      scales(xs, ws, p, g, ex, ew);
+#pragma unroll
+      for (int r = 0; r < T * T / 64; ++r) sum[r] += __builtin_amdgcn_ldexpf(s[r], ex + ew - 254);
+    }
+    return sum;
+  }
+
+  // group g's
+  static __device__ __forceinline__ void scales(const uint32_t* xs, const uint32_t* ws, const Fp8Args& p, int g,
+                                                int& ex, int& ew) {
+    const int64_t word = g >> 2;
+    ex = static_cast<int>(xs[word * p.xs_ld] >> (8 * (g & 3)) & 255);
+    ew = static_cast<int>(ws[word * p.ws_ld] >> (8 * (g & 3)) & 255);
+  }
+
+  // whether the row's results of those groups are NaN, and if not, whether they leave bf16's range
+  static __device__ __forceinline__ void look(const Fp8Args& p, int row, int col, int first, int step, bool& far,
+                                              bool& nan) {
+    const uint32_t* xs = p.xs + min(row, p.M - 1);
+    const uint32_t* ws = p.ws + min(col, p.N - 1) / kFp8Group;
+    const int groups = (p.K + kFp8Group - 1) / kFp8Group;
+    far = nan = false;
+#pragma unroll 8
+    for (int g = first; g < groups; g += step) {
+      int ex, ew;
+      scales(xs, ws, p, g, ex, ew);
+      far |= wide_far(wide_rest(ex, ew));
+      nan |= max(ex, ew) == kScaleNan;
+    }
+    far = far && !nan;
+  }
+};
+
+// WIDE: the largest scales that a lane has seen of its rows of x, and of w's.
+struct Seen {
+  int rest = 0, ex = 0, ew = 0;
+  // the scale of x's operand for a row's e and the wave's w
+  __device__ __forceinline__ int take(int e, int w) {
+    const int r = wide_rest(e, w);
+    rest = max(rest, r);
+    ex = max(ex, e);
+    return wide_x(r);
+  }
+  // whether results of the wave have to be made anew
+  __device__ __forceinline__ bool any() const { return __any(wide_far(rest) || max(ex, ew) == kScaleNan); }
+};
 
 // MT x 16 rows of x, NT x 16 of w a workgroup; wave v of WAVES takes the groups v, v + WAVES ..
 // of K, AHEAD (2 to 4) of them in flight.
@@ -222,6 +317,7 @@ __device__ __forceinline__ void fp8_direct(const Fp8Args& p) {
     for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   // A lane has row r of a tile, chunks q and q + 4.
   const int at_lo = r * kFp8Group + 16 * (q ^ (r >> 1)), at_hi = at_lo ^ 64;
+  Seen seen;
   const auto multiply = [&](int a) {
     Frag w[NT], x[MT];
 #pragma unroll
@@ -232,6 +328,19 @@ __device__ __forceinline__ void fp8_direct(const Fp8Args& p) {
     for (int i = 0; i < MT; ++i)
       x[i] = Frag{*reinterpret_cast<const u32x4*>(slot(a) + (NT + i) * 2048 + at_lo),
                   *reinterpret_cast<const u32x4*>(slot(a) + (NT + i) * 2048 + at_hi)};
+    if constexpr (WIDE) {
+      // (volatile: the compiler would move what depends on a scale alone in front of the wait above, right
+      // behind the scale's load, and wait there: 100 x 4000 x 4096 12.3 us in place of 10.1)
+      asm volatile("" : "+v"(sw[a]));
+      const int ew = __builtin_amdgcn_readfirstlane(sw[a]);
+      seen.ew = max(seen.ew, ew);
+      sw[a] = wide_w(ew);
+#pragma unroll
+      for (int i = 0; i < MT; ++i) {
+        asm volatile("" : "+v"(sx[a][i]));
+        sx[a][i] = seen.take(sx[a][i], ew);
+      }
+    }
 #pragma unroll
     for (int i = 0; i < MT; ++i)
 #pragma unroll
@@ -265,6 +374,24 @@ __device__ __forceinline__ void fp8_direct(const Fp8Args& p) {
   for (int i = 0; i < MT; ++i)
 #pragma unroll
     for (int j = 0; j < NT; ++j) part[(wave * MT * NT + i * NT + j) * 64 + lane] = acc[i][j];
+  if constexpr (WIDE) {
+    if (seen.any()) {
+#pragma unroll 1
+      for (int i = 0; i < MT; ++i) {
+        const int row = m0 + 16 * i + r;
+        bool far, nan;
+        FarTile<16>::look(p, row, n0, wave, WAVES, far, nan);
+        const bool some = __any(far);
+#pragma unroll 1
+        for (int j = 0; j < NT; ++j) {
+          f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
+          if (some) s = FarTile<16>::of(p, row, n0 + 16 * j, wave, WAVES);
+          if (nan) s += __builtin_nanf("");
+          if (far || nan) part[(wave * MT * NT + i * NT + j) * 64 + lane] = s;
+        }
+      }
+    }
+  }
   __syncthreads();
   for (int t = wave; t < MT * NT; t += WAVES) {
     f32x4 s = part[t * 64 + lane];
@@ -284,21 +411,20 @@ __global__ __launch_bounds__(WAVES * 64) void fp8_direct_kernel(const Fp8Args p)
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 
-// One k = 64 step of a 32 x 32 tile; e: the scales' byte
+// One k = 64 step of a 32 x 32 tile; E: the scales' byte (WIDE: as in mma16)
 template <bool WIDE, int E>
 __device__ __forceinline__ f32x16 mma32(const Frag& a, const Frag& b, f32x16 acc, uint32_t sa, uint32_t sb) {
   if constexpr (!WIDE) {
     return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(all8(a), all8(b), acc, 0, 0, E, static_cast<int>(sa), E,
                                                            static_cast<int>(sb));
   } else {
-    const uint32_t ea = sa >> (8 * E) & 255, eb = sb >> (8 * E) & 255;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const u32x4 u = h ? a.hi : a.lo, v = h ? b.hi : b.lo;
 #pragma unroll
       for (int i = 0; i < 2; ++i)
-        acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(widened(u[2 * i], u[2 * i + 1], ea),
-                                                      widened(v[2 * i], v[2 * i + 1], eb), acc, 0, 0, 0);
+        acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(widened(u[2 * i], u[2 * i + 1], sa),
+                                                      widened(v[2 * i], v[2 * i + 1], sb), acc, 0, 0, 0);
     }
     return acc;
   }
@@ -358,7 +484,7 @@ __device__ __forceinline__ void store_tiles(const Fp8Args& p, int m0, int n0, co
 
 // The scales of a wave's TX x 32 rows of x (a lane's in each tile) and of its rows of w, which are
 // in one block: a word, four groups, at a time, one ahead.
-template <int TX>
+template <int TX, bool WIDE>
 struct Scales {
   const uint32_t* ws;
   const uint32_t* xs[TX];
@@ -388,6 +514,7 @@ struct Scales {
   __device__ __forceinline__ void take(const Fp8Args& p, int word) {
     const uint32_t none = word == words - 1 ? past : 0u;  // (their codes are zeros, their scale 1 / 2^127)
     w = next_w & ~none;
+    if constexpr (WIDE) w = __builtin_amdgcn_readfirstlane(w);  // (what is made of it is scalar, and free)
 #pragma unroll
     for (int i = 0; i < TX; ++i) x[i] = next_x[i] & ~none;
     load(p, word + 1);
@@ -469,7 +596,8 @@ __device__ __forceinline__ void fp8_block(const Fp8Args& p) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
 
-  Scales<TX> scale(p, m0 + wm, n0 + wn);
+  Scales<TX, WIDE> scale(p, m0 + wm, n0 + wn);
+  Seen seen;
   each_until([&](auto q) {
 #pragma unroll
     for (int i = 0; i < kLoads; ++i)
@@ -488,17 +616,26 @@ __device__ __forceinline__ void fp8_block(const Fp8Args& p) {
     constexpr int U = decltype(uu)::value, E = U % 4;
     using Next = std::integral_constant<int, U + 1>;
     if constexpr (E == 0) scale.take(p, s >> 2);
+    uint32_t sw = scale.w, sx[TX];
+#pragma unroll
+    for (int i = 0; i < TX; ++i)
+      sx[i] = WIDE ? seen.take(scale_byte<E>(scale.x[i]), scale_byte<E>(sw)) : scale.x[i];
+    if constexpr (WIDE) {
+      seen.ew = max(seen.ew, scale_byte<E>(sw));
+      sw = wide_w(scale_byte<E>(sw));
+    }
+    if constexpr (WIDE) __builtin_amdgcn_sched_barrier(0);  // (in front of the barrier, where waves wait)
     const int k2 = (s + RING) * kFp8Group;
     const bool there = k2 + chunk < p.K;
     __builtin_amdgcn_s_waitcnt(kLdsDone);
     // (are the scales' loads, at a word's first group, among those behind group s + 1's?)
-    __builtin_amdgcn_s_waitcnt(vmcnt_imm((RING - 2) * kLoads + (E <= RING - 2 ? Scales<TX>::kLoads : 0)));
+    __builtin_amdgcn_s_waitcnt(vmcnt_imm((RING - 2) * kLoads + (E <= RING - 2 ? Scales<TX, WIDE>::kLoads : 0)));
     __builtin_amdgcn_s_barrier();
     constexpr int kMma = 2 * TX * TW;
 #pragma unroll
     for (int v = 0; v < kMma; ++v) {
       const int k = v / (TX * TW), i = v / TW % TX, j = v % TW;
-      acc[i][j] = mma32<WIDE, E>(cur.w[j][k], cur.x[i][k], acc[i][j], scale.w, scale.x[i]);
+      acc[i][j] = mma32<WIDE, E>(cur.w[j][k], cur.x[i][k], acc[i][j], sw, sx[i]);
       // the reads in the first three quarters, so that they are done at the barrier
       const int r0 = min(kReads, v * kReads * 4 / (3 * kMma)), r1 = min(kReads, (v + 1) * kReads * 4 / (3 * kMma));
 #pragma unroll
@@ -520,6 +657,29 @@ __device__ __forceinline__ void fp8_block(const Fp8Args& p) {
     }, std::make_integer_sequence<int, kTurn>());
   __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));  // (no load is left to land in LDS that another has by then)
   store_tiles(p, m0 + wm, n0 + wn, acc);
+  if constexpr (WIDE) {
+    if (seen.any()) {
+#pragma unroll 1
+      for (int i = 0; i < TX; ++i) {
+        const int row = m0 + wm + 32 * i + l32;
+        bool far, nan;
+        FarTile<32>::look(p, row, n0 + wn, 0, 1, far, nan);
+        const bool some = __any(far);
+#pragma unroll 1
+        for (int j = 0; j < TW; ++j) {
+          const int col = n0 + wn + 32 * j;
+          f32x16 v = {};
+          if (some) v = FarTile<32>::of(p, row, col, 0, 1);
+          if (nan) v += __builtin_nanf("");
+          if (far || nan) {  // (the lane that has stored these results before)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              store4(p, row, col + 8 * r + 4 * h, f32x4{v[4 * r], v[4 * r + 1], v[4 * r + 2], v[4 * r + 3]});
+          }
+        }
+      }
+    }
+  }
 }
 
 template <int TX, int TW, int RING, bool WIDE>
@@ -612,7 +772,7 @@ __device__ __forceinline__ void fp8_large(const Fp8Args& p) {
 
   using I0 = std::integral_constant<int, 0>;
   using I1 = std::integral_constant<int, 1>;
-  Scales<4> scale(p, m0 + 128 * wm, n0 + 128 * wn);
+  Scales<4, false> scale(p, m0 + 128 * wm, n0 + 128 * wn);
   // the first group, and of the second what the first one's turn does not load
   {
     const int second_k = begin(1);
@@ -674,7 +834,7 @@ __device__ __forceinline__ void fp8_large(const Fp8Args& p) {
         __builtin_amdgcn_s_waitcnt(kLdsDone);
         // Behind the loads that have to have landed there are 16 (12 of the group after the next,
         // four of the next one's tiles 2 and 3), and in a word's first group the scales' four or five.
-        __builtin_amdgcn_s_waitcnt(vmcnt_imm(16 + (U == 0 ? Scales<4>::kLoads : 0)));
+        __builtin_amdgcn_s_waitcnt(vmcnt_imm(16 + (U == 0 ? Scales<4, false>::kLoads : 0)));
         __builtin_amdgcn_s_barrier();
         __builtin_amdgcn_sched_barrier(0);
       }

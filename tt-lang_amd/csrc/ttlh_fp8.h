@@ -54,4 +54,19 @@ TTLH_FP8_HD uint32_t inverse_scale_bits(int code) {
   return static_cast<uint32_t>(254 - code) << 23;
 }
 
+// Codes as bf16 operands of a product (results in fp32), times powers of two whose product is that of
+// their scales 2^(ex - 127) and 2^(ew - 127).  bf16 has neither 256 x 2^120 nor 2^-9 x 2^-126, so ex and ew
+// themselves will not do: w's operand gets half of ew's exponent and 2^-21 (it is between 2^-94 and 2^51 then,
+// whatever ew is), and x's the rest.  Where that is below 2^-117, x's operand may lose bits (or is held at
+// 2^-126), but w's is less than 2^-25 then: products that are off are off by less than 2^-149.  Where it
+// is above 2^119 bf16 may not hold it: wide_far.  (NaN scales, ex or ew 255: the caller's.)
+constexpr int kWideMost = 246;  // 448 x 2^(246 - 127) is the largest that bf16 holds
+
+TTLH_FP8_HD int wide_w(int ew) { return (ew >> 1) + 42; }
+TTLH_FP8_HD int wide_rest(int ex, int ew) { return ex + (ew - wide_w(ew)); }  // before its limits
+TTLH_FP8_HD int wide_x(int rest) {
+  return rest < kScaleLeast ? kScaleLeast : rest > kWideMost ? kWideMost : rest;
+}
+TTLH_FP8_HD bool wide_far(int rest) { return rest > kWideMost; }
+
 }  // namespace ttlh

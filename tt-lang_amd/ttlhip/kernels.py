@@ -1217,7 +1217,8 @@ def matmul_fp8(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale:
     K is a multiple of 16; rows of codes start on 16 bytes.  fp32 accumulation; for a bf16
     result each eight neighbouring products are aligned to 2^-13 of the largest of them (the
     fp8 matrix instruction), for an f32 result they are added as fp32 (bf16 instructions, at
-    half the rate).  A NaN scale makes its row (of w: the block's outputs) NaN."""
+    half the rate).  Any scales, 0 (2^-127) among them; products and sums below 2^-126 may be lost.
+    A NaN scale makes its row (of w: the block's outputs) NaN."""
     what = "matmul_fp8"
     (M, K), xl = _fp8_rows(what, "x", x)
     (N, kw), wl = _fp8_rows(what, "w", w)
