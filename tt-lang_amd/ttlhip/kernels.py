@@ -1029,7 +1029,9 @@ def fp8_weights(w: torch.Tensor):
     full = full.view(blocks, FP8_GROUP, groups, FP8_GROUP)
     m, e = torch.frexp(full.abs().amax((1, 3)))  # 448 = 0.875 x 2^9
     e = torch.where(m > 0, e - 9 + (m > 0.875).int(), torch.full_like(e, -126)).clamp(min=-126)
-    codes = torch.ldexp(full, -e[:, None, :, None]).to(_E4M3).view(blocks * FP8_GROUP, -1)
+    # 2^-e by its bits (torch.ldexp takes it from pow(), which on the device is off by half a unit)
+    inv = (127 - e << 23).to(torch.int32).view(torch.float32)
+    codes = (full * inv[:, None, :, None]).to(_E4M3).view(blocks * FP8_GROUP, -1)
     scales = fp8_scales(blocks, k, w.device)
     bits = torch.ones(blocks, 4 * scales.shape[0], dtype=torch.uint8, device=w.device)
     bits[:, :groups] = (e + 127).to(torch.uint8)
