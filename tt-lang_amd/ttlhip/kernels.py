@@ -1016,12 +1016,14 @@ def fp8_scales(rows: int, dim: int, device=None) -> torch.Tensor:
 def fp8_weights(w: torch.Tensor):
     """(codes, scales) of weights w [outputs, inputs] for matmul_fp8(): e4m3 codes with
     the smallest power of two for each 128 x 128 block whose 448 fold holds it; made once,
-    with torch, where w is.  Weights that are not finite are refused."""
+    with torch, where w is.  Weights that are not finite in fp32 are refused."""
     if w.dim() != 2 or w.shape[1] == 0 or not w.is_floating_point():
         raise ValueError(f"fp8_weights: w must be a matrix of numbers, got {w.dtype} {tuple(w.shape)}")
-    w = w.detach().float()
-    if not bool(torch.isfinite(w).all()):
-        raise ValueError("fp8_weights: w must be finite")
+    w = w.detach()
+    if w.dtype != torch.float64:
+        w = w.float()
+    if not bool(torch.isfinite(w.float()).all()):
+        raise ValueError("fp8_weights: w must be finite in fp32")
     n, k = w.shape
     blocks, groups = -(-n // FP8_GROUP), -(-k // FP8_GROUP)
     full = w.new_zeros(blocks * FP8_GROUP, groups * FP8_GROUP)
@@ -1031,7 +1033,13 @@ def fp8_weights(w: torch.Tensor):
     e = torch.where(m > 0, e - 9 + (m > 0.875).int(), torch.full_like(e, -126)).clamp(min=-126)
     # 2^-e by its bits (torch.ldexp takes it from pow(), which on the device is off by half a unit)
     inv = (127 - e << 23).to(torch.int32).view(torch.float32)
-    codes = (full * inv[:, None, :, None]).to(_E4M3).view(blocks * FP8_GROUP, -1)
+    full = full * inv[:, None, :, None]
+    if full.dtype == torch.float64:
+        # to fp32 towards zero, the last place odd where something was lost: the codes are one rounding of w
+        near = full.float()
+        bits = near.view(torch.int32) - (near.double().abs() > full.abs()).int()
+        full = torch.where(near.double() == full, near, (bits | 1).view(torch.float32))
+    codes = full.to(_E4M3).view(blocks * FP8_GROUP, -1)
     scales = fp8_scales(blocks, k, w.device)
     bits = torch.ones(blocks, 4 * scales.shape[0], dtype=torch.uint8, device=w.device)
     bits[:, :groups] = (e + 127).to(torch.uint8)
