@@ -51,6 +51,20 @@ def test_weights_of_64_bits_that_fp32_does_not_hold_are_refused():
         K.fp8_weights(torch.full((2, 2), 1e39, dtype=F64))
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32, F64])
+def test_no_outputs(dtype):
+    codes, scales = K.fp8_weights(torch.empty(0, 640, dtype=dtype))
+    assert codes.shape == (0, 640) and codes.dtype == E4M3
+    assert scales.shape == (2, 0, 4) and scales.dtype == K.fp8_scales(0, 640, "cpu").dtype
+
+
+@pytest.mark.gpu
+def test_a_product_with_no_outputs():
+    c = torch.empty(3, 640, dtype=E4M3, device="cuda")
+    K.matmul_fp8(c, K.fp8_scales(3, 640), *K.fp8_weights(torch.empty(0, 640, device="cuda")),
+                 torch.empty(3, 0, dtype=torch.bfloat16, device="cuda"))
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32, F64])
 def test_weights_on_the_device_are_those_on_the_host(dtype):

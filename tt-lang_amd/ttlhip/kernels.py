@@ -1039,11 +1039,11 @@ def fp8_weights(w: torch.Tensor):
         near = full.float()
         bits = near.view(torch.int32) - (near.double().abs() > full.abs()).int()
         full = torch.where(near.double() == full, near, (bits | 1).view(torch.float32))
-    codes = full.to(_E4M3).view(blocks * FP8_GROUP, -1)
+    codes = full.to(_E4M3).view(blocks * FP8_GROUP, groups * FP8_GROUP)
     scales = fp8_scales(blocks, k, w.device)
     bits = torch.ones(blocks, 4 * scales.shape[0], dtype=torch.uint8, device=w.device)
     bits[:, :groups] = (e + 127).to(torch.uint8)
-    scales.view(torch.uint8).copy_(bits.view(blocks, -1, 4).transpose(0, 1))
+    scales.view(torch.uint8).copy_(bits.view(blocks, scales.shape[0], 4).transpose(0, 1))
     return codes[:n, :k].contiguous(), scales
 
 
