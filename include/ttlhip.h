@@ -574,10 +574,12 @@ int ttlh_rope(const void* x, void* out, int dtype, const void* positions, int po
  * The three operators that write codes give each group the smallest scale s = 2^e, e
  * from -126 on, with largest magnitude <= 448 s, and code = y / s rounded to nearest even
  * (ties to even); bytes of groups past the last one are 1 (2^-126).  Scales and codes are
- * those of the exact y; magnitudes below 2^-126, of y or of a gate's exponential, are right
- * to 2^-149.  A y that is not finite in fp32 makes its group's scale NaN and its codes 0:
- * products with that row are NaN.  dtype: bf16 or f32; *_ld: elements (codes: bytes) from
- * row to row.                                                                         */
+ * those of y computed in fp64, to 2^-40: where the exact y lies nearer to a border than that, the
+ * code or scale may be that of its other side (silu of 64 is 64 in fp64).  Magnitudes below 2^-126,
+ * of y or on the way to it (t / sqrt(..), act(g), act's exponential, gelu's integral
+ * (1 + erf(..)) / 2), are right to 2^-149.  A y or t that is not finite in fp32 makes its group's
+ * scale NaN and its codes 0: products with that row are NaN.  dtype: bf16 or f32; *_ld: elements
+ * (codes: bytes) from row to row.                                                     */
 /* y = x */
 int ttlh_fp8_quant(const void* x, int64_t x_ld, int dtype, void* codes, int64_t codes_ld,
                    void* scales, int64_t scales_ld, int64_t rows, int64_t dim, void* stream);

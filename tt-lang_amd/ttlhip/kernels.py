@@ -1151,7 +1151,7 @@ def rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, codes: torch.Tensor, sca
 
     x, residual: bf16 or f32 [rows, dim], any row pitch; weight: bf16 or f32 [dim]; eps
     positive.  total: gets t, rounded to x's dtype; it may be residual or x itself.  The norm is that
-    of t before this rounding."""
+    of t before this rounding.  Codes and scales are those of the norm in 64 bits."""
     what = "rms_norm_fp8"
     shape, ld = _fp8_rows(what, "x", x)
     rows, dim = shape
@@ -1198,7 +1198,8 @@ def glu_fp8(gate: torch.Tensor, up: torch.Tensor, codes: torch.Tensor, scales: t
             act: str = "silu", stream=None) -> None:
     """The gated activation act(gate) * up into codes and scales as quant_fp8() makes
     them.  gate, up: bf16 or f32 [rows, dim], any row pitch (the halves of one product's
-    result).  act: "silu", g / (1 + e^-g), or "gelu", g (1 + erf(g / sqrt 2)) / 2."""
+    result).  act: "silu", g / (1 + e^-g), or "gelu", g (1 + erf(g / sqrt 2)) / 2.  Codes and
+    scales are those of the product in 64 bits."""
     shape, gl = _fp8_rows("glu_fp8", "gate", gate)
     _, ul = _fp8_rows("glu_fp8", "up", up, shape)
     if up.dtype != gate.dtype:
