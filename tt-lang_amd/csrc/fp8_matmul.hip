@@ -488,26 +488,30 @@ template <int TX, bool WIDE>
 struct Scales {
   const uint32_t* ws;
   const uint32_t* xs[TX];
+  uint32_t lane0 = 0;
   uint32_t w, x[TX], next_w, next_x[TX];
   int words;
   uint32_t past;  // bytes of the last word that are of no group: those scales may be anything
-  // What the waits below count: the vector loads that load() cannot do without, x's, whose addresses are a
-  // lane's own.  w's address is the same for a wave, so its load may be a scalar one, which vmcnt does not
-  // see; where it is a vector load, the waits are one load stricter than they have to be.
-  static constexpr int kLoads = TX;
+  // What the waits below count: loads that are vector loads whatever the compiler does.  x's addresses are a
+  // lane's own.  w's is the same for a wave, so its load may be a scalar one, which vmcnt does not see; but
+  // for `lane0`, which the compiler does not know to be 0.  (WIDE: not counted, the waits one load stricter
+  // than they may have to be, and w's scales in scalar registers.  2048 x 4096 x 4096 into f32 64.3 us, 67 the
+  // other way; 250 x 4000 x 4096 into bf16 11.2 us so, 10.8 the other way.)
+  static constexpr int kLoads = WIDE ? TX : TX + 1;
 
   __device__ __forceinline__ Scales(const Fp8Args& p, int m, int n) {
     words = (p.K + kFp8Word - 1) / kFp8Word;
     const int last = (p.K - 1) / kFp8Group & 3;
     past = last == 3 ? 0u : ~0u << (8 * last + 8);
     ws = p.ws + min(n, p.N - 1) / kFp8Group;
+    if constexpr (!WIDE) asm volatile("" : "+v"(lane0));
 #pragma unroll
     for (int i = 0; i < TX; ++i) xs[i] = p.xs + min(m + 32 * i + static_cast<int>(threadIdx.x & 31), p.M - 1);
     load(p, 0);
   }
   __device__ __forceinline__ void load(const Fp8Args& p, int word) {
     word = min(word, words - 1);
-    next_w = ws[word * p.ws_ld];
+    next_w = (ws + word * p.ws_ld)[lane0];
 #pragma unroll
     for (int i = 0; i < TX; ++i) next_x[i] = xs[i][word * p.xs_ld];
   }
@@ -833,7 +837,7 @@ __device__ __forceinline__ void fp8_large(const Fp8Args& p) {
       if (i == 0 || i == 2) {
         __builtin_amdgcn_s_waitcnt(kLdsDone);
         // Behind the loads that have to have landed there are 16 (12 of the group after the next,
-        // four of the next one's tiles 2 and 3), and in a word's first group the scales' four or five.
+        // four of the next one's tiles 2 and 3), and in a word's first group the scales' five.
         __builtin_amdgcn_s_waitcnt(vmcnt_imm(16 + (U == 0 ? Scales<4, false>::kLoads : 0)));
         __builtin_amdgcn_s_barrier();
         __builtin_amdgcn_sched_barrier(0);
