@@ -55,12 +55,11 @@ typedef __attribute__((address_space(3))) void lds_void;
 constexpr int vmcnt_imm(int n) { return 0x0F70 | (n & 0xF) | ((n >> 4) << 14); }
 constexpr int kLdsDone = 0xC07F;
 
-// until at most n rounds of LOADS loads are outstanding
+// until at most n (to 2) rounds of LOADS loads are outstanding
 template <int LOADS>
 __device__ __forceinline__ void wait_behind(int n) {
   static_assert(2 * LOADS < 64, "what the counter holds");
-  if (n >= 3) __builtin_amdgcn_s_waitcnt(vmcnt_imm(3 * LOADS < 63 ? 3 * LOADS : 63));
-  else if (n == 2) __builtin_amdgcn_s_waitcnt(vmcnt_imm(2 * LOADS));
+  if (n == 2) __builtin_amdgcn_s_waitcnt(vmcnt_imm(2 * LOADS));
   else if (n == 1) __builtin_amdgcn_s_waitcnt(vmcnt_imm(LOADS));
   else __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
 }
@@ -115,12 +114,11 @@ __device__ __forceinline__ int scale_byte(uint32_t s) {
   return static_cast<int>(s >> (8 * J) & 255);
 }
 
-// acc += A . B over one group; sa, sb: dwords of scales, the group's in byte J (WIDE: the operands'
-// scales, of wide_w and wide_x)
-template <bool WIDE, int J>
+// acc += A . B over one group; sa, sb: its scales (WIDE: those of the operands, of wide_w and wide_x)
+template <bool WIDE>
 __device__ __forceinline__ f32x4 mma16(const Frag& a, const Frag& b, f32x4 acc, uint32_t sa, uint32_t sb) {
   if constexpr (!WIDE) {
-    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(all8(a), all8(b), acc, 0, 0, J, static_cast<int>(sa), J,
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(all8(a), all8(b), acc, 0, 0, 0, static_cast<int>(sa), 0,
                                                             static_cast<int>(sb));
   } else {
 #pragma unroll
@@ -258,22 +256,19 @@ struct Seen {
 };
 
 // MT x 16 rows of x, NT x 16 of w a workgroup; wave v of WAVES takes the groups v, v + WAVES ..
-// of K, AHEAD (2 to 4) of them in flight.
-template <int MT, int NT, int WAVES, int AHEAD, bool WIDE>
-__device__ __forceinline__ void fp8_direct(const Fp8Args& p) {
+// of K, two of them in flight.
+template <int MT, int NT, int WAVES, bool WIDE>
+__global__ __launch_bounds__(WAVES * 64) void fp8_direct_kernel(const Fp8Args p) {
   static_assert(WAVES % 4 == 0 && 128 % (NT * 16) == 0, "one byte of the scales a wave, one block of w's");
   constexpr int kRows = (MT + NT) * 16;  // of a wave's group: those of w, then those of x
   constexpr int kSlot = kRows * kFp8Group;
-  __shared__ __attribute__((aligned(16))) uint8_t b0[WAVES * kSlot], b1[WAVES * kSlot],
-      b2[AHEAD > 2 ? WAVES * kSlot : 16], b3[AHEAD > 3 ? WAVES * kSlot : 16];
+  __shared__ __attribute__((aligned(16))) uint8_t b0[WAVES * kSlot], b1[WAVES * kSlot];
   int bm, bn;
   block_of(p, bm, bn);
   // (uniform, and known to be: an MFMA behind a branch that the compiler takes for divergent
   // runs whether or not its lanes are masked)
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const auto slot = [&](int a) -> uint8_t* {
-    return (a == 0 ? b0 : a == 1 ? b1 : a == 2 ? b2 : b3) + wave * kSlot;
-  };
+  const auto slot = [&](int a) -> uint8_t* { return (a ? b1 : b0) + wave * kSlot; };
   const int m0 = bm * MT * 16, n0 = bn * NT * 16;
   const int groups = (p.K + kFp8Group - 1) / kFp8Group;
   const int n = groups > wave ? (groups - wave + WAVES - 1) / WAVES : 0;  // of this wave
@@ -296,7 +291,7 @@ __device__ __forceinline__ void fp8_direct(const Fp8Args& p) {
 #pragma unroll
   for (int i = 0; i < MT; ++i)
     xs[i] = reinterpret_cast<const uint8_t*>(p.xs + min(m0 + 16 * i + r, p.M - 1)) + (wave & 3);
-  uint32_t sw[AHEAD], sx[AHEAD][MT];
+  uint32_t sw[2], sx[2][MT];
   const auto load = [&](int a, int i) {  // (past the wave's last group: zeros)
     const int g = wave + WAVES * i, k = g * kFp8Group, word = min(g, groups - 1) >> 2;
     const bool even = k + chunk < p.K, odd = k + (chunk ^ 64) < p.K;
@@ -344,24 +339,24 @@ __device__ __forceinline__ void fp8_direct(const Fp8Args& p) {
 #pragma unroll
     for (int i = 0; i < MT; ++i)
 #pragma unroll
-      for (int j = 0; j < NT; ++j) acc[i][j] = mma16<WIDE, 0>(w[j], x[i], acc[i][j], sw[a], sx[a][i]);
+      for (int j = 0; j < NT; ++j) acc[i][j] = mma16<WIDE>(w[j], x[i], acc[i][j], sw[a], sx[a][i]);
     __builtin_amdgcn_sched_barrier(0);  // (the slot is read before it is loaded anew)
   };
 #pragma unroll
-  for (int a = 0; a < AHEAD; ++a) load(a, a);
+  for (int a = 0; a < 2; ++a) load(a, a);
   int i = 0;
-  for (; i + AHEAD < n; i += AHEAD) {
+  for (; i + 2 < n; i += 2) {
 #pragma unroll
-    for (int a = 0; a < AHEAD; ++a) {
-      wait_behind<kLoads>(AHEAD - 1);
+    for (int a = 0; a < 2; ++a) {
+      wait_behind<kLoads>(1);
       multiply(a);
-      load(a, i + a + AHEAD);
+      load(a, i + a + 2);
     }
   }
 #pragma unroll
-  for (int a = 0; a < AHEAD; ++a)
+  for (int a = 0; a < 2; ++a)
     if (i + a < n) {
-      wait_behind<kLoads>(AHEAD - 1 - a);
+      wait_behind<kLoads>(1 - a);
       multiply(a);
     }
   __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));  // (no load of a wave without groups is left to land)
@@ -401,15 +396,9 @@ __device__ __forceinline__ void fp8_direct(const Fp8Args& p) {
   }
 }
 
-template <int MT, int NT, int WAVES, int AHEAD, bool WIDE>
-__global__ __launch_bounds__(WAVES * 64) void fp8_direct_kernel(const Fp8Args p) {
-  fp8_direct<MT, NT, WAVES, AHEAD, WIDE>(p);
-}
-
 // --- more results ---------------------------------------------------------------
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
-
 
 // One k = 64 step of a 32 x 32 tile; E: the scales' byte (WIDE: as in mma16)
 template <bool WIDE, int E>
@@ -532,19 +521,20 @@ __device__ __forceinline__ void each_until(F f, std::integer_sequence<int, I...>
 }
 
 // A wave has TX x TW tiles of 32 x 32 (of x's rows, of w's), four waves a block of 64 TX x 64 TW; a
-// ring of RING (3 or 4) buffers.  A group's fragments are read while the one before it is multiplied.
-template <int TX, int TW, int RING, bool WIDE>
-__device__ __forceinline__ void fp8_block(const Fp8Args& p) {
+// ring of three buffers.  A group's fragments are read while the one before it is multiplied.
+template <int TX, int TW, bool WIDE>
+__global__ __launch_bounds__(256, TX * TW < 3 ? 2 : 1) void fp8_block_kernel(const Fp8Args p) {
+  constexpr int kRing = 3;
   constexpr int kXBytes = 64 * TX * kFp8Group, kWBytes = 64 * TW * kFp8Group;
-  __shared__ __attribute__((aligned(16))) uint8_t x0[kXBytes], x1[kXBytes], x2[kXBytes],
-      x3[RING > 3 ? kXBytes : 16], w0[kWBytes], w1[kWBytes], w2[kWBytes], w3[RING > 3 ? kWBytes : 16];
+  __shared__ __attribute__((aligned(16))) uint8_t x0[kXBytes], x1[kXBytes], x2[kXBytes], w0[kWBytes], w1[kWBytes],
+      w2[kWBytes];
   const auto xbuf = [&](auto q) -> uint8_t* {
-    constexpr int Q = decltype(q)::value % RING;
-    return Q == 0 ? x0 : Q == 1 ? x1 : Q == 2 ? x2 : x3;
+    constexpr int Q = decltype(q)::value % kRing;
+    return Q == 0 ? x0 : Q == 1 ? x1 : x2;
   };
   const auto wbuf = [&](auto q) -> uint8_t* {
-    constexpr int Q = decltype(q)::value % RING;
-    return Q == 0 ? w0 : Q == 1 ? w1 : Q == 2 ? w2 : w3;
+    constexpr int Q = decltype(q)::value % kRing;
+    return Q == 0 ? w0 : Q == 1 ? w1 : w2;
   };
   const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
   int bm, bn;
@@ -607,14 +597,14 @@ __device__ __forceinline__ void fp8_block(const Fp8Args& p) {
     for (int i = 0; i < kLoads; ++i)
       load_piece(q, decltype(q)::value * kFp8Group, decltype(q)::value * kFp8Group + chunk < p.K, i);
     return true;
-  }, std::make_integer_sequence<int, RING>());
-  wait_behind<kLoads>(RING - 1);
+  }, std::make_integer_sequence<int, kRing>());
+  wait_behind<kLoads>(kRing - 1);
   __builtin_amdgcn_s_barrier();
 #pragma unroll
   for (int y = 0; y < kReads; ++y) read_piece(std::integral_constant<int, 0>(), f0, y);
 
   // Group s = U of a turn of the loop, whose fragments are in cur.  Behind the barrier every wave
-  // has read its fragments of group s, so its buffers take group s + RING (past the last one:
+  // has read its fragments of group s, so its buffers take group s + kRing (past the last one:
   // zeros), and group s + 1 has landed.
   const auto group = [&](auto uu, Frags& cur, Frags& nxt, int s) {
     constexpr int U = decltype(uu)::value, E = U % 4;
@@ -629,11 +619,11 @@ __device__ __forceinline__ void fp8_block(const Fp8Args& p) {
       sw = wide_w(scale_byte<E>(sw));
     }
     if constexpr (WIDE) __builtin_amdgcn_sched_barrier(0);  // (in front of the barrier, where waves wait)
-    const int k2 = (s + RING) * kFp8Group;
+    const int k2 = (s + kRing) * kFp8Group;
     const bool there = k2 + chunk < p.K;
     __builtin_amdgcn_s_waitcnt(kLdsDone);
     // (are the scales' loads, at a word's first group, among those behind group s + 1's?)
-    __builtin_amdgcn_s_waitcnt(vmcnt_imm((RING - 2) * kLoads + (E <= RING - 2 ? Scales<TX, WIDE>::kLoads : 0)));
+    __builtin_amdgcn_s_waitcnt(vmcnt_imm((kRing - 2) * kLoads + (E <= kRing - 2 ? Scales<TX, WIDE>::kLoads : 0)));
     __builtin_amdgcn_s_barrier();
     constexpr int kMma = 2 * TX * TW;
 #pragma unroll
@@ -653,7 +643,7 @@ __device__ __forceinline__ void fp8_block(const Fp8Args& p) {
     }
     return s + 1 < groups;
   };
-  constexpr int kTurn = RING == 3 ? 12 : 4;
+  constexpr int kTurn = 12;  // whole rings, words and pairs of fragments
   for (int s = 0; s < groups; s += kTurn)
     each_until([&](auto uu) {
       constexpr int U = decltype(uu)::value;
@@ -686,11 +676,6 @@ __device__ __forceinline__ void fp8_block(const Fp8Args& p) {
   }
 }
 
-template <int TX, int TW, int RING, bool WIDE>
-__global__ __launch_bounds__(256, TX * TW * RING < 8 ? 2 : 1) void fp8_block_kernel(const Fp8Args p) {
-  fp8_block<TX, TW, RING, WIDE>(p);
-}
-
 // 256 x 256 results a workgroup, 128 x 128 a wave.  Two buffers of a group are all that LDS holds, so
 // a buffer is given back in parts.  A wave keeps all fragments of w of a group, and goes through
 // x's four tiles in turn, one read ahead; while the last one is multiplied it reads the next
@@ -703,7 +688,7 @@ __global__ __launch_bounds__(256, TX * TW * RING < 8 ? 2 : 1) void fp8_block_ker
 // what bounds this kernel is power (workgroups set apart in time by up to 6 us, so that their stores do
 // not meet: no change).
 template <bool CUT>
-__device__ __forceinline__ void fp8_large(const Fp8Args& p) {
+__global__ __launch_bounds__(256, 1) void fp8_large_kernel(const Fp8Args p) {
   constexpr int kBytes = 256 * kFp8Group;
   __shared__ __attribute__((aligned(16))) uint8_t xa0[kBytes / 2], xb0[kBytes / 2], xa1[kBytes / 2],
       xb1[kBytes / 2], w0[kBytes], w1[kBytes];  // xa: tiles 0 and 1 of both halves of the rows
@@ -856,11 +841,6 @@ __device__ __forceinline__ void fp8_large(const Fp8Args& p) {
   store_tiles(p, m0 + 128 * wm, n0 + 128 * wn, acc);
 }
 
-template <bool CUT>
-__global__ __launch_bounds__(256, 1) void fp8_large_kernel(const Fp8Args p) {
-  fp8_large<CUT>(p);
-}
-
 // --- which of them ------------------------------------------------------------------
 
 // A kernel's block of results, and how long a group of K takes it, in us, measured with cold
@@ -973,16 +953,16 @@ extern "C" int ttlh_matmul_fp8(const void* x, int64_t x_ld, const void* x_scale,
     return check_launch("a kernel of ttlh_matmul_fp8");
   };
   switch (i) {
-    case 0: return run(fp8_direct_kernel<1, 1, 8, 2, false>, fp8_direct_kernel<1, 1, 8, 2, true>);
-    case 1: return run(fp8_direct_kernel<2, 1, 8, 2, false>, fp8_direct_kernel<2, 1, 8, 2, true>);
-    case 2: return run(fp8_direct_kernel<2, 2, 4, 2, false>, fp8_direct_kernel<2, 2, 4, 2, true>);
-    case 3: return run(fp8_direct_kernel<2, 2, 8, 2, false>, fp8_direct_kernel<2, 2, 8, 2, true>);
-    case 4: return run(fp8_direct_kernel<2, 4, 4, 2, false>, fp8_direct_kernel<2, 4, 4, 2, true>);
-    case 5: return run(fp8_direct_kernel<4, 4, 4, 2, false>, fp8_direct_kernel<4, 4, 4, 2, true>);
-    case 6: return run(fp8_block_kernel<1, 1, 3, false>, fp8_block_kernel<1, 1, 3, true>);
-    case 7: return run(fp8_block_kernel<1, 2, 3, false>, fp8_block_kernel<1, 2, 3, true>);
-    case 8: return run(fp8_block_kernel<2, 2, 3, false>, fp8_block_kernel<2, 2, 3, true>);
-    case 9: return run(fp8_block_kernel<2, 4, 3, false>, fp8_block_kernel<2, 4, 3, true>);
+    case 0: return run(fp8_direct_kernel<1, 1, 8, false>, fp8_direct_kernel<1, 1, 8, true>);
+    case 1: return run(fp8_direct_kernel<2, 1, 8, false>, fp8_direct_kernel<2, 1, 8, true>);
+    case 2: return run(fp8_direct_kernel<2, 2, 4, false>, fp8_direct_kernel<2, 2, 4, true>);
+    case 3: return run(fp8_direct_kernel<2, 2, 8, false>, fp8_direct_kernel<2, 2, 8, true>);
+    case 4: return run(fp8_direct_kernel<2, 4, 4, false>, fp8_direct_kernel<2, 4, 4, true>);
+    case 5: return run(fp8_direct_kernel<4, 4, 4, false>, fp8_direct_kernel<4, 4, 4, true>);
+    case 6: return run(fp8_block_kernel<1, 1, false>, fp8_block_kernel<1, 1, true>);
+    case 7: return run(fp8_block_kernel<1, 2, false>, fp8_block_kernel<1, 2, true>);
+    case 8: return run(fp8_block_kernel<2, 2, false>, fp8_block_kernel<2, 2, true>);
+    case 9: return run(fp8_block_kernel<2, 4, false>, fp8_block_kernel<2, 4, true>);
     default:  // (bf16 results alone)
       return K % kFp8Group ? run(fp8_large_kernel<true>, fp8_large_kernel<true>)
                            : run(fp8_large_kernel<false>, fp8_large_kernel<false>);
