@@ -600,7 +600,8 @@ int ttlh_fp8_glu(const void* gate, int64_t gate_ld, const void* up, int64_t up_l
  * multiple of 16, rows of codes 16-byte aligned.  fp32 accumulation.  Into bf16, each eight
  * neighbouring products are aligned to 2^-13 of the largest of them before they are added
  * (the fp8 MFMA); into f32 they are added as fp32.  Any scales, 0 (2^-127) among them; products
- * and sums below 2^-126 may be lost.                                                  */
+ * and sums below 2^-126 may be lost.  M, N below 2^28, K up to 2^28, and no more blocks of results
+ * (ttlh_matmul_fp8_form) than a launch has: fewer than 2^23 of the smaller ones.      */
 int ttlh_matmul_fp8(const void* x, int64_t x_ld, const void* x_scale, int64_t xs_ld, const void* w,
                     int64_t w_ld, const void* w_scale, int64_t ws_ld, void* c, int c_dtype,
                     int64_t c_ld, int64_t M, int64_t N, int64_t K, void* stream);
